@@ -139,7 +139,7 @@ sa_status sa_kvcache_reset(sa_kvcache* cache, sa_stream_t stream);
 sa_status sa_kvcache_reserve(sa_kvcache* cache, int seq, int n_tokens, sa_stream_t stream);
 /* Give sequence seq an explicit page list (host array; replaces its current
  * pages).  Each page must be in the pool, listed once, and free or already
- * seq's (SA_ERANGE / SA_EINVAL otherwise).  A committed length beyond the new
+ * one of seq's (SA_ERANGE / SA_EINVAL otherwise).  A committed length beyond the new
  * capacity is cut to it. */
 sa_status sa_kvcache_set_pages(sa_kvcache* cache, int seq, const int32_t* pages,
                                int n_pages, sa_stream_t stream);
@@ -155,6 +155,35 @@ int sa_kvcache_capacity(const sa_kvcache* cache, int seq);
  * once; NULL = 0..n_seqs-1). */
 sa_status sa_kvcache_commit(sa_kvcache* cache, const int32_t* seqs, int n_seqs, int n,
                             sa_stream_t stream);
+/* ---- Sequences that share pages ----
+ * No counterpart in the reference, whose cache has one dense row per
+ * sequence.  A page that several sequences list is never written: an append
+ * whose tokens would fall into one is refused (SA_EINVAL), which only happens
+ * after sa_kvcache_set_len has moved a length back into shared pages.  A page
+ * returns to the pool when the last sequence drops it.  Both calls decide on
+ * the host and enqueue one small launch per 64 rows (more where many table
+ * entries change); a refused call changes and enqueues nothing.  They are
+ * refused while another device than the cache's is current. */
+
+/* Sequence dst gives its pages back and becomes the first n_tokens committed
+ * tokens of src (n_tokens <= src's length, else SA_ERANGE): src's whole pages
+ * are shared, and where n_tokens ends inside a page dst gets a page of its own
+ * with a copy of those tokens (every layer).  dst has room for n_tokens
+ * rounded up to whole pages; reserve more before appending past that.
+ * SA_EFULL if there is no page for the copy. */
+sa_status sa_kvcache_fork(sa_kvcache* cache, int dst, int src, int n_tokens, sa_stream_t stream);
+
+/* The reordering of states of a beam search, at once for all i: sequence
+ * rows[i] becomes what sequence parents[i] was before the call (host arrays of
+ * n; each row listed once, any parents, which need not be among the rows).
+ * Whole pages are shared.  The page that a parent's length ends inside moves
+ * to one of its children where the parent itself is replaced; every other
+ * child gets a page of its own with a copy.  A row keeps its capacity, or gets
+ * the parent's whole and partial pages where those are more.  A row that is
+ * its own parent is left as it is.  SA_EFULL if the pool has too few pages. */
+sa_status sa_kvcache_reorder(sa_kvcache* cache, const int32_t* rows, const int32_t* parents, int n,
+                             sa_stream_t stream);
+
 /* Device pointers into the cache, for callers that drive kernels themselves. */
 void* sa_kvcache_k_pool(sa_kvcache* cache, int layer);
 void* sa_kvcache_v_pool(sa_kvcache* cache, int layer);
@@ -246,6 +275,45 @@ sa_status sa_paged_decode(const sa_kvcache* cache, int layer, const float* q,
                           int n_seq, const int32_t* seq_ids, int n_q_heads, int n_pending,
                           float scale, float* out, void* ws, size_t ws_bytes,
                           sa_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Paged decode attention with a sliding window and sinks.
+ *
+ * No counterpart in the reference.  As sa_paged_decode, but sequence i, of
+ * n = seq_len[seq_ids[i]] + n_pending tokens, attends over its last `window`
+ * tokens (window >= 1; all of them if n is smaller) and its first n_sink
+ * (n_sink >= 0), each token once:
+ *   out = softmax(scale q k_t) v over t < n with n - 1 - t < window or t < n_sink.
+ * Only the pages of those tokens are read.  A sequence of length 0 gets a zero
+ * output.  head_dim 64 or 128, at most 64 query heads per KV head; q
+ * [n_seq][n_q_heads][D] fp32, out likewise, accumulation in fp32.  q, out and
+ * ws 16-byte aligned; ws of sa_paged_decode_window_ws_bytes(...) bytes
+ * (n_seq as in the call); calls that overlap on one workspace race.
+ * ------------------------------------------------------------------------ */
+size_t sa_paged_decode_window_ws_bytes(const sa_kvcache* cache, int n_seq, int n_q_heads, int window, int n_sink);
+sa_status sa_paged_decode_window(const sa_kvcache* cache, int layer, const float* q,
+                                 int n_seq, const int32_t* seq_ids, int n_q_heads, int n_pending,
+                                 int window, int n_sink, float scale, float* out,
+                                 void* ws, size_t ws_bytes, sa_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Paged decode attention of sequences that share their leading pages.
+ *
+ * No counterpart in the reference.  Results as sa_paged_decode's (to fp32
+ * rounding), with the n_seq rows in groups of consecutive rows: group_sizes
+ * [n_groups] (host, each >= 1, adding up to n_seq), or NULL with n_groups = 0
+ * for one group of all.  What a group shares is found from the page table: the
+ * whole pages that all its rows list alike from the start on
+ * (sa_kvcache_fork, sa_kvcache_reorder).  They are read once for up to 64 rows
+ * of the group; the tokens behind them, and rows that share nothing, are
+ * attended row by row.  Other arguments, shapes and ws as in
+ * sa_paged_decode_window.
+ * ------------------------------------------------------------------------ */
+size_t sa_paged_decode_shared_ws_bytes(const sa_kvcache* cache, int n_seq, int n_q_heads);
+sa_status sa_paged_decode_shared(const sa_kvcache* cache, int layer, const float* q,
+                                 int n_seq, const int32_t* seq_ids, const int32_t* group_sizes, int n_groups,
+                                 int n_q_heads, int n_pending, float scale, float* out,
+                                 void* ws, size_t ws_bytes, sa_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * One decode step of a layer in one call: sa_qknorm_rope_append with S = 1,

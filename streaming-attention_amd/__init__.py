@@ -76,6 +76,8 @@ SIGNATURES = {
     "sa_kvcache_len": (_I, [_P, _I]),
     "sa_kvcache_capacity": (_I, [_P, _I]),
     "sa_kvcache_commit": (_I, [_P, _P, _I, _I, _P]),
+    "sa_kvcache_fork": (_I, [_P, _I, _I, _I, _P]),
+    "sa_kvcache_reorder": (_I, [_P, _P, _P, _I, _P]),
     "sa_kvcache_k_pool": (_P, [_P, _I]),
     "sa_kvcache_v_pool": (_P, [_P, _I]),
     "sa_kvcache_block_table": (_P, [_P]),
@@ -93,6 +95,10 @@ SIGNATURES = {
     "sa_axpby_f32": (_I, [_P, _F, _P, _F, _SZ, _P, _P]),
     "sa_paged_decode_ws_bytes": (_SZ, [_P, _I, _I]),
     "sa_paged_decode": (_I, [_P, _I, _P, _I, _P, _I, _I, _F, _P, _P, _SZ, _P]),
+    "sa_paged_decode_window_ws_bytes": (_SZ, [_P, _I, _I, _I, _I]),
+    "sa_paged_decode_window": (_I, [_P, _I, _P, _I, _P, _I, _I, _I, _I, _F, _P, _P, _SZ, _P]),
+    "sa_paged_decode_shared_ws_bytes": (_SZ, [_P, _I, _I]),
+    "sa_paged_decode_shared": (_I, [_P, _I, _P, _I, _P, _P, _I, _I, _I, _F, _P, _P, _SZ, _P]),
     "sa_append_decode_partials": (_I, [_P, _I, _P, _I, _I, _P, _I, _P, _P, _F, _P, _P, _I, _F, _P, _P, _P,
                                        _SZ, _I, _P]),
     "sa_kvcache_gather": (_I, [_P, _I, _I, _I, _P, _P, _P]),
@@ -145,6 +151,10 @@ def check(status: int) -> None:
 
 def _ptr(t) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+def _nbytes(t) -> int:
+    return t.numel() * t.element_size()
 
 
 def _rows(ids, n: int):
@@ -261,6 +271,17 @@ class KVCache:
             arr = (C.c_int32 * len(seqs))(*[int(s) for s in seqs])
             check(lib().sa_kvcache_commit(self.handle, arr, len(seqs), n, _stream(stream)))
 
+    def fork(self, dst: int, src: int, n_tokens: int, stream=None) -> None:
+        """Sequence dst becomes the first n_tokens tokens of src (whole pages
+        shared, a page that they end inside copied)."""
+        check(lib().sa_kvcache_fork(self.handle, dst, src, n_tokens, _stream(stream)))
+
+    def reorder(self, rows, parents, stream=None) -> None:
+        """At once: sequence rows[i] becomes what parents[i] was (host ints)."""
+        rows = [int(r) for r in rows]
+        check(lib().sa_kvcache_reorder(self.handle, _rows(rows, len(rows)), _rows(parents, len(rows)), len(rows),
+                                       _stream(stream)))
+
     def k_pool(self, layer: int) -> int:
         return lib().sa_kvcache_k_pool(self.handle, layer)
 
@@ -303,6 +324,50 @@ class KVCache:
         check(lib().sa_paged_decode(self.handle, layer, _ptr(_f32(q, "q")), n_seq, _rows(seq_ids, n_seq), Hq,
                                     n_pending, scale, _ptr(out), _ptr(ws), ws.numel(), _stream(stream)))
         return out
+
+    def decode_window_ws_bytes(self, n_seq: int, n_q_heads: int, window: int, n_sink: int = 0) -> int:
+        return lib().sa_paged_decode_window_ws_bytes(self.handle, n_seq, n_q_heads, window, n_sink)
+
+    def decode_window(self, layer: int, q, scale: float, window: int, n_sink: int = 0, n_pending: int = 0, out=None,
+                      ws=None, seq_ids=None, stream=None):
+        """decode over each sequence's last `window` tokens and its first
+        n_sink: q [n_seq, Hq, D] -> out [n_seq, Hq, D]."""
+        n_seq, Hq, _ = q.shape
+        out, ws = self._out_ws(q, out, ws, lambda: self.decode_window_ws_bytes(n_seq, Hq, window, n_sink))
+        check(lib().sa_paged_decode_window(self.handle, layer, _ptr(_f32(q, "q")), n_seq, _rows(seq_ids, n_seq), Hq,
+                                           n_pending, window, n_sink, scale, _ptr(out), _ptr(ws), _nbytes(ws),
+                                           _stream(stream)))
+        return out
+
+    def decode_shared_ws_bytes(self, n_seq: int, n_q_heads: int) -> int:
+        return lib().sa_paged_decode_shared_ws_bytes(self.handle, n_seq, n_q_heads)
+
+    def decode_shared(self, layer: int, q, scale: float, groups=None, n_pending: int = 0, out=None, ws=None,
+                      seq_ids=None, stream=None):
+        """decode of rows in groups (sizes of runs of consecutive rows; None:
+        one group) whose shared leading pages are read once per group:
+        q [n_seq, Hq, D] -> out [n_seq, Hq, D]."""
+        n_seq, Hq, _ = q.shape
+        out, ws = self._out_ws(q, out, ws, lambda: self.decode_shared_ws_bytes(n_seq, Hq))
+        n_groups = 0 if groups is None else len(groups)
+        check(lib().sa_paged_decode_shared(self.handle, layer, _ptr(_f32(q, "q")), n_seq, _rows(seq_ids, n_seq),
+                                           _rows(groups, n_groups), n_groups, Hq, n_pending, scale, _ptr(out),
+                                           _ptr(ws), _nbytes(ws), _stream(stream)))
+        return out
+
+    def _out_ws(self, q, out, ws, need):
+        """The output and workspace of a decode of q, made where not given."""
+        import torch
+        if q.shape[-1] != self.desc.head_dim:
+            raise ValueError("q must be [n_seq, Hq, head_dim]")
+        if out is None:
+            out = torch.empty_like(q)
+        elif out.shape != q.shape:
+            raise ValueError("out must have q's shape")
+        if ws is None:
+            ws = torch.empty(max(need(), 16), dtype=torch.uint8, device=q.device)
+        _f32(out, "out")
+        return out, ws
 
     def append_decode(self, layer: int, q, k, v, scale: float, q_norm_w=None, k_norm_w=None, eps: float = 1e-6,
                       rope=None, out=None, q_out=None, ws=None, commit: bool = False, seq_ids=None, stream=None):

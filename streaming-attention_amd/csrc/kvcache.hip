@@ -16,10 +16,12 @@
 // the order they were called.
 #include "sa_internal.h"
 #include "page_table.h"
+#include "ranges.h"
 
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
+#include <new>
 #include <vector>
 
 struct sa_kvcache {
@@ -99,6 +101,98 @@ sa_status publish_lens(sa_kvcache* c, const int32_t* rows, int n, int val, int a
 }
 
 sa_status refused(const Verdict& v) { return fail(v.status, v.msg); }
+
+// Kernels of a cache run on its own device; a call made while another one is
+// current is refused.
+sa_status on_cache_device(const sa_kvcache* c) {
+    int dev = 0;
+    SA_HIP_TRY(hipGetDevice(&dev));
+    if (dev != c->device) return fail(SA_EINVAL, "the cache lives on another device than the current one");
+    return SA_OK;
+}
+
+// ---------------------------------------------------------------------------
+// Publishing a fork or a reorder: table entries, lengths and page copies of
+// several rows in one launch.  Rows that share their prompt differ in a few
+// entries behind it, so only entries that change are sent.
+// ---------------------------------------------------------------------------
+constexpr int kEdits = 160, kCopies = 64;
+struct TableEdit {
+    int32_t row, col, page;
+};
+struct RowsArgs {
+    int32_t* table;
+    int32_t* lens;
+    char* pool;
+    size_t layer_bytes;
+    int max_pages, n_kv, head_bytes, row_bytes;   // head_bytes: 64 rows of one head of a page
+    int n_edits, n_lens, n_copies;
+    TableEdit edit[kEdits];
+    int32_t len_row[kRowsPerLaunch], len[kRowsPerLaunch];
+    PageCopy copy[kCopies];
+};
+static_assert(sizeof(RowsArgs) <= 4096, "kernel arguments");
+
+// Block (x, y) copies head slice x (layer, K or V, head) of page pair y.  No
+// page is both read and written in a launch.  Bound: HBM; the whole launch is
+// the latency of a round trip for a few pages.
+__global__ void __launch_bounds__(256) update_rows_kernel(RowsArgs a) {
+    if (blockIdx.x == 0 && blockIdx.y == 0) {
+        for (int i = threadIdx.x; i < a.n_edits; i += 256)
+            a.table[(size_t)a.edit[i].row * a.max_pages + a.edit[i].col] = a.edit[i].page;
+        if ((int)threadIdx.x < a.n_lens) a.lens[a.len_row[threadIdx.x]] = a.len[threadIdx.x];
+    }
+    if ((int)blockIdx.y >= a.n_copies) return;
+    const PageCopy cp = a.copy[blockIdx.y];
+    const int head = blockIdx.x % a.n_kv, half = blockIdx.x / a.n_kv;   // half: 2 layer + (V)
+    char* base = a.pool + (size_t)half * (a.layer_bytes / 2);
+    const uint4* src = reinterpret_cast<const uint4*>(base + ((size_t)cp.src * a.n_kv + head) * a.head_bytes);
+    uint4* dst = reinterpret_cast<uint4*>(base + ((size_t)cp.dst * a.n_kv + head) * a.head_bytes);
+    const int n = cp.tokens * a.row_bytes / 16;
+    for (int i = threadIdx.x; i < n; i += 256) dst[i] = src[i];
+}
+
+// The device side of what fork and reorder decided for rows[0, n): `before`
+// holds each row's table entries (before_n of them) as they were.
+sa_status publish_rows(sa_kvcache* c, const std::vector<int32_t>& rows,
+                       const std::vector<std::vector<int32_t>>& before, const std::vector<PageCopy>& copies,
+                       hipStream_t st) {
+    std::vector<TableEdit> edits;
+    for (size_t i = 0; i < rows.size(); ++i) {
+        const int32_t* now = c->pt.row(rows[i]);
+        const int old_n = (int)before[i].size(), n = std::max(old_n, c->pt.npages(rows[i]));
+        for (int j = 0; j < n; ++j)
+            if (now[j] != (j < old_n ? before[i][j] : -1)) edits.push_back(TableEdit{rows[i], j, now[j]});
+    }
+    size_t e = 0, l = 0, k = 0;
+    while (e < edits.size() || l < rows.size() || k < copies.size()) {
+        RowsArgs a{};
+        a.table = c->d_table; a.lens = c->d_lens; a.pool = c->pool; a.layer_bytes = c->layer_bytes;
+        a.max_pages = c->desc.max_pages_per_seq; a.n_kv = c->desc.num_kv_heads;
+        a.row_bytes = (int)(c->desc.head_dim * c->elem_bytes);
+        a.head_bytes = SA_PAGE_TOKENS * a.row_bytes;
+        for (; a.n_edits < kEdits && e < edits.size(); ++e) a.edit[a.n_edits++] = edits[e];
+        for (; a.n_lens < kRowsPerLaunch && l < rows.size(); ++l) {
+            a.len_row[a.n_lens] = rows[l];
+            a.len[a.n_lens++] = c->pt.len(rows[l]);
+        }
+        for (; a.n_copies < kCopies && k < copies.size(); ++k) a.copy[a.n_copies++] = copies[k];
+        const dim3 grid(a.n_copies ? 2 * c->desc.num_layers * a.n_kv : 1, std::max(1, a.n_copies));
+        hipLaunchKernelGGL(update_rows_kernel, grid, dim3(256), 0, st, a);
+        SA_CHECK_LAUNCH();
+    }
+    return SA_OK;
+}
+
+// Entry points that allocate host memory: nothing is thrown across the C ABI.
+template <class F>
+sa_status no_throw(F&& body) {
+    try {
+        return body();
+    } catch (const std::bad_alloc&) {
+        return fail(SA_ENOMEM, "out of host memory");
+    }
+}
 
 // ---------------------------------------------------------------------------
 // Fused QK-norm + RoPE + append.  A head row (query, key or value) of a prompt is
@@ -505,6 +599,42 @@ extern "C" sa_status sa_kvcache_commit(sa_kvcache* c, const int32_t* seqs, int n
     return publish_lens(c, seqs, n_seqs, n, 1, st);
 }
 
+extern "C" sa_status sa_kvcache_fork(sa_kvcache* c, int dst, int src, int n_tokens, sa_stream_t stream) {
+    clear_error();
+    if (!valid_cache(c)) return fail(SA_EINVAL, "invalid cache");
+    return no_throw([&]() -> sa_status {
+        SA_TRY(on_cache_device(c));
+        const std::vector<int32_t> rows{dst};
+        std::vector<std::vector<int32_t>> before(1);
+        if (c->pt.valid_seq(dst)) before[0].assign(c->pt.row(dst), c->pt.row(dst) + c->pt.npages(dst));
+        std::vector<PageCopy> copies;
+        const Verdict v = c->pt.fork(dst, src, n_tokens, &copies);
+        if (!v.ok()) return refused(v);
+        return publish_rows(c, rows, before, copies, as_stream(stream));
+    });
+}
+
+extern "C" sa_status sa_kvcache_reorder(sa_kvcache* c, const int32_t* rows, const int32_t* parents, int n,
+                                        sa_stream_t stream) {
+    clear_error();
+    if (!valid_cache(c)) return fail(SA_EINVAL, "invalid cache");
+    return no_throw([&]() -> sa_status {
+        SA_TRY(on_cache_device(c));
+        std::vector<int32_t> changed;
+        std::vector<std::vector<int32_t>> before;
+        for (int i = 0; rows && parents && i < n; ++i) {
+            if (!c->pt.valid_seq(rows[i])) return fail(SA_ERANGE, "sequence index out of range");
+            if (rows[i] == parents[i]) continue;
+            changed.push_back(rows[i]);
+            before.emplace_back(c->pt.row(rows[i]), c->pt.row(rows[i]) + c->pt.npages(rows[i]));
+        }
+        std::vector<PageCopy> copies;
+        const Verdict v = c->pt.reorder(rows, parents, n, &copies);
+        if (!v.ok()) return refused(v);
+        return publish_rows(c, changed, before, copies, as_stream(stream));
+    });
+}
+
 extern "C" sa_status sa_kvcache_get_desc(const sa_kvcache* c, sa_kv_desc* out) {
     clear_error();
     if (!valid_cache(c) || !out) return fail(SA_EINVAL, "invalid cache or null output");
@@ -694,6 +824,115 @@ extern "C" sa_status sa_paged_decode(const sa_kvcache* c, int layer, const float
     for (int i = 0; i < n_seq; ++i) lens[i] = c->pt.len(seq_ids ? seq_ids[i] : i);
     return decode_paged(pv, q, n_seq, seq_ids, lens.data(), n_q_heads, n_pending, max_len, total, scale, out, ws,
                         ws_bytes, as_stream(stream));
+}
+
+namespace sa {
+namespace {
+
+// What the decodes over ranges share: the checks of their arguments and the
+// view of a layer's pools.
+sa_status check_ranges(const sa_kvcache* c, int layer, const float* q, int n_seq, int n_q_heads, const float* out,
+                       const void* ws) {
+    if (layer < 0 || layer >= c->desc.num_layers) return fail(SA_ERANGE, "Layer index out of range");
+    if (!q || !out) return fail(SA_EINVAL, "null pointer");
+    if (n_seq <= 0) return fail(SA_EINVAL, "n_seq must be positive");
+    if (n_q_heads <= 0 || n_q_heads % c->desc.num_kv_heads) return fail(SA_EINVAL, "bad head counts");
+    if (n_q_heads / c->desc.num_kv_heads > kRangesMaxRep || n_q_heads > 65535)
+        return fail(SA_EINVAL, "at most 64 query heads per KV head");
+    if (!ranges_head_dim(c->desc.head_dim)) return fail(SA_EINVAL, "head_dim must be 64 or 128");
+    if (!aligned16(q) || !aligned16(out) || !aligned16(ws))
+        return fail(SA_EINVAL, "q, out and ws must be 16-byte aligned");
+    return on_cache_device(c);
+}
+
+PagedView view_of(const sa_kvcache* c, int layer) {
+    PagedView pv;
+    pv.k_pool = k_pool_of(c, layer); pv.v_pool = v_pool_of(c, layer);
+    pv.block_table = c->d_table; pv.seq_lens = c->d_lens;
+    pv.n_kv = c->desc.num_kv_heads; pv.d = c->desc.head_dim;
+    pv.max_pages = c->desc.max_pages_per_seq; pv.num_pages = c->desc.num_pages;
+    pv.bf16 = c->desc.kv_dtype == SA_DTYPE_BF16;
+    return pv;
+}
+
+}  // namespace
+}  // namespace sa
+
+extern "C" size_t sa_paged_decode_window_ws_bytes(const sa_kvcache* c, int n_seq, int n_q_heads, int window,
+                                                  int n_sink) {
+    if (!valid_cache(c) || n_seq <= 0 || n_q_heads <= 0 || window <= 0 || n_sink < 0) return 0;
+    const long long seen = std::min<long long>((long long)c->desc.max_pages_per_seq * SA_PAGE_TOKENS,
+                                               (long long)window + n_sink);
+    return ranges_ws(n_seq, n_q_heads, c->desc.head_dim, seen, 0);
+}
+
+extern "C" sa_status sa_paged_decode_window(const sa_kvcache* c, int layer, const float* q, int n_seq,
+                                            const int32_t* seq_ids, int n_q_heads, int n_pending, int window,
+                                            int n_sink, float scale, float* out, void* ws, size_t ws_bytes,
+                                            sa_stream_t stream) {
+    clear_error();
+    if (!valid_cache(c)) return fail(SA_EINVAL, "invalid cache");
+    if (window <= 0) return fail(SA_EINVAL, "window must be positive");
+    if (n_sink < 0) return fail(SA_EINVAL, "n_sink must be >= 0");
+    return no_throw([&]() -> sa_status {
+        SA_TRY(check_ranges(c, layer, q, n_seq, n_q_heads, out, ws));
+        const Verdict vd = c->pt.check_decode(seq_ids, n_seq, n_pending, nullptr, nullptr);
+        if (!vd.ok()) return refused(vd);
+        std::vector<RangeSource> own(n_seq);
+        for (int i = 0; i < n_seq; ++i) {
+            const int row = seq_ids ? seq_ids[i] : i;
+            const int len = c->pt.len(row) + n_pending, first = std::max(0, len - window);
+            // sinks that reach the window leave one range
+            own[i] = n_sink < first ? RangeSource{row, n_sink, first, len} : RangeSource{row, 0, 0, len};
+        }
+        return decode_ranges(view_of(c, layer), q, n_q_heads, RangePlan{n_seq, own.data(), 0, nullptr, nullptr}, scale,
+                             out, ws, ws_bytes, as_stream(stream));
+    });
+}
+
+extern "C" size_t sa_paged_decode_shared_ws_bytes(const sa_kvcache* c, int n_seq, int n_q_heads) {
+    if (!valid_cache(c) || n_seq <= 0 || n_q_heads <= 0) return 0;
+    const long long tokens = (long long)c->desc.max_pages_per_seq * SA_PAGE_TOKENS;
+    return ranges_ws(n_seq, n_q_heads, c->desc.head_dim, tokens, tokens);
+}
+
+extern "C" sa_status sa_paged_decode_shared(const sa_kvcache* c, int layer, const float* q, int n_seq,
+                                            const int32_t* seq_ids, const int32_t* group_sizes, int n_groups,
+                                            int n_q_heads, int n_pending, float scale, float* out, void* ws,
+                                            size_t ws_bytes, sa_stream_t stream) {
+    clear_error();
+    if (!valid_cache(c)) return fail(SA_EINVAL, "invalid cache");
+    if (group_sizes ? n_groups <= 0 : n_groups != 0) return fail(SA_EINVAL, "group_sizes and n_groups go together");
+    return no_throw([&]() -> sa_status {
+        SA_TRY(check_ranges(c, layer, q, n_seq, n_q_heads, out, ws));
+        const Verdict vd = c->pt.check_decode(seq_ids, n_seq, n_pending, nullptr, nullptr);
+        if (!vd.ok()) return refused(vd);
+        const std::vector<int32_t> sizes = group_sizes ? std::vector<int32_t>(group_sizes, group_sizes + n_groups)
+                                                       : std::vector<int32_t>{n_seq};
+        long long rows = 0;
+        for (int32_t n : sizes) {
+            if (n <= 0) return fail(SA_EINVAL, "group sizes must be positive");
+            rows += n;
+        }
+        if (rows != n_seq) return fail(SA_EINVAL, "group sizes must add up to n_seq");
+        std::vector<RangeSource> own(n_seq), group;
+        bool any = false;
+        int at = 0;
+        for (int32_t n : sizes) {
+            const int first = seq_ids ? seq_ids[at] : at;
+            const int shared = c->pt.shared_tokens(seq_ids ? seq_ids + at : nullptr, first, n, n_pending);
+            group.push_back(RangeSource{first, shared, shared, shared});
+            any = any || shared > 0;
+            for (int i = at; i < at + n; ++i) {
+                const int row = seq_ids ? seq_ids[i] : i;
+                own[i] = RangeSource{row, 0, shared, c->pt.len(row) + n_pending};
+            }
+            at += n;
+        }
+        return decode_ranges(view_of(c, layer), q, n_q_heads,
+                             RangePlan{n_seq, own.data(), any ? (int)sizes.size() : 0, sizes.data(), group.data()},
+                             scale, out, ws, ws_bytes, as_stream(stream));
+    });
 }
 
 namespace sa {
