@@ -456,6 +456,30 @@ sa_status sa_swiglu_f32(const float* gate, const float* up, size_t n, float* out
 sa_status sa_axpby_f32(const float* x, float a, const float* y, float b, size_t n, float* out,
                        sa_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * One selection of a beam search (no counterpart in the reference, which
+ * decodes greedily).
+ *
+ * Row g * n_beams + b of logits (fp32, row_stride floats from one row to the
+ * next, row_stride >= vocab) holds beam b of search g; scores
+ * [n_groups][n_beams] their accumulated log probabilities.  With
+ *   c(b, t) = scores[g][b] + logits[b][t] - log sum_t' exp(logits[b][t'])
+ * each search's n_select largest c are written in order, largest first and of
+ * equal ones the lowest b * vocab + t: out_scores, out_tokens and out_beams
+ * [n_groups][n_select].  Ask for twice as many as beams where some may end.
+ * A continuation of probability 0 (logit -inf) is never selected, nor one of
+ * a beam whose score is -inf (beams not yet begun) or NaN or whose normaliser
+ * is not finite (a NaN or +inf among its logits, or nothing but -inf).  Places
+ * left over hold -inf, -1 and -1.  The order is decided in 64 bits.
+ * n_beams and n_select 1 .. 64, n_beams * vocab < 2^31.  ws: 8-byte aligned,
+ * sa_beam_select_ws_bytes bytes; calls that overlap on one workspace race.
+ * The parents (out_beams) are what sa_kvcache_reorder takes, on the host.
+ * ------------------------------------------------------------------------ */
+size_t sa_beam_select_ws_bytes(int n_groups, int n_beams, int vocab, int n_select);
+sa_status sa_beam_select(const float* logits, int64_t row_stride, const float* scores, int n_groups,
+                         int n_beams, int vocab, int n_select, float* out_scores, int32_t* out_tokens,
+                         int32_t* out_beams, void* ws, size_t ws_bytes, sa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -113,6 +113,8 @@ SIGNATURES = {
     "sa_set_attention_blocks": (_I, [_I, _I]),
     "sa_get_attention_blocks": (_I, [C.POINTER(_I), C.POINTER(_I)]),
     "sa_prefill_query_tile": (_I, [_I, _I, _I, _I, _I, _I]),
+    "sa_beam_select_ws_bytes": (_SZ, [_I, _I, _I, _I]),
+    "sa_beam_select": (_I, [_P, C.c_int64, _P, _I, _I, _I, _I, _P, _P, _P, _P, _SZ, _P]),
     "sa_qwen3_create": (_I, [C.POINTER(Qwen3Desc), _I, C.POINTER(_P)]),
     "sa_qwen3_destroy": (_I, [_P]),
     "sa_qwen3_get_desc": (_I, [_P, C.POINTER(Qwen3Desc)]),
@@ -498,6 +500,38 @@ def axpby(x, a: float, y=None, b: float = 0.0, out=None, stream=None):
     out = torch.empty_like(x) if out is None else out
     check(lib().sa_axpby_f32(_ptr(_f32(x, "x")), a, _ptr(_f32(y, "y")) if y is not None else None, b,
                              x.numel(), _ptr(out), _stream(stream)))
+    return out
+
+
+# ---------------------------------------------------------------- beam search
+
+def beam_select_ws_bytes(n_groups: int, n_beams: int, vocab: int, n_select: int) -> int:
+    return lib().sa_beam_select_ws_bytes(n_groups, n_beams, vocab, n_select)
+
+
+def beam_select(logits, scores, n_select: int, out=None, ws=None, stream=None):
+    """The n_select best continuations of each search: logits [G, B, vocab] fp32
+    (rows may be strided), accumulated log probabilities scores [G, B] ->
+    (scores, tokens, beams), each [G, n_select], best first."""
+    import torch
+    G, B, V = logits.shape
+    if logits.dtype != torch.float32 or not logits.is_cuda or (V > 1 and logits.stride(2) != 1):
+        raise ValueError("logits must be a float32 CUDA tensor with contiguous rows")
+    stride = logits.stride(1) if B > 1 else logits.stride(0) if G > 1 else V
+    if G > 1 and logits.stride(0) != B * stride:
+        raise ValueError("the rows of logits must be evenly spaced")
+    if tuple(scores.shape) != (G, B):
+        raise ValueError("scores must be [G, B]")
+    if out is None:
+        out = (torch.empty(G, n_select, dtype=torch.float32, device=logits.device),
+               *(torch.empty(G, n_select, dtype=torch.int32, device=logits.device) for _ in range(2)))
+    for t, dt in zip(out, (torch.float32, torch.int32, torch.int32)):
+        if t.dtype != dt or tuple(t.shape) != (G, n_select) or not t.is_cuda or not t.is_contiguous():
+            raise ValueError("out must be contiguous CUDA tensors [G, n_select]: float32, int32, int32")
+    if ws is None:
+        ws = torch.empty(max(beam_select_ws_bytes(G, B, V, n_select), 8), dtype=torch.uint8, device=logits.device)
+    check(lib().sa_beam_select(_ptr(logits), stride, _ptr(_f32(scores, "scores")), G, B, V, n_select, _ptr(out[0]),
+                               _ptr(out[1]), _ptr(out[2]), _ptr(ws), _nbytes(ws), _stream(stream)))
     return out
 
 
