@@ -402,6 +402,29 @@ sa_status sa_prefill_causal_strided_ws(const void* q, const void* k, const void*
                                        void* ws, size_t ws_bytes, sa_stream_t stream);
 
 /* ------------------------------------------------------------------------
+ * Causal prefill attention with a sliding window and sinks, on MFMA.
+ *
+ * No counterpart in the reference.  As sa_prefill_causal_strided, but query i
+ * attends to its last `window` keys (window >= 1) and the first n_sink
+ * (n_sink >= 0): out_i = softmax(scale q_i k_j) v_j over j <= i with
+ * i - j < window or j < n_sink.  The form that fills a cache for
+ * sa_paged_decode_window.  q and out [batch][n_q_heads][L][D], k and v
+ * [batch][n_kv_heads][L][D], all in dtype: bf16 in and bf16 out (products of
+ * bf16 operands, fp32 sums and softmax), or fp32 throughout.  D 64 or 128,
+ * L <= 2^30 (0: nothing to do).  Strides in elements {batch, head, row}, as in
+ * sa_prefill_causal_strided, for all tensors or NULL for all (dense); rows
+ * contiguous; tensors and strides multiples of 16 bytes.  out must not
+ * overlap an input.  The keys and values of a tile enter the products
+ * together: a value that is not finite may reach queries up to 63 keys away
+ * that do not see it.
+ * ------------------------------------------------------------------------ */
+sa_status sa_prefill_window(const void* q, const void* k, const void* v, sa_dtype dtype,
+                            int batch, int n_q_heads, int n_kv_heads, int L, int D,
+                            const int64_t q_strides[3], const int64_t kv_strides[3],
+                            const int64_t out_strides[3], int window, int n_sink, float scale,
+                            void* out, sa_stream_t stream);
+
+/* ------------------------------------------------------------------------
  * Tile sizes of the attention kernels, for the whole process: the
  * counterpart of the reference's tensor_cpp::g_q_block_size and
  * g_kv_block_size (tensor_cpp/src/ops.cpp:1630-1631), which benchmark_qwen3

@@ -110,6 +110,7 @@ SIGNATURES = {
     "sa_prefill_causal_ws": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P, _P, _SZ, _P]),
     "sa_prefill_causal_strided_ws": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _F, _P, _P, _SZ,
                                           _P]),
+    "sa_prefill_window": (_I, [_P, _P, _P, _I, _I, _I, _I, _I, _I, _P, _P, _P, _I, _I, _F, _P, _P]),
     "sa_set_attention_blocks": (_I, [_I, _I]),
     "sa_get_attention_blocks": (_I, [C.POINTER(_I), C.POINTER(_I)]),
     "sa_prefill_query_tile": (_I, [_I, _I, _I, _I, _I, _I]),
@@ -585,6 +586,29 @@ def prefill_causal(q, k, v, scale: float, out=None, stream=None, ws=None):
     else:
         check(lib().sa_prefill_causal_ws(_ptr(q), _ptr(k), _ptr(v), dt, B, Hq, Hkv, L, D, scale, _ptr(out),
                                          _ptr(ws), ws.numel() * ws.element_size(), _stream(stream)))
+    return out
+
+
+def prefill_window(q, k, v, scale: float, window: int, n_sink: int = 0, out=None, stream=None):
+    """Causal attention over the last `window` keys and the first n_sink: q [B, Hq,
+    L, D], k/v [B, Hkv, L, D], all fp32 or all bf16 -> out like q.  Views with
+    contiguous rows are taken as they are (k and v of one layout)."""
+    import torch
+    if q.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError("q must be float32 or bfloat16")
+    out = torch.empty_like(q) if out is None else out
+    for t, n in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
+        if t.dtype != q.dtype or not t.is_cuda or t.dim() != 4 or t.stride(3) != 1:
+            raise ValueError(f"{n} must be a CUDA tensor [B, H, L, D] of q's dtype with contiguous rows")
+    B, Hq, L, D = q.shape
+    if out.shape != q.shape or k.shape != v.shape or k.stride() != v.stride():
+        raise ValueError("out must have q's shape, and k and v one shape and layout")
+    if (k.shape[0], *k.shape[2:]) != (B, L, D):
+        raise ValueError("k and v must be [B, Hkv, L, D]")
+    strides = [C.cast((C.c_int64 * 3)(*t.stride()[:3]), C.c_void_p) for t in (q, k, out)]
+    dt = SA_DTYPE_F32 if q.dtype == torch.float32 else SA_DTYPE_BF16
+    check(lib().sa_prefill_window(_ptr(q), _ptr(k), _ptr(v), dt, B, Hq, k.shape[1], L, D, *strides, window, n_sink,
+                                  scale, _ptr(out), _stream(stream)))
     return out
 
 
