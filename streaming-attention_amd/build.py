@@ -40,11 +40,13 @@ DEVICE = [
 ]
 
 
-# Per-file device flags.  The prefill kernels keep MFMA accumulators in arch
+# Per-file device flags.  The attention kernels on MFMA keep accumulators in arch
 # VGPRs (their softmax rescales them with VALU ops); the register-staged bf16
 # kernel parks Q in AGPRs.
 EXTRA = {
     "prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "ranges.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "window.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -7,7 +7,7 @@
 // segments, and each leaves its largest logit and its sum of exponentials
 // relative to it (fp32, at most 64 VPT values a sum).  The second, a workgroup
 // per group, joins the sums in 64 bits and selects.  c is non-decreasing in x,
-// so with tau the n_select-th largest of any set of segment maxima, only
+// so with tau a value that at least n_select segment maxima reach, only
 // segments whose maximum reaches tau hold candidates, and only their elements
 // that reach tau are candidates: a few dozen, put in order by counting for
 // each how many precede it.  Comparisons with tau are in fp32 (rounding is
@@ -27,11 +27,11 @@ namespace {
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / kWave;
 constexpr int kMaxBeams = 64, kMaxSelect = 64;
-constexpr int kSegsPerThread = 4;
-constexpr int kMaxSegs = kSelThreads * kSegsPerThread;   // segments of a group
+constexpr int kSlots = 8;                                // segments of a thread of the second launch
+constexpr int kBeamsPerWave = kMaxBeams / kSelWaves;
 constexpr int kBlock = 8 * kWave;                        // elements of a wave's step
-constexpr int kSegList = 128, kCandList = 1024;
-static_assert(kMaxSelect <= kSegList && kMaxSelect <= kWave, "rounds fill the segment list; ranks come from one list per wave");
+constexpr int kSegList = 256, kCandList = 1024;
+static_assert(kMaxSelect <= kSegList, "the rounds fill the segment list");
 constexpr float kNone = -INFINITY;
 
 struct BeamArgs {
@@ -46,6 +46,9 @@ struct BeamArgs {
     int n_seg, seg_len;      // segments of a row, elements of a segment
     int steps;               // steps of kBlock elements per wave
     int wg_per_row;
+    // Second launch: a beam's segments on waves_per_beam waves, or
+    // beams_per_wave beams on a wave, per_beam segments of a beam per thread.
+    int waves_per_beam, beams_per_wave, per_beam;
 };
 
 // exp(d) for d <= 0; log2(e) in two parts, so that the argument's rounding
@@ -100,6 +103,15 @@ __global__ void __launch_bounds__(256) beam_scan_kernel(BeamArgs a) {
     }
 }
 
+// Floats as unsigned integers of the same order (NaN aside), and back.
+__device__ __forceinline__ uint32_t ordered(float f) {
+    const uint32_t u = __float_as_uint(f);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float unordered(uint32_t u) {
+    return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
+}
+
 // Candidate order: larger value first, of equal ones the lower index.
 __device__ __forceinline__ bool ahead(double v, int i, double w, int j) { return v > w || (v == w && i < j); }
 
@@ -130,92 +142,139 @@ __device__ void first_of_all(double& v, int& idx, double* sv, int* si) {
 
 __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
     __shared__ double base[kMaxBeams];              // score - log sum exp; NaN: the beam offers nothing
-    __shared__ float top[kSelWaves * kWave];
+    __shared__ float wave_max[kSelWaves][kBeamsPerWave];
+    __shared__ double wave_sum[kSelWaves][kBeamsPerWave];
+    __shared__ float beam_max[kMaxBeams];
+    __shared__ float top[kSelWaves];
+    __shared__ int counts[2][kSelWaves];
     __shared__ int seg_list[kSegList];
     __shared__ double cand_v[kCandList];
     __shared__ int cand_i[kCandList];
     __shared__ int n_segs, n_cand;
-    __shared__ float tau;
     __shared__ double red_v[kSelWaves];
     __shared__ int red_i[kSelWaves];
 
     const int group = blockIdx.x;
-    const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+    const int tid = threadIdx.x, lane = tid & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
     const float2* seg = a.seg + (long long)group * a.n_beams * a.n_seg;
-    const int n_all = a.n_beams * a.n_seg;
     const int want = a.n_select;
     if (tid == 0) {
         n_segs = 0;
         n_cand = 0;
-        tau = kNone;
+    }
+
+    // ---- this thread's segments: slot j is part j % per_beam of its wave's beam
+    // j / per_beam, whose segments are dealt out to the beam's waves first ----
+    float2 sg[kSlots];
+    int id[kSlots];      // beam * n_seg + segment, -1: none
+    int of[kSlots];      // the beam's place in the wave
+    {
+        int bi = 0, k = 0;
+#pragma unroll
+        for (int j = 0; j < kSlots; ++j) {
+            const int beam = a.beams_per_wave > 1 ? wave * a.beams_per_wave + bi : wave / a.waves_per_beam;
+            const int s = (k * kWave + lane) * a.waves_per_beam + wave % a.waves_per_beam;
+            of[j] = bi;
+            id[j] = bi < a.beams_per_wave && beam < a.n_beams && s < a.n_seg ? beam * a.n_seg + s : -1;
+            sg[j] = id[j] >= 0 ? seg[id[j]] : make_float2(kNone, 0.f);
+            if (++k == a.per_beam) {
+                k = 0;
+                ++bi;
+            }
+        }
     }
 
     // ---- the beams' normalisers ----
-    for (int b = wave; b < a.n_beams; b += kSelWaves) {
+    auto first_of = [&](int b) { return a.beams_per_wave > 1 ? b / a.beams_per_wave : b * a.waves_per_beam; };
+    auto place_of = [&](int b) { return a.beams_per_wave > 1 ? b % a.beams_per_wave : 0; };
+    for (int bi = 0; bi < a.beams_per_wave; ++bi) {
         float m = kNone;
-        for (int i = lane; i < a.n_seg; i += kWave) m = fmaxf(m, seg[b * a.n_seg + i].x);
+#pragma unroll
+        for (int j = 0; j < kSlots; ++j) m = of[j] == bi ? fmaxf(m, sg[j].x) : m;
         m = group_reduce<OpMax, 1, kWave>(m);
+        if (lane == 0) wave_max[wave][bi] = m;
+    }
+    __syncthreads();
+    for (int bi = 0; bi < a.beams_per_wave; ++bi) {
+        const int w0 = a.beams_per_wave > 1 ? wave : wave / a.waves_per_beam * a.waves_per_beam;
+        float m = kNone;
+        for (int w = w0; w < min(w0 + a.waves_per_beam, kSelWaves); ++w) m = fmaxf(m, wave_max[w][bi]);
         double l = 0.0;
-        for (int i = lane; i < a.n_seg; i += kWave) {
-            const float2 s = seg[b * a.n_seg + i];
-            // an empty segment (maximum -inf) has sum 0, or NaN where it held one
-            l += s.x == kNone ? (double)s.y : (double)s.y * exp((double)s.x - (double)m);
-        }
+#pragma unroll
+        for (int j = 0; j < kSlots; ++j)
+            if (id[j] >= 0 && of[j] == bi) l += (double)(sg[j].y * exp_diff(sg[j].x - m));
 #pragma unroll
         for (int d = 1; d < kWave; d <<= 1) l += __shfl_xor(l, d, kWave);
+        const int beam = a.beams_per_wave > 1 ? wave * a.beams_per_wave + bi : wave / a.waves_per_beam;
         if (lane == 0) {
-            const double lse = (double)m + log(l);
-            base[b] = isfinite(lse) ? (double)a.scores[(long long)group * a.n_beams + b] - lse : (double)NAN;
+            wave_sum[wave][bi] = l;
+            if (wave == w0 && beam < a.n_beams) beam_max[beam] = m;
         }
+    }
+    __syncthreads();
+    if (tid < a.n_beams) {
+        const int w0 = first_of(tid), bi = place_of(tid);
+        double l = 0.0;
+        for (int w = w0; w < w0 + a.waves_per_beam; ++w) l += wave_sum[w][bi];
+        const double lse = (double)beam_max[tid] + log(l);
+        base[tid] = isfinite(lse) ? (double)a.scores[(long long)group * a.n_beams + tid] - lse : (double)NAN;
     }
     __syncthreads();
 
-    // ---- tau: the want-th largest of the threads' largest segment maxima (-inf:
-    // fewer threads have one) ----
-    float key[kSegsPerThread];
+    // ---- tau: a value that at least `want`, and rarely more than twice as many,
+    // of the threads' largest segment maxima reach (-inf: fewer threads have one).
+    // Bisection over the values' bit patterns, from 16 below the largest on. ----
+    float key[kSlots];
     float best = kNone;
 #pragma unroll
-    for (int j = 0; j < kSegsPerThread; ++j) {
-        const int s = tid + j * kSelThreads;
-        key[j] = kNone;
-        if (s < n_all) {
-            const float k = (float)(base[s / a.n_seg] + (double)seg[s].x);
-            if (k > kNone) key[j] = k;   // also leaves NaN out
-        }
+    for (int j = 0; j < kSlots; ++j) {
+        const float k = id[j] >= 0 ? (float)(base[id[j] / a.n_seg] + (double)sg[j].x) : kNone;
+        key[j] = k > kNone ? k : kNone;   // also leaves NaN out
         best = fmaxf(best, key[j]);
     }
-    int rank = 0;
-    for (int j = 0; j < kWave; ++j) {
-        const float o = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(best), j));
-        rank += o > best || (o == best && j < lane);
+    {
+        const float m = group_reduce<OpMax, 1, kWave>(best);
+        if (lane == 0) top[wave] = m;
     }
-    top[wave * kWave + rank] = best;    // the wave's maxima in order
     __syncthreads();
-    if (rank < want) {
-        int above = rank;
-        for (int w = 0; w < kSelWaves; ++w) {
-            if (w == wave) continue;
-            // entries of wave w's list before this one: larger, or equal in an earlier wave
-            int lo = 0, hi = kWave;
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                const float o = top[w * kWave + mid];
-                if (o > best || (o == best && w < wave)) lo = mid + 1;
-                else hi = mid;
-            }
-            above += lo;
+    float most = top[0];
+#pragma unroll
+    for (int w = 1; w < kSelWaves; ++w) most = fmaxf(most, top[w]);
+    const uint32_t mine = ordered(best);
+    int parity = 0;
+    auto reach = [&](uint32_t v) {   // threads whose best is at least v
+        const int n = __popcll(__ballot(mine >= v));
+        if (lane == 0) counts[parity][wave] = n;
+        __syncthreads();
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < kSelWaves; ++w) all += counts[parity][w];
+        parity ^= 1;
+        return all;
+    };
+    uint32_t lo = ordered(kNone) + 1, hi = ordered(most) + 1;
+    float t = kNone;
+    if (most > kNone && reach(lo) >= want) {
+        const uint32_t near = ordered(most - 16.f);
+        if (near > lo && reach(near) >= want) lo = near;
+        while (hi - lo > 1) {
+            const uint32_t mid = lo + (hi - lo) / 2;
+            const int n = reach(mid);
+            if (n >= want) lo = mid;
+            else hi = mid;
+            if (n >= want && n <= 2 * want) break;
         }
-        if (above == want - 1) tau = best;
+        t = unordered(lo);
     }
-    __syncthreads();
-    const float t = tau;
+
 
     // ---- the segments and elements that reach it ----
 #pragma unroll
-    for (int j = 0; j < kSegsPerThread; ++j) {
+    for (int j = 0; j < kSlots; ++j) {
         if (key[j] > kNone && key[j] >= t) {
             const int at = atomicAdd(&n_segs, 1);
-            if (at < kSegList) seg_list[at] = tid + j * kSelThreads;
+            if (at < kSegList) seg_list[at] = id[j];
         }
     }
     __syncthreads();
@@ -230,15 +289,28 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
         return c;
     };
     if (n_segs <= kSegList) {
-        const long long n = (long long)n_segs * a.seg_len;
-        for (long long i = tid; i < n; i += kSelThreads) {
-            int idx;
-            const double c = value(seg_list[i / a.seg_len], (int)(i % a.seg_len), idx);
-            if (idx >= 0 && (float)c >= t) {
-                const int at = atomicAdd(&n_cand, 1);
-                if (at < kCandList) {
-                    cand_v[at] = c;
-                    cand_i[at] = idx;
+        // a wave per segment, four rows of 64 elements in flight
+        for (int i = wave; i < n_segs; i += kSelWaves) {
+            const int s = seg_list[i];
+            const int b = s / a.n_seg;
+            const long long tok0 = (long long)(s % a.n_seg) * a.seg_len;
+            const float* xr = x + b * a.row_stride + tok0;
+            const int left = (int)min((long long)a.seg_len, a.vocab - tok0);
+            const double bb = base[b];
+            for (int o = 0; o < left; o += 4 * kWave) {
+                float v[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = o + j * kWave + lane < left ? xr[o + j * kWave + lane] : kNone;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const double c = bb + (double)v[j];
+                    if (c > (double)kNone && (float)c >= t) {
+                        const int at = atomicAdd(&n_cand, 1);
+                        if (at < kCandList) {
+                            cand_v[at] = c;
+                            cand_i[at] = b * a.vocab + (int)tok0 + o + j * kWave + lane;
+                        }
+                    }
                 }
             }
         }
@@ -271,10 +343,10 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
         double v = 0.0;
         int idx = -1;
 #pragma unroll
-        for (int j = 0; j < kSegsPerThread; ++j) {
-            const int s = tid + j * kSelThreads;
+        for (int j = 0; j < kSlots; ++j) {
+            const int s = id[j];
             if (!(key[j] > kNone)) continue;
-            const double c = base[s / a.n_seg] + (double)seg[s].x;
+            const double c = base[s / a.n_seg] + (double)sg[j].x;
             if (picked && !ahead(last_v, last_i, c, s)) continue;
             if (idx < 0 || ahead(c, s, v, idx)) {
                 v = c;
@@ -312,16 +384,18 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
 
 struct BeamShape {
     int vpt, steps, n_seg;
+    int waves_per_beam, beams_per_wave, per_beam;
 };
-// The shortest segments of which a group has at most kMaxSegs.
+// The shortest segments that the second launch's threads hold.
 BeamShape beam_shape(int n_beams, int vocab) {
-    for (int vpt = 1; vpt < 8; vpt *= 2) {
-        const int n = (vocab + kWave * vpt - 1) / (kWave * vpt);
-        if ((long long)n * n_beams <= kMaxSegs) return {vpt, 1, n};
-    }
-    for (int steps = 1;; steps *= 2) {
-        const int n = (int)((vocab + (long long)kBlock * steps - 1) / ((long long)kBlock * steps));
-        if ((long long)n * n_beams <= kMaxSegs) return {8, steps, n};
+    BeamShape s{1, 1, 0, std::max(1, kSelWaves / n_beams), (n_beams + kSelWaves - 1) / kSelWaves, 0};
+    for (;;) {
+        const long long len = (long long)kWave * s.vpt * s.steps;
+        s.n_seg = (int)((vocab + len - 1) / len);
+        s.per_beam = (s.n_seg + kWave * s.waves_per_beam - 1) / (kWave * s.waves_per_beam);
+        if (s.per_beam * s.beams_per_wave <= kSlots) return s;
+        if (s.vpt < 8) s.vpt *= 2;
+        else s.steps *= 2;
     }
 }
 
@@ -357,6 +431,7 @@ extern "C" sa_status sa_beam_select(const float* logits, int64_t row_stride, con
     a.out_scores = out_scores; a.out_tokens = out_tokens; a.out_beams = out_beams;
     a.row_stride = row_stride;
     a.n_groups = n_groups; a.n_beams = n_beams; a.vocab = vocab; a.n_select = n_select;
+    a.waves_per_beam = sh.waves_per_beam; a.beams_per_wave = sh.beams_per_wave; a.per_beam = sh.per_beam;
     a.n_seg = sh.n_seg; a.seg_len = kWave * sh.vpt * sh.steps; a.steps = sh.steps;
     const long long per_wave = (long long)kBlock * sh.steps;
     a.wg_per_row = (int)((vocab + 4 * per_wave - 1) / (4 * per_wave));

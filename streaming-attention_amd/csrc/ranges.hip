@@ -446,7 +446,7 @@ __device__ __forceinline__ void attend(const RangeArgs& a, const Item& it, lds_u
 }
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads) range_attn_kernel(RangeArgs a) {
+__global__ void __launch_bounds__(kThreads, BF16 ? 2 : 1) range_attn_kernel(RangeArgs a) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ int32_t pages[kChunkTiles];
     __shared__ float ml[kWaves * 32][2];
