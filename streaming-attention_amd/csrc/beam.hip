@@ -30,7 +30,7 @@ constexpr int kMaxBeams = 64, kMaxSelect = 64;
 constexpr int kSlots = 8;                                // segments of a thread of the second launch
 constexpr int kBeamsPerWave = kMaxBeams / kSelWaves;
 constexpr int kBlock = 8 * kWave;                        // elements of a wave's step
-constexpr int kSegList = 256, kCandList = 1024;
+constexpr int kSegList = 256, kCandList = 1024, kGather = 8;
 static_assert(kMaxSelect <= kSegList, "the rounds fill the segment list");
 constexpr float kNone = -INFINITY;
 
@@ -57,12 +57,14 @@ __device__ __forceinline__ float exp_diff(float d) {
     return __builtin_amdgcn_exp2f(fmaf(d, 1.44269502162933349609f, d * 1.92596299112661746887e-8f));
 }
 
-// A wave takes `steps` steps of kBlock consecutive elements of a row.  VPT < 8:
-// every VPT rows of 64 elements are a segment; VPT = 8: the wave's steps are
-// one segment.
-template <int VPT>
+// A wave takes `steps` steps of kBlock consecutive elements of a row, four
+// neighbouring ones per lane and load (VEC: rows start 16-byte aligned, else
+// four loads).  VPT < 8: the 64 VPT elements of 16 VPT lanes are a segment, so
+// one reduction serves all segments of a load; VPT = 8: the wave's steps are one.
+template <int VPT, bool VEC>
 __global__ void __launch_bounds__(256) beam_scan_kernel(BeamArgs a) {
-    constexpr int SEGS = 8 / VPT;
+    constexpr int LANES = VPT < 4 ? 16 * VPT : kWave;   // lanes of a segment
+    constexpr int JOIN = VPT == 8 ? 2 : 1;              // loads of a segment
     const int row = blockIdx.x / a.wg_per_row;
     const int block = (blockIdx.x % a.wg_per_row) * 4 + threadIdx.x / kWave;
     const int lane = threadIdx.x & (kWave - 1);
@@ -72,25 +74,33 @@ __global__ void __launch_bounds__(256) beam_scan_kernel(BeamArgs a) {
     float m_run = kNone, l_run = 0.f;
     for (int s = 0; s < a.steps; ++s) {
         const long long at = first + (long long)s * kBlock;
-        float v[8];
+        float v[2][4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const long long i = at + j * kWave + lane;
-            v[j] = i < a.vocab ? x[i] : kNone;
+        for (int j = 0; j < 2; ++j) {
+            const long long i = at + j * 4 * kWave + 4 * lane;
+            if (VEC && i + 4 <= a.vocab) {
+                const float4 q = *reinterpret_cast<const float4*>(x + i);
+                v[j][0] = q.x; v[j][1] = q.y; v[j][2] = q.z; v[j][3] = q.w;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[j][e] = i + e < a.vocab ? x[i + e] : kNone;
+            }
         }
 #pragma unroll
-        for (int g = 0; g < SEGS; ++g) {
-            float m = v[g * VPT];
+        for (int g = 0; g < 2; g += JOIN) {
+            float m = kNone;
 #pragma unroll
-            for (int j = 1; j < VPT; ++j) m = fmaxf(m, v[g * VPT + j]);
-            m = group_reduce<OpMax, 1, kWave>(m);
+            for (int j = g; j < g + JOIN; ++j) m = fmaxf(m, fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])));
+            m = group_reduce<OpMax, 1, LANES>(m);
             float l = 0.f;
 #pragma unroll
-            for (int j = 0; j < VPT; ++j) l += m == kNone && v[g * VPT + j] == kNone ? 0.f : exp_diff(v[g * VPT + j] - m);
-            l = group_reduce<OpSum, 1, kWave>(l);
+            for (int j = g; j < g + JOIN; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) l += m == kNone && v[j][e] == kNone ? 0.f : exp_diff(v[j][e] - m);
+            l = group_reduce<OpSum, 1, LANES>(l);
             if constexpr (VPT < 8) {
-                const long long seg = at / (kWave * VPT) + g;
-                if (lane == 0 && seg < a.n_seg) a.seg[(long long)row * a.n_seg + seg] = make_float2(m, l);
+                const long long seg = (at + g * 4 * kWave + 4 * lane) / (kWave * VPT);
+                if (lane % LANES == 0 && seg < a.n_seg) a.seg[(long long)row * a.n_seg + seg] = make_float2(m, l);
             } else {
                 const float mn = fmaxf(m_run, m);
                 l_run = (m_run == kNone ? l_run : l_run * exp_diff(m_run - mn)) + (m == kNone ? l : l * exp_diff(m - mn));
@@ -101,6 +111,26 @@ __global__ void __launch_bounds__(256) beam_scan_kernel(BeamArgs a) {
     if constexpr (VPT == 8) {
         if (lane == 0) a.seg[(long long)row * a.n_seg + block] = make_float2(m_run, l_run);
     }
+}
+
+// The sum over a wave, in 64 bits: lane exchanges inside 16 lanes with DPP
+// (after each step groups are uniform, so the mirrors act as xor 4 and 8), then
+// halves of 32 and of the wave.
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t u = __double_as_longlong(v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
+    return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+    v += dpp_f64<kDppXor1>(v);
+    v += dpp_f64<kDppXor2>(v);
+    v += dpp_f64<kDppHalfMirror>(v);
+    v += dpp_f64<kDppMirror>(v);
+    v += __shfl_xor(v, 16, kWave);
+    v += __shfl_xor(v, 32, kWave);
+    return v;
 }
 
 // Floats as unsigned integers of the same order (NaN aside), and back.
@@ -167,17 +197,18 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
     // ---- this thread's segments: slot j is part j % per_beam of its wave's beam
     // j / per_beam, whose segments are dealt out to the beam's waves first ----
     float2 sg[kSlots];
-    int id[kSlots];      // beam * n_seg + segment, -1: none
-    int of[kSlots];      // the beam's place in the wave
+    int id[kSlots];      // segment of the beam, -1: none
+    int of[kSlots];      // the beam's place in the wave (uniform)
+    const int n_slots = a.per_beam * a.beams_per_wave;
+    const int beam0 = a.beams_per_wave > 1 ? wave * a.beams_per_wave : wave / a.waves_per_beam;
     {
         int bi = 0, k = 0;
 #pragma unroll
         for (int j = 0; j < kSlots; ++j) {
-            const int beam = a.beams_per_wave > 1 ? wave * a.beams_per_wave + bi : wave / a.waves_per_beam;
             const int s = (k * kWave + lane) * a.waves_per_beam + wave % a.waves_per_beam;
             of[j] = bi;
-            id[j] = bi < a.beams_per_wave && beam < a.n_beams && s < a.n_seg ? beam * a.n_seg + s : -1;
-            sg[j] = id[j] >= 0 ? seg[id[j]] : make_float2(kNone, 0.f);
+            id[j] = j < n_slots && beam0 + bi < a.n_beams && s < a.n_seg ? s : -1;
+            sg[j] = id[j] >= 0 ? seg[(beam0 + bi) * a.n_seg + s] : make_float2(kNone, 0.f);
             if (++k == a.per_beam) {
                 k = 0;
                 ++bi;
@@ -203,13 +234,11 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
         double l = 0.0;
 #pragma unroll
         for (int j = 0; j < kSlots; ++j)
-            if (id[j] >= 0 && of[j] == bi) l += (double)(sg[j].y * exp_diff(sg[j].x - m));
-#pragma unroll
-        for (int d = 1; d < kWave; d <<= 1) l += __shfl_xor(l, d, kWave);
-        const int beam = a.beams_per_wave > 1 ? wave * a.beams_per_wave + bi : wave / a.waves_per_beam;
+            if (j < n_slots && of[j] == bi) l += id[j] >= 0 ? (double)(sg[j].y * exp_diff(sg[j].x - m)) : 0.0;
+        l = wave_sum_f64(l);
         if (lane == 0) {
             wave_sum[wave][bi] = l;
-            if (wave == w0 && beam < a.n_beams) beam_max[beam] = m;
+            if (wave == w0 && beam0 + bi < a.n_beams) beam_max[beam0 + bi] = m;
         }
     }
     __syncthreads();
@@ -229,8 +258,11 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
     float best = kNone;
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
-        const float k = id[j] >= 0 ? (float)(base[id[j] / a.n_seg] + (double)sg[j].x) : kNone;
-        key[j] = k > kNone ? k : kNone;   // also leaves NaN out
+        key[j] = kNone;
+        if (j < n_slots && beam0 + of[j] < a.n_beams) {
+            const float k = (float)(base[beam0 + of[j]] + (double)sg[j].x);
+            if (k > kNone) key[j] = k;   // also leaves NaN out
+        }
         best = fmaxf(best, key[j]);
     }
     {
@@ -274,7 +306,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
     for (int j = 0; j < kSlots; ++j) {
         if (key[j] > kNone && key[j] >= t) {
             const int at = atomicAdd(&n_segs, 1);
-            if (at < kSegList) seg_list[at] = id[j];
+            if (at < kSegList) seg_list[at] = (beam0 + of[j]) * a.n_seg + id[j];
         }
     }
     __syncthreads();
@@ -289,27 +321,35 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
         return c;
     };
     if (n_segs <= kSegList) {
-        // a wave per segment, four rows of 64 elements in flight
-        for (int i = wave; i < n_segs; i += kSelWaves) {
-            const int s = seg_list[i];
-            const int b = s / a.n_seg;
-            const long long tok0 = (long long)(s % a.n_seg) * a.seg_len;
-            const float* xr = x + b * a.row_stride + tok0;
-            const int left = (int)min((long long)a.seg_len, a.vocab - tok0);
-            const double bb = base[b];
-            for (int o = 0; o < left; o += 4 * kWave) {
-                float v[4];
+        // all their elements at once, kGather per thread in flight
+        const int shift = 31 - __clz(a.seg_len);
+        const long long n = (long long)n_segs << shift;
+        for (long long at0 = tid; at0 < n; at0 += kGather * kSelThreads) {
+            float v[kGather];
+            int idx[kGather], beam[kGather];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = o + j * kWave + lane < left ? xr[o + j * kWave + lane] : kNone;
+            for (int j = 0; j < kGather; ++j) {
+                const long long at = at0 + j * kSelThreads;
+                idx[j] = -1;
+                if (at < n) {
+                    const int s = seg_list[at >> shift];
+                    beam[j] = s / a.n_seg;
+                    const long long tok = (((long long)s - beam[j] * a.n_seg) << shift) + (at & (a.seg_len - 1));
+                    if (tok < a.vocab) {
+                        idx[j] = beam[j] * a.vocab + (int)tok;
+                        v[j] = x[beam[j] * a.row_stride + tok];
+                    }
+                }
+            }
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const double c = bb + (double)v[j];
-                    if (c > (double)kNone && (float)c >= t) {
-                        const int at = atomicAdd(&n_cand, 1);
-                        if (at < kCandList) {
-                            cand_v[at] = c;
-                            cand_i[at] = b * a.vocab + (int)tok0 + o + j * kWave + lane;
-                        }
+            for (int j = 0; j < kGather; ++j) {
+                if (idx[j] < 0) continue;
+                const double c = base[beam[j]] + (double)v[j];
+                if (c > (double)kNone && (float)c >= t) {
+                    const int at = atomicAdd(&n_cand, 1);
+                    if (at < kCandList) {
+                        cand_v[at] = c;
+                        cand_i[at] = idx[j];
                     }
                 }
             }
@@ -344,9 +384,9 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
         int idx = -1;
 #pragma unroll
         for (int j = 0; j < kSlots; ++j) {
-            const int s = id[j];
             if (!(key[j] > kNone)) continue;
-            const double c = base[s / a.n_seg] + (double)sg[j].x;
+            const int s = (beam0 + of[j]) * a.n_seg + id[j];
+            const double c = base[beam0 + of[j]] + (double)sg[j].x;
             if (picked && !ahead(last_v, last_i, c, s)) continue;
             if (idx < 0 || ahead(c, s, v, idx)) {
                 v = c;
@@ -439,11 +479,18 @@ extern "C" sa_status sa_beam_select(const float* logits, int64_t row_stride, con
     const long long wgs = (long long)n_groups * n_beams * a.wg_per_row;
     if (wgs >= (1LL << 31)) return fail(SA_EINVAL, "too many rows");
     const dim3 grid((unsigned)wgs);
+    const bool vec = aligned16(logits) && row_stride % 4 == 0;
     switch (sh.vpt) {
-        case 1: hipLaunchKernelGGL(beam_scan_kernel<1>, grid, dim3(256), 0, st, a); break;
-        case 2: hipLaunchKernelGGL(beam_scan_kernel<2>, grid, dim3(256), 0, st, a); break;
-        case 4: hipLaunchKernelGGL(beam_scan_kernel<4>, grid, dim3(256), 0, st, a); break;
-        default: hipLaunchKernelGGL(beam_scan_kernel<8>, grid, dim3(256), 0, st, a); break;
+#define SA_BEAM_SCAN(VV)                                                                              \
+    case VV:                                                                                          \
+        if (vec) hipLaunchKernelGGL((beam_scan_kernel<VV, true>), grid, dim3(256), 0, st, a);         \
+        else hipLaunchKernelGGL((beam_scan_kernel<VV, false>), grid, dim3(256), 0, st, a);            \
+        break;
+        SA_BEAM_SCAN(1)
+        SA_BEAM_SCAN(2)
+        SA_BEAM_SCAN(4)
+        SA_BEAM_SCAN(8)
+#undef SA_BEAM_SCAN
     }
     SA_CHECK_LAUNCH();
     hipLaunchKernelGGL(beam_pick_kernel, dim3(n_groups), dim3(kSelThreads), 0, st, a);
