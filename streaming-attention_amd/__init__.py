@@ -170,10 +170,21 @@ def _rows(ids, n: int):
     return C.cast((C.c_int32 * n)(*ids), C.c_void_p)
 
 
+_raw_stream = None   # the current stream's handle, without a Stream object (2.9 -> 0.4 us per call)
+
+
 def _stream(stream) -> int | None:
+    global _raw_stream
     if stream is None:
-        import torch
-        return torch.cuda.current_stream().cuda_stream
+        if _raw_stream is None:
+            import torch
+            raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+            current = torch.cuda.current_device
+            if raw is None:
+                _raw_stream = lambda: torch.cuda.current_stream().cuda_stream  # noqa: E731
+            else:
+                _raw_stream = lambda: raw(current())  # noqa: E731
+        return _raw_stream()
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else stream
 
 
@@ -516,23 +527,29 @@ def beam_select(logits, scores, n_select: int, out=None, ws=None, stream=None):
     (scores, tokens, beams), each [G, n_select], best first."""
     import torch
     G, B, V = logits.shape
-    if logits.dtype != torch.float32 or not logits.is_cuda or (V > 1 and logits.stride(2) != 1):
-        raise ValueError("logits must be a float32 CUDA tensor with contiguous rows")
-    stride = logits.stride(1) if B > 1 else logits.stride(0) if G > 1 else V
-    if G > 1 and logits.stride(0) != B * stride:
-        raise ValueError("the rows of logits must be evenly spaced")
-    if tuple(scores.shape) != (G, B):
+    if logits.dtype != torch.float32 or not logits.is_cuda:
+        raise ValueError("logits must be a float32 CUDA tensor")
+    if logits.is_contiguous():
+        stride = V
+    else:
+        s0, s1, s2 = logits.stride()
+        stride = s1 if B > 1 else s0 if G > 1 else V
+        if (V > 1 and s2 != 1) or (G > 1 and s0 != B * stride):
+            raise ValueError("the rows of logits must be contiguous and evenly spaced")
+    if scores.shape != (G, B):
         raise ValueError("scores must be [G, B]")
     if out is None:
         out = (torch.empty(G, n_select, dtype=torch.float32, device=logits.device),
                *(torch.empty(G, n_select, dtype=torch.int32, device=logits.device) for _ in range(2)))
-    for t, dt in zip(out, (torch.float32, torch.int32, torch.int32)):
-        if t.dtype != dt or tuple(t.shape) != (G, n_select) or not t.is_cuda or not t.is_contiguous():
-            raise ValueError("out must be contiguous CUDA tensors [G, n_select]: float32, int32, int32")
+    o, t, b = out
+    if not (o.shape == t.shape == b.shape == (G, n_select) and o.is_contiguous() and t.is_contiguous() and
+            b.is_contiguous() and o.is_cuda and t.is_cuda and b.is_cuda and o.dtype == torch.float32 and
+            t.dtype == torch.int32 and b.dtype == torch.int32):
+        raise ValueError("out must be contiguous CUDA tensors [G, n_select]: float32, int32, int32")
     if ws is None:
         ws = torch.empty(max(beam_select_ws_bytes(G, B, V, n_select), 8), dtype=torch.uint8, device=logits.device)
-    check(lib().sa_beam_select(_ptr(logits), stride, _ptr(_f32(scores, "scores")), G, B, V, n_select, _ptr(out[0]),
-                               _ptr(out[1]), _ptr(out[2]), _ptr(ws), _nbytes(ws), _stream(stream)))
+    check(lib().sa_beam_select(logits.data_ptr(), stride, _ptr(_f32(scores, "scores")), G, B, V, n_select, o.data_ptr(),
+                               t.data_ptr(), b.data_ptr(), ws.data_ptr(), _nbytes(ws), _stream(stream)))
     return out
 
 
@@ -594,21 +611,29 @@ def prefill_window(q, k, v, scale: float, window: int, n_sink: int = 0, out=None
     L, D], k/v [B, Hkv, L, D], all fp32 or all bf16 -> out like q.  Views with
     contiguous rows are taken as they are (k and v of one layout)."""
     import torch
-    if q.dtype not in (torch.float32, torch.bfloat16):
+    dtype, shape, layout = q.dtype, q.shape, k.stride()
+    if dtype != torch.float32 and dtype != torch.bfloat16:
         raise ValueError("q must be float32 or bfloat16")
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("q, k and v must be [B, H, L, D]")
     out = torch.empty_like(q) if out is None else out
-    for t, n in ((q, "q"), (k, "k"), (v, "v"), (out, "out")):
-        if t.dtype != q.dtype or not t.is_cuda or t.dim() != 4 or t.stride(3) != 1:
-            raise ValueError(f"{n} must be a CUDA tensor [B, H, L, D] of q's dtype with contiguous rows")
-    B, Hq, L, D = q.shape
-    if out.shape != q.shape or k.shape != v.shape or k.stride() != v.stride():
-        raise ValueError("out must have q's shape, and k and v one shape and layout")
-    if (k.shape[0], *k.shape[2:]) != (B, L, D):
-        raise ValueError("k and v must be [B, Hkv, L, D]")
-    strides = [C.cast((C.c_int64 * 3)(*t.stride()[:3]), C.c_void_p) for t in (q, k, out)]
-    dt = SA_DTYPE_F32 if q.dtype == torch.float32 else SA_DTYPE_BF16
-    check(lib().sa_prefill_window(_ptr(q), _ptr(k), _ptr(v), dt, B, Hq, k.shape[1], L, D, *strides, window, n_sink,
-                                  scale, _ptr(out), _stream(stream)))
+    B, Hq, L, D = shape
+    Hkv = k.shape[1]
+    if k.shape != (B, Hkv, L, D) or v.shape != k.shape or v.stride() != layout or out.shape != shape:
+        raise ValueError("k and v must be [B, Hkv, L, D] of one layout, and out like q")
+    if k.dtype != dtype or v.dtype != dtype or out.dtype != dtype:
+        raise ValueError("q, k, v and out must have one dtype")
+    if not (q.is_cuda and k.is_cuda and v.is_cuda and out.is_cuda):
+        raise ValueError("q, k, v and out must be CUDA tensors")
+    if q.is_contiguous() and k.is_contiguous() and out.is_contiguous():
+        qs = ks = os_ = None
+    else:
+        if q.stride(3) != 1 or layout[3] != 1 or out.stride(3) != 1:
+            raise ValueError("the rows of q, k, v and out must be contiguous")
+        qs, ks, os_ = (C.cast((C.c_int64 * 3)(*t.stride()[:3]), C.c_void_p) for t in (q, k, out))
+    dt = SA_DTYPE_F32 if dtype == torch.float32 else SA_DTYPE_BF16
+    check(lib().sa_prefill_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, B, Hq, Hkv, L, D, qs, ks, os_, window,
+                                  n_sink, scale, out.data_ptr(), _stream(stream)))
     return out
 
 
