@@ -5,7 +5,7 @@
 // and its own (the tokens behind the prefix, or the sinks and the window of a
 // windowed decode).  A source's tokens are cut into chunks; one workgroup
 // takes a chunk of one KV head for all query rows of the source (rows of the
-// group x query heads of the KV head, up to kRowBlock at a time) and leaves a
+// group x query heads of the KV head, up to Geo::ROWS at a time) and leaves a
 // partial (m, l, O) per query row; a second launch joins a row's partials,
 // O = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c.  A row with one partial
 // is written by the first launch, and a launch of such rows has no second.
@@ -18,12 +18,12 @@
 //
 // Layout: v_mfma_f32_16x16x32_bf16 with S^T = K Q^T (rows: keys, columns: query
 // rows), so that a lane's eight scores of a 32-key tile are the operand that
-// O^T += V^T P^T takes.  Four waves: RG of them take 16 RT query rows each, and
-// 4 / RG groups of RG waves take every (4 / RG)-th tile of the chunk.
+// O^T += V^T P^T takes.  Four waves: RG of them take 16 RT query
+// rows each (RT 1, fp32 also 2), and KG = 4 / RG groups of RG waves take every KG-th tile of the chunk.
 //   RG = 1 (up to 16 RT rows): a wave reads its own tiles and never waits for
 //     another; the next tile's K load into LDS while P V is computed, the next
 //     tile's V while the scores are.
-//   RG = 2, 4: the waves of a key group share its tiles, a ring of RG of them.
+//   RG > 1: the waves of a key group share its tiles, a ring of RG of them.
 #include "ranges.h"
 
 #include <algorithm>
@@ -36,15 +36,13 @@
 namespace sa {
 namespace {
 
-using pf::dma16;
 using pf::lds_s16x4_t;
 using pf::lds_u8_t;
 using pf::s16x4_t;
 
+constexpr int kTile = 32;                    // keys per tile; divides a page
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * kWave;
-constexpr int kTile = 32;                    // keys per tile; divides a page
-constexpr int kRowBlock = kWaves * 2 * 16;   // query rows of one workgroup
 constexpr int kMaxChunks = 64;               // chunks of one source
 constexpr int kChunkTiles = 1024;            // tiles of one chunk, whose page ids sit in LDS
 constexpr int kSources = 2 * kRowsPerLaunch;
@@ -60,7 +58,10 @@ struct RangeArgs {
     float* part_ml;          // [partial rows][n_kv][2]
     int n_kv, n_q, rep, max_pages, num_pages;
     int n_groups, n_rows;
+    int row_block;                           // query rows of a workgroup
     int chunk_group, chunk_own;              // tiles
+    uint32_t rep_inv;                        // ceil(2^20 / rep): j / rep = j rep_inv >> 20 for query rows j
+    uint64_t single;                         // rows with one partial, which is the output
     float sl2;                               // scale * log2(e)
     // Sources 0 .. n_groups - 1 are the groups', n_groups + i is row i's own.
     RangeSource src[kSources];
@@ -73,6 +74,7 @@ struct RangeArgs {
     int32_t group_of[kRowsPerLaunch];        // a row's group
 };
 static_assert(sizeof(RangeArgs) <= 4096, "kernel arguments");
+static_assert(kRowsPerLaunch <= 64, "a bit of `single` per row");
 
 // The tiles of a source: those of [0, a1), then those of [b0, b1).
 __host__ __device__ inline int tiles_a(const RangeSource& s) { return (s.a1 + kTile - 1) / kTile; }
@@ -107,8 +109,10 @@ struct Geo {
     static constexpr int NL = kTile / RPL;            // wave loads per half
     static constexpr int KS = D / 32, DB = D / 16;
     static constexpr int NT = BF16 ? 1 : kTerms;      // terms of a cached value
+    static constexpr int RT = BF16 ? 1 : 2;           // most tiles of 16 query rows of a wave
+    static constexpr int ROWS = kWaves * RT * 16;     // query rows of a workgroup
     // LDS: one tile per wave, or the partials of the waves' query rows at the end.
-    static constexpr int LDS = kWaves * (TILEB > 32 * D * 4 ? TILEB : 32 * D * 4);
+    static constexpr int LDS = kWaves * (TILEB > 16 * RT * D * 4 ? TILEB : 16 * RT * D * 4);
 
     // Chunk c of row r sits at chunk c ^ swz(r) of the row: the 16 rows 8a + 4kb
     // + b (a, b < 4) of a K fragment read, and the rows of a V^T read (bf16: 8g
@@ -124,6 +128,12 @@ struct Geo {
 
 __device__ __forceinline__ f32x4_t lds_f4(const lds_u8_t* p) {
     return *reinterpret_cast<const __attribute__((address_space(3))) f32x4_t*>(p);
+}
+
+// pf::dma16 for data that is read once: non-temporal.
+__device__ __forceinline__ void dma16_nt(const void* g, lds_u8_t* dst) {
+    const uint32_t m = static_cast<uint32_t>(reinterpret_cast<size_t>(dst));
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(g), "s"(m) : "memory", "m0");
 }
 
 template <int N>
@@ -167,12 +177,13 @@ struct WaveState {
         }
     }
     __device__ __forceinline__ void load_q(int rt, const float* row, float sl2) {
+        f32x4_t x[G::KS][2];
 #pragma unroll
-        for (int ks = 0; ks < G::KS; ++ks) {
-            f32x4_t x = *reinterpret_cast<const f32x4_t*>(row + 32 * ks + 8 * g);
-            f32x4_t y = *reinterpret_cast<const f32x4_t*>(row + 32 * ks + 8 * g + 4);
-            split_terms(x * sl2, y * sl2, q[rt][ks]);
-        }
+        for (int ks = 0; ks < G::KS; ++ks)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) x[ks][i] = *reinterpret_cast<const f32x4_t*>(row + 32 * ks + 8 * g + 4 * i);
+#pragma unroll
+        for (int ks = 0; ks < G::KS; ++ks) split_terms(x[ks][0] * sl2, x[ks][1] * sl2, q[rt][ks]);
     }
 
     // Scores of the tile whose K sits at kb, masked to its tokens [lo, hi), and
@@ -281,28 +292,31 @@ struct Item {
     int row0, rows;    // the source's first row of the launch, and its query rows
     int q0, q1;        // the workgroup's query rows of those
     int part0;         // the chunk's first partial row
+    uint64_t single;   // RangeArgs::single from row0 on
 };
 
 // Query row j of an item: row row0 + j / rep of the launch, head j % rep of the
-// KV head.  Whether that row has one partial only is decided by its sources.
-__device__ __forceinline__ int row_blocks(int rows) { return (rows + kRowBlock - 1) / kRowBlock; }
+// KV head.  j <= 64 rep and rep <= 64, so j rep < 2^20 and the product's quotient
+// is exact.
+static_assert(kRowsPerLaunch * kRangesMaxRep * kRangesMaxRep < (1 << 20), "query rows divided by a product");
+__device__ __forceinline__ int row_of(const RangeArgs& a, int j) { return (int)(((uint32_t)j * a.rep_inv) >> 20); }
+
 __device__ __forceinline__ int group_chunks(const RangeArgs& a, int g) {
-    return (a.start[g + 1] - a.start[g]) / row_blocks((a.first[g + 1] - a.first[g]) * a.rep);
+    const int rows = (a.first[g + 1] - a.first[g]) * a.rep;
+    return (a.start[g + 1] - a.start[g]) / ((rows + a.row_block - 1) / a.row_block);
 }
 __device__ __forceinline__ int own_chunks(const RangeArgs& a, int row) {
     return a.start[a.n_groups + row + 1] - a.start[a.n_groups + row];
-}
-__device__ __forceinline__ int row_partials(const RangeArgs& a, int row) {
-    return own_chunks(a, row) + (a.n_groups ? group_chunks(a, a.group_of[row]) : 0);
 }
 
 // O (unnormalised), m and l of query row j of an item: the output itself if it
 // is the row's only partial.  c: float4 column.
 template <int D>
 __device__ __forceinline__ void put(const RangeArgs& a, const Item& it, int j, int c, f32x4_t o, float m, float l) {
-    const int row = it.row0 + j / a.rep, head = it.kvh * a.rep + j % a.rep;
-    if (row_partials(a, row) == 1) {
-        *reinterpret_cast<f32x4_t*>(a.out + ((size_t)row * a.n_q + head) * D + 4 * c) = o * (1.0f / l);
+    const int r = row_of(a, j);
+    if (it.single >> r & 1) {
+        const int head = it.kvh * a.rep + j - r * a.rep;
+        *reinterpret_cast<f32x4_t*>(a.out + ((size_t)(it.row0 + r) * a.n_q + head) * D + 4 * c) = o * (1.0f / l);
         return;
     }
     const size_t at = (size_t)(it.part0 + j) * a.n_kv + it.kvh;
@@ -323,69 +337,69 @@ __device__ __forceinline__ void attend(const RangeArgs& a, const Item& it, lds_u
     WaveState<D, BF16, RT> w;
     w.init(lane);
 
-    // N of the wave loads of K or V of tile u, from load `first` on, into the half
-    // at dst.  Rows outside the source's tokens read the nearest one inside.
-    auto load_half = [&](const void* pool, int u, lds_u8_t* dst, auto n_c, int first) {
+    // Wave loads [first, first + N) of the 2 NL of tile u (K's, then V's) into the
+    // tile at dst.  Rows outside the source's tokens read the nearest one inside.
+    auto load = [&](int u, lds_u8_t* dst, int first, auto n_c) {
         const TileSpan sp = tile_span(it.src, u);
-        const char* base = static_cast<const char*>(pool) +
-                           (((size_t)pages[u - it.u0] * a.n_kv + it.kvh) * SA_PAGE_TOKENS) * G::ROWB;
+        const size_t at = (((size_t)pages[u - it.u0] * a.n_kv + it.kvh) * SA_PAGE_TOKENS) * G::ROWB;
 #pragma unroll
         for (int i = 0; i < decltype(n_c)::value; ++i) {
-            const int r = (first + i) * G::RPL + lane / G::CPR;
+            const bool is_v = first + i >= G::NL;
+            const int r = (first + i - (is_v ? G::NL : 0)) * G::RPL + lane / G::CPR;
             const int tok = min(max(sp.t0 + r, sp.lo), sp.hi - 1) & (SA_PAGE_TOKENS - 1);
             const int col = ((lane % G::CPR) ^ G::swz(r)) * 16;
-            dma16(reinterpret_cast<const uint16_t*>(base + (size_t)tok * G::ROWB + col), dst + (first + i) * 1024);
+            const char* pool = static_cast<const char*>(is_v ? a.v : a.k);
+            dma16_nt(pool + at + (size_t)tok * G::ROWB + col, dst + (first + i) * 1024);
+        }
+    };
+    auto load_queries = [&]() {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+            const int j = min(q_base + 16 * rt + w.r16, it.q1 - 1), r = row_of(a, j);
+            w.load_q(rt, a.q + ((size_t)(it.row0 + r) * a.n_q + it.kvh * a.rep + j - r * a.rep) * D, a.sl2);
         }
     };
 
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int j = min(q_base + 16 * rt + w.r16, it.q1 - 1);
-        w.load_q(rt, a.q + ((size_t)(it.row0 + j / a.rep) * a.n_q + it.kvh * a.rep + j % a.rep) * D, a.sl2);
-    }
-
     if constexpr (RG == 1) {
-        using All = std::integral_constant<int, G::NL>;
+        using Half = std::integral_constant<int, G::NL>;
         lds_u8_t* const kb = smem + wave * G::TILEB;
         lds_u8_t* const vb = kb + G::HALF;
         int u = it.u0 + kg;
         if (u < it.u1) {
-            load_half(a.k, u, kb, All{}, 0);
-            load_half(a.v, u, vb, All{}, 0);
+            load(u, kb, 0, Half{});
+            load(u, kb, G::NL, Half{});
         }
+        load_queries();   // behind the first tile's loads, so that the two latencies are one
         for (; u < it.u1; u += KG) {
             const bool more = u + KG < it.u1;
             wait_loads<G::NL>();                               // K; V may be in flight
             w.scores(kb, tile_span(it.src, u));
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // K has been read
             if (more) {
-                load_half(a.k, u + KG, kb, All{}, 0);
+                load(u + KG, kb, 0, Half{});
                 wait_loads<G::NL>();                           // V; the next K may be in flight
             } else {
                 wait_loads<0>();
             }
             w.weigh(vb);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (more) load_half(a.v, u + KG, vb, All{}, 0);
+            if (more) load(u + KG, kb, G::NL, Half{});
         }
     } else {
         // RG stages per key group; each wave loads its share of a tile.
-        constexpr int MINE = G::NL / RG;
-        static_assert(MINE * RG == G::NL, "a tile's loads are shared evenly");
+        constexpr int MINE = 2 * G::NL / RG;
+        static_assert(MINE * RG == 2 * G::NL, "a tile's loads are shared evenly");
         using Mine = std::integral_constant<int, MINE>;
         lds_u8_t* const ring = smem + kg * RG * G::TILEB;
         const int n_all = (it.u1 - it.u0 + KG - 1) / KG;                  // steps of the workgroup
         const int n = it.u0 + kg < it.u1 ? (it.u1 - it.u0 - kg + KG - 1) / KG : 0;   // of this key group
-        auto load_tile = [&](int t) {
-            lds_u8_t* dst = ring + (t % RG) * G::TILEB;
-            load_half(a.k, it.u0 + kg + t * KG, dst, Mine{}, rg * MINE);
-            load_half(a.v, it.u0 + kg + t * KG, dst + G::HALF, Mine{}, rg * MINE);
-        };
+        auto load_tile = [&](int t) { load(it.u0 + kg + t * KG, ring + (t % RG) * G::TILEB, rg * MINE, Mine{}); };
         for (int t = 0; t < RG - 1; ++t)
             if (t < n) load_tile(t);
+        load_queries();
         for (int t = 0; t < n_all; ++t) {
             // tiles t .. t + RG - 2 are in flight where the chunk has them
-            if (t + RG - 1 <= n) wait_loads<(RG - 2) * 2 * MINE>();
+            if (t + RG - 1 <= n) wait_loads<(RG - 2) * MINE>();
             else wait_loads<0>();
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (t + RG - 1 < n) load_tile(t + RG - 1);
@@ -446,34 +460,35 @@ __device__ __forceinline__ void attend(const RangeArgs& a, const Item& it, lds_u
 }
 
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kThreads, BF16 ? 2 : 1) range_attn_kernel(RangeArgs a) {
+__global__ void __launch_bounds__(kThreads) range_attn_kernel(RangeArgs a) {
+    using G = Geo<D, BF16>;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ int32_t pages[kChunkTiles];
-    __shared__ float ml[kWaves * 32][2];
+    __shared__ float ml[G::ROWS][2];
     lds_u8_t* const smem = (lds_u8_t*)smem_raw;
 
     // The KV head varies fastest: with 8 of them each XCD has one head's chunks.
     Item it;
     it.kvh = blockIdx.x;
     const int n_src = a.n_groups + a.n_rows;
-    int lo = 0, hi = n_src;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.start[mid] <= (int)blockIdx.y) lo = mid;
-        else hi = mid;
-    }
+    // The last source that starts at or before blockIdx.y: every lane looks at
+    // one or two of them.
+    const int lane = threadIdx.x & (kWave - 1);
+    int lo = __popcll(__ballot(lane < n_src && a.start[lane] <= (int)blockIdx.y)) - 1;
+    if (n_src > kWave) lo += __popcll(__ballot(lane + kWave < n_src && a.start[lane + kWave] <= (int)blockIdx.y));
     it.src = a.src[lo];
     const bool grouped = lo < a.n_groups;
     it.row0 = grouped ? a.first[lo] : lo - a.n_groups;
     it.rows = (grouped ? a.first[lo + 1] - a.first[lo] : 1) * a.rep;
-    const int nb = row_blocks(it.rows);
+    const int nb = (it.rows + G::ROWS - 1) / G::ROWS;
     const int local = blockIdx.y - a.start[lo];
     const int chunk = local / nb, tiles = grouped ? a.chunk_group : a.chunk_own;
     it.u0 = chunk * tiles;
     it.u1 = min(it.u0 + tiles, tiles_of(it.src));
-    it.q0 = (local % nb) * kRowBlock;
-    it.q1 = min(it.q0 + kRowBlock, it.rows);
+    it.q0 = (local % nb) * G::ROWS;
+    it.q1 = min(it.q0 + G::ROWS, it.rows);
     it.part0 = a.base[lo] + chunk * it.rows;
+    it.single = a.single >> it.row0;
 
     // The tiles' pages; an id outside the pool (a table entry that was never
     // set) is clamped so that no load can fault.
@@ -483,10 +498,16 @@ __global__ void __launch_bounds__(kThreads, BF16 ? 2 : 1) range_attn_kernel(Rang
     __syncthreads();
 
     const int rows = it.q1 - it.q0;
-    if (rows <= 16) attend<D, BF16, 1, 1>(a, it, smem, pages, ml);
-    else if (rows <= 32) attend<D, BF16, 1, 2>(a, it, smem, pages, ml);
-    else if (rows <= 64) attend<D, BF16, 2, 2>(a, it, smem, pages, ml);
-    else attend<D, BF16, 4, 2>(a, it, smem, pages, ml);
+    if constexpr (BF16) {
+        if (rows <= 16) attend<D, BF16, 1, 1>(a, it, smem, pages, ml);
+        else if (rows <= 32) attend<D, BF16, 2, 1>(a, it, smem, pages, ml);
+        else attend<D, BF16, 4, 1>(a, it, smem, pages, ml);
+    } else {
+        if (rows <= 16) attend<D, BF16, 1, 1>(a, it, smem, pages, ml);
+        else if (rows <= 32) attend<D, BF16, 1, 2>(a, it, smem, pages, ml);
+        else if (rows <= 64) attend<D, BF16, 2, 2>(a, it, smem, pages, ml);
+        else attend<D, BF16, 4, 2>(a, it, smem, pages, ml);
+    }
 }
 
 // Joins the partials of row blockIdx.y's query head blockIdx.x: thread (s, c)
@@ -495,6 +516,7 @@ template <int D>
 __global__ void __launch_bounds__(256) range_merge_kernel(RangeArgs a) {
     constexpr int C = D / 4, S = 256 / C;
     const int head = blockIdx.x, row = blockIdx.y;
+    if (a.single >> row & 1) return;
     const int kvh = head / a.rep;
     const int no = own_chunks(a, row);
     int ng = 0, gbase = 0, grows = 0, gj = 0;
@@ -506,7 +528,6 @@ __global__ void __launch_bounds__(256) range_merge_kernel(RangeArgs a) {
         gbase = a.base[g];
     }
     const int n = ng + no;
-    if (n == 1) return;
     const int c = threadIdx.x % C, s = threadIdx.x / C;
     const int obase = a.base[a.n_groups + row];
     float M = -INFINITY, L = 0.f;
@@ -566,6 +587,27 @@ sa_status launch(const RangeArgs& a, bool merge, hipStream_t st) {
 
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
+// Tiles per chunk.  A launch without groups whose rows have few tiles gives each
+// row one chunk, which saves the second launch: up to four tiles per wave (7 rows
+// of 403 tokens, bf16, d = 64: 6.7 against 7.8 us in four chunks; 16 query rows
+// of 512 tokens, d = 128: a second, third and fourth tile per wave cost 0.8, 1.7
+// and 2.7 us, the second launch 3.5), in fp32 two (a tile per wave costs 3 us).
+// Otherwise the shortest chunk whose workgroups are about one round (2 per CU in
+// bf16, 1 in fp32), since a workgroup costs 5 us besides its tiles (16 rows in 4
+// groups behind 1500 - 2100 tokens, fp32: 12 tiles 20.3, 8 25.7, 4 30.8 us), and
+// kLongChunk where that would be longer (64 rows of 4100 tokens, bf16: 16 tiles
+// 158.3, 24 155.3, 32 156.2, 64 158.6, one round 174 us; 64 rows behind 32768
+// shared tokens: 16 tiles 82, 24 76, 32 74, 48 75 us).
+constexpr int kLongChunk = 32;
+template <class F>
+int pick_tiles(bool bf16, int longest, long long work, const F& workgroups) {
+    if (longest > 0 && longest <= (bf16 ? 4 : 2) * kWaves) return longest;
+    const long long slots = (bf16 ? 2LL : 1LL) * device_cu_count(), round = slots + slots / 4;
+    for (int t = kWaves; t < kLongChunk; t += kWaves)
+        if (work <= round * t && workgroups(t) <= round) return t;
+    return kLongChunk;
+}
+
 }  // namespace
 
 size_t ranges_ws(int n_rows, int n_q, int d, long long own_tokens, long long group_tokens) {
@@ -586,6 +628,8 @@ sa_status decode_ranges(const PagedView& c, const float* q, int n_q, const Range
     a.n_kv = c.n_kv; a.n_q = n_q; a.rep = n_q / c.n_kv;
     a.max_pages = c.max_pages; a.num_pages = c.num_pages;
     a.sl2 = scale * pf::kLog2eP;
+    a.row_block = c.bf16 ? Geo<128, true>::ROWS : Geo<128, false>::ROWS;
+    a.rep_inv = ((1u << 20) + a.rep - 1) / a.rep;
     int g = 0, done = 0;   // the group of the launch's first row, and its rows already attended
     for (int i0 = 0; i0 < plan.n_rows; i0 += kRowsPerLaunch) {
         a.n_rows = std::min(kRowsPerLaunch, plan.n_rows - i0);
@@ -608,23 +652,28 @@ sa_status decode_ranges(const PagedView& c, const float* q, int n_q, const Range
         a.first[a.n_groups] = a.n_rows;
         for (int i = 0; i < a.n_rows; ++i) a.src[a.n_groups + i] = plan.own[i0 + i];
 
-        // Chunks: about two workgroups per CU, at least a tile per wave, at
-        // most kMaxChunks per source (more only where kChunkTiles asks for it).
+        // Chunks of the sources, at most kMaxChunks each (more only where
+        // kChunkTiles asks for it).
         const int n_src = a.n_groups + a.n_rows;
         auto rows_of = [&](int s) { return (s < a.n_groups ? a.first[s + 1] - a.first[s] : 1) * a.rep; };
-        auto blocks_of = [&](int s) { return ceil_div(rows_of(s), kRowBlock); };
-        long long work = 0;
+        auto blocks_of = [&](int s) { return ceil_div(rows_of(s), a.row_block); };
         int longest_group = 0, longest_own = 0;
+        long long work = 0;
         for (int s = 0; s < n_src; ++s) {
             const int t = tiles_of(a.src[s]);
             work += (long long)t * blocks_of(s) * a.n_kv;
             int& longest = s < a.n_groups ? longest_group : longest_own;
             longest = std::max(longest, t);
         }
-        long long chunk = std::max<long long>(kWaves, ceil_div(work, 2LL * device_cu_count()));
+        auto workgroups = [&](int tiles) {
+            long long n = 0;
+            for (int s = 0; s < n_src; ++s) n += (long long)ceil_div(tiles_of(a.src[s]), tiles) * blocks_of(s) * a.n_kv;
+            return n;
+        };
+        int chunk = pick_tiles(c.bf16, a.n_groups ? 0 : longest_own, work, workgroups);
         if (attn_kv_block() > 0) chunk = attn_kv_block() / kTile;
-        a.chunk_group = (int)std::max<long long>(chunk, ceil_div(longest_group, kMaxChunks));
-        a.chunk_own = (int)std::max<long long>(chunk, ceil_div(longest_own, kMaxChunks));
+        a.chunk_group = std::max(chunk, ceil_div(longest_group, kMaxChunks));
+        a.chunk_own = std::max(chunk, ceil_div(longest_own, kMaxChunks));
         a.chunk_group = std::min(a.chunk_group, kChunkTiles);
         a.chunk_own = std::min(a.chunk_own, kChunkTiles);
 
@@ -637,9 +686,10 @@ sa_status decode_ranges(const PagedView& c, const float* q, int n_q, const Range
             parts += (long long)chunks[s] * rows_of(s);
             a.start[s + 1] = a.start[s] + chunks[s] * blocks_of(s);
         }
-        bool merge = false;
+        a.single = 0;
         for (int i = 0; i < a.n_rows; ++i)
-            merge = merge || chunks[a.n_groups + i] + (a.n_groups ? chunks[a.group_of[i]] : 0) != 1;
+            if (chunks[a.n_groups + i] + (a.n_groups ? chunks[a.group_of[i]] : 0) == 1) a.single |= 1ull << i;
+        const bool merge = a.single != (a.n_rows < 64 ? (1ull << a.n_rows) - 1 : ~0ull);
         if (merge) {
             const size_t need = (size_t)parts * a.n_kv * (c.d + 2) * sizeof(float);
             if (need > 0 && (!ws || ws_bytes < need)) return fail(SA_ENOMEM, "workspace too small for the partials");
