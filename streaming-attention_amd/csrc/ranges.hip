@@ -255,31 +255,39 @@ struct WaveState {
 
     // O^T += V^T P^T for the tile whose V sits at vb.
     __device__ __forceinline__ void weigh(const lds_u8_t* vb) {
+        // ND d blocks at a time: consecutive MFMAs do not wait for each other
+        constexpr int ND = 2;
 #pragma unroll
-        for (int db = 0; db < G::DB; ++db) {
-            bf16x8_t vf[G::NT];
-            if constexpr (BF16) {
-                // Lane s of a group of 16 reads row 8 g + 4 u + s / 4, columns
-                // 16 db + 4 (s % 4) ..; lane r16 receives V[8 g + 4 u + e][16 db + r16].
-                const int c = 2 * db + ((r16 & 3) >> 1), h8 = (r16 & 1) * 8;
-                const int r = 8 * g + (r16 >> 2);
-                const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vb + G::off(r, c) + h8));
-                const s16x4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vb + G::off(r + 4, c) + h8));
-                vf[0] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
-            } else {
-                f32x4_t x[2];
+        for (int d0 = 0; d0 < G::DB; d0 += ND) {
+            bf16x8_t vf[ND][G::NT];
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    x[j >> 2][j & 3] = *reinterpret_cast<const __attribute__((address_space(3))) float*>(
-                        vb + G::off(8 * g + j, 4 * db + (r16 >> 2)) + (r16 & 3) * 4);
-                split_terms(x[0], x[1], vf);
+            for (int d = 0; d < ND; ++d) {
+                if constexpr (BF16) {
+                    // Lane s of a group of 16 reads row 8 g + 4 u + s / 4, columns
+                    // 16 db + 4 (s % 4) ..; lane r16 receives V[8 g + 4 u + e][16 db + r16].
+                    const int c = 2 * (d0 + d) + ((r16 & 3) >> 1), h8 = (r16 & 1) * 8;
+                    const int r = 8 * g + (r16 >> 2);
+                    const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vb + G::off(r, c) + h8));
+                    const s16x4_t y =
+                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vb + G::off(r + 4, c) + h8));
+                    vf[d][0] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+                } else {
+                    f32x4_t x[2];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        x[j >> 2][j & 3] = *reinterpret_cast<const __attribute__((address_space(3))) float*>(
+                            vb + G::off(8 * g + j, 4 * (d0 + d) + (r16 >> 2)) + (r16 & 3) * 4);
+                    split_terms(x[0], x[1], vf[d]);
+                }
             }
 #pragma unroll
             for (int pr = 0; pr < PAIRS; ++pr)
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt)
-                    acc[rt][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[pair_a(pr)], p[rt][pair_b(pr)],
-                                                                          acc[rt][db], 0, 0, 0);
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt)
+                        acc[rt][d0 + d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            vf[d][pair_a(pr)], p[rt][pair_b(pr)], acc[rt][d0 + d], 0, 0, 0);
         }
     }
 };
