@@ -129,6 +129,23 @@ sa_status sa_qwen3_prefill(sa_qwen3* model, sa_kvcache* cache, const int32_t* to
 sa_status sa_qwen3_decode_step(sa_qwen3* model, sa_kvcache* cache, const int32_t* tokens, int batch,
                                int32_t* next_tokens, float* logits, sa_stream_t stream);
 
+/* One step of a beam search (no counterpart in the reference): the step of
+ * sa_qwen3_decode_step for rows 0 .. n_groups * n_beams - 1 of the cache, row g
+ * * n_beams + b holding beam b of search g, and sa_beam_select over its logits.
+ * tokens: device int32 [n_groups * n_beams]; scores: device fp32, the beams'
+ * accumulated log probabilities; out_scores, out_tokens, out_beams: device
+ * [n_groups][n_select], as sa_beam_select's.  Every row's length grows by one.
+ * Where the beams of a search share enough leading pages (sa_kvcache_fork,
+ * sa_kvcache_reorder), the attention reads them once per search
+ * (sa_paged_decode_shared), else row by row.  The search goes on with the beams
+ * that the caller picks: sa_kvcache_reorder with their rows as parents, their
+ * tokens and scores as the next step's.  The caller must have reserved pages
+ * of every row's own for the new token.  Asynchronous on stream; the first call
+ * with a given cache geometry and selection allocates workspaces. */
+sa_status sa_qwen3_beam_step(sa_qwen3* model, sa_kvcache* cache, const int32_t* tokens, int n_groups, int n_beams,
+                             const float* scores, int n_select, float* out_scores, int32_t* out_tokens,
+                             int32_t* out_beams, sa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -125,6 +125,7 @@ SIGNATURES = {
     "sa_qwen3_init_random": (_I, [_P, C.c_uint64, _F, _P]),
     "sa_qwen3_decode_step": (_I, [_P, _P, _P, _I, _P, _P, _P]),
     "sa_qwen3_prefill": (_I, [_P, _P, _P, _I, _I, _P, _P, _P]),
+    "sa_qwen3_beam_step": (_I, [_P, _P, _P, _I, _I, _P, _I, _P, _P, _P, _P]),
 }
 
 _lib = None
@@ -729,6 +730,81 @@ class Qwen3:
         check(lib().sa_qwen3_decode_step(self.handle, cache.handle, _ptr(tokens), B, _ptr(next_tokens),
                                          _ptr(logits), _stream(stream)))
         return next_tokens
+
+
+    def beam_step(self, cache: "KVCache", tokens, scores, n_select: int, out=None, stream=None):
+        """One beam search step: tokens int32 CUDA [G, B] (row g * B + b of the
+        cache holds beam b of search g) and accumulated log probabilities scores
+        fp32 CUDA [G, B] -> (scores, tokens, beams), each [G, n_select], best first."""
+        import torch
+        G, B = tokens.shape
+        if tokens.dtype != torch.int32 or not tokens.is_cuda or not tokens.is_contiguous():
+            raise ValueError("tokens must be a contiguous int32 CUDA tensor [G, B]")
+        if tuple(scores.shape) != (G, B):
+            raise ValueError("scores must be [G, B]")
+        if out is None:
+            out = (torch.empty(G, n_select, dtype=torch.float32, device=tokens.device),
+                   *(torch.empty(G, n_select, dtype=torch.int32, device=tokens.device) for _ in range(2)))
+        for t, dt in zip(out, (torch.float32, torch.int32, torch.int32)):
+            if t.dtype != dt or tuple(t.shape) != (G, n_select) or not t.is_cuda or not t.is_contiguous():
+                raise ValueError("out must be contiguous CUDA tensors [G, n_select]: float32, int32, int32")
+        check(lib().sa_qwen3_beam_step(self.handle, cache.handle, _ptr(tokens), G, B, _ptr(_f32(scores, "scores")),
+                                       n_select, _ptr(out[0]), _ptr(out[1]), _ptr(out[2]), _stream(stream)))
+        return out
+
+    def beam_search(self, cache: "KVCache", prompts, n_beams: int, n_tokens: int, eos: int | None = None):
+        """Beam search from prompts int32 CUDA [G, L] over an empty cache of G *
+        n_beams rows: up to n_tokens tokens per continuation, ended early by eos.
+        Returns, per prompt, its n_beams best as (accumulated log probability,
+        tokens), best first.  Ends for a prompt when n_beams ended continuations
+        score above its running ones."""
+        import torch
+        G, L = prompts.shape
+        B, dev = n_beams, prompts.device
+        n_select = min(2 * B, 64)
+        for g in range(G):
+            cache.reserve(g, L)
+        logits = torch.empty(G, self.desc.vocab, dtype=torch.float32, device=dev)
+        self.prefill(cache, prompts, logits=logits)
+        done = [[] for _ in range(G)]
+        step = beam_select(logits.view(G, 1, -1), torch.zeros(G, 1, device=dev), n_select)
+        paths = [[[]] for _ in range(G)]         # tokens of each running beam
+        rows = list(range(G * B))
+        for n in range(1, n_tokens + 1):
+            best = [t.tolist() for t in step]
+            tokens, scores, parents, running = [], [], [], False
+            for g in range(G):
+                kept = []
+                for rank, (s, t, b) in enumerate(zip(*(x[g] for x in best))):
+                    if b < 0:
+                        break
+                    if eos is not None and t == eos:
+                        if rank < B:
+                            done[g].append((s, paths[g][b] + [t]))
+                    elif len(kept) < B:
+                        kept.append((s, t, b))
+                ended = sorted((s for s, _ in done[g]), reverse=True)[:B]
+                if kept and not (len(ended) == B and ended[-1] >= kept[0][0]):
+                    running = True
+                # a search with fewer continuations than beams, or none, goes on with beams of probability 0
+                kept += [(float("-inf"), 0, 0)] * (B - len(kept))
+                paths[g] = [paths[g][b] + [t] for _, t, b in kept]
+                first = g if n == 1 else g * B     # the prompts were rows 0 .. G - 1
+                parents += [first + b for _, _, b in kept]
+                tokens.append([t for _, t, _ in kept])
+                scores.append([s for s, _, _ in kept])
+            if n == n_tokens or not running:
+                break
+            cache.reorder(rows, parents)
+            for r in rows:
+                cache.reserve(r, L + n)
+            step = self.beam_step(cache, torch.tensor(tokens, dtype=torch.int32, device=dev),
+                                  torch.tensor(scores, dtype=torch.float32, device=dev), n_select)
+        out = []
+        for g in range(G):
+            last = [(s, p) for s, p in zip(scores[g], paths[g]) if s > float("-inf")]
+            out.append(sorted(done[g] + last, key=lambda x: -x[0])[:B])
+        return out
 
 
 class _CudaArray:

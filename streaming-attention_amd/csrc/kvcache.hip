@@ -858,6 +858,13 @@ PagedView view_of(const sa_kvcache* c, int layer) {
 }  // namespace
 }  // namespace sa
 
+long long sa::shared_tokens_saved(const sa_kvcache* c, const int32_t* sizes, int n_groups) {
+    long long saved = 0;
+    for (int g = 0, at = 0; g < n_groups; at += sizes[g], ++g)
+        saved += (long long)(sizes[g] - 1) * c->pt.shared_tokens(nullptr, at, sizes[g], 1);
+    return saved;
+}
+
 extern "C" size_t sa_paged_decode_window_ws_bytes(const sa_kvcache* c, int n_seq, int n_q_heads, int window,
                                                   int n_sink) {
     if (!valid_cache(c) || n_seq <= 0 || n_q_heads <= 0 || window <= 0 || n_sink < 0) return 0;

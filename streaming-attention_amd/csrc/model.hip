@@ -17,6 +17,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <new>
 #include <vector>
 
 #include "bf16_terms.h"
@@ -70,6 +71,8 @@ struct sa_qwen3 {
     float* part2 = nullptr;
     void* ws2 = nullptr;
     size_t ws2_bytes = 0;
+    void* beam_ws = nullptr;   // a beam step's greedy tokens, selection and shared attention (grow-only)
+    size_t beam_ws_bytes = 0;
     hipStream_t side = nullptr;
     std::vector<hipEvent_t> events;   // fork, join, the first half's first attention done
 };
@@ -513,6 +516,8 @@ void release(sa_qwen3* m) {
     m->ws = nullptr;
     if (m->ws2) (void)hipFree(m->ws2);
     m->ws2 = nullptr;
+    if (m->beam_ws) (void)hipFree(m->beam_ws);
+    m->beam_ws = nullptr;
     if (m->pf) (void)hipFree(m->pf);
     m->pf = nullptr;
 }
@@ -791,9 +796,28 @@ extern "C" sa_status sa_qwen3_prefill(sa_qwen3* m, sa_kvcache* cache, const int3
     return sa_kvcache_commit(cache, nullptr, batch, L, stream);
 }
 
-extern "C" sa_status sa_qwen3_decode_step(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int batch,
-                                          int32_t* next_tokens, float* logits, sa_stream_t stream) {
-    clear_error();
+namespace sa {
+namespace {
+
+// Tokens that a grouped step has to save reading for its attention to take the
+// shared form (an append and the two launches of sa_paged_decode_shared instead
+// of one or two).  us per layer, one launch / shared, 16 / 8 heads of 128, bf16:
+// 4 rows behind 2048 tokens 13.4 / 12.9, 4096 17.9 / 15.8; 8 behind 1024 13.4 / 13.1,
+// 2048 17.9 / 13.9; 64 behind 128 9.7 / 17.5, 512 28.5 / 18.6; 2 behind 8192 18.8 / 21.4.
+constexpr long long kSharedTokens = 12000;
+
+// Consecutive rows that may share leading pages (sizes adding up to the
+// batch), and the workspace of their attention.
+struct RowGroups {
+    const int32_t* sizes;
+    int n;
+    void* ws;
+    size_t ws_bytes;
+};
+
+// One step of rows 0 .. batch-1, in groups or (NULL) not.
+sa_status decode_rows(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int batch, const RowGroups* groups,
+                      int32_t* next_tokens, float* logits, sa_stream_t stream) {
     if (!m || !cache || !tokens || !next_tokens) return fail(SA_EINVAL, "null argument");
     if (batch < 1 || batch > m->max_batch) return fail(SA_ERANGE, "batch outside [1, max_batch]");
     sa_kv_desc kd;
@@ -808,6 +832,7 @@ extern "C" sa_status sa_qwen3_decode_step(sa_qwen3* m, sa_kvcache* cache, const 
         if (len + 1 > sa_kvcache_capacity(cache, i)) return fail(SA_EFULL, "KV cache full, cannot append more tokens");
     }
     hipStream_t st = as_stream(stream);
+    const bool shared = groups && shared_tokens_saved(cache, groups->sizes, groups->n) >= kSharedTokens;
     const size_t need = sa_paged_decode_ws_bytes(cache, batch, d.n_q_heads);
     SA_TRY(grow(&m->ws, &m->ws_bytes, need));
     const Shapes s = shapes_of(d);
@@ -834,8 +859,8 @@ extern "C" sa_status sa_qwen3_decode_step(sa_qwen3* m, sa_kvcache* cache, const 
     const int kv_elem = kd.kv_dtype == SA_DTYPE_BF16 ? 2 : 4;
     const long long attn_bytes = total * d.n_kv_heads * d.head_dim * 2LL * kv_elem;
     const char* fenv = std::getenv("SA_DECODE_INTERLEAVE");
-    const bool interleave = M >= 2 && (fenv ? std::atoi(fenv) != 0 : attn_bytes >= kInterleaveBytes);
-    const bool long_attn = attn_bytes >= kBesideBytes;
+    const bool interleave = !shared && M >= 2 && (fenv ? std::atoi(fenv) != 0 : attn_bytes >= kInterleaveBytes);
+    const bool long_attn = !shared && attn_bytes >= kBesideBytes;
     bool few_head_rows = false;   // the head takes the last layer's residual sum of all rows
 
     // Rows [r0, r0 + n) of the batch on one stream: its own split-K partials
@@ -880,9 +905,17 @@ extern "C" sa_status sa_qwen3_decode_step(sa_qwen3* m, sa_kvcache* cache, const 
     // the paged decode in one launch per 64 sequences (plus the LSE merge of
     // multi-chunk sequences); the last layer's call also commits the token.
     // (A separate split kernel cost 4.7 us per layer.)
-    auto attention = [&](Rows& r, int l) {
+    // A shared step appends first and commits behind the last layer.
+    auto attention = [&](Rows& r, int l) -> sa_status {
         const sa_qwen3::Layer& L = m->layers[l];
         const int n_part = r.few ? 1 : r.beside ? r.gb.qkv.S : r.g.qkv.split;
+        if (shared) {
+            SA_TRY(qknorm_rope_append_partials(cache, l, r.part, n_part, r.n, 1, s.Hq, L.q_norm, L.k_norm, eps,
+                                               m->rope_cos, m->rope_sin, d.max_pos, m->q_rope, nullptr, nullptr, r.st));
+            SA_TRY(sa_paged_decode_shared(cache, l, m->q_rope, r.n, nullptr, groups->sizes, groups->n, s.Hq, 1, scale,
+                                          m->attn, groups->ws, groups->ws_bytes, r.st));
+            return l + 1 == d.num_layers ? sa_kvcache_commit(cache, nullptr, r.n, 1, r.st) : SA_OK;
+        }
         return sa::append_decode_partials(cache, l, r.part, n_part, r.n, r.ids.data(), s.Hq, L.q_norm, L.k_norm, eps,
                                           m->rope_cos, m->rope_sin, d.max_pos, scale,
                                           m->attn + (size_t)r.r0 * s.Nq, nullptr, r.ws, r.ws_bytes,
@@ -980,5 +1013,41 @@ extern "C" sa_status sa_qwen3_decode_step(sa_qwen3* m, sa_kvcache* cache, const 
     FewInput last{m->h, nullptr, 0, nullptr, 0.f, nullptr};   // normed by the last layer's residual launch
     if (few_head_rows) last = {all.x, all.down_part, kFewSplit, m->final_norm, eps, nullptr};
     SA_TRY(head(m, s, last, M, out_logits, next_tokens, st));
-    return SA_OK;   // the last layer's sa_append_decode committed the token
+    return SA_OK;   // the last layer's attention committed the token
+}
+
+}  // namespace
+}  // namespace sa
+
+extern "C" sa_status sa_qwen3_decode_step(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int batch,
+                                          int32_t* next_tokens, float* logits, sa_stream_t stream) {
+    clear_error();
+    return decode_rows(m, cache, tokens, batch, nullptr, next_tokens, logits, stream);
+}
+
+extern "C" sa_status sa_qwen3_beam_step(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int n_groups,
+                                        int n_beams, const float* scores, int n_select, float* out_scores,
+                                        int32_t* out_tokens, int32_t* out_beams, sa_stream_t stream) {
+    clear_error();
+    if (!m || !cache || !tokens || !scores || !out_scores || !out_tokens || !out_beams)
+        return fail(SA_EINVAL, "null argument");
+    if (n_groups < 1 || n_beams < 1 || (long long)n_groups * n_beams > m->max_batch)
+        return fail(SA_ERANGE, "n_groups * n_beams outside [1, max_batch]");
+    // Refused before anything is enqueued, as the selection would be.
+    const int rows = n_groups * n_beams;
+    const size_t select = sa_beam_select_ws_bytes(n_groups, n_beams, m->d.vocab, n_select);
+    if (select == 0) return fail(SA_EINVAL, "beam selection takes 1 to 64 beams, 1 to 64 selected");
+    auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    const size_t next = up(rows * sizeof(int32_t)), attn = sa_paged_decode_shared_ws_bytes(cache, rows, m->d.n_q_heads);
+    try {
+        const std::vector<int32_t> sizes(n_groups, n_beams);
+        SA_TRY(grow(&m->beam_ws, &m->beam_ws_bytes, next + up(select) + attn));
+        char* ws = static_cast<char*>(m->beam_ws);
+        const RowGroups groups{sizes.data(), n_groups, ws + next + up(select), attn};
+        SA_TRY(decode_rows(m, cache, tokens, rows, &groups, static_cast<int32_t*>(m->beam_ws), m->logits, stream));
+    } catch (const std::bad_alloc&) {
+        return fail(SA_ENOMEM, "out of host memory");
+    }
+    return sa_beam_select(m->logits, m->d.vocab, scores, n_groups, n_beams, m->d.vocab, n_select, out_scores, out_tokens,
+                          out_beams, static_cast<char*>(m->beam_ws) + next, select, stream);
 }

@@ -28,6 +28,7 @@
 
 #include <algorithm>
 #include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "bf16_terms.h"
@@ -595,22 +596,21 @@ sa_status launch(const RangeArgs& a, bool merge, hipStream_t st) {
 
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
-// Tiles per chunk.  A launch without groups whose rows have few tiles gives each
-// row one chunk, which saves the second launch: up to four tiles per wave (7 rows
-// of 403 tokens, bf16, d = 64: 6.7 against 7.8 us in four chunks; 16 query rows
-// of 512 tokens, d = 128: a second, third and fourth tile per wave cost 0.8, 1.7
-// and 2.7 us, the second launch 3.5), in fp32 two (a tile per wave costs 3 us).
-// Otherwise the shortest chunk whose workgroups are about one round (2 per CU in
-// bf16, 1 in fp32), since a workgroup costs 5 us besides its tiles (16 rows in 4
-// groups behind 1500 - 2100 tokens, fp32: 12 tiles 20.3, 8 25.7, 4 30.8 us), and
-// kLongChunk where that would be longer (64 rows of 4100 tokens, bf16: 16 tiles
-// 158.3, 24 155.3, 32 156.2, 64 158.6, one round 174 us; 64 rows behind 32768
+// Tiles per chunk: the shortest chunk whose workgroups are about one round (2
+// per CU in bf16, 1 in fp32; the groups' sources half a round at least, what the
+// rows' own leave otherwise), since a workgroup costs 5 us besides its tiles (16
+// rows in 4 groups behind 1500 - 2100 tokens, fp32: 12 tiles 20.3, 8 25.7, 4 30.8
+// us), and kLongChunk where that would be longer (64 rows of 4100 tokens, bf16: 16
+// tiles 158.3, 24 155.3, 32 156.2, 64 158.6, one round 174 us; 64 rows behind 32768
 // shared tokens: 16 tiles 82, 24 76, 32 74, 48 75 us).
+// A launch without groups whose rows have few tiles gives each row one chunk,
+// which saves the second launch: up to four tiles per wave (7 rows of 403 tokens,
+// bf16, d = 64: 6.7 against 7.8 us in four chunks; 16 query rows of 512 tokens,
+// d = 128: a second, third and fourth tile per wave cost 0.8, 1.7 and 2.7 us, the
+// second launch 3.5), in fp32 two (a tile per wave costs 3 us).
 constexpr int kLongChunk = 32;
 template <class F>
-int pick_tiles(bool bf16, int longest, long long work, const F& workgroups) {
-    if (longest > 0 && longest <= (bf16 ? 4 : 2) * kWaves) return longest;
-    const long long slots = (bf16 ? 2LL : 1LL) * device_cu_count(), round = slots + slots / 4;
+int pick_tiles(long long round, long long work, const F& workgroups) {
     for (int t = kWaves; t < kLongChunk; t += kWaves)
         if (work <= round * t && workgroups(t) <= round) return t;
     return kLongChunk;
@@ -665,25 +665,30 @@ sa_status decode_ranges(const PagedView& c, const float* q, int n_q, const Range
         const int n_src = a.n_groups + a.n_rows;
         auto rows_of = [&](int s) { return (s < a.n_groups ? a.first[s + 1] - a.first[s] : 1) * a.rep; };
         auto blocks_of = [&](int s) { return ceil_div(rows_of(s), a.row_block); };
-        int longest_group = 0, longest_own = 0;
-        long long work = 0;
-        for (int s = 0; s < n_src; ++s) {
-            const int t = tiles_of(a.src[s]);
-            work += (long long)t * blocks_of(s) * a.n_kv;
-            int& longest = s < a.n_groups ? longest_group : longest_own;
-            longest = std::max(longest, t);
-        }
-        auto workgroups = [&](int tiles) {
-            long long n = 0;
-            for (int s = 0; s < n_src; ++s) n += (long long)ceil_div(tiles_of(a.src[s]), tiles) * blocks_of(s) * a.n_kv;
-            return n;
+        // Chunks of the sources first .. last - 1 for about `round` workgroups.
+        auto pick = [&](int first, int last, long long round, bool whole) {
+            int longest = 0;
+            long long work = 0;
+            for (int s = first; s < last; ++s) {
+                longest = std::max(longest, tiles_of(a.src[s]));
+                work += (long long)tiles_of(a.src[s]) * blocks_of(s) * a.n_kv;
+            }
+            auto workgroups = [&](int tiles) {
+                long long n = 0;
+                for (int s = first; s < last; ++s)
+                    n += (long long)ceil_div(tiles_of(a.src[s]), tiles) * blocks_of(s) * a.n_kv;
+                return n;
+            };
+            int chunk = whole && longest <= (c.bf16 ? 4 : 2) * kWaves ? std::max(1, longest)
+                                                                      : pick_tiles(round, work, workgroups);
+            if (attn_kv_block() > 0) chunk = attn_kv_block() / kTile;
+            chunk = std::min(std::max(chunk, ceil_div(longest, kMaxChunks)), kChunkTiles);
+            return std::pair<int, long long>(chunk, workgroups(chunk));
         };
-        int chunk = pick_tiles(c.bf16, a.n_groups ? 0 : longest_own, work, workgroups);
-        if (attn_kv_block() > 0) chunk = attn_kv_block() / kTile;
-        a.chunk_group = std::max(chunk, ceil_div(longest_group, kMaxChunks));
-        a.chunk_own = std::max(chunk, ceil_div(longest_own, kMaxChunks));
-        a.chunk_group = std::min(a.chunk_group, kChunkTiles);
-        a.chunk_own = std::min(a.chunk_own, kChunkTiles);
+        const long long slots = (c.bf16 ? 2LL : 1LL) * device_cu_count(), round = slots + slots / 4;
+        const auto own = pick(a.n_groups, n_src, round, a.n_groups == 0);
+        a.chunk_own = own.first;
+        a.chunk_group = pick(0, a.n_groups, std::max(round - own.second, round / 2), false).first;
 
         long long parts = 0;
         std::vector<int> chunks(n_src);

@@ -274,6 +274,10 @@ sa_status append_decode_partials(sa_kvcache* c, int layer, const float* part, in
                                  int rope_max_pos, float scale, float* out, float* q_out, void* ws,
                                  size_t ws_bytes, int commit, hipStream_t st, DecodeParts* parts = nullptr);
 
+// Tokens that a shared decode of rows 0 .. in groups of sizes[0, n_groups)
+// reads once instead of once per row, with one token pending in each row.
+long long shared_tokens_saved(const sa_kvcache* c, const int32_t* sizes, int n_groups);
+
 size_t paged_ws(int n_seq, int n_q, int n_kv, int d, int max_pages);
 // seq_ids: host array of cache rows (NULL: 0 .. n_seq-1), already checked.
 // lens: the rows' committed lengths (host array in call order, the page
