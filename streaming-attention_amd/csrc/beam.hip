@@ -30,6 +30,8 @@ constexpr int kMaxBeams = 64, kMaxSelect = 64;
 constexpr int kSlots = 8;                                // segments of a thread of the second launch
 constexpr int kBeamsPerWave = kMaxBeams / kSelWaves;
 constexpr int kBlock = 8 * kWave;                        // elements of a wave's step
+constexpr int kWays = 4;                                 // thresholds tried at once
+static_assert(kWays * kSelWaves == kWave && kSelWaves == 16, "a lane per threshold and wave");
 constexpr int kSegList = 256, kCandList = 1024, kGather = 8;
 static_assert(kMaxSelect <= kSegList, "the rounds fill the segment list");
 constexpr float kNone = -INFINITY;
@@ -142,6 +144,18 @@ __device__ __forceinline__ float unordered(uint32_t u) {
     return __uint_as_float(u & 0x80000000u ? u & 0x7fffffffu : ~u);
 }
 
+// A beam's segment in one integer of the segments' order.
+constexpr int kSegBits = 16;
+static_assert(kSelWaves * kWave * kSlots <= 1 << kSegBits, "segments of a beam");
+__device__ __forceinline__ int segment_id(int beam, int seg) { return beam << kSegBits | seg; }
+__device__ __forceinline__ int beam_of(int id) { return id >> kSegBits; }
+__device__ __forceinline__ int seg_of(int id) { return id & ((1 << kSegBits) - 1); }
+
+struct alignas(16) Candidate {
+    double c;
+    int idx;
+};
+
 // Candidate order: larger value first, of equal ones the lower index.
 __device__ __forceinline__ bool ahead(double v, int i, double w, int j) { return v > w || (v == w && i < j); }
 
@@ -176,10 +190,9 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
     __shared__ double wave_sum[kSelWaves][kBeamsPerWave];
     __shared__ float beam_max[kMaxBeams];
     __shared__ float top[kSelWaves];
-    __shared__ int counts[2][kSelWaves];
+    __shared__ float counts[2][kWays * kSelWaves];
     __shared__ int seg_list[kSegList];
-    __shared__ double cand_v[kCandList];
-    __shared__ int cand_i[kCandList];
+    __shared__ Candidate cand[kCandList];
     __shared__ int n_segs, n_cand;
     __shared__ double red_v[kSelWaves];
     __shared__ int red_i[kSelWaves];
@@ -196,6 +209,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
 
     // ---- this thread's segments: slot j is part j % per_beam of its wave's beam
     // j / per_beam, whose segments are dealt out to the beam's waves first ----
+    const float score = tid < a.n_beams ? a.scores[(long long)group * a.n_beams + tid] : 0.f;
     float2 sg[kSlots];
     int id[kSlots];      // segment of the beam, -1: none
     int of[kSlots];      // the beam's place in the wave (uniform)
@@ -247,13 +261,14 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
         double l = 0.0;
         for (int w = w0; w < w0 + a.waves_per_beam; ++w) l += wave_sum[w][bi];
         const double lse = (double)beam_max[tid] + log(l);
-        base[tid] = isfinite(lse) ? (double)a.scores[(long long)group * a.n_beams + tid] - lse : (double)NAN;
+        base[tid] = isfinite(lse) ? (double)score - lse : (double)NAN;
     }
     __syncthreads();
 
     // ---- tau: a value that at least `want`, and rarely more than twice as many,
     // of the threads' largest segment maxima reach (-inf: fewer threads have one).
-    // Bisection over the values' bit patterns, from 16 below the largest on. ----
+    // kWays thresholds at once, then equal parts of the range that is left, by
+    // the values' bit patterns. ----
     float key[kSlots];
     float best = kNone;
 #pragma unroll
@@ -270,50 +285,62 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
         if (lane == 0) top[wave] = m;
     }
     __syncthreads();
-    float most = top[0];
-#pragma unroll
-    for (int w = 1; w < kSelWaves; ++w) most = fmaxf(most, top[w]);
+    const float most = group_reduce<OpMax, 1, kSelWaves>(top[lane % kSelWaves]);
     const uint32_t mine = ordered(best);
     int parity = 0;
-    auto reach = [&](uint32_t v) {   // threads whose best is at least v
-        const int n = __popcll(__ballot(mine >= v));
-        if (lane == 0) counts[parity][wave] = n;
-        __syncthreads();
-        int all = 0;
+    // Threads whose best is at least v[0], .., v[kWays - 1] (increasing).  Lanes 16 i
+    // .. add up the waves' counts for v[i] (whole numbers, exact in fp32).
+    auto reach = [&](const uint32_t (&v)[kWays], int (&n)[kWays]) {
 #pragma unroll
-        for (int w = 0; w < kSelWaves; ++w) all += counts[parity][w];
-        parity ^= 1;
-        return all;
-    };
-    uint32_t lo = ordered(kNone) + 1, hi = ordered(most) + 1;
-    float t = kNone;
-    if (most > kNone && reach(lo) >= want) {
-        const uint32_t near = ordered(most - 16.f);
-        if (near > lo && reach(near) >= want) lo = near;
-        while (hi - lo > 1) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            const int n = reach(mid);
-            if (n >= want) lo = mid;
-            else hi = mid;
-            if (n >= want && n <= 2 * want) break;
+        for (int i = 0; i < kWays; ++i) {
+            const int here = __popcll(__ballot(mine >= v[i]));
+            if (lane == 0) counts[parity][i * kSelWaves + wave] = (float)here;
         }
-        t = unordered(lo);
+        __syncthreads();
+        const float all = group_reduce<OpSum, 1, kSelWaves>(counts[parity][lane]);
+#pragma unroll
+        for (int i = 0; i < kWays; ++i)
+            n[i] = (int)__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(all), i * kSelWaves));
+        parity ^= 1;
+    };
+    float t = kNone;
+    if (most > kNone) {
+        const uint32_t bottom = ordered(kNone) + 1;
+        uint32_t v[kWays] = {bottom, max(bottom, ordered(most - 16.f)), max(bottom, ordered(most - 8.f)),
+                             max(bottom, ordered(most - 4.f))};
+        uint32_t lo = bottom, hi = ordered(most) + 1;
+        int n[kWays];
+        reach(v, n);
+        bool go = n[0] >= want;      // else every value is wanted
+        while (go) {
+#pragma unroll
+            for (int i = 0; i < kWays; ++i) {
+                if (n[i] >= want) lo = v[i];
+                if (n[i] >= want && n[i] <= 2 * want) go = false;
+                if (n[i] < want) hi = min(hi, v[i]);
+            }
+            t = unordered(lo);
+            if (!go || hi - lo <= 1) break;
+            const uint32_t step = (hi - lo) / (kWays + 1);
+#pragma unroll
+            for (int i = 0; i < kWays; ++i) v[i] = lo + (step ? (i + 1) * step : min(i + 1u, hi - 1 - lo));
+            reach(v, n);
+        }
     }
-
 
     // ---- the segments and elements that reach it ----
 #pragma unroll
     for (int j = 0; j < kSlots; ++j) {
         if (key[j] > kNone && key[j] >= t) {
             const int at = atomicAdd(&n_segs, 1);
-            if (at < kSegList) seg_list[at] = (beam0 + of[j]) * a.n_seg + id[j];
+            if (at < kSegList) seg_list[at] = segment_id(beam0 + of[j], id[j]);
         }
     }
     __syncthreads();
     const float* x = a.logits + (long long)group * a.n_beams * a.row_stride;
     auto value = [&](int s, int off, int& idx) -> double {
-        const int b = s / a.n_seg;
-        const long long tok = (long long)(s % a.n_seg) * a.seg_len + off;
+        const int b = beam_of(s);
+        const long long tok = (long long)seg_of(s) * a.seg_len + off;
         idx = -1;
         if (tok >= a.vocab) return 0.0;
         const double c = base[b] + (double)x[b * a.row_stride + tok];
@@ -333,8 +360,8 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
                 idx[j] = -1;
                 if (at < n) {
                     const int s = seg_list[at >> shift];
-                    beam[j] = s / a.n_seg;
-                    const long long tok = (((long long)s - beam[j] * a.n_seg) << shift) + (at & (a.seg_len - 1));
+                    beam[j] = beam_of(s);
+                    const long long tok = ((long long)seg_of(s) << shift) + (at & (a.seg_len - 1));
                     if (tok < a.vocab) {
                         idx[j] = beam[j] * a.vocab + (int)tok;
                         v[j] = x[beam[j] * a.row_stride + tok];
@@ -347,10 +374,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
                 const double c = base[beam[j]] + (double)v[j];
                 if (c > (double)kNone && (float)c >= t) {
                     const int at = atomicAdd(&n_cand, 1);
-                    if (at < kCandList) {
-                        cand_v[at] = c;
-                        cand_i[at] = idx[j];
-                    }
+                    if (at < kCandList) cand[at] = Candidate{c, idx[j]};
                 }
             }
         }
@@ -365,11 +389,11 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
     if (n_segs <= kSegList && n_cand <= kCandList) {
         const int n = n_cand;
         if (tid < n) {
-            const double c = cand_v[tid];
-            const int idx = cand_i[tid];
+            const Candidate mine = cand[tid];
             int r = 0;
-            for (int j = 0; j < n; ++j) r += ahead(cand_v[j], cand_i[j], c, idx);
-            if (r < a.n_select) put(r, c, idx);
+#pragma unroll 8
+            for (int j = 0; j < n; ++j) r += ahead(cand[j].c, cand[j].idx, mine.c, mine.idx);
+            if (r < a.n_select) put(r, mine.c, mine.idx);
         }
         if (tid >= n && tid < a.n_select) put(tid, 0.0, -1);
         return;
@@ -385,7 +409,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
 #pragma unroll
         for (int j = 0; j < kSlots; ++j) {
             if (!(key[j] > kNone)) continue;
-            const int s = (beam0 + of[j]) * a.n_seg + id[j];
+            const int s = segment_id(beam0 + of[j], id[j]);
             const double c = base[beam0 + of[j]] + (double)sg[j].x;
             if (picked && !ahead(last_v, last_i, c, s)) continue;
             if (idx < 0 || ahead(c, s, v, idx)) {
