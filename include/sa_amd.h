@@ -163,7 +163,9 @@ sa_status sa_kvcache_commit(sa_kvcache* cache, const int32_t* seqs, int n_seqs, 
  * returns to the pool when the last sequence drops it.  Both calls decide on
  * the host and enqueue one small launch per 64 rows (more where many table
  * entries change); a refused call changes and enqueues nothing.  They are
- * refused while another device than the cache's is current. */
+ * refused while another device than the cache's is current.  A graph that
+ * captures one repeats, at each replay, what was decided at the call: replay it
+ * only in the state that the call found. */
 
 /* Sequence dst gives its pages back and becomes the first n_tokens committed
  * tokens of src (n_tokens <= src's length, else SA_ERANGE): src's whole pages
@@ -288,7 +290,10 @@ sa_status sa_paged_decode(const sa_kvcache* cache, int layer, const float* q,
  * output.  head_dim 64 or 128, at most 64 query heads per KV head; q
  * [n_seq][n_q_heads][D] fp32, out likewise, accumulation in fp32.  q, out and
  * ws 16-byte aligned; ws of sa_paged_decode_window_ws_bytes(...) bytes
- * (n_seq as in the call); calls that overlap on one workspace race.
+ * (n_seq as in the call); calls that overlap on one workspace race.  The
+ * tokens are those of the lengths at the call, also where a graph that holds
+ * the call is replayed; with 33 million tokens or more per sequence a call may
+ * be refused (SA_EINVAL).
  * ------------------------------------------------------------------------ */
 size_t sa_paged_decode_window_ws_bytes(const sa_kvcache* cache, int n_seq, int n_q_heads, int window, int n_sink);
 sa_status sa_paged_decode_window(const sa_kvcache* cache, int layer, const float* q,
@@ -413,8 +418,9 @@ sa_status sa_prefill_causal_strided_ws(const void* q, const void* k, const void*
  * bf16 operands, fp32 sums and softmax), or fp32 throughout.  D 64 or 128,
  * L <= 2^30 (0: nothing to do).  Strides in elements {batch, head, row}, as in
  * sa_prefill_causal_strided, for all tensors or NULL for all (dense); rows
- * contiguous; tensors and strides multiples of 16 bytes.  out must not
- * overlap an input.  The keys and values of a tile enter the products
+ * contiguous; tensors and strides multiples of 16 bytes, the row stride of k
+ * and v below 2^24 elements.  More than 2^23 query tiles (of 16 to 256 rows) are
+ * refused.  out must not overlap an input.  The keys and values of a tile enter the products
  * together: a value that is not finite may reach queries up to 63 keys away
  * that do not see it.
  * ------------------------------------------------------------------------ */
@@ -494,7 +500,8 @@ sa_status sa_axpby_f32(const float* x, float a, const float* y, float b, size_t 
  * a beam whose score is -inf (beams not yet begun) or NaN or whose normaliser
  * is not finite (a NaN or +inf among its logits, or nothing but -inf).  Places
  * left over hold -inf, -1 and -1.  The order is decided in 64 bits.
- * n_beams and n_select 1 .. 64, n_beams * vocab < 2^31.  ws: 8-byte aligned,
+ * n_beams and n_select 1 .. 64, n_beams * vocab < 2^31, n_groups at most 2^20
+ * and n_groups * n_beams * ceil(vocab / 2048) below 2^24.  out_scores may be scores itself.  ws: 8-byte aligned,
  * sa_beam_select_ws_bytes bytes; calls that overlap on one workspace race.
  * The parents (out_beams) are what sa_kvcache_reorder takes, on the host.
  * ------------------------------------------------------------------------ */

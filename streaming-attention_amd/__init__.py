@@ -189,6 +189,28 @@ def _stream(stream) -> int | None:
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else stream
 
 
+def _alloc(stream, make):
+    """make() with its tensors allocated for the stream that the call runs on."""
+    if stream is None:
+        return make()
+    import torch
+    s = stream if hasattr(stream, "cuda_stream") else torch.cuda.ExternalStream(stream)
+    with torch.cuda.stream(s):
+        return make()
+
+
+def _on_device(*tensors) -> None:
+    """Kernels run on the current device, and so must their tensors be."""
+    import torch
+    device = torch.cuda.current_device()
+    for t in tensors:
+        if t.get_device() != device:
+            raise ValueError("the tensors must be on the current CUDA device")
+
+
+_INT_MAX = 2 ** 31 - 1
+
+
 _float32 = None   # torch.float32 (torch is imported by the first call that needs it)
 
 
@@ -348,8 +370,9 @@ class KVCache:
         """decode over each sequence's last `window` tokens and its first
         n_sink: q [n_seq, Hq, D] -> out [n_seq, Hq, D]."""
         n_seq, Hq, _ = q.shape
-        out, ws = self._out_ws(q, out, ws, lambda: self.decode_window_ws_bytes(n_seq, Hq, window, n_sink))
-        check(lib().sa_paged_decode_window(self.handle, layer, _ptr(_f32(q, "q")), n_seq, _rows(seq_ids, n_seq), Hq,
+        window, n_sink = min(window, _INT_MAX), min(n_sink, _INT_MAX)
+        out, ws = self._out_ws(q, out, ws, lambda: self.decode_window_ws_bytes(n_seq, Hq, window, n_sink), stream)
+        check(lib().sa_paged_decode_window(self.handle, layer, _ptr(q), n_seq, _rows(seq_ids, n_seq), Hq,
                                            n_pending, window, n_sink, scale, _ptr(out), _ptr(ws), _nbytes(ws),
                                            _stream(stream)))
         return out
@@ -363,25 +386,26 @@ class KVCache:
         one group) whose shared leading pages are read once per group:
         q [n_seq, Hq, D] -> out [n_seq, Hq, D]."""
         n_seq, Hq, _ = q.shape
-        out, ws = self._out_ws(q, out, ws, lambda: self.decode_shared_ws_bytes(n_seq, Hq))
+        out, ws = self._out_ws(q, out, ws, lambda: self.decode_shared_ws_bytes(n_seq, Hq), stream)
         n_groups = 0 if groups is None else len(groups)
-        check(lib().sa_paged_decode_shared(self.handle, layer, _ptr(_f32(q, "q")), n_seq, _rows(seq_ids, n_seq),
+        check(lib().sa_paged_decode_shared(self.handle, layer, _ptr(q), n_seq, _rows(seq_ids, n_seq),
                                            _rows(groups, n_groups), n_groups, Hq, n_pending, scale, _ptr(out),
                                            _ptr(ws), _nbytes(ws), _stream(stream)))
         return out
 
-    def _out_ws(self, q, out, ws, need):
+    def _out_ws(self, q, out, ws, need, stream):
         """The output and workspace of a decode of q, made where not given."""
         import torch
+        _f32(q, "q")
         if q.shape[-1] != self.desc.head_dim:
             raise ValueError("q must be [n_seq, Hq, head_dim]")
         if out is None:
-            out = torch.empty_like(q)
+            out = _alloc(stream, lambda: torch.empty_like(q))
         elif out.shape != q.shape:
             raise ValueError("out must have q's shape")
         if ws is None:
-            ws = torch.empty(max(need(), 16), dtype=torch.uint8, device=q.device)
-        _f32(out, "out")
+            ws = _alloc(stream, lambda: torch.empty(max(need(), 16), dtype=torch.uint8, device=q.device))
+        _on_device(q, _f32(out, "out"), ws)
         return out, ws
 
     def append_decode(self, layer: int, q, k, v, scale: float, q_norm_w=None, k_norm_w=None, eps: float = 1e-6,
@@ -522,6 +546,12 @@ def beam_select_ws_bytes(n_groups: int, n_beams: int, vocab: int, n_select: int)
     return lib().sa_beam_select_ws_bytes(n_groups, n_beams, vocab, n_select)
 
 
+def _selection(G: int, n_select: int, device):
+    import torch
+    return (torch.empty(G, n_select, dtype=torch.float32, device=device),
+            *(torch.empty(G, n_select, dtype=torch.int32, device=device) for _ in range(2)))
+
+
 def beam_select(logits, scores, n_select: int, out=None, ws=None, stream=None):
     """The n_select best continuations of each search: logits [G, B, vocab] fp32
     (rows may be strided), accumulated log probabilities scores [G, B] ->
@@ -540,16 +570,17 @@ def beam_select(logits, scores, n_select: int, out=None, ws=None, stream=None):
     if scores.shape != (G, B):
         raise ValueError("scores must be [G, B]")
     if out is None:
-        out = (torch.empty(G, n_select, dtype=torch.float32, device=logits.device),
-               *(torch.empty(G, n_select, dtype=torch.int32, device=logits.device) for _ in range(2)))
+        out = _alloc(stream, lambda: _selection(G, n_select, logits.device))
     o, t, b = out
     if not (o.shape == t.shape == b.shape == (G, n_select) and o.is_contiguous() and t.is_contiguous() and
             b.is_contiguous() and o.is_cuda and t.is_cuda and b.is_cuda and o.dtype == torch.float32 and
             t.dtype == torch.int32 and b.dtype == torch.int32):
         raise ValueError("out must be contiguous CUDA tensors [G, n_select]: float32, int32, int32")
     if ws is None:
-        ws = torch.empty(max(beam_select_ws_bytes(G, B, V, n_select), 8), dtype=torch.uint8, device=logits.device)
-    check(lib().sa_beam_select(logits.data_ptr(), stride, _ptr(_f32(scores, "scores")), G, B, V, n_select, o.data_ptr(),
+        ws = _alloc(stream, lambda: torch.empty(max(beam_select_ws_bytes(G, B, V, n_select), 8), dtype=torch.uint8,
+                                                device=logits.device))
+    _on_device(logits, _f32(scores, "scores"), o, t, b, ws)
+    check(lib().sa_beam_select(logits.data_ptr(), stride, _ptr(scores), G, B, V, n_select, o.data_ptr(),
                                t.data_ptr(), b.data_ptr(), ws.data_ptr(), _nbytes(ws), _stream(stream)))
     return out
 
@@ -617,15 +648,14 @@ def prefill_window(q, k, v, scale: float, window: int, n_sink: int = 0, out=None
         raise ValueError("q must be float32 or bfloat16")
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError("q, k and v must be [B, H, L, D]")
-    out = torch.empty_like(q) if out is None else out
+    out = _alloc(stream, lambda: torch.empty_like(q)) if out is None else out
     B, Hq, L, D = shape
     Hkv = k.shape[1]
     if k.shape != (B, Hkv, L, D) or v.shape != k.shape or v.stride() != layout or out.shape != shape:
         raise ValueError("k and v must be [B, Hkv, L, D] of one layout, and out like q")
     if k.dtype != dtype or v.dtype != dtype or out.dtype != dtype:
         raise ValueError("q, k, v and out must have one dtype")
-    if not (q.is_cuda and k.is_cuda and v.is_cuda and out.is_cuda):
-        raise ValueError("q, k, v and out must be CUDA tensors")
+    _on_device(q, k, v, out)
     if q.is_contiguous() and k.is_contiguous() and out.is_contiguous():
         qs = ks = os_ = None
     else:
@@ -633,8 +663,8 @@ def prefill_window(q, k, v, scale: float, window: int, n_sink: int = 0, out=None
             raise ValueError("the rows of q, k, v and out must be contiguous")
         qs, ks, os_ = (C.cast((C.c_int64 * 3)(*t.stride()[:3]), C.c_void_p) for t in (q, k, out))
     dt = SA_DTYPE_F32 if dtype == torch.float32 else SA_DTYPE_BF16
-    check(lib().sa_prefill_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, B, Hq, Hkv, L, D, qs, ks, os_, window,
-                                  n_sink, scale, out.data_ptr(), _stream(stream)))
+    check(lib().sa_prefill_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, B, Hq, Hkv, L, D, qs, ks, os_,
+                                  min(window, _INT_MAX), min(n_sink, _INT_MAX), scale, out.data_ptr(), _stream(stream)))
     return out
 
 
@@ -743,12 +773,12 @@ class Qwen3:
         if tuple(scores.shape) != (G, B):
             raise ValueError("scores must be [G, B]")
         if out is None:
-            out = (torch.empty(G, n_select, dtype=torch.float32, device=tokens.device),
-                   *(torch.empty(G, n_select, dtype=torch.int32, device=tokens.device) for _ in range(2)))
+            out = _alloc(stream, lambda: _selection(G, n_select, tokens.device))
         for t, dt in zip(out, (torch.float32, torch.int32, torch.int32)):
             if t.dtype != dt or tuple(t.shape) != (G, n_select) or not t.is_cuda or not t.is_contiguous():
                 raise ValueError("out must be contiguous CUDA tensors [G, n_select]: float32, int32, int32")
-        check(lib().sa_qwen3_beam_step(self.handle, cache.handle, _ptr(tokens), G, B, _ptr(_f32(scores, "scores")),
+        _on_device(tokens, _f32(scores, "scores"), *out)
+        check(lib().sa_qwen3_beam_step(self.handle, cache.handle, _ptr(tokens), G, B, _ptr(scores),
                                        n_select, _ptr(out[0]), _ptr(out[1]), _ptr(out[2]), _stream(stream)))
         return out
 
@@ -757,9 +787,15 @@ class Qwen3:
         n_beams rows: up to n_tokens tokens per continuation, ended early by eos.
         Returns, per prompt, its n_beams best as (accumulated log probability,
         tokens), best first.  Ends for a prompt when n_beams ended continuations
-        score above its running ones."""
+        score above its running ones.  Up to 64 beams; a step offers min(2 *
+        n_beams, 64) continuations, so with more than 32 beams fewer may run on
+        where some end.  The cache holds the last beams afterwards: reset it."""
         import torch
+        if not 1 <= n_beams <= 64 or n_tokens < 1:
+            raise ValueError("beam_search takes 1 to 64 beams and at least one token")
         G, L = prompts.shape
+        if G * n_beams > cache.desc.max_seqs:
+            raise ValueError("the cache needs a row per beam")
         B, dev = n_beams, prompts.device
         n_select = min(2 * B, 64)
         for g in range(G):

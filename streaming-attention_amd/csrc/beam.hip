@@ -27,6 +27,7 @@ namespace {
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / kWave;
 constexpr int kMaxBeams = 64, kMaxSelect = 64;
+constexpr int kMaxGroups = 1 << 20;                      // a grid has fewer than 2^32 threads
 constexpr int kSlots = 8;                                // segments of a thread of the second launch
 constexpr int kBeamsPerWave = kMaxBeams / kSelWaves;
 constexpr int kBlock = 8 * kWave;                        // elements of a wave's step
@@ -465,7 +466,7 @@ BeamShape beam_shape(int n_beams, int vocab) {
 
 bool beam_sizes_ok(int n_groups, int n_beams, int vocab, int n_select) {
     return n_groups > 0 && n_beams > 0 && n_beams <= kMaxBeams && vocab > 0 && n_select > 0 && n_select <= kMaxSelect &&
-           (long long)n_beams * vocab < (1LL << 31) && (long long)n_groups * n_beams < (1LL << 24);
+           (long long)n_beams * vocab < (1LL << 31) && n_groups <= kMaxGroups;
 }
 
 }  // namespace
@@ -484,7 +485,7 @@ extern "C" sa_status sa_beam_select(const float* logits, int64_t row_stride, con
     clear_error();
     if (!logits || !scores || !out_scores || !out_tokens || !out_beams) return fail(SA_EINVAL, "null pointer");
     if (!beam_sizes_ok(n_groups, n_beams, vocab, n_select))
-        return fail(SA_EINVAL, "beam selection takes 1 to 64 beams, 1 to 64 selected, n_beams * vocab < 2^31");
+        return fail(SA_EINVAL, "beam selection takes 1 to 64 beams, 1 to 64 selected, n_beams * vocab < 2^31, 2^20 groups");
     if (row_stride < vocab) return fail(SA_EINVAL, "row_stride must be at least vocab");
     const BeamShape sh = beam_shape(n_beams, vocab);
     if (!ws || ws_bytes < sa_beam_select_ws_bytes(n_groups, n_beams, vocab, n_select))
@@ -501,7 +502,7 @@ extern "C" sa_status sa_beam_select(const float* logits, int64_t row_stride, con
     a.wg_per_row = (int)((vocab + 4 * per_wave - 1) / (4 * per_wave));
     hipStream_t st = as_stream(stream);
     const long long wgs = (long long)n_groups * n_beams * a.wg_per_row;
-    if (wgs >= (1LL << 31)) return fail(SA_EINVAL, "too many rows");
+    if (wgs >= (1LL << 24)) return fail(SA_EINVAL, "too many logits for one call");
     const dim3 grid((unsigned)wgs);
     const bool vec = aligned16(logits) && row_stride % 4 == 0;
     switch (sh.vpt) {

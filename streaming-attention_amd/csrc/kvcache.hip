@@ -858,6 +858,11 @@ PagedView view_of(const sa_kvcache* c, int layer) {
 }  // namespace
 }  // namespace sa
 
+sa_status sa::check_append(const sa_kvcache* c, int n, int S, int max_pos) {
+    const Verdict v = c->pt.check_append(nullptr, n, S, max_pos);
+    return v.ok() ? SA_OK : refused(v);
+}
+
 long long sa::shared_tokens_saved(const sa_kvcache* c, const int32_t* sizes, int n_groups) {
     long long saved = 0;
     for (int g = 0, at = 0; g < n_groups; at += sizes[g], ++g)

@@ -723,6 +723,7 @@ extern "C" sa_status sa_qwen3_prefill(sa_qwen3* m, sa_kvcache* cache, const int3
         if (sa_kvcache_len(cache, i) != 0) return fail(SA_EINVAL, "prefill needs empty sequences");
         if (sa_kvcache_capacity(cache, i) < L) return fail(SA_EFULL, "KV cache full, reserve pages for the prompt");
     }
+    SA_TRY(check_append(cache, batch, L, d.max_pos));
     hipStream_t st = as_stream(stream);
     const Shapes s = shapes_of(d);
     const long long M = (long long)batch * L;
@@ -831,6 +832,7 @@ sa_status decode_rows(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int
         if (len < 0 || len >= d.max_pos) return fail(SA_ERANGE, "position outside the RoPE table");
         if (len + 1 > sa_kvcache_capacity(cache, i)) return fail(SA_EFULL, "KV cache full, cannot append more tokens");
     }
+    SA_TRY(check_append(cache, batch, 1, d.max_pos));
     hipStream_t st = as_stream(stream);
     const bool shared = groups && shared_tokens_saved(cache, groups->sizes, groups->n) >= kSharedTokens;
     const size_t need = sa_paged_decode_ws_bytes(cache, batch, d.n_q_heads);

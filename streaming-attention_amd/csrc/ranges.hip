@@ -699,6 +699,7 @@ sa_status decode_ranges(const PagedView& c, const float* q, int n_q, const Range
             parts += (long long)chunks[s] * rows_of(s);
             a.start[s + 1] = a.start[s] + chunks[s] * blocks_of(s);
         }
+        if (a.start[n_src] > 65535) return fail(SA_EINVAL, "too many tokens for one call");   // the grid's y
         a.single = 0;
         for (int i = 0; i < a.n_rows; ++i)
             if (chunks[a.n_groups + i] + (a.n_groups ? chunks[a.group_of[i]] : 0) == 1) a.single |= 1ull << i;

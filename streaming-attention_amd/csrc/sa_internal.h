@@ -274,6 +274,10 @@ sa_status append_decode_partials(sa_kvcache* c, int layer, const float* part, in
                                  int rope_max_pos, float scale, float* out, float* q_out, void* ws,
                                  size_t ws_bytes, int commit, hipStream_t st, DecodeParts* parts = nullptr);
 
+// Whether the next S tokens of rows 0 .. n - 1 can be appended: pages of their
+// own for them, and positions below max_pos.
+sa_status check_append(const sa_kvcache* c, int n, int S, int max_pos);
+
 // Tokens that a shared decode of rows 0 .. in groups of sizes[0, n_groups)
 // reads once instead of once per row, with one token pending in each row.
 long long shared_tokens_saved(const sa_kvcache* c, const int32_t* sizes, int n_groups);

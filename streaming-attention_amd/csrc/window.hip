@@ -644,7 +644,9 @@ extern "C" sa_status sa_prefill_window(const void* q, const void* k, const void*
     a.gh = s.gh;
     a.q_tile = s.q_tile;
     a.n_qt = (L + s.q_tile - 1) / s.q_tile;
-    if ((long long)batch * (n_q_heads / s.gh) * a.n_qt >= (1LL << 31)) return fail(SA_EINVAL, "too many query tiles");
+    // a grid has fewer than 2^32 threads
+    if ((long long)batch * (n_q_heads / s.gh) * a.n_qt >= (1LL << 32) / (s.waves * kWave))
+        return fail(SA_EINVAL, "too many query tiles");
     const long long groups = (long long)batch * n_kv_heads;
     a.xcd_groups = groups % 8 == 0 ? (int)(groups / 8) : 0;
     // bf16: the sign goes to q, so that the scores' factor is not negative

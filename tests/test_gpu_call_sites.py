@@ -1,0 +1,134 @@
+"""GPU tests of how the windowed, shared-prefix and beam-search calls sit in a
+program: outputs and workspaces made on the stream that the call runs on,
+tensors of another device, sizes beyond a C int, refusals of a step."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def filled_cache(sa, rows, n):
+    c = sa.KVCache(1, 2, 64, rows, (n + 64) // 64, rows * ((n + 64) // 64), sa.SA_DTYPE_BF16)
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    for r in range(rows):
+        c.reserve(r, n + 1)
+    c.append(0, None, *(torch.randn(rows, n, 2, 64, device="cuda", generator=gen) for _ in range(2)))
+    c.commit(n, n_seqs=rows)
+    return c
+
+
+def calls(sa):
+    """Each operator as a call(stream) whose output takes 4 MiB, or a little."""
+    c = filled_cache(sa, 1024, 5)
+    q = torch.randn(1024, 16, 64, device="cuda")
+    qw, kw = torch.randn(1, 16, 1024, 64, device="cuda"), torch.randn(1, 2, 1024, 64, device="cuda")
+    x, s = torch.randn(2, 4, 1000, device="cuda"), torch.zeros(2, 4, device="cuda")
+    return c, [(q.numel() * 4, lambda st: c.decode_window(0, q, 0.1, 3, 1, stream=st)),
+               (q.numel() * 4, lambda st: c.decode_shared(0, q, 0.1, stream=st)),
+               (q.numel() * 4, lambda st: sa.prefill_window(qw, kw, kw, 0.1, 100, 2, stream=st)),
+               (2 * 8 * 4, lambda st: sa.beam_select(x, s, 8, stream=st))]
+
+
+@pytest.mark.parametrize("raw", [False, True])
+def test_outputs_belong_to_the_calls_stream(sa, raw):
+    c, todo = calls(sa)
+    side = torch.cuda.Stream()
+    for nbytes, call in todo:
+        want = call(None)
+        torch.cuda.synchronize()
+        # memory that the current stream has just given back, perhaps with work
+        # still reading it, is not another stream's to write
+        old = [torch.empty(nbytes, dtype=torch.uint8, device="cuda") for _ in range(8)]
+        freed = {t.data_ptr() for t in old}
+        del old
+        got = call(side.cuda_stream if raw else side)
+        side.synchronize()
+        for g, w in zip(got if isinstance(got, tuple) else [got], want if isinstance(want, tuple) else [want]):
+            assert g.data_ptr() not in freed
+            assert torch.equal(g, w)
+    c.close()
+
+
+def test_other_devices(sa, monkeypatch):
+    c, todo = calls(sa)
+    q = torch.randn(1, 16, 64)
+    for bad in (lambda: c.decode_window(0, q, 0.1, 3), lambda: c.decode_shared(0, q, 0.1),
+                lambda: c.decode_shared(0, q.cuda(), 0.1, ws=torch.empty(1 << 20, dtype=torch.uint8)),
+                lambda: sa.prefill_window(q[None], q[None], q[None], 0.1, 5),
+                lambda: sa.prefill_window(q[None].cuda(), q[None].cuda(), q[None], 0.1, 5),
+                lambda: sa.beam_select(torch.zeros(1, 1, 9), torch.zeros(1, 1), 2),
+                lambda: sa.beam_select(torch.zeros(1, 1, 9).cuda(), torch.zeros(1, 1), 2)):
+        with pytest.raises(ValueError):
+            bad()
+    # tensors on device 0 while another one is current
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    for _, call in todo:
+        with pytest.raises(ValueError):
+            call(None)
+    monkeypatch.undo()
+    c.close()
+
+
+def test_sizes_beyond_a_c_int(sa):
+    """A window without end, as Python writes it."""
+    c = filled_cache(sa, 3, 200)
+    q = torch.randn(3, 4, 64, device="cuda")
+    full = c.decode_window(0, q, 0.1, 201)
+    for window, sink in ((2**32 + 1, 0), (10**18, 2**40), (1, 2**33 + 1)):
+        assert torch.equal(c.decode_window(0, q, 0.1, window, sink), full)
+    with pytest.raises(RuntimeError):
+        c.decode_window(0, q, 0.1, 0)
+    qw, kw = torch.randn(1, 4, 300, 64, device="cuda"), torch.randn(1, 2, 300, 64, device="cuda")
+    full = sa.prefill_window(qw, kw, kw, 0.1, 300)
+    for window, sink in ((2**32 + 1, 0), (2**31, 2**32), (1, 2**33 + 1)):
+        assert torch.equal(sa.prefill_window(qw, kw, kw, 0.1, window, sink), full)
+    c.close()
+
+
+def test_scores_in_place(sa):
+    """A selection of as many as there are beams, into the scores themselves."""
+    x = torch.randn(5, 6, 4001, device="cuda")
+    s = -torch.rand(5, 6, device="cuda")
+    want = sa.beam_select(x, s, 6)
+    out = (s, *(torch.empty(5, 6, dtype=torch.int32, device="cuda") for _ in range(2)))
+    got = sa.beam_select(x, s, 6, out=out)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("interleave", ["0", "1"])
+def test_steps_into_shared_pages_are_refused_whole(sa, monkeypatch, interleave):
+    """Rows whose next token would fall into a shared page: no other row of the
+    step gets a token either, in a one-layer model whose halves overlap."""
+    monkeypatch.setenv("SA_DECODE_INTERLEAVE", interleave)
+    model = sa.Qwen3(4, 200, num_layers=1, hidden=256, intermediate=512, vocab=1024, n_q_heads=4, n_kv_heads=2,
+                     head_dim=64, rms_eps=1e-6, rope_theta=1e6)
+    model.init_random(3, 0.1)
+    cache = sa.KVCache(1, 2, 64, 4, 3, 12, sa.SA_DTYPE_F32)
+    for r in range(4):
+        cache.reserve(r, 100)
+    tokens = torch.zeros(4, 64, dtype=torch.int32, device="cuda")
+    model.prefill(cache, tokens)
+    cache.fork(3, 2, 64)
+    cache.reserve(3, 100)
+    cache.set_len(3, 60)
+    one = torch.zeros(4, dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="shares"):
+        model.decode_step(cache, one)
+    with pytest.raises(RuntimeError, match="shares"):
+        model.beam_step(cache, one.view(1, 4), torch.zeros(1, 4, device="cuda"), 4)
+    assert [cache.length(r) for r in range(4)] == [64, 64, 64, 60]
+    for r in range(4):
+        cache.set_len(r, 0)
+    with pytest.raises(RuntimeError, match="shares"):
+        model.prefill(cache, tokens)
+    assert [cache.length(r) for r in range(4)] == [0] * 4
+    cache.fork(3, 2, 0)             # pages of its own again
+    cache.reserve(3, 100)
+    model.prefill(cache, tokens)
+    model.decode_step(cache, one)
+    torch.cuda.synchronize()
+    assert [cache.length(r) for r in range(4)] == [65] * 4
+    cache.close()
+    model.close()
