@@ -140,7 +140,9 @@ sa_status sa_qwen3_decode_step(sa_qwen3* model, sa_kvcache* cache, const int32_t
  * (sa_paged_decode_shared), else row by row.  The search goes on with the beams
  * that the caller picks: sa_kvcache_reorder with their rows as parents, their
  * tokens and scores as the next step's.  The caller must have reserved pages
- * of every row's own for the new token.  Asynchronous on stream; the first call
+ * of every row's own for the new token (SA_EFULL, or SA_EINVAL where it is a
+ * shared one; nothing is enqueued then).  Asynchronous on stream; a graph that
+ * holds a step repeats it for the lengths at the call.  The first call
  * with a given cache geometry and selection allocates workspaces. */
 sa_status sa_qwen3_beam_step(sa_qwen3* model, sa_kvcache* cache, const int32_t* tokens, int n_groups, int n_beams,
                              const float* scores, int n_select, float* out_scores, int32_t* out_tokens,
