@@ -71,12 +71,12 @@ __global__ void add_lens_range_kernel(int32_t* lens, int n, int val) {
     if (i < n) lens[i] += val;
 }
 
-// Publish entries [0, n) of seq's host table row (the rest of the device row
-// already holds -1 or is overwritten here).
-sa_status write_table_row(sa_kvcache* c, int seq, int n, hipStream_t st) {
+// Publish entries [first, n) of seq's host table row (the others are on the
+// device already).
+sa_status write_table_row(sa_kvcache* c, int seq, int first, int n, hipStream_t st) {
     const int mp = c->desc.max_pages_per_seq;
     const int32_t* src = c->pt.row(seq);
-    for (int j0 = 0; j0 < n; j0 += 64) {
+    for (int j0 = first; j0 < n; j0 += 64) {
         TableRow row;
         const int m = std::min(64, n - j0);
         for (int j = 0; j < m; ++j) row.v[j] = src[j0 + j];
@@ -114,7 +114,8 @@ sa_status on_cache_device(const sa_kvcache* c) {
 // ---------------------------------------------------------------------------
 // Publishing a fork or a reorder: table entries, lengths and page copies of
 // several rows in one launch.  Rows that share their prompt differ in a few
-// entries behind it, so only entries that change are sent.
+// entries behind it, so only entries that change are sent; a fork's shared
+// entries are copied on the device.
 // ---------------------------------------------------------------------------
 constexpr int kEdits = 160, kCopies = 64;
 struct TableEdit {
@@ -127,6 +128,7 @@ struct RowsArgs {
     size_t layer_bytes;
     int max_pages, n_kv, head_bytes, row_bytes;   // head_bytes: 64 rows of one head of a page
     int n_edits, n_lens, n_copies;
+    int like_dst, like_src, like_n;               // a fork: row dst's first n entries are row src's
     TableEdit edit[kEdits];
     int32_t len_row[kRowsPerLaunch], len[kRowsPerLaunch];
     PageCopy copy[kCopies];
@@ -138,6 +140,8 @@ static_assert(sizeof(RowsArgs) <= 4096, "kernel arguments");
 // the latency of a round trip for a few pages.
 __global__ void __launch_bounds__(256) update_rows_kernel(RowsArgs a) {
     if (blockIdx.x == 0 && blockIdx.y == 0) {
+        for (int i = threadIdx.x; i < a.like_n; i += 256)
+            a.table[(size_t)a.like_dst * a.max_pages + i] = a.table[(size_t)a.like_src * a.max_pages + i];
         for (int i = threadIdx.x; i < a.n_edits; i += 256)
             a.table[(size_t)a.edit[i].row * a.max_pages + a.edit[i].col] = a.edit[i].page;
         if ((int)threadIdx.x < a.n_lens) a.lens[a.len_row[threadIdx.x]] = a.len[threadIdx.x];
@@ -153,24 +157,28 @@ __global__ void __launch_bounds__(256) update_rows_kernel(RowsArgs a) {
 }
 
 // The device side of what fork and reorder decided for rows[0, n): `before`
-// holds each row's table entries (before_n of them) as they were.
+// holds each row's table entries as they were.  like: the row whose first
+// `alike` entries the one row of a fork has, which the device copies itself.
 sa_status publish_rows(sa_kvcache* c, const std::vector<int32_t>& rows,
                        const std::vector<std::vector<int32_t>>& before, const std::vector<PageCopy>& copies,
-                       hipStream_t st) {
+                       hipStream_t st, int like = 0, int alike = 0) {
     std::vector<TableEdit> edits;
     for (size_t i = 0; i < rows.size(); ++i) {
         const int32_t* now = c->pt.row(rows[i]);
         const int old_n = (int)before[i].size(), n = std::max(old_n, c->pt.npages(rows[i]));
-        for (int j = 0; j < n; ++j)
+        for (int j = alike; j < n; ++j)
             if (now[j] != (j < old_n ? before[i][j] : -1)) edits.push_back(TableEdit{rows[i], j, now[j]});
     }
-    size_t e = 0, l = 0, k = 0;
+    size_t e = 0, l = 0, k = 0;   // a changed row has a length to publish: one launch at least
     while (e < edits.size() || l < rows.size() || k < copies.size()) {
         RowsArgs a{};
         a.table = c->d_table; a.lens = c->d_lens; a.pool = c->pool; a.layer_bytes = c->layer_bytes;
         a.max_pages = c->desc.max_pages_per_seq; a.n_kv = c->desc.num_kv_heads;
         a.row_bytes = (int)(c->desc.head_dim * c->elem_bytes);
         a.head_bytes = SA_PAGE_TOKENS * a.row_bytes;
+        if (l == 0 && alike > 0) {
+            a.like_dst = rows[0]; a.like_src = like; a.like_n = alike;
+        }
         for (; a.n_edits < kEdits && e < edits.size(); ++e) a.edit[a.n_edits++] = edits[e];
         for (; a.n_lens < kRowsPerLaunch && l < rows.size(); ++l) {
             a.len_row[a.n_lens] = rows[l];
@@ -543,7 +551,7 @@ extern "C" sa_status sa_kvcache_reserve(sa_kvcache* c, int seq, int n_tokens, sa
     const Verdict v = c->pt.reserve(seq, n_tokens);
     if (!v.ok()) return refused(v);
     if (c->pt.npages(seq) == before) return SA_OK;
-    return write_table_row(c, seq, c->pt.npages(seq), as_stream(stream));
+    return write_table_row(c, seq, before, c->pt.npages(seq), as_stream(stream));   // pages are only added
 }
 
 extern "C" sa_status sa_kvcache_set_pages(sa_kvcache* c, int seq, const int32_t* pages, int n_pages,
@@ -556,7 +564,7 @@ extern "C" sa_status sa_kvcache_set_pages(sa_kvcache* c, int seq, const int32_t*
     if (!v.ok()) return refused(v);
     hipStream_t st = as_stream(stream);
     // Entries past the new list become -1 on the device too.
-    SA_TRY(write_table_row(c, seq, std::max(before, n_pages), st));
+    SA_TRY(write_table_row(c, seq, 0, std::max(before, n_pages), st));
     if (len_cut) {
         const int32_t row = seq;
         SA_TRY(publish_lens(c, &row, 1, c->pt.len(seq), 0, st));
@@ -610,7 +618,7 @@ extern "C" sa_status sa_kvcache_fork(sa_kvcache* c, int dst, int src, int n_toke
         std::vector<PageCopy> copies;
         const Verdict v = c->pt.fork(dst, src, n_tokens, &copies);
         if (!v.ok()) return refused(v);
-        return publish_rows(c, rows, before, copies, as_stream(stream));
+        return publish_rows(c, rows, before, copies, as_stream(stream), src, n_tokens / SA_PAGE_TOKENS);
     });
 }
 

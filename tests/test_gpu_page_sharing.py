@@ -167,3 +167,24 @@ def test_on_a_stream_of_the_callers(sa):
         for r, n in enumerate([190, 190, 190, 200]):
             assert torch.equal(got[layer][r], want[layer][:, :, :n]), (layer, r)
     cache.close()
+
+
+@pytest.mark.parametrize("n,old", [(300 * 64, 0), (300 * 64 + 5, 400 * 64), (64, 350 * 64), (0, 200 * 64)])
+def test_fork_of_many_pages(sa, n, old):
+    """Tables of more entries than a launch's arguments hold; room is added to a
+    forked row in two steps."""
+    cache = sa.KVCache(1, 1, 8, 3, 420, 1260, sa.SA_DTYPE_BF16)
+    cache.reserve(2, 310 * 64)
+    cache.set_len(2, 310 * 64 - 9)
+    cache.reserve(0, old)
+    cache.fork(0, 2, n)
+    shared, own = n // 64, (n + 63) // 64
+    for more in (0, 1, 100):
+        cache.reserve(0, (own + more) * 64)
+        table, lens = device_table(sa, cache)
+        assert lens.tolist() == [n, 0, 310 * 64 - 9]
+        assert (table[0, :shared] == table[2, :shared]).all() and (table[0, own + more:] == -1).all()
+        fresh = table[0, shared:own + more]
+        assert (fresh >= 0).all() and len(set(fresh) | set(table[2, :310])) == len(fresh) + 310
+        assert (table[1] == -1).all() and (table[2, 310:] == -1).all()
+    cache.close()
