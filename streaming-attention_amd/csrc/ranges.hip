@@ -118,13 +118,16 @@ struct Geo {
     // Chunk c of row r sits at chunk c ^ swz(r) of the row: the 16 rows 8a + 4kb
     // + b (a, b < 4) of a K fragment read, and the rows of a V^T read (bf16: 8g
     // + 4u + b with b < 4 and g of one half wave; fp32: 8g + e, g < 4), fall on
-    // different banks.
+    // different banks; for fp32 products (F32) 16 neighbouring rows, and 4g + e.
+    template <bool F32>
     static __device__ __forceinline__ int swz(int r) {
-        if constexpr (!BF16) return (((r >> 3) & 3) << 2) | (r & 3);
+        if constexpr (F32) return r & 15;
+        else if constexpr (!BF16) return (((r >> 3) & 3) << 2) | (r & 3);
         else if constexpr (CPR == 16) return ((r & 3) << 2) | (((r >> 3) & 1) << 1) | ((r >> 4) & 1);
         else return (((r >> 1) & 1) << 2) | (((r >> 3) & 1) << 1) | ((r >> 4) & 1);
     }
-    static __device__ __forceinline__ int off(int r, int c) { return r * ROWB + ((c ^ swz(r)) << 4); }
+    template <bool F32>
+    static __device__ __forceinline__ int off(int r, int c) { return r * ROWB + ((c ^ swz<F32>(r)) << 4); }
 };
 
 __device__ __forceinline__ f32x4_t lds_f4(const lds_u8_t* p) {
@@ -151,11 +154,16 @@ template <int D, bool BF16, int RT>
 struct WaveState {
     using G = Geo<D, BF16>;
     static constexpr int PAIRS = BF16 ? 3 : 6;
+    // fp32 values whose split into terms would serve one tile of query rows only:
+    // v_mfma_f32_16x16x4_f32 instead.
+    static constexpr bool F32 = !BF16 && RT == 1;
+    static __device__ __forceinline__ int off(int r, int c) { return G::template off<F32>(r, c); }
     // Terms of the cached and of the other operand of a product, largest first.
     static constexpr int pair_a(int pr) { return BF16 ? 0 : (pr == 2 || pr == 4 ? 1 : pr == 5 ? 2 : 0); }
     static constexpr int pair_b(int pr) { return BF16 ? pr : (pr == 1 || pr == 4 ? 1 : pr == 3 ? 2 : 0); }
 
     bf16x8_t q[RT][G::KS][kTerms];
+    f32x4_t qf[D / 16], pf[2];   // F32: q from D / 4 g on, the weights
     f32x4_t acc[RT][G::DB];
     float m[RT];     // running max (log2 domain) at the last raise
     float b[RT];     // -m once finite: the score chain's start
@@ -178,6 +186,11 @@ struct WaveState {
         }
     }
     __device__ __forceinline__ void load_q(int rt, const float* row, float sl2) {
+        if constexpr (F32) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) qf[i] = *reinterpret_cast<const f32x4_t*>(row + D / 4 * g + 4 * i) * sl2;
+            return;
+        }
         f32x4_t x[G::KS][2];
 #pragma unroll
         for (int ks = 0; ks < G::KS; ++ks)
@@ -189,22 +202,36 @@ struct WaveState {
 
     // Scores of the tile whose K sits at kb, masked to its tokens [lo, hi), and
     // the weights p = 2^(s - m) as three bf16 terms.  Element 4 h + e of a lane
-    // is key 8 g + 4 h + e.
+    // is key 8 g + 4 h + e (F32: 16 h + 4 g + e, the operand of V^T P^T as it is;
+    // the products take d in the order that lets a lane read 16 bytes of K).
     __device__ __forceinline__ void scores(const lds_u8_t* kb, const TileSpan& sp) {
         f32x4_t s[RT][2];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) s[rt][0] = s[rt][1] = f32x4_t{b[rt], b[rt], b[rt], b[rt]};
+        if constexpr (F32) {
 #pragma unroll
-        for (int ks = 0; ks < G::KS; ++ks) {
+            for (int i = 0; i < D / 16; ++i) {
+                f32x4_t kf[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) kf[h] = lds_f4(kb + off(16 * h + r16, D / 16 * g + i));
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        s[0][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[h][e], qf[i][e], s[0][h], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int ks = 0; ks < (F32 ? 0 : G::KS); ++ks) {
             bf16x8_t kf[2][G::NT];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int r = 8 * (r16 >> 2) + 4 * h + (r16 & 3);
                 if constexpr (BF16) {
                     kf[h][0] = *reinterpret_cast<const __attribute__((address_space(3))) bf16x8_t*>(
-                        kb + G::off(r, 4 * ks + g));
+                        kb + off(r, 4 * ks + g));
                 } else {
-                    split_terms(lds_f4(kb + G::off(r, 8 * ks + 2 * g)), lds_f4(kb + G::off(r, 8 * ks + 2 * g + 1)),
+                    split_terms(lds_f4(kb + off(r, 8 * ks + 2 * g)), lds_f4(kb + off(r, 8 * ks + 2 * g + 1)),
                                 kf[h]);
                 }
             }
@@ -223,7 +250,7 @@ struct WaveState {
             if (ragged) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const int t = sp.t0 + 8 * g + j;
+                    const int t = sp.t0 + (F32 ? 16 * (j >> 2) + 4 * g + (j & 3) : 8 * g + j);
                     if (t < sp.lo || t >= sp.hi) s[rt][j >> 2][j & 3] = -INFINITY;
                 }
             }
@@ -250,7 +277,9 @@ struct WaveState {
                 cap[rt] = m_new == -INFINITY ? -1.f : kRaiseAt;
             }
             l[rt] += sum;
-            split_terms(f32x4_t{w[0], w[1], w[2], w[3]}, f32x4_t{w[4], w[5], w[6], w[7]}, p[rt]);
+            pf[0] = f32x4_t{w[0], w[1], w[2], w[3]};
+            pf[1] = f32x4_t{w[4], w[5], w[6], w[7]};
+            if constexpr (!F32) split_terms(pf[0], pf[1], p[rt]);
         }
     }
 
@@ -260,6 +289,22 @@ struct WaveState {
         constexpr int ND = 2;
 #pragma unroll
         for (int d0 = 0; d0 < G::DB; d0 += ND) {
+            if constexpr (F32) {
+                float x[ND][8];
+#pragma unroll
+                for (int d = 0; d < ND; ++d)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        x[d][j] = *reinterpret_cast<const __attribute__((address_space(3))) float*>(
+                            vb + off(16 * (j >> 2) + 4 * g + (j & 3), 4 * (d0 + d) + (r16 >> 2)) + (r16 & 3) * 4);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                    for (int d = 0; d < ND; ++d)
+                        acc[0][d0 + d] =
+                            __builtin_amdgcn_mfma_f32_16x16x4f32(x[d][j], pf[j >> 2][j & 3], acc[0][d0 + d], 0, 0, 0);
+                continue;
+            }
             bf16x8_t vf[ND][G::NT];
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
@@ -268,16 +313,16 @@ struct WaveState {
                     // 16 db + 4 (s % 4) ..; lane r16 receives V[8 g + 4 u + e][16 db + r16].
                     const int c = 2 * (d0 + d) + ((r16 & 3) >> 1), h8 = (r16 & 1) * 8;
                     const int r = 8 * g + (r16 >> 2);
-                    const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vb + G::off(r, c) + h8));
+                    const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vb + off(r, c) + h8));
                     const s16x4_t y =
-                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vb + G::off(r + 4, c) + h8));
+                        __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vb + off(r + 4, c) + h8));
                     vf[d][0] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
                 } else {
                     f32x4_t x[2];
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         x[j >> 2][j & 3] = *reinterpret_cast<const __attribute__((address_space(3))) float*>(
-                            vb + G::off(8 * g + j, 4 * (d0 + d) + (r16 >> 2)) + (r16 & 3) * 4);
+                            vb + off(8 * g + j, 4 * (d0 + d) + (r16 >> 2)) + (r16 & 3) * 4);
                     split_terms(x[0], x[1], vf[d]);
                 }
             }
@@ -356,7 +401,7 @@ __device__ __forceinline__ void attend(const RangeArgs& a, const Item& it, lds_u
             const bool is_v = first + i >= G::NL;
             const int r = (first + i - (is_v ? G::NL : 0)) * G::RPL + lane / G::CPR;
             const int tok = min(max(sp.t0 + r, sp.lo), sp.hi - 1) & (SA_PAGE_TOKENS - 1);
-            const int col = ((lane % G::CPR) ^ G::swz(r)) * 16;
+            const int col = ((lane % G::CPR) ^ G::template swz<decltype(w)::F32>(r)) * 16;
             const char* pool = static_cast<const char*>(is_v ? a.v : a.k);
             dma16_nt(pool + at + (size_t)tok * G::ROWB + col, dst + (first + i) * 1024);
         }
