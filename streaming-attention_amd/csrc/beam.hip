@@ -28,7 +28,7 @@ constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / kWave;
 constexpr int kMaxBeams = 64, kMaxSelect = 64;
 constexpr int kMaxGroups = 1 << 20;                      // a grid has fewer than 2^32 threads
-constexpr int kSlots = 8;                                // segments of a thread of the second launch
+constexpr int kFewSlots = 4, kMaxSlots = 8;              // segments of a thread of the second launch
 constexpr int kBeamsPerWave = kMaxBeams / kSelWaves;
 constexpr int kBlock = 8 * kWave;                        // elements of a wave's step
 constexpr int kWays = 4;                                 // thresholds tried at once
@@ -147,7 +147,7 @@ __device__ __forceinline__ float unordered(uint32_t u) {
 
 // A beam's segment in one integer of the segments' order.
 constexpr int kSegBits = 16;
-static_assert(kSelWaves * kWave * kSlots <= 1 << kSegBits, "segments of a beam");
+static_assert(kSelWaves * kWave * kMaxSlots <= 1 << kSegBits, "segments of a beam");
 __device__ __forceinline__ int segment_id(int beam, int seg) { return beam << kSegBits | seg; }
 __device__ __forceinline__ int beam_of(int id) { return id >> kSegBits; }
 __device__ __forceinline__ int seg_of(int id) { return id & ((1 << kSegBits) - 1); }
@@ -185,6 +185,7 @@ __device__ void first_of_all(double& v, int& idx, double* sv, int* si) {
         }
 }
 
+template <int SLOTS>
 __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
     __shared__ double base[kMaxBeams];              // score - log sum exp; NaN: the beam offers nothing
     __shared__ float wave_max[kSelWaves][kBeamsPerWave];
@@ -211,15 +212,15 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
     // ---- this thread's segments: slot j is part j % per_beam of its wave's beam
     // j / per_beam, whose segments are dealt out to the beam's waves first ----
     const float score = tid < a.n_beams ? a.scores[(long long)group * a.n_beams + tid] : 0.f;
-    float2 sg[kSlots];
-    int id[kSlots];      // segment of the beam, -1: none
-    int of[kSlots];      // the beam's place in the wave (uniform)
+    float2 sg[SLOTS];
+    int id[SLOTS];      // segment of the beam, -1: none
+    int of[SLOTS];      // the beam's place in the wave (uniform)
     const int n_slots = a.per_beam * a.beams_per_wave;
     const int beam0 = a.beams_per_wave > 1 ? wave * a.beams_per_wave : wave / a.waves_per_beam;
     {
         int bi = 0, k = 0;
 #pragma unroll
-        for (int j = 0; j < kSlots; ++j) {
+        for (int j = 0; j < SLOTS; ++j) {
             const int s = (k * kWave + lane) * a.waves_per_beam + wave % a.waves_per_beam;
             of[j] = bi;
             id[j] = j < n_slots && beam0 + bi < a.n_beams && s < a.n_seg ? s : -1;
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
     for (int bi = 0; bi < a.beams_per_wave; ++bi) {
         float m = kNone;
 #pragma unroll
-        for (int j = 0; j < kSlots; ++j) m = of[j] == bi ? fmaxf(m, sg[j].x) : m;
+        for (int j = 0; j < SLOTS; ++j) m = of[j] == bi ? fmaxf(m, sg[j].x) : m;
         m = group_reduce<OpMax, 1, kWave>(m);
         if (lane == 0) wave_max[wave][bi] = m;
     }
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
         for (int w = w0; w < min(w0 + a.waves_per_beam, kSelWaves); ++w) m = fmaxf(m, wave_max[w][bi]);
         double l = 0.0;
 #pragma unroll
-        for (int j = 0; j < kSlots; ++j)
+        for (int j = 0; j < SLOTS; ++j)
             if (j < n_slots && of[j] == bi) l += id[j] >= 0 ? (double)(sg[j].y * exp_diff(sg[j].x - m)) : 0.0;
         l = wave_sum_f64(l);
         if (lane == 0) {
@@ -270,10 +271,10 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
     // of the threads' largest segment maxima reach (-inf: fewer threads have one).
     // kWays thresholds at once, then equal parts of the range that is left, by
     // the values' bit patterns. ----
-    float key[kSlots];
+    float key[SLOTS];
     float best = kNone;
 #pragma unroll
-    for (int j = 0; j < kSlots; ++j) {
+    for (int j = 0; j < SLOTS; ++j) {
         key[j] = kNone;
         if (j < n_slots && beam0 + of[j] < a.n_beams) {
             const float k = (float)(base[beam0 + of[j]] + (double)sg[j].x);
@@ -331,7 +332,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
 
     // ---- the segments and elements that reach it ----
 #pragma unroll
-    for (int j = 0; j < kSlots; ++j) {
+    for (int j = 0; j < SLOTS; ++j) {
         if (key[j] > kNone && key[j] >= t) {
             const int at = atomicAdd(&n_segs, 1);
             if (at < kSegList) seg_list[at] = segment_id(beam0 + of[j], id[j]);
@@ -408,7 +409,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
         double v = 0.0;
         int idx = -1;
 #pragma unroll
-        for (int j = 0; j < kSlots; ++j) {
+        for (int j = 0; j < SLOTS; ++j) {
             if (!(key[j] > kNone)) continue;
             const int s = segment_id(beam0 + of[j], id[j]);
             const double c = base[beam0 + of[j]] + (double)sg[j].x;
@@ -448,18 +449,23 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
 }
 
 struct BeamShape {
-    int vpt, steps, n_seg;
+    int slots, vpt, steps, n_seg;
     int waves_per_beam, beams_per_wave, per_beam;
 };
-// The shortest segments that the second launch's threads hold.
+// The shortest segments that the second launch's threads hold: in four slots
+// each where segments of 256 elements do, since its time is mostly that of
+// fetching its instructions (4 beams of 151,936 tokens 12.0 us against 12.5 in
+// eight, 3 x 5 of 32,003 12.7 against 13.3), else in eight (8 x 8 of 151,936
+// 21.7 against 24.2 us).
 BeamShape beam_shape(int n_beams, int vocab) {
-    BeamShape s{1, 1, 0, std::max(1, kSelWaves / n_beams), (n_beams + kSelWaves - 1) / kSelWaves, 0};
+    BeamShape s{kFewSlots, 1, 1, 0, std::max(1, kSelWaves / n_beams), (n_beams + kSelWaves - 1) / kSelWaves, 0};
     for (;;) {
         const long long len = (long long)kWave * s.vpt * s.steps;
         s.n_seg = (int)((vocab + len - 1) / len);
         s.per_beam = (s.n_seg + kWave * s.waves_per_beam - 1) / (kWave * s.waves_per_beam);
-        if (s.per_beam * s.beams_per_wave <= kSlots) return s;
-        if (s.vpt < 8) s.vpt *= 2;
+        if (s.per_beam * s.beams_per_wave <= s.slots) return s;
+        if (s.slots == kFewSlots && s.vpt == 4) s.slots = kMaxSlots, s.vpt = 1;
+        else if (s.vpt < 8) s.vpt *= 2;
         else s.steps *= 2;
     }
 }
@@ -518,7 +524,8 @@ extern "C" sa_status sa_beam_select(const float* logits, int64_t row_stride, con
 #undef SA_BEAM_SCAN
     }
     SA_CHECK_LAUNCH();
-    hipLaunchKernelGGL(beam_pick_kernel, dim3(n_groups), dim3(kSelThreads), 0, st, a);
+    if (sh.slots == kFewSlots) hipLaunchKernelGGL(beam_pick_kernel<kFewSlots>, dim3(n_groups), dim3(kSelThreads), 0, st, a);
+    else hipLaunchKernelGGL(beam_pick_kernel<kMaxSlots>, dim3(n_groups), dim3(kSelThreads), 0, st, a);
     SA_CHECK_LAUNCH();
     return SA_OK;
 }
