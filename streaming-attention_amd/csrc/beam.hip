@@ -16,7 +16,10 @@
 // Where equal maxima make the lists overflow, the selection goes in n_select
 // rounds over (c, index) instead.
 //
-// Bound: HBM, the logits read once.
+// Bound: HBM for the first launch (64 rows of 151,936: 38.9 MB in 8.3 us), latency
+// for the second: a lone workgroup per search fetches every instruction that it
+// runs once, 9 us for 4 beams and 11.6 for 8 x 8.  Both, graph-replayed: 4 beams
+// of 151,936 tokens 12.1 us, 8 searches of 8 21.6, 3 of 5 beams of 32,003 12.6.
 #include "sa_internal.h"
 
 #include <algorithm>

@@ -136,8 +136,9 @@ struct RowsArgs {
 static_assert(sizeof(RowsArgs) <= 4096, "kernel arguments");
 
 // Block (x, y) copies head slice x (layer, K or V, head) of page pair y.  No
-// page is both read and written in a launch.  Bound: HBM; the whole launch is
-// the latency of a round trip for a few pages.
+// page is both read and written in a launch.  Bound: for a few pages the latency
+// of a round trip, hidden behind the host's part (28 layers, 8 heads of 128, bf16:
+// a reorder of 4 rows 9 us a call, of 64 rows behind 2,000 tokens 25, a fork 6.7).
 __global__ void __launch_bounds__(256) update_rows_kernel(RowsArgs a) {
     if (blockIdx.x == 0 && blockIdx.y == 0) {
         for (int i = threadIdx.x; i < a.like_n; i += 256)

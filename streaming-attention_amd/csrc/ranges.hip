@@ -14,7 +14,9 @@
 // weights enter the products as the exact sum of three bf16 terms; cached bf16
 // values are one term, cached fp32 ones three, split where they are used.  Of
 // the products of three by three terms the six largest are taken: what is left
-// out is below 2^-24 of the product, the rounding of an fp32 one.
+// out is below 2^-24 of the product, the rounding of an fp32 one.  fp32 values
+// that only one tile of 16 query rows uses are not split: fp32 MFMA takes them as
+// they are (4 searches of 4 beams behind 1500 - 2100 tokens 19.4 us against 19.8).
 //
 // Layout: v_mfma_f32_16x16x32_bf16 with S^T = K Q^T (rows: keys, columns: query
 // rows), so that a lane's eight scores of a 32-key tile are the operand that
@@ -24,6 +26,13 @@
 //     another; the next tile's K load into LDS while P V is computed, the next
 //     tile's V while the scores are.
 //   RG > 1: the waves of a key group share its tiles, a ring of RG of them.
+//
+// Bound, 16 / 8 heads of 128: HBM for many rows (64 rows, window 4096 and 4 sinks,
+// bf16: 992 MB in 157 us, 6.3 TB/s); the products and the softmax between for many
+// rows behind one prefix (64 behind 32768 tokens, bf16: 73 us, MFMA 41 % and VALU
+// 45 % busy; loads alone 55, computing alone 66, of both 15 for launches, queries
+// and partials); the latency of the tiles for few rows (4 x 4 beams, fp32: 19.4 us,
+// 2.65 per tile of a wave; 4 rows behind 512 tokens, bf16: 9.0).
 #include "ranges.h"
 
 #include <algorithm>
@@ -652,7 +661,7 @@ int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 // which saves the second launch: up to four tiles per wave (7 rows of 403 tokens,
 // bf16, d = 64: 6.7 against 7.8 us in four chunks; 16 query rows of 512 tokens,
 // d = 128: a second, third and fourth tile per wave cost 0.8, 1.7 and 2.7 us, the
-// second launch 3.5), in fp32 two (a tile per wave costs 3 us).
+// second launch 3.5), in fp32 two (a tile per wave costs 2.65 us).
 constexpr int kLongChunk = 32;
 template <class F>
 int pick_tiles(long long round, long long work, const F& workgroups) {

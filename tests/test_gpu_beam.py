@@ -165,3 +165,14 @@ def test_graph_replays(sa):
         want = reference(x, s, 8)
         assert torch.equal(out[1].cpu().long(), want[1]) and torch.equal(out[2].cpu().long(), want[2])
     del graph
+
+
+@pytest.mark.parametrize("B,V,n", [(8, 151936, 16), (16, 151936, 64), (33, 70001, 64)])
+def test_equal_values_in_eight_segments_a_thread(sa, B, V, n):
+    z = torch.zeros(1, B, V, device="cuda")
+    s = torch.zeros(1, B, device="cuda")
+    check(sa, z, s, n)
+    gen = torch.Generator(device="cuda").manual_seed(V + B)
+    check(sa, torch.randint(0, 3, (1, B, V), device="cuda", generator=gen).float(), s, n)
+    z[:, -1, V - 1] = 1.0
+    check(sa, z, s, n)
