@@ -35,7 +35,9 @@ constexpr int kFewSlots = 4, kMaxSlots = 8;              // segments of a thread
 constexpr int kBeamsPerWave = kMaxBeams / kSelWaves;
 constexpr int kBlock = 8 * kWave;                        // elements of a wave's step
 constexpr int kWays = 4;                                 // thresholds tried at once
+constexpr int kTopLanes = kSelThreads / kWave;           // lanes of a first guess
 static_assert(kWays * kSelWaves == kWave && kSelWaves == 16, "a lane per threshold and wave");
+static_assert(kMaxSelect <= kWave, "a first guess for every place");
 constexpr int kSegList = 256, kCandList = 1024, kGather = 8;
 static_assert(kMaxSelect <= kSegList, "the rounds fill the segment list");
 constexpr float kNone = -INFINITY;
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
     __shared__ float wave_max[kSelWaves][kBeamsPerWave];
     __shared__ double wave_sum[kSelWaves][kBeamsPerWave];
     __shared__ float beam_max[kMaxBeams];
-    __shared__ float top[kSelWaves];
+    __shared__ float tops[kWave], ranked[kWave];    // the largest segment maximum of 16 lanes each
     __shared__ float counts[2][kWays * kSelWaves];
     __shared__ int seg_list[kSegList];
     __shared__ Candidate cand[kCandList];
@@ -272,8 +274,9 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
 
     // ---- tau: a value that at least `want`, and rarely more than twice as many,
     // of the threads' largest segment maxima reach (-inf: fewer threads have one).
-    // kWays thresholds at once, then equal parts of the range that is left, by
-    // the values' bit patterns. ----
+    // The first guesses are largest values of 16 lanes each, of which the want-th
+    // largest is seldom reached by many more threads; then kWays thresholds at once,
+    // equal parts of the range that is left, by the values' bit patterns. ----
     float key[SLOTS];
     float best = kNone;
 #pragma unroll
@@ -286,11 +289,21 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
         best = fmaxf(best, key[j]);
     }
     {
-        const float m = group_reduce<OpMax, 1, kWave>(best);
-        if (lane == 0) top[wave] = m;
+        const float m = group_reduce<OpMax, 1, kTopLanes>(best);
+        if (lane % kTopLanes == 0) tops[tid / kTopLanes] = m;
     }
     __syncthreads();
-    const float most = group_reduce<OpMax, 1, kSelWaves>(top[lane % kSelWaves]);
+    const float a_top = tops[lane];
+    // tops in order, largest first: each wave finds the places of its own four.
+#pragma unroll
+    for (int j = 0; j < kWave / kSelWaves; ++j) {
+        const int i = wave * (kWave / kSelWaves) + j;
+        const float v = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(a_top), i));
+        const int place = __popcll(__ballot(a_top > v || (a_top == v && lane < i)));
+        if (lane == 0) ranked[place] = v;
+    }
+    __syncthreads();
+    const float most = ranked[0];
     const uint32_t mine = ordered(best);
     int parity = 0;
     // Threads whose best is at least v[0], .., v[kWays - 1] (increasing).  Lanes 16 i
@@ -311,8 +324,8 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
     float t = kNone;
     if (most > kNone) {
         const uint32_t bottom = ordered(kNone) + 1;
-        uint32_t v[kWays] = {bottom, max(bottom, ordered(most - 16.f)), max(bottom, ordered(most - 8.f)),
-                             max(bottom, ordered(most - 4.f))};
+        uint32_t v[kWays] = {max(bottom, ordered(ranked[want - 1])), max(bottom, ordered(ranked[(want - 1) / 2])),
+                             max(bottom, ordered(ranked[(want - 1) / 4])), ordered(most)};
         uint32_t lo = bottom, hi = ordered(most) + 1;
         int n[kWays];
         reach(v, n);
