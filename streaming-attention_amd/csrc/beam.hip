@@ -159,7 +159,7 @@ __device__ __forceinline__ int seg_of(int id) { return id & ((1 << kSegBits) - 1
 
 struct alignas(16) Candidate {
     double c;
-    int idx;
+    int idx, beam;
 };
 
 // Candidate order: larger value first, of equal ones the lower index.
@@ -195,7 +195,6 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
     __shared__ double base[kMaxBeams];              // score - log sum exp; NaN: the beam offers nothing
     __shared__ float wave_max[kSelWaves][kBeamsPerWave];
     __shared__ double wave_sum[kSelWaves][kBeamsPerWave];
-    __shared__ float beam_max[kMaxBeams];
     __shared__ float tops[kWave], ranked[kWave];    // the largest segment maximum of 16 lanes each
     __shared__ float counts[2][kWays * kSelWaves];
     __shared__ int seg_list[kSegList];
@@ -245,29 +244,28 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
 #pragma unroll
         for (int j = 0; j < SLOTS; ++j) m = of[j] == bi ? fmaxf(m, sg[j].x) : m;
         m = group_reduce<OpMax, 1, kWave>(m);
-        if (lane == 0) wave_max[wave][bi] = m;
-    }
-    __syncthreads();
-    for (int bi = 0; bi < a.beams_per_wave; ++bi) {
-        const int w0 = a.beams_per_wave > 1 ? wave : wave / a.waves_per_beam * a.waves_per_beam;
-        float m = kNone;
-        for (int w = w0; w < min(w0 + a.waves_per_beam, kSelWaves); ++w) m = fmaxf(m, wave_max[w][bi]);
         double l = 0.0;
 #pragma unroll
         for (int j = 0; j < SLOTS; ++j)
-            if (j < n_slots && of[j] == bi) l += id[j] >= 0 ? (double)(sg[j].y * exp_diff(sg[j].x - m)) : 0.0;
+            if (j < n_slots && of[j] == bi) l += sg[j].x == kNone ? sg[j].y : (double)(sg[j].y * exp_diff(sg[j].x - m));
         l = wave_sum_f64(l);
         if (lane == 0) {
+            wave_max[wave][bi] = m;
             wave_sum[wave][bi] = l;
-            if (wave == w0 && beam0 + bi < a.n_beams) beam_max[beam0 + bi] = m;
         }
     }
     __syncthreads();
     if (tid < a.n_beams) {
         const int w0 = first_of(tid), bi = place_of(tid);
+        float m = kNone;
         double l = 0.0;
-        for (int w = w0; w < w0 + a.waves_per_beam; ++w) l += wave_sum[w][bi];
-        const double lse = (double)beam_max[tid] + log(l);
+        for (int w = w0; w < w0 + a.waves_per_beam; ++w) {
+            const float x = wave_max[w][bi], y = fmaxf(m, x);
+            l = (m == kNone ? l : l * (double)exp_diff(m - y)) +
+                (x == kNone ? wave_sum[w][bi] : wave_sum[w][bi] * (double)exp_diff(x - y));
+            m = y;
+        }
+        const double lse = (double)m + log(l);
         base[tid] = isfinite(lse) ? (double)score - lse : (double)NAN;
     }
     __syncthreads();
@@ -392,17 +390,17 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
                 const double c = base[beam[j]] + (double)v[j];
                 if (c > (double)kNone && (float)c >= t) {
                     const int at = atomicAdd(&n_cand, 1);
-                    if (at < kCandList) cand[at] = Candidate{c, idx[j]};
+                    if (at < kCandList) cand[at] = Candidate{c, idx[j], beam[j]};
                 }
             }
         }
     }
     __syncthreads();
     const long long out0 = (long long)group * a.n_select;
-    auto put = [&](int r, double c, int idx) {
+    auto put = [&](int r, double c, int idx, int beam) {
         a.out_scores[out0 + r] = idx < 0 ? kNone : (float)c;
-        a.out_tokens[out0 + r] = idx < 0 ? -1 : idx % a.vocab;
-        a.out_beams[out0 + r] = idx < 0 ? -1 : idx / a.vocab;
+        a.out_tokens[out0 + r] = idx < 0 ? -1 : idx - beam * a.vocab;
+        a.out_beams[out0 + r] = idx < 0 ? -1 : beam;
     };
     if (n_segs <= kSegList && n_cand <= kCandList) {
         const int n = n_cand;
@@ -411,9 +409,9 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
             int r = 0;
 #pragma unroll 8
             for (int j = 0; j < n; ++j) r += ahead(cand[j].c, cand[j].idx, mine.c, mine.idx);
-            if (r < a.n_select) put(r, mine.c, mine.idx);
+            if (r < a.n_select) put(r, mine.c, mine.idx, mine.beam);
         }
-        if (tid >= n && tid < a.n_select) put(tid, 0.0, -1);
+        if (tid >= n && tid < a.n_select) put(tid, 0.0, -1, -1);
         return;
     }
 
@@ -460,7 +458,7 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
         more = idx >= 0;
         last_v = v;
         last_i = idx;
-        if (tid == 0) put(r, v, idx);
+        if (tid == 0) put(r, v, idx, idx / a.vocab);
     }
 }
 

@@ -176,3 +176,17 @@ def test_equal_values_in_eight_segments_a_thread(sa, B, V, n):
     check(sa, torch.randint(0, 3, (1, B, V), device="cuda", generator=gen).float(), s, n)
     z[:, -1, V - 1] = 1.0
     check(sa, z, s, n)
+
+
+@pytest.mark.parametrize("B", [1, 4, 8, 16])
+def test_few_tokens_allowed(sa, B):
+    """A mask that leaves a few tokens of a long vocabulary: most segments, and
+    whole waves of them, hold nothing but -inf, one of them a NaN beside it."""
+    V = 151936
+    x, s = inputs(2, B, V, 60 + B)
+    allowed = torch.tensor([3, 70000, 70001, V - 1], device="cuda")
+    masked = torch.full_like(x, -math.inf)
+    masked[..., allowed] = x[..., allowed]
+    check(sa, masked, s, 8)
+    masked[1, B - 1, 40000] = math.nan
+    check(sa, masked, s, 8)
