@@ -18,8 +18,8 @@
 //
 // Bound: HBM for the first launch (64 rows of 151,936: 38.9 MB in 8.3 us), latency
 // for the second: a lone workgroup per search fetches every instruction that it
-// runs once, 9 us for 4 beams and 11.6 for 8 x 8.  Both, graph-replayed: 4 beams
-// of 151,936 tokens 12.1 us, 8 searches of 8 21.6, 3 of 5 beams of 32,003 12.6.
+// runs once, 7.7 us for 4 beams and 10.8 for 8 x 8.  Both, graph-replayed: 4 beams
+// of 151,936 tokens 10.9 us, 8 searches of 8 21.4, 3 of 5 beams of 32,003 11.8.
 #include "sa_internal.h"
 
 #include <algorithm>
@@ -468,9 +468,9 @@ struct BeamShape {
 };
 // The shortest segments that the second launch's threads hold: in four slots
 // each where segments of 256 elements do, since its time is mostly that of
-// fetching its instructions (4 beams of 151,936 tokens 12.0 us against 12.5 in
-// eight, 3 x 5 of 32,003 12.7 against 13.3), else in eight (8 x 8 of 151,936
-// 21.7 against 24.2 us).
+// fetching its instructions (when written, 4 beams of 151,936 tokens 12.0 us
+// against 12.5 in eight, 3 x 5 of 32,003 12.7 against 13.3), else in eight (8 x 8
+// of 151,936 21.7 against 24.2 us).
 BeamShape beam_shape(int n_beams, int vocab) {
     BeamShape s{kFewSlots, 1, 1, 0, std::max(1, kSelWaves / n_beams), (n_beams + kSelWaves - 1) / kSelWaves, 0};
     for (;;) {
