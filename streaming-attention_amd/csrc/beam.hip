@@ -100,11 +100,12 @@ __global__ void __launch_bounds__(256) beam_scan_kernel(BeamArgs a) {
 #pragma unroll
             for (int j = g; j < g + JOIN; ++j) m = fmaxf(m, fmaxf(fmaxf(v[j][0], v[j][1]), fmaxf(v[j][2], v[j][3])));
             m = group_reduce<OpMax, 1, LANES>(m);
+            const float from = m == kNone ? 0.f : m;   // -inf itself adds 0
             float l = 0.f;
 #pragma unroll
             for (int j = g; j < g + JOIN; ++j)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) l += m == kNone && v[j][e] == kNone ? 0.f : exp_diff(v[j][e] - m);
+                for (int e = 0; e < 4; ++e) l += exp_diff(v[j][e] - from);
             l = group_reduce<OpSum, 1, LANES>(l);
             if constexpr (VPT < 8) {
                 const long long seg = (at + g * 4 * kWave + 4 * lane) / (kWave * VPT);
