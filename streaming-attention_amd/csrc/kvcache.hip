@@ -841,7 +841,7 @@ namespace {
 // What the decodes over ranges share: the checks of their arguments and the
 // view of a layer's pools.
 sa_status check_ranges(const sa_kvcache* c, int layer, const float* q, int n_seq, int n_q_heads, const float* out,
-                       const void* ws) {
+                       const void* ws, size_t ws_bytes, size_t ws_need) {
     if (layer < 0 || layer >= c->desc.num_layers) return fail(SA_ERANGE, "Layer index out of range");
     if (!q || !out) return fail(SA_EINVAL, "null pointer");
     if (n_seq <= 0) return fail(SA_EINVAL, "n_seq must be positive");
@@ -851,6 +851,9 @@ sa_status check_ranges(const sa_kvcache* c, int layer, const float* q, int n_seq
     if (!ranges_head_dim(c->desc.head_dim)) return fail(SA_EINVAL, "head_dim must be 64 or 128");
     if (!aligned16(q) || !aligned16(out) || !aligned16(ws))
         return fail(SA_EINVAL, "q, out and ws must be 16-byte aligned");
+    // A call of one launch is refused by that launch, which may need less.
+    if (n_seq > kRowsPerLaunch && (!ws || ws_bytes < ws_need))
+        return fail(SA_ENOMEM, "workspace too small for the partials");
     return on_cache_device(c);
 }
 
@@ -896,7 +899,8 @@ extern "C" sa_status sa_paged_decode_window(const sa_kvcache* c, int layer, cons
     if (window <= 0) return fail(SA_EINVAL, "window must be positive");
     if (n_sink < 0) return fail(SA_EINVAL, "n_sink must be >= 0");
     return no_throw([&]() -> sa_status {
-        SA_TRY(check_ranges(c, layer, q, n_seq, n_q_heads, out, ws));
+        SA_TRY(check_ranges(c, layer, q, n_seq, n_q_heads, out, ws, ws_bytes,
+                            sa_paged_decode_window_ws_bytes(c, n_seq, n_q_heads, window, n_sink)));
         const Verdict vd = c->pt.check_decode(seq_ids, n_seq, n_pending, nullptr, nullptr);
         if (!vd.ok()) return refused(vd);
         std::vector<RangeSource> own(n_seq);
@@ -925,7 +929,8 @@ extern "C" sa_status sa_paged_decode_shared(const sa_kvcache* c, int layer, cons
     if (!valid_cache(c)) return fail(SA_EINVAL, "invalid cache");
     if (group_sizes ? n_groups <= 0 : n_groups != 0) return fail(SA_EINVAL, "group_sizes and n_groups go together");
     return no_throw([&]() -> sa_status {
-        SA_TRY(check_ranges(c, layer, q, n_seq, n_q_heads, out, ws));
+        SA_TRY(check_ranges(c, layer, q, n_seq, n_q_heads, out, ws, ws_bytes,
+                            sa_paged_decode_shared_ws_bytes(c, n_seq, n_q_heads)));
         const Verdict vd = c->pt.check_decode(seq_ids, n_seq, n_pending, nullptr, nullptr);
         if (!vd.ok()) return refused(vd);
         const std::vector<int32_t> sizes = group_sizes ? std::vector<int32_t>(group_sizes, group_sizes + n_groups)

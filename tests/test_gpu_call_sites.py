@@ -132,3 +132,66 @@ def test_steps_into_shared_pages_are_refused_whole(sa, monkeypatch, interleave):
     assert [cache.length(r) for r in range(4)] == [65] * 4
     cache.close()
     model.close()
+
+
+def test_small_workspaces_refuse_many_rows_whole(sa):
+    """70 rows take two launches; the first would fit the workspace."""
+    lens = [64] * 64 + [4000] * 6
+    c = sa.KVCache(1, 1, 64, 70, 63, 64 + 6 * 63, sa.SA_DTYPE_BF16)
+    for r, n in enumerate(lens):
+        c.reserve(r, n)
+        c.set_len(r, n)
+    q = torch.randn(70, 4, 64, device="cuda")
+    out = torch.full_like(q, 7.0)
+    ws = torch.empty(4096, dtype=torch.uint8, device="cuda")
+    for call in (lambda: c.decode_window(0, q, 0.1, 4000, out=out, ws=ws), lambda: c.decode_shared(0, q, 0.1, out=out, ws=ws)):
+        with pytest.raises(RuntimeError, match="workspace"):
+            call()
+        torch.cuda.synchronize()
+        assert (out == 7).all()
+    c.close()
+
+
+@pytest.mark.parametrize("P", [200, 4100])
+def test_beam_step_replayed(sa, P):
+    """A step captured into a graph and replayed from the state of the call, row
+    by row (200 tokens) and over shared pages (4100)."""
+    model = sa.Qwen3(4, P + 10, num_layers=2, hidden=256, intermediate=512, vocab=1024, n_q_heads=4, n_kv_heads=2,
+                     head_dim=64, rms_eps=1e-6, rope_theta=1e6)
+    model.init_random(7, 0.1)
+    cache = sa.KVCache(2, 2, 64, 4, P // 64 + 1, 4 * (P // 64 + 1), sa.SA_DTYPE_BF16)
+    cache.reserve(0, P)
+    for layer in range(2):
+        cache.append(layer, None, *(torch.randn(1, P, 2, 64, device="cuda") for _ in range(2)), seq_ids=[0])
+    cache.commit(P, seqs=[0])
+    for r in range(1, 4):
+        cache.fork(r, 0, P)
+    for r in range(4):
+        cache.reserve(r, P + 1)
+    tokens = torch.tensor([[5, 6, 7, 8]], dtype=torch.int32, device="cuda")
+    scores = torch.tensor([[-1.0, -2.0, -3.0, -4.0]], device="cuda")
+    out = (torch.empty(1, 8, device="cuda"), *(torch.empty(1, 8, dtype=torch.int32, device="cuda") for _ in range(2)))
+
+    def back():
+        for r in range(4):
+            cache.set_len(r, P)
+
+    want = [t.clone() for t in model.beam_step(cache, tokens, scores, 8, out=out)]
+    back()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        model.beam_step(cache, tokens, scores, 8, out=out)
+    for _ in range(3):
+        back()
+        for t in out:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+        back()
+        again = model.beam_step(cache, tokens, scores, 8)
+        assert all(torch.equal(a, b) for a, b in zip(again, want))
+    del graph
+    cache.close()
+    model.close()
