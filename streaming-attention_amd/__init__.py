@@ -172,10 +172,11 @@ def _rows(ids, n: int):
 
 
 _raw_stream = None   # the current stream's handle, without a Stream object (2.9 -> 0.4 us per call)
+_raw_of = None       # the same for a device that is known
 
 
 def _stream(stream) -> int | None:
-    global _raw_stream
+    global _raw_stream, _raw_of
     if stream is None:
         if _raw_stream is None:
             import torch
@@ -184,7 +185,7 @@ def _stream(stream) -> int | None:
             if raw is None:
                 _raw_stream = lambda: torch.cuda.current_stream().cuda_stream  # noqa: E731
             else:
-                _raw_stream = lambda: raw(current())  # noqa: E731
+                _raw_stream, _raw_of = lambda: raw(current()), raw
         return _raw_stream()
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else stream
 
@@ -199,13 +200,21 @@ def _alloc(stream, make):
         return make()
 
 
-def _on_device(*tensors) -> None:
-    """Kernels run on the current device, and so must their tensors be."""
-    import torch
-    device = torch.cuda.current_device()
+_cuda = None         # torch.cuda
+
+
+def _on(stream, *tensors) -> int | None:
+    """The handle of the stream of a call: kernels run on the current device, and
+    so must their tensors be."""
+    global _cuda
+    if _cuda is None:
+        import torch
+        _cuda = torch.cuda
+    device = _cuda.current_device()
     for t in tensors:
         if t.get_device() != device:
             raise ValueError("the tensors must be on the current CUDA device")
+    return _stream(stream) if stream is not None or _raw_of is None else _raw_of(device)
 
 
 _INT_MAX = 2 ** 31 - 1
@@ -370,11 +379,12 @@ class KVCache:
         """decode over each sequence's last `window` tokens and its first
         n_sink: q [n_seq, Hq, D] -> out [n_seq, Hq, D]."""
         n_seq, Hq, _ = q.shape
-        window, n_sink = min(window, _INT_MAX), min(n_sink, _INT_MAX)
-        out, ws = self._out_ws(q, out, ws, lambda: self.decode_window_ws_bytes(n_seq, Hq, window, n_sink), stream)
-        check(lib().sa_paged_decode_window(self.handle, layer, _ptr(q), n_seq, _rows(seq_ids, n_seq), Hq,
-                                           n_pending, window, n_sink, scale, _ptr(out), _ptr(ws), _nbytes(ws),
-                                           _stream(stream)))
+        if window > _INT_MAX or n_sink > _INT_MAX:
+            window, n_sink = min(window, _INT_MAX), min(n_sink, _INT_MAX)
+        out, ws, st = self._out_ws(q, out, ws, stream, self.decode_window_ws_bytes, n_seq, Hq, window, n_sink)
+        check(lib().sa_paged_decode_window(self.handle, layer, q.data_ptr(), n_seq, _rows(seq_ids, n_seq), Hq,
+                                           n_pending, window, n_sink, scale, out.data_ptr(), ws.data_ptr(),
+                                           _nbytes(ws), st))
         return out
 
     def decode_shared_ws_bytes(self, n_seq: int, n_q_heads: int) -> int:
@@ -386,27 +396,28 @@ class KVCache:
         one group) whose shared leading pages are read once per group:
         q [n_seq, Hq, D] -> out [n_seq, Hq, D]."""
         n_seq, Hq, _ = q.shape
-        out, ws = self._out_ws(q, out, ws, lambda: self.decode_shared_ws_bytes(n_seq, Hq), stream)
+        out, ws, st = self._out_ws(q, out, ws, stream, self.decode_shared_ws_bytes, n_seq, Hq)
         n_groups = 0 if groups is None else len(groups)
-        check(lib().sa_paged_decode_shared(self.handle, layer, _ptr(q), n_seq, _rows(seq_ids, n_seq),
-                                           _rows(groups, n_groups), n_groups, Hq, n_pending, scale, _ptr(out),
-                                           _ptr(ws), _nbytes(ws), _stream(stream)))
+        check(lib().sa_paged_decode_shared(self.handle, layer, q.data_ptr(), n_seq, _rows(seq_ids, n_seq),
+                                           _rows(groups, n_groups), n_groups, Hq, n_pending, scale,
+                                           out.data_ptr(), ws.data_ptr(), _nbytes(ws), st))
         return out
 
-    def _out_ws(self, q, out, ws, need, stream):
-        """The output and workspace of a decode of q, made where not given."""
-        import torch
+    def _out_ws(self, q, out, ws, stream, need, *args):
+        """The output and workspace (of need(*args) bytes) of a decode of q, made
+        where not given, and the stream's handle."""
         _f32(q, "q")
         if q.shape[-1] != self.desc.head_dim:
             raise ValueError("q must be [n_seq, Hq, head_dim]")
         if out is None:
+            import torch
             out = _alloc(stream, lambda: torch.empty_like(q))
         elif out.shape != q.shape:
             raise ValueError("out must have q's shape")
         if ws is None:
-            ws = _alloc(stream, lambda: torch.empty(max(need(), 16), dtype=torch.uint8, device=q.device))
-        _on_device(q, _f32(out, "out"), ws)
-        return out, ws
+            import torch
+            ws = _alloc(stream, lambda: torch.empty(max(need(*args), 16), dtype=torch.uint8, device=q.device))
+        return out, ws, _on(stream, q, _f32(out, "out"), ws)
 
     def append_decode(self, layer: int, q, k, v, scale: float, q_norm_w=None, k_norm_w=None, eps: float = 1e-6,
                       rope=None, out=None, q_out=None, ws=None, commit: bool = False, seq_ids=None, stream=None):
@@ -579,9 +590,9 @@ def beam_select(logits, scores, n_select: int, out=None, ws=None, stream=None):
     if ws is None:
         ws = _alloc(stream, lambda: torch.empty(max(beam_select_ws_bytes(G, B, V, n_select), 8), dtype=torch.uint8,
                                                 device=logits.device))
-    _on_device(logits, _f32(scores, "scores"), o, t, b, ws)
-    check(lib().sa_beam_select(logits.data_ptr(), stride, _ptr(scores), G, B, V, n_select, o.data_ptr(),
-                               t.data_ptr(), b.data_ptr(), ws.data_ptr(), _nbytes(ws), _stream(stream)))
+    st = _on(stream, logits, _f32(scores, "scores"), o, t, b, ws)
+    check(lib().sa_beam_select(logits.data_ptr(), stride, scores.data_ptr(), G, B, V, n_select, o.data_ptr(),
+                               t.data_ptr(), b.data_ptr(), ws.data_ptr(), _nbytes(ws), st))
     return out
 
 
@@ -655,7 +666,7 @@ def prefill_window(q, k, v, scale: float, window: int, n_sink: int = 0, out=None
         raise ValueError("k and v must be [B, Hkv, L, D] of one layout, and out like q")
     if k.dtype != dtype or v.dtype != dtype or out.dtype != dtype:
         raise ValueError("q, k, v and out must have one dtype")
-    _on_device(q, k, v, out)
+    st = _on(stream, q, k, v, out)
     if q.is_contiguous() and k.is_contiguous() and out.is_contiguous():
         qs = ks = os_ = None
     else:
@@ -663,8 +674,10 @@ def prefill_window(q, k, v, scale: float, window: int, n_sink: int = 0, out=None
             raise ValueError("the rows of q, k, v and out must be contiguous")
         qs, ks, os_ = (C.cast((C.c_int64 * 3)(*t.stride()[:3]), C.c_void_p) for t in (q, k, out))
     dt = SA_DTYPE_F32 if dtype == torch.float32 else SA_DTYPE_BF16
-    check(lib().sa_prefill_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, B, Hq, Hkv, L, D, qs, ks, os_,
-                                  min(window, _INT_MAX), min(n_sink, _INT_MAX), scale, out.data_ptr(), _stream(stream)))
+    if window > _INT_MAX or n_sink > _INT_MAX:
+        window, n_sink = min(window, _INT_MAX), min(n_sink, _INT_MAX)
+    check(lib().sa_prefill_window(q.data_ptr(), k.data_ptr(), v.data_ptr(), dt, B, Hq, Hkv, L, D, qs, ks, os_, window,
+                                  n_sink, scale, out.data_ptr(), st))
     return out
 
 
@@ -777,9 +790,9 @@ class Qwen3:
         for t, dt in zip(out, (torch.float32, torch.int32, torch.int32)):
             if t.dtype != dt or tuple(t.shape) != (G, n_select) or not t.is_cuda or not t.is_contiguous():
                 raise ValueError("out must be contiguous CUDA tensors [G, n_select]: float32, int32, int32")
-        _on_device(tokens, _f32(scores, "scores"), *out)
+        st = _on(stream, tokens, _f32(scores, "scores"), *out)
         check(lib().sa_qwen3_beam_step(self.handle, cache.handle, _ptr(tokens), G, B, _ptr(scores),
-                                       n_select, _ptr(out[0]), _ptr(out[1]), _ptr(out[2]), _stream(stream)))
+                                       n_select, _ptr(out[0]), _ptr(out[1]), _ptr(out[2]), st))
         return out
 
     def beam_search(self, cache: "KVCache", prompts, n_beams: int, n_tokens: int, eos: int | None = None):
