@@ -501,7 +501,10 @@ sa_status sa_axpby_f32(const float* x, float a, const float* y, float b, size_t 
  * is not finite (a NaN or +inf among its logits, or nothing but -inf).  Places
  * left over hold -inf, -1 and -1.  The order is decided in 64 bits.
  * n_beams and n_select 1 .. 64, n_beams * vocab < 2^31, n_groups at most 2^20
- * and n_groups * n_beams * ceil(vocab / 2048) below 2^24.  out_scores may be scores itself.  ws: 8-byte aligned,
+ * and n_groups * n_beams * ceil(vocab / 2048) below 2^24.  out_scores may be
+ * scores itself where n_select == n_beams or n_groups == 1, since each search
+ * reads its scores before it writes; the two may not overlap otherwise
+ * (SA_EINVAL), nor may another output overlap an input.  ws: 8-byte aligned,
  * sa_beam_select_ws_bytes bytes; calls that overlap on one workspace race.
  * The parents (out_beams) are what sa_kvcache_reorder takes, on the host.
  * ------------------------------------------------------------------------ */

@@ -134,7 +134,8 @@ sa_status sa_qwen3_decode_step(sa_qwen3* model, sa_kvcache* cache, const int32_t
  * * n_beams + b holding beam b of search g, and sa_beam_select over its logits.
  * tokens: device int32 [n_groups * n_beams]; scores: device fp32, the beams'
  * accumulated log probabilities; out_scores, out_tokens, out_beams: device
- * [n_groups][n_select], as sa_beam_select's.  Every row's length grows by one.
+ * [n_groups][n_select], as sa_beam_select's (out_scores may be scores itself
+ * where n_select == n_beams or n_groups == 1).  Every row's length grows by one.
  * Where the beams of a search share enough leading pages (sa_kvcache_fork,
  * sa_kvcache_reorder), the attention reads them once per search
  * (sa_paged_decode_shared), else row by row.  The search goes on with the beams

@@ -216,6 +216,8 @@ __global__ void __launch_bounds__(kSelThreads) beam_pick_kernel(BeamArgs a) {
 
     // ---- this thread's segments: slot j is part j % per_beam of its wave's beam
     // j / per_beam, whose segments are dealt out to the beam's waves first ----
+    // A search's scores are read here and its results written at the end: they may
+    // share their place, while no search's results may fall on another's scores.
     const float score = tid < a.n_beams ? a.scores[(long long)group * a.n_beams + tid] : 0.f;
     float2 sg[SLOTS];
     int id[SLOTS];      // segment of the beam, -1: none
@@ -495,6 +497,17 @@ bool beam_sizes_ok(int n_groups, int n_beams, int vocab, int n_select) {
 
 using namespace sa;
 
+sa_status sa::check_beam_scores(const float* scores, const float* out_scores, int n_groups, int n_beams, int n_select) {
+    if (n_groups <= 0 || n_beams <= 0 || n_select <= 0) return SA_OK;   // refused as sizes
+    if (out_scores == scores && (n_select == n_beams || n_groups == 1)) return SA_OK;
+    const uintptr_t in = reinterpret_cast<uintptr_t>(scores), out = reinterpret_cast<uintptr_t>(out_scores);
+    const unsigned long long n = n_groups;
+    if (in < out + n * n_select * sizeof(float) && out < in + n * n_beams * sizeof(float))
+        return fail(SA_EINVAL, "out_scores may be scores itself for as many selected as beams, or for one search, "
+                               "and not overlap it otherwise");
+    return SA_OK;
+}
+
 extern "C" size_t sa_beam_select_ws_bytes(int n_groups, int n_beams, int vocab, int n_select) {
     if (!beam_sizes_ok(n_groups, n_beams, vocab, n_select)) return 0;
     return (size_t)n_groups * n_beams * beam_shape(n_beams, vocab).n_seg * sizeof(float2);
@@ -508,6 +521,7 @@ extern "C" sa_status sa_beam_select(const float* logits, int64_t row_stride, con
     if (!beam_sizes_ok(n_groups, n_beams, vocab, n_select))
         return fail(SA_EINVAL, "beam selection takes 1 to 64 beams, 1 to 64 selected, n_beams * vocab < 2^31, 2^20 groups");
     if (row_stride < vocab) return fail(SA_EINVAL, "row_stride must be at least vocab");
+    SA_TRY(check_beam_scores(scores, out_scores, n_groups, n_beams, n_select));
     const BeamShape sh = beam_shape(n_beams, vocab);
     if (!ws || ws_bytes < sa_beam_select_ws_bytes(n_groups, n_beams, vocab, n_select))
         return fail(SA_ENOMEM, "workspace too small for the segments");

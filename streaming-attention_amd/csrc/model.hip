@@ -1033,6 +1033,7 @@ extern "C" sa_status sa_qwen3_beam_step(sa_qwen3* m, sa_kvcache* cache, const in
     clear_error();
     if (!m || !cache || !tokens || !scores || !out_scores || !out_tokens || !out_beams)
         return fail(SA_EINVAL, "null argument");
+    SA_TRY(check_beam_scores(scores, out_scores, n_groups, n_beams, n_select));
     if (n_groups < 1 || n_beams < 1 || (long long)n_groups * n_beams > m->max_batch)
         return fail(SA_ERANGE, "n_groups * n_beams outside [1, max_batch]");
     // Refused before anything is enqueued, as the selection would be.

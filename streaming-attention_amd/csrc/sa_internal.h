@@ -282,6 +282,10 @@ sa_status check_append(const sa_kvcache* c, int n, int S, int max_pos);
 // reads once instead of once per row, with one token pending in each row.
 long long shared_tokens_saved(const sa_kvcache* c, const int32_t* sizes, int n_groups);
 
+// A beam selection's results may not fall on scores that another search of the
+// launch has yet to read.
+sa_status check_beam_scores(const float* scores, const float* out_scores, int n_groups, int n_beams, int n_select);
+
 size_t paged_ws(int n_seq, int n_q, int n_kv, int d, int max_pages);
 // seq_ids: host array of cache rows (NULL: 0 .. n_seq-1), already checked.
 // lens: the rows' committed lengths (host array in call order, the page

@@ -195,3 +195,23 @@ def test_beam_step_replayed(sa, P):
     del graph
     cache.close()
     model.close()
+
+
+@pytest.mark.parametrize("B,n", [(3, 6), (6, 3), (4, 64)])
+def test_one_search_in_place(sa, B, n):
+    """One search may select more or fewer than it has beams over its scores;
+    several may not, and are refused with nothing written."""
+    x = torch.randn(3, B, 4001, device="cuda")
+    buf = -torch.rand(3 * max(B, n), device="cuda")
+    s = buf[:B].view(1, B)
+    want = sa.beam_select(x[:1], s, n)
+    ints = [torch.full((3, n), 7, dtype=torch.int32, device="cuda") for _ in range(2)]
+    got = sa.beam_select(x[:1], s, n, out=(buf[:n].view(1, n), *(t[:1] for t in ints)))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    before = buf.clone()
+    for t in ints:
+        t.fill_(7)
+    with pytest.raises(RuntimeError, match="out_scores"):
+        sa.beam_select(x, buf[:3 * B].view(3, B), n, out=(buf[:3 * n].view(3, n), *ints))
+    torch.cuda.synchronize()
+    assert torch.equal(buf, before) and all((t == 7).all() for t in ints)

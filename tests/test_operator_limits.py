@@ -50,3 +50,27 @@ def test_beam_search_arguments(sa):
     for beams, tokens in ((0, 5), (65, 5), (4, 0), (4, -1)):
         with pytest.raises(ValueError):
             model.beam_search(None, None, beams, tokens)
+
+
+def test_scores_in_place_where_searches_would_meet(sa):
+    """Searches run side by side: results of one may not fall on scores that
+    another has yet to read.  (A workspace too small is what the calls that may
+    run in place are refused for.)"""
+    buf = (C.c_uint8 * 4096)()
+    at = (C.addressof(buf) + 15) // 16 * 16
+    model = (C.c_uint8 * 4096)()                # no call reads it
+    far = at + 2048
+
+    def select(G, B, n, scores, out):
+        return sa.lib().sa_beam_select(at, 50, scores, G, B, 50, n, out, far, far + 512, far + 1024, 8, None)
+
+    def step(G, B, n, scores, out):
+        return sa.lib().sa_qwen3_beam_step(C.addressof(model), at, at, G, B, scores, n, out, far, far + 512, None)
+
+    for call in (select, step):
+        for G, B, n, shift in ((2, 2, 4, 0), (2, 4, 2, 0), (3, 1, 2, 0), (2, 4, 4, 4), (2, 4, 4, -4), (2, 2, 8, -60),
+                               (1, 4, 4, 4), (1, 4, 8, -28), (3, 4, 4, 44)):
+            assert call(G, B, n, at + 256, at + 256 + shift) == sa.SA_EINVAL, (call, G, B, n, shift)
+            assert b"out_scores" in sa.lib().sa_last_error()
+    for G, B, n, shift in ((2, 4, 4, 0), (1, 2, 4, 0), (1, 4, 2, 0), (2, 4, 2, 32), (2, 4, 8, -64), (1, 4, 4, 16)):
+        assert select(G, B, n, at + 256, at + 256 + shift) == sa.SA_ENOMEM, (G, B, n, shift)
