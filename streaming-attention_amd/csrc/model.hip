@@ -1033,9 +1033,10 @@ extern "C" sa_status sa_qwen3_beam_step(sa_qwen3* m, sa_kvcache* cache, const in
     clear_error();
     if (!m || !cache || !tokens || !scores || !out_scores || !out_tokens || !out_beams)
         return fail(SA_EINVAL, "null argument");
-    SA_TRY(check_beam_scores(scores, out_scores, n_groups, n_beams, n_select));
-    if (n_groups < 1 || n_beams < 1 || (long long)n_groups * n_beams > m->max_batch)
+    if (n_groups < 1 || n_beams < 1 || (long long)n_groups * n_beams > kMaxBatch)
         return fail(SA_ERANGE, "n_groups * n_beams outside [1, max_batch]");
+    SA_TRY(check_beam_scores(scores, out_scores, n_groups, n_beams, n_select));
+    if (n_groups * n_beams > m->max_batch) return fail(SA_ERANGE, "n_groups * n_beams outside [1, max_batch]");
     // Refused before anything is enqueued, as the selection would be.
     const int rows = n_groups * n_beams;
     const size_t select = sa_beam_select_ws_bytes(n_groups, n_beams, m->d.vocab, n_select);
