@@ -112,7 +112,9 @@ sa_status sa_qwen3_load_safetensors(sa_qwen3* model, const char* path);
  * the last position's logits; logits: device fp32 [batch][vocab] (that
  * position) or NULL.  The caller must have reserved L tokens of pages.
  * Activations of batch * L rows live in a grow-only device buffer of the
- * model (allocated on the first call of a larger size).  Asynchronous. */
+ * model (allocated on the first call of a larger size, which frees the smaller
+ * one: a graph that captured a prefill must not be replayed after it).
+ * Asynchronous. */
 sa_status sa_qwen3_prefill(sa_qwen3* model, sa_kvcache* cache, const int32_t* tokens, int batch, int L,
                            int32_t* next_tokens, float* logits, sa_stream_t stream);
 
@@ -125,7 +127,9 @@ sa_status sa_qwen3_prefill(sa_qwen3* model, sa_kvcache* cache, const int32_t* to
  * (lowest index on ties).  logits: device fp32 [batch][vocab] or NULL.  The
  * caller must have reserved cache pages for the new tokens.  Input ids
  * outside [0, vocab) embed as zeros.  Asynchronous on stream; the first call
- * with a given cache geometry allocates the attention workspace. */
+ * with a given cache geometry allocates the attention workspace.  Workspaces
+ * that are outgrown live until the model is destroyed, so that a graph that
+ * captured a step stays valid after a larger one. */
 sa_status sa_qwen3_decode_step(sa_qwen3* model, sa_kvcache* cache, const int32_t* tokens, int batch,
                                int32_t* next_tokens, float* logits, sa_stream_t stream);
 
@@ -143,8 +147,9 @@ sa_status sa_qwen3_decode_step(sa_qwen3* model, sa_kvcache* cache, const int32_t
  * tokens and scores as the next step's.  The caller must have reserved pages
  * of every row's own for the new token (SA_EFULL, or SA_EINVAL where it is a
  * shared one; nothing is enqueued then).  Asynchronous on stream; a graph that
- * holds a step repeats it for the lengths at the call.  The first call
- * with a given cache geometry and selection allocates workspaces. */
+ * holds a step repeats it for the lengths at the call, also after larger steps.
+ * The first call with a given cache geometry and selection allocates
+ * workspaces. */
 sa_status sa_qwen3_beam_step(sa_qwen3* model, sa_kvcache* cache, const int32_t* tokens, int n_groups, int n_beams,
                              const float* scores, int n_select, float* out_scores, int32_t* out_tokens,
                              int32_t* out_beams, sa_stream_t stream);

@@ -61,7 +61,7 @@ struct sa_qwen3 {
     float* logits = nullptr;   // [B][vocab]
     float* am_val = nullptr;   // argmax partials [B][max(kArgBlocks, kFewHeadBlocks)]
     int32_t* am_idx = nullptr;
-    void* ws = nullptr;        // paged decode workspace (grow-only)
+    void* ws = nullptr;        // paged decode workspace (see grow)
     size_t ws_bytes = 0;
     void* pf = nullptr;        // prefill activations for batch x prompt rows (grow-only)
     size_t pf_bytes = 0;
@@ -71,7 +71,7 @@ struct sa_qwen3 {
     float* part2 = nullptr;
     void* ws2 = nullptr;
     size_t ws2_bytes = 0;
-    void* beam_ws = nullptr;   // a beam step's greedy tokens, selection and shared attention (grow-only)
+    void* beam_ws = nullptr;   // a beam step's greedy tokens, selection and shared attention (see grow)
     size_t beam_ws_bytes = 0;
     hipStream_t side = nullptr;
     std::vector<hipEvent_t> events;   // fork, join, the first half's first attention done
@@ -522,14 +522,24 @@ void release(sa_qwen3* m) {
     m->pf = nullptr;
 }
 
-// Grow-only device buffer.
-sa_status grow(void** p, size_t* have, size_t need) {
+// Workspace of at least need bytes.  An outgrown block lives on until the model
+// is destroyed: captured steps hold pointers into it.  A new one is at least
+// twice as large, so the outgrown ones together are smaller than the last.
+sa_status grow(sa_qwen3* m, void** p, size_t* have, size_t need) {
     if (need <= *have) return SA_OK;
-    if (*p) SA_HIP_TRY(hipFree(*p));
-    *p = nullptr;
-    *have = 0;
-    SA_HIP_TRY(hipMalloc(p, need));
-    *have = need;
+    m->allocs.reserve(m->allocs.size() + 1);
+    void* block = nullptr;
+    size_t size = std::max(need, 2 * *have);
+    hipError_t e = hipMalloc(&block, size);
+    if (e != hipSuccess && size > need) {
+        (void)hipGetLastError();
+        size = need;
+        e = hipMalloc(&block, size);
+    }
+    if (e != hipSuccess) return hip_fail(e, "hipMalloc of a workspace");
+    if (*p) m->allocs.push_back(*p);
+    *p = block;
+    *have = size;
     return SA_OK;
 }
 
@@ -836,7 +846,7 @@ sa_status decode_rows(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int
     hipStream_t st = as_stream(stream);
     const bool shared = groups && shared_tokens_saved(cache, groups->sizes, groups->n) >= kSharedTokens;
     const size_t need = sa_paged_decode_ws_bytes(cache, batch, d.n_q_heads);
-    SA_TRY(grow(&m->ws, &m->ws_bytes, need));
+    SA_TRY(grow(m, &m->ws, &m->ws_bytes, need));
     const Shapes s = shapes_of(d);
     const int M = batch;
     const float eps = d.rms_eps;
@@ -981,7 +991,7 @@ sa_status decode_rows(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int
         }
     } else {
         SA_TRY(make_side(m, part_floats(s, m->max_batch)));
-        SA_TRY(grow(&m->ws2, &m->ws2_bytes, need));
+        SA_TRY(grow(m, &m->ws2, &m->ws2_bytes, need));
         int cut = 1;
         while (cut < M - 1 && 2 * prefix[cut] < total) ++cut;
         Rows a = make_rows(0, cut, m->part, m->ws, m->ws_bytes, st, true);
@@ -1045,7 +1055,7 @@ extern "C" sa_status sa_qwen3_beam_step(sa_qwen3* m, sa_kvcache* cache, const in
     const size_t next = up(rows * sizeof(int32_t)), attn = sa_paged_decode_shared_ws_bytes(cache, rows, m->d.n_q_heads);
     try {
         const std::vector<int32_t> sizes(n_groups, n_beams);
-        SA_TRY(grow(&m->beam_ws, &m->beam_ws_bytes, next + up(select) + attn));
+        SA_TRY(grow(m, &m->beam_ws, &m->beam_ws_bytes, next + up(select) + attn));
         char* ws = static_cast<char*>(m->beam_ws);
         const RowGroups groups{sizes.data(), n_groups, ws + next + up(select), attn};
         SA_TRY(decode_rows(m, cache, tokens, rows, &groups, static_cast<int32_t*>(m->beam_ws), m->logits, stream));

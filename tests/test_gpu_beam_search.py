@@ -180,3 +180,67 @@ def test_one_probability_left(sa):
     assert (b == 1).all() and torch.isfinite(s).all() and (s.diff() <= 0).all()
     cache.close()
     model.close()
+
+
+@pytest.mark.parametrize("P", [200, 4100])
+def test_captured_steps_outlive_larger_ones(sa, P):
+    """A beam step and a decode step captured into graphs, then steps of more
+    rows, pages and selections, which need larger workspaces, and new tensors
+    where a freed workspace would be: the graphs' replays still give what the
+    eager steps gave, and leave the new tensors alone."""
+    model = make_model(sa, 16, 9000, 8)
+    small, large = make_cache(sa, 4, P + 80, sa.SA_DTYPE_F32), make_cache(sa, 16, 8800, sa.SA_DTYPE_F32)
+    gen = torch.Generator(device="cuda").manual_seed(P)
+
+    def fill(cache, rows, n):
+        cache.reserve(0, n)
+        for layer in range(SMALL["num_layers"]):
+            kv = (torch.randn(1, n, 2, 64, device="cuda", generator=gen) for _ in range(2))
+            cache.append(layer, None, *kv, seq_ids=[0])
+        cache.commit(n, seqs=[0])
+        for r in range(1, rows):
+            cache.fork(r, 0, n)
+        for r in range(rows):
+            cache.reserve(r, n + 1)
+
+    fill(small, 4, P)
+    tokens = torch.tensor([[5, 6, 7, 8]], dtype=torch.int32, device="cuda")
+    scores = torch.tensor([[-1.0, -2.0, -1.5, -0.5]], device="cuda")
+    out = (torch.empty(1, 6, device="cuda"), *(torch.empty(1, 6, dtype=torch.int32, device="cuda") for _ in range(2)))
+    logits = torch.empty(4, SMALL["vocab"], device="cuda")
+
+    def back(cache, rows, n):
+        for r in range(rows):
+            cache.set_len(r, n)
+        torch.cuda.synchronize()
+
+    steps = (lambda: model.beam_step(small, tokens, scores, 6, out=out),
+             lambda: model.decode_step(small, tokens.view(-1), logits=logits))
+    want, graphs = [], []
+    for step in steps:
+        step()
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in (*out, logits)])
+        back(small, 4, P)
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            step()
+        back(small, 4, P)
+    fill(large, 16, 8700)
+    model.beam_step(large, torch.arange(16, dtype=torch.int32, device="cuda").view(2, 8), torch.zeros(2, 8, device="cuda"), 64)
+    back(large, 16, 8700)
+    model.decode_step(large, torch.arange(16, dtype=torch.int32, device="cuda"))
+    fresh = [torch.full((1 << n,), 0xa5, dtype=torch.uint8, device="cuda") for n in range(12, 27) for _ in range(2)]
+    for rep in range(3):
+        for graph, w, some in zip(graphs, want, (slice(0, 3), slice(3, 4))):
+            for t in (*out, logits):
+                t.fill_(9)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip((*out, logits)[some], w[some])), rep
+            back(small, 4, P)
+    assert all((t == 0xa5).all() for t in fresh)
+    del graphs
+    for c in (small, large):
+        c.close()
+    model.close()
