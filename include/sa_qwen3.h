@@ -142,7 +142,9 @@ sa_status sa_qwen3_decode_step(sa_qwen3* model, sa_kvcache* cache, const int32_t
  * where n_select == n_beams or n_groups == 1).  Every row's length grows by one.
  * Where the beams of a search share enough leading pages (sa_kvcache_fork,
  * sa_kvcache_reorder), the attention reads them once per search
- * (sa_paged_decode_shared), else row by row.  The search goes on with the beams
+ * (sa_paged_decode_shared), else row by row.  Models of up to 64 query heads
+ * per KV head are taken (sa_qwen3_decode_step: 1, 2, 4 or 8; both refuse others
+ * before anything is enqueued).  The search goes on with the beams
  * that the caller picks: sa_kvcache_reorder with their rows as parents, their
  * tokens and scores as the next step's.  The caller must have reserved pages
  * of every row's own for the new token (SA_EFULL, or SA_EINVAL where it is a

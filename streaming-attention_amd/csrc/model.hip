@@ -23,6 +23,7 @@
 #include "bf16_terms.h"
 #include "few_rows.h"
 #include "proj.h"
+#include "ranges.h"
 #include "sa_internal.h"
 #include "sa_qwen3.h"
 
@@ -812,7 +813,7 @@ namespace {
 
 // Tokens that a grouped step has to save reading for its attention to take the
 // shared form (an append and the two launches of sa_paged_decode_shared instead
-// of one or two).  us per layer, one launch / shared, 16 / 8 heads of 128, bf16:
+// of one or two).  Measured at one shape only; us per layer, one launch / shared, 16 / 8 heads of 128, bf16:
 // 4 rows behind 2048 tokens 13.4 / 12.9, 4096 17.9 / 15.8; 8 behind 1024 13.4 / 13.1,
 // 2048 17.9 / 13.9; 64 behind 128 9.7 / 17.5, 512 28.5 / 18.6; 2 behind 8192 18.8 / 21.4.
 constexpr long long kSharedTokens = 12000;
@@ -843,8 +844,15 @@ sa_status decode_rows(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int
         if (len + 1 > sa_kvcache_capacity(cache, i)) return fail(SA_EFULL, "KV cache full, cannot append more tokens");
     }
     SA_TRY(check_append(cache, batch, 1, d.max_pos));
+    // The row-by-row form is made for some head ratios; the shared one takes
+    // rows that share nothing too.
+    const int rep = d.n_q_heads / d.n_kv_heads;
+    const bool by_rows = decode_rep_ok(rep);
+    if (!by_rows && !groups) return fail(SA_EINVAL, "n_q_heads / n_kv_heads must be 1, 2, 4 or 8");
+    if (!by_rows && rep > kRangesMaxRep) return fail(SA_EINVAL, "at most 64 query heads per KV head");
     hipStream_t st = as_stream(stream);
-    const bool shared = groups && shared_tokens_saved(cache, groups->sizes, groups->n) >= kSharedTokens;
+    const bool shared =
+        groups && (!by_rows || shared_tokens_saved(cache, groups->sizes, groups->n) >= kSharedTokens);
     const size_t need = sa_paged_decode_ws_bytes(cache, batch, d.n_q_heads);
     SA_TRY(grow(m, &m->ws, &m->ws_bytes, need));
     const Shapes s = shapes_of(d);

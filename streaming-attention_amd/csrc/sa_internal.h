@@ -286,6 +286,9 @@ long long shared_tokens_saved(const sa_kvcache* c, const int32_t* sizes, int n_g
 // launch has yet to read.
 sa_status check_beam_scores(const float* scores, const float* out_scores, int n_groups, int n_beams, int n_select);
 
+// Query heads per KV head that the paged decode has a kernel for.
+inline bool decode_rep_ok(int rep) { return rep == 1 || rep == 2 || rep == 4 || rep == 8; }
+
 size_t paged_ws(int n_seq, int n_q, int n_kv, int d, int max_pages);
 // seq_ids: host array of cache rows (NULL: 0 .. n_seq-1), already checked.
 // lens: the rows' committed lengths (host array in call order, the page

@@ -244,3 +244,46 @@ def test_captured_steps_outlive_larger_ones(sa, P):
     for c in (small, large):
         c.close()
     model.close()
+
+
+@pytest.mark.parametrize("Hq,Hkv", [(6, 2), (16, 1), (5, 1)])
+@pytest.mark.parametrize("P", [70, 4100])
+def test_head_ratios(sa, Hq, Hkv, P):
+    """Head ratios that the row-by-row attention has no kernel for, behind short
+    and long prompts, against the paths prefilled anew."""
+    desc = dict(SMALL, n_q_heads=Hq, n_kv_heads=Hkv)
+    model = sa.Qwen3(4, P + 10, **desc)
+    model.init_random(9, 0.1)
+    per = P // 64 + 1
+
+    def cache_of(rows):
+        return sa.KVCache(desc["num_layers"], Hkv, 64, rows, per, rows * per, sa.SA_DTYPE_F32)
+
+    gen = torch.Generator(device="cuda").manual_seed(P)
+    prompt = torch.randint(0, SMALL["vocab"], (1, P), dtype=torch.int32, device="cuda", generator=gen)
+    cache = cache_of(4)
+    cache.reserve(0, P)
+    model.prefill(cache, prompt)
+    cache.reorder(range(4), [0] * 4)
+    for r in range(4):
+        cache.reserve(r, P + 2)
+    tokens = torch.tensor([[3, 900, 17, 4]], dtype=torch.int32, device="cuda")
+    scores = torch.tensor([[-1.0, -3.0, -2.0, -1.5]], device="cuda")
+    got = model.beam_step(cache, tokens, scores, 6)
+    paths = torch.cat([prompt.expand(4, P), tokens.view(4, 1)], 1)
+    anew = cache_of(4)
+    for r in range(4):
+        anew.reserve(r, P + 1)
+    logits = torch.empty(4, SMALL["vocab"], device="cuda")
+    model.prefill(anew, paths.contiguous(), logits=logits)
+    lp = torch.log_softmax(logits.double(), -1).view(1, 4, -1) + scores.double()[..., None]
+    at = got[2].long() * SMALL["vocab"] + got[1].long()
+    assert (torch.gather(lp.view(1, -1), 1, at) - got[0].double()).abs().max() <= 2e-4
+    assert (torch.topk(lp.view(1, -1), 6).values - got[0].double()).abs().max() <= 2e-4
+    # the ordinary step has no kernel for them and says so before it does anything
+    with pytest.raises(RuntimeError, match="n_q_heads"):
+        model.decode_step(cache, tokens.view(-1))
+    assert [cache.length(r) for r in range(4)] == [P + 1] * 4
+    for c in (cache, anew):
+        c.close()
+    model.close()
