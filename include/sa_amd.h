@@ -305,7 +305,8 @@ sa_status sa_paged_decode_window(const sa_kvcache* cache, int layer, const float
  * Paged decode attention of sequences that share their leading pages.
  *
  * No counterpart in the reference.  Results as sa_paged_decode's (to fp32
- * rounding), with the n_seq rows in groups of consecutive rows: group_sizes
+ * rounding; infinite keys and values that a row sees come out alike in both,
+ * and in sa_paged_decode_window), with the n_seq rows in groups of consecutive rows: group_sizes
  * [n_groups] (host, each >= 1, adding up to n_seq), or NULL with n_groups = 0
  * for one group of all.  What a group shares is found from the page table: the
  * whole pages that all its rows list alike from the start on

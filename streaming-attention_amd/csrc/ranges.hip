@@ -17,6 +17,9 @@
 // out is below 2^-24 of the product, the rounding of an fp32 one.  fp32 values
 // that only one tile of 16 query rows uses are not split: fp32 MFMA takes them as
 // they are (4 searches of 4 beams behind 1500 - 2100 tokens 19.4 us against 19.8).
+// A chunk's row whose sums are not finite is computed anew without terms
+// (plain_row.h), so that infinities and values near fp32's limit come out as in
+// the paged decode that does not split.
 //
 // Layout: v_mfma_f32_16x16x32_bf16 with S^T = K Q^T (rows: keys, columns: query
 // rows), so that a lane's eight scores of a 32-key tile are the operand that
@@ -41,6 +44,7 @@
 #include <vector>
 
 #include "bf16_terms.h"
+#include "plain_row.h"
 #include "prefill_shared.h"
 
 namespace sa {
@@ -387,8 +391,10 @@ __device__ __forceinline__ void put(const RangeArgs& a, const Item& it, int j, i
     if (c == 0) *reinterpret_cast<f32x2_t*>(a.part_ml + at * 2) = f32x2_t{m, l};
 }
 
+// Returns the query rows, from it.q0 (RG = 4: the wave's first) on a bit each, that
+// the wave has to compute anew: their sums are not finite and nothing was put.
 template <int D, bool BF16, int RG, int RT>
-__device__ __forceinline__ void attend(const RangeArgs& a, const Item& it, lds_u8_t* smem, const int32_t* pages,
+__device__ __forceinline__ uint64_t attend(const RangeArgs& a, const Item& it, lds_u8_t* smem, const int32_t* pages,
                                        float (*ml)[2]) {
     using G = Geo<D, BF16>;
     constexpr int KG = kWaves / RG;
@@ -477,11 +483,14 @@ __device__ __forceinline__ void attend(const RangeArgs& a, const Item& it, lds_u
     float l[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) l[rt] = row_sum(w.l[rt]);
+    uint64_t anew = 0;
     if constexpr (KG == 1) {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const int j = q_base + 16 * rt + w.r16;
-            if (j < it.q1) {
+            const bool fine = l[rt] + row_sum(not_finite<G::DB>(w.acc[rt])) < INFINITY;
+            anew |= (__ballot(j < it.q1 && !fine) & 0xffff) << (16 * rt);
+            if (j < it.q1 && fine) {
 #pragma unroll
                 for (int db = 0; db < G::DB; ++db) put<D>(a, it, j, 4 * db + w.g, w.acc[rt][db], w.m[rt], l[rt]);
             }
@@ -502,9 +511,11 @@ __device__ __forceinline__ void attend(const RangeArgs& a, const Item& it, lds_u
             }
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < ROWS * (D / 4); i += kThreads) {
-            const int j = i / (D / 4), c = i % (D / 4);
-            if (it.q0 + j >= it.q1) break;
+        constexpr int C = D / 4;
+        const int c = lane % C;
+        for (int j0 = wave * (kWave / C); j0 < ROWS; j0 += kThreads / C) {   // the wave's rows
+            if (it.q0 + j0 >= it.q1) break;
+            const int j = j0 + lane / C;
             float M = ml[j][0];
 #pragma unroll
             for (int k = 1; k < KG; ++k) M = fmaxf(M, ml[k * ROWS + j][0]);
@@ -514,11 +525,48 @@ __device__ __forceinline__ void attend(const RangeArgs& a, const Item& it, lds_u
             for (int k = 0; k < KG; ++k) {
                 const float mk = ml[k * ROWS + j][0];
                 const float wk = mk == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mk - M);
-                o += po[(k * ROWS + j) * (D / 4) + c] * wk;
+                o += po[(k * ROWS + j) * C + c] * wk;
                 L += ml[k * ROWS + j][1] * wk;
             }
-            put<D>(a, it, it.q0 + j, c, o, M, L);
+            const bool mine = it.q0 + j < it.q1;
+            const uint64_t bad = __ballot(mine && !(L + not_finite<1>(&o) < INFINITY));
+            constexpr uint64_t row = (1ull << C) - 1;
+            static_assert(ROWS <= 64, "a bit per row");
+            if (mine && !(bad >> (lane / C * C) & row)) put<D>(a, it, it.q0 + j, c, o, M, L);
+#pragma unroll
+            for (int g = 0; g < kWave / C; ++g)
+                if (bad >> (g * C) & row) anew |= 1ull << (j0 + g);
         }
+    }
+    return anew;
+}
+
+// Query row j of an item without matrix instructions.
+template <int D, bool BF16>
+__device__ __forceinline__ void attend_plain(const RangeArgs& a, const Item& it, const int32_t* pages, int j) {
+    using T = std::conditional_t<BF16, uint16_t, float>;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int r = row_of(a, j), head = it.kvh * a.rep + j - r * a.rep;
+    const size_t row = ((size_t)(it.row0 + r) * a.n_q + head) * D;
+    PlainRow<D> p;
+    for (int u = it.u0; u < it.u1; ++u) {
+        const TileSpan sp = tile_span(it.src, u);
+        const size_t at = (((size_t)pages[u - it.u0] * a.n_kv + it.kvh) * SA_PAGE_TOKENS + (sp.lo & (SA_PAGE_TOKENS - 1))) * D;
+        p.keys(sp.hi - sp.lo, a.q + row, a.sl2,
+               [&](int i) { return static_cast<const T*>(a.k) + at + (size_t)i * D; },
+               [&](int i) { return static_cast<const T*>(a.v) + at + (size_t)i * D; });
+    }
+    if (it.single >> r & 1) {
+#pragma unroll
+        for (int e = 0; e < p.E; ++e) a.out[row + lane * p.E + e] = p.o[e] / p.l;
+        return;
+    }
+    const size_t at = (size_t)(it.part0 + j) * a.n_kv + it.kvh;
+#pragma unroll
+    for (int e = 0; e < p.E; ++e) a.part_o[at * D + lane * p.E + e] = p.o[e];
+    if (lane == 0) {
+        a.part_ml[at * 2] = p.m;
+        a.part_ml[at * 2 + 1] = p.l;
     }
 }
 
@@ -561,16 +609,20 @@ __global__ void __launch_bounds__(kThreads) range_attn_kernel(RangeArgs a) {
     __syncthreads();
 
     const int rows = it.q1 - it.q0;
+    uint64_t anew;
+    int first = it.q0;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     if constexpr (BF16) {
-        if (rows <= 16) attend<D, BF16, 1, 1>(a, it, smem, pages, ml);
-        else if (rows <= 32) attend<D, BF16, 2, 1>(a, it, smem, pages, ml);
-        else attend<D, BF16, 4, 1>(a, it, smem, pages, ml);
+        if (rows <= 16) anew = attend<D, BF16, 1, 1>(a, it, smem, pages, ml);
+        else if (rows <= 32) anew = attend<D, BF16, 2, 1>(a, it, smem, pages, ml);
+        else anew = attend<D, BF16, 4, 1>(a, it, smem, pages, ml), first += 16 * wave;
     } else {
-        if (rows <= 16) attend<D, BF16, 1, 1>(a, it, smem, pages, ml);
-        else if (rows <= 32) attend<D, BF16, 1, 2>(a, it, smem, pages, ml);
-        else if (rows <= 64) attend<D, BF16, 2, 2>(a, it, smem, pages, ml);
-        else attend<D, BF16, 4, 2>(a, it, smem, pages, ml);
+        if (rows <= 16) anew = attend<D, BF16, 1, 1>(a, it, smem, pages, ml);
+        else if (rows <= 32) anew = attend<D, BF16, 1, 2>(a, it, smem, pages, ml);
+        else if (rows <= 64) anew = attend<D, BF16, 2, 2>(a, it, smem, pages, ml);
+        else anew = attend<D, BF16, 4, 2>(a, it, smem, pages, ml), first += 32 * wave;
     }
+    for (; anew; anew &= anew - 1) attend_plain<D, BF16>(a, it, pages, first + __builtin_ctzll(anew));
 }
 
 // Joins the partials of row blockIdx.y's query head blockIdx.x: thread (s, c)

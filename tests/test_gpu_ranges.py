@@ -346,3 +346,56 @@ def test_streams_at_once(sa):
     for got, w in outs:
         close(got, w)
     r.cache.close()
+
+
+def same_with_infinities(got, want):
+    """Of one kind everywhere; finite values within 1e-4, or within 3e-4 of
+    themselves where one value near fp32's limit makes them (twice the error of
+    its weight, which a score's 5.6e-5 and a normaliser's make)."""
+    got, want = got.double(), want.double()
+    for kind in (torch.isnan, torch.isposinf, torch.isneginf):
+        assert torch.equal(kind(got), kind(want)), (kind, kind(got).sum().item(), kind(want).sum().item())
+        assert kind(want).any()
+    fine = torch.isfinite(want)
+    over = ((got - want).abs()[fine] / torch.clamp(3e-4 * want.abs()[fine], min=1e-4)).max().item()
+    assert over <= 1, over
+
+
+@pytest.mark.parametrize("kv", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows", [2, 8, 12, 20, 40, 64])
+def test_infinities_in_sight(sa, kv, D, rows):
+    """Infinite keys and values, and values near the types' limits, that the rows
+    see: what the formula makes of them, whichever split of the waves a number of
+    rows takes, and as the ordinary paged decode has it."""
+    P, Hkv, rep = 300, 2, 2
+    r = Rows(sa, kv, Hkv, D, [P] + [0] * (rows - 1), 20 + rows, spare=12 * rows, width=8)
+    k, v = r.k[0], r.v[0]
+    v[70, :, 3], v[71, :, 5] = np.inf, -np.inf
+    v[299, :, 6], v[0, :, 7], v[40, :, 8] = np.inf, -np.inf, 3.4e38 if kv == "f32" else 3.3e38
+    v[90, :, 10], v[91, :, 10] = np.inf, -np.inf        # NaN
+    k[33, 0, 0] = np.inf                                # head 0: a weight of 0, or NaN, by the sign of q
+    r.cache.set_len(0, 0)
+    r.cache.append(0, None, k[None], v[None], seq_ids=[0])
+    r.cache.commit(P, seqs=[0])
+    r.k[0], r.v[0] = (x.to(r.dtype).float() for x in (k, v))      # as they are stored
+    for i in range(1, rows):
+        r.fork(i, 0, P)
+    for i in range(rows):
+        r.cache.reserve(i, P + 5)
+        r.append(i, 1 + i % 5)
+    q = r.query(rows, rep)
+    ids = range(rows)
+    scale = D ** -0.5
+    for kv_block in (0, 64):
+        sa.set_attention_blocks(0, kv_block)
+        try:
+            want = r.want(q, ids, scale)
+            same_with_infinities(r.cache.decode_shared(0, q, scale), want)
+            same_with_infinities(r.cache.decode_shared(0, q, scale, [1] * rows), want)
+            same_with_infinities(r.cache.decode(0, q, scale), want)
+            for window, sink in ((1000, 0), (260, 5), (6, 92)):
+                same_with_infinities(r.cache.decode_window(0, q, scale, window, sink), r.want(q, ids, scale, window, sink))
+        finally:
+            sa.set_attention_blocks(0, 0)
+    r.cache.close()
