@@ -421,9 +421,9 @@ sa_status sa_prefill_causal_strided_ws(const void* q, const void* k, const void*
  * sa_prefill_causal_strided, for all tensors or NULL for all (dense); rows
  * contiguous; tensors and strides multiples of 16 bytes, the row stride of k
  * and v below 2^24 elements.  More than 2^23 query tiles (of 16 to 256 rows) are
- * refused.  out must not overlap an input.  The keys and values of a tile enter the products
- * together: a value that is not finite may reach queries up to 63 keys away
- * that do not see it.
+ * refused.  out must not overlap an input.  What a query does not see does not
+ * reach it, NaN and infinities included; rows whose tiles hold such values take
+ * longer.
  * ------------------------------------------------------------------------ */
 sa_status sa_prefill_window(const void* q, const void* k, const void* v, sa_dtype dtype,
                             int batch, int n_q_heads, int n_kv_heads, int L, int D,

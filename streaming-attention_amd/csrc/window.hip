@@ -21,6 +21,10 @@
 // v_mfma_f32_16x16x32_bf16; a wave owns 16 queries, tiles of 32 keys are split
 // into terms on their way into LDS.
 //
+// A hidden key's weight of 0 makes NaN of an infinite or NaN value, and a split
+// makes NaN of an infinity: rows whose sums are not finite are computed anew over
+// the keys that they see (plain_row.h).
+//
 // Bound: MFMA, with the softmax between.  16 / 8 heads of 128: 8192 queries,
 // window 1024, 4 sinks, bf16 86.9 us (64.7 GF of visible products, 0.74 PFLOP/s;
 // MFMA alone at a large product's rate 53); 2048 queries, window 512, fp32 54.8
@@ -30,6 +34,7 @@
 #include <cmath>
 
 #include "bf16_terms.h"
+#include "plain_row.h"
 #include "prefill_shared.h"
 
 namespace sa {
@@ -70,6 +75,39 @@ __device__ __forceinline__ Seen seen(const WindowArgs& a, int q0, int q1, int k0
 }
 __device__ __forceinline__ bool hidden(const WindowArgs& a, int q, int k) {
     return k > q || (q - k >= a.window && k >= a.sink);
+}
+
+// Query row `row` of the workgroup's head h0 + dh without matrix instructions, one
+// wave.  The launch's arguments (the kernel's first) are read anew, so that no
+// register holds them until here.
+template <int D, class T>
+__device__ __forceinline__ void window_plain(int dh, int row) {
+    const int lane = threadIdx.x & (kWave - 1);
+    auto args = (const __attribute__((address_space(4))) WindowArgs*)__builtin_amdgcn_kernarg_segment_ptr();
+    int block = blockIdx.x;
+    asm volatile("" : "+s"(args), "+s"(block));
+    const WindowArgs& a = *(const WindowArgs*)args;
+    const float factor = a.q_sign ? -a.sl2 : a.sl2;   // bf16: the sign went to q
+    const pf::Work wk = pf::map_work(a, block);
+    const T* Q = static_cast<const T*>(a.q) + wk.b * a.qs[0] + (wk.h0 + dh) * a.qs[1];
+    const T* K = static_cast<const T*>(a.k) + wk.b * a.kvs[0] + wk.kvh * a.kvs[1];
+    const T* V = static_cast<const T*>(a.v) + wk.b * a.kvs[0] + wk.kvh * a.kvs[1];
+    T* out = static_cast<T*>(a.dst) + wk.b * a.os[0] + (wk.h0 + dh) * a.os[1];
+    const int from = max(0, row - a.window + 1);
+    PlainRow<D> p;
+    auto span = [&](int k0, int k1) {
+        for (int k = k0; k < k1; k += kWave)
+            p.keys(min(kWave, k1 - k), Q + row * a.qs[2], factor, [&](int i) { return K + (k + i) * a.kvs[2]; },
+                   [&](int i) { return V + (k + i) * a.kvs[2]; });
+    };
+    span(0, min(a.sink, from));
+    span(from, row + 1);
+#pragma unroll
+    for (int e = 0; e < p.E; ++e) {
+        const float v = p.o[e] / p.l;
+        if constexpr (sizeof(T) == 2) out[row * a.os[2] + lane * p.E + e] = f32_to_bf16_rne(v);
+        else out[row * a.os[2] + lane * p.E + e] = v;
+    }
 }
 
 // pf::dma16 with a uniform base and a byte offset per lane.
@@ -224,34 +262,43 @@ struct BfWave {
     }
 
     // O / l: every lane's columns into the wave's part of LDS (chunks of a row
-    // permuted as the tiles' are), then rows of 16-byte pieces to memory.
-    __device__ __forceinline__ void store(uint16_t* head, long long row, int L, lds_u8_t* buf, int lane) const {
+    // permuted as the tiles' are), then rows of 16-byte pieces to memory.  Returns
+    // the rows, a bit each, that are not finite and not written.
+    __device__ __forceinline__ uint32_t store(uint16_t* head, long long row, int L, lds_u8_t* buf, int lane) const {
         const float inv = 1.0f / (l + xor32(l));
+        const bf16x2_t one = {(__bf16)1.0f, (__bf16)1.0f};
+        float sum[4] = {};   // of the outputs: finite where they are
 #pragma unroll
         for (int db = 0; db < G::NDB; ++db)
 #pragma unroll
             for (int jj = 0; jj < 4; ++jj) {
                 const f32x2_t x = {acc[db][4 * jj] * inv, acc[db][4 * jj + 1] * inv};
                 const f32x2_t y = {acc[db][4 * jj + 2] * inv, acc[db][4 * jj + 3] * inv};
+                const bf16x2_t bx = __builtin_convertvector(x, bf16x2_t), by = __builtin_convertvector(y, bf16x2_t);
+                sum[jj] = __builtin_amdgcn_fdot2_f32_bf16(bx, one, sum[jj], false);
+                sum[jj] = __builtin_amdgcn_fdot2_f32_bf16(by, one, sum[jj], false);
                 *reinterpret_cast<__attribute__((address_space(3))) uint64_t*>(
                     buf + n * G::ROWB + (((4 * db + jj) ^ G::swz(n & 15)) << 4) + 8 * hh) =
-                    (uint64_t)__builtin_bit_cast(uint32_t, __builtin_convertvector(y, bf16x2_t)) << 32 |
-                    __builtin_bit_cast(uint32_t, __builtin_convertvector(x, bf16x2_t));
+                    (uint64_t)__builtin_bit_cast(uint32_t, by) << 32 | __builtin_bit_cast(uint32_t, bx);
             }
+        const uint64_t bad = __ballot(q0 + n < L && !(fabsf((sum[0] + sum[1]) + (sum[2] + sum[3])) < INFINITY));
+        const uint32_t anew = (uint32_t)bad | (uint32_t)(bad >> 32);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // a wave's own part: no barrier
 #pragma unroll
         for (int i = 0; i < 32 / G::RPL; ++i) {
             const int r = i * G::RPL + lane / G::CPR, ch = lane % G::CPR;
             const u32x4_t v = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(
                 buf + r * G::ROWB + ((ch ^ G::swz(r & 15)) << 4));
-            if (q0 + r < L) *reinterpret_cast<u32x4_t*>(head + (q0 + r) * row + 8 * ch) = v;
+            if (q0 + r < L && !(anew >> r & 1)) *reinterpret_cast<u32x4_t*>(head + (q0 + r) * row + 8 * ch) = v;
         }
+        return anew;
     }
 };
 
-// W waves: W / gh query blocks of 32 for each of gh heads.
+// W waves: W / gh query blocks of 32 for each of gh heads.  Eight at D = 64: the registers
+// of four waves per SIMD, two workgroups of eight per CU.
 template <int D, int W>
-__global__ void __launch_bounds__(W * kWave) window_bf16_kernel(WindowArgs a) {
+__global__ void __launch_bounds__(W * kWave, W == 8 && D == 64 ? 4 : 1) window_bf16_kernel(WindowArgs a) {
     using G = BfGeo<D>;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     lds_u8_t* const smem = (lds_u8_t*)smem_raw;
@@ -382,7 +429,10 @@ __global__ void __launch_bounds__(W * kWave) window_bf16_kernel(WindowArgs a) {
     }
     for (; it < tiles.n; ++it) edge_tile(it);
     // The output through LDS, 32 rows per wave, so that stores are whole rows.
-    w.store(static_cast<uint16_t*>(a.dst) + wk.b * a.os[0] + h * a.os[1], a.os[2], a.L, smem + wave * 32 * G::ROWB, lane);
+    uint32_t anew = w.store(static_cast<uint16_t*>(a.dst) + wk.b * a.os[0] + h * a.os[1], a.os[2], a.L,
+                            smem + wave * 32 * G::ROWB, lane);
+    for (; anew; anew &= anew - 1)
+        window_plain<D, uint16_t>(wave / wph, w.q0 + __builtin_ctz(anew));
 }
 
 // ---------------------------------------------------------------- fp32
@@ -561,12 +611,15 @@ __global__ void __launch_bounds__(W * kWave) window_f32_kernel(WindowArgs a) {
         __syncthreads();
     }
 
-    const float inv = 1.0f / group_reduce<OpSum, 16, kWave>(l);
-    if (q0 + r16 < a.L) {
+    const float sum = group_reduce<OpSum, 16, kWave>(l + not_finite<G::DB>(acc)), inv = 1.0f / sum;
+    const bool fine = sum < INFINITY;
+    if (q0 + r16 < a.L && fine) {
         float* o = static_cast<float*>(a.dst) + wk.b * a.os[0] + h * a.os[1] + (long long)(q0 + r16) * a.os[2] + 4 * g;
 #pragma unroll
         for (int db = 0; db < G::DB; ++db) *reinterpret_cast<f32x4_t*>(o + 16 * db) = acc[db] * inv;
     }
+    for (uint32_t anew = __ballot(q0 + r16 < a.L && !fine) & 0xffff; anew; anew &= anew - 1)
+        window_plain<D, float>(wave / wph, q0 + __builtin_ctz(anew));
 }
 
 // ---------------------------------------------------------------- launch
@@ -660,7 +713,7 @@ extern "C" sa_status sa_prefill_window(const void* q, const void* k, const void*
     a.xcd_groups = groups % 8 == 0 ? (int)(groups / 8) : 0;
     // bf16: the sign goes to q, so that the scores' factor is not negative
     a.sl2 = (bf16 ? std::fabs(scale) : scale) * pf::kLog2eP;
-    a.q_sign = scale < 0 ? 0x80008000u : 0u;
+    a.q_sign = bf16 && scale < 0 ? 0x80008000u : 0u;
     return D == 64 ? dispatch_window<64>(a, bf16, batch, s, as_stream(stream))
                    : dispatch_window<128>(a, bf16, batch, s, as_stream(stream));
 }

@@ -177,3 +177,37 @@ def test_graph_replays_and_streams(sa, dtype):
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(other, want)
     del graph
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("B,Hq,Hkv,L,D,window,sink", [(1, 4, 2, 200, 64, 40, 3), (1, 4, 2, 200, 128, 40, 120),
+                                                      (40, 16, 8, 200, 64, 1000, 0), (9, 16, 8, 460, 128, 150, 4)])
+def test_not_finite(sa, dtype, B, Hq, Hkv, L, D, window, sink):
+    """NaN and infinite keys and values, a padded tail among them: queries that do
+    not see them are untouched, others get what the formula makes of them."""
+    q, k, v = tensors(dtype, B, Hq, Hkv, L, D, 12)
+    k[:, :, L - 30:], v[:, :, L - 30:] = float("nan"), float("nan")      # padding behind the prompts
+    v[:, :, 20, 3], v[:, :, 70, 5] = float("inf"), -float("inf")
+    v[:, :, 100, 7], v[:, :, 101, 7] = float("inf"), -float("inf")       # NaN for who sees both
+    v[:, :, 130, 9] = float("nan")
+    k[:, :, 110, 0] = float("inf")                                       # a weight of 0, or NaN, by the sign of q
+    i, j = torch.arange(L, device="cuda")[:, None], torch.arange(L, device="cuda")[None]
+    unseen = (j > i) | ((i - j >= window) & (j >= sink))
+    before = [t.clone() for t in (q, k, v)]
+    got = sa.prefill_window(q, k, v, 0.1, window, sink)
+    for b, h in {(0, 0), (B - 1, Hq - 1), (B // 2, Hq // 2)}:
+        s = (q[b, h].double() @ k[b, h * Hkv // Hq].double().T * 0.1).masked_fill(unseen, float("-inf"))
+        p = torch.softmax(s, -1)
+        vd = v[b, h * Hkv // Hq].double()
+        want, mag = torch.empty(L, D, device="cuda", dtype=torch.float64), torch.empty(L, D, device="cuda", dtype=torch.float64)
+        for r in range(L):
+            see = ~unseen[r]
+            want[r], mag[r] = p[r][see] @ vd[see], p[r][see] @ vd[see].abs()
+        g = got[b, h].double()
+        for kind in (torch.isnan, torch.isposinf, torch.isneginf):
+            assert torch.equal(kind(g), kind(want)), (kind, (kind(g) != kind(want)).nonzero()[:4].tolist())
+        fine = torch.isfinite(want)
+        assert fine[:20].all() and not fine[L - 30:].any()
+        bound = 1e-4 + (0.0 if dtype == "f32" else 2.0 ** -8 * mag + 2.0 ** -9 * want.abs())
+        assert ((g - want).abs() <= bound)[fine].all()
+    assert all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip((q, k, v), before))
