@@ -500,7 +500,12 @@ sa_status sa_axpby_f32(const float* x, float a, const float* y, float b, size_t 
  * A continuation of probability 0 (logit -inf) is never selected, nor one of
  * a beam whose score is -inf (beams not yet begun) or NaN or whose normaliser
  * is not finite (a NaN or +inf among its logits, or nothing but -inf).  Places
- * left over hold -inf, -1 and -1.  The order is decided in 64 bits.
+ * left over hold -inf, -1 and -1.  c is formed and the order decided in 64 bits,
+ * from normalisers whose sums of exponentials are fp32 (each off by some 1e-7):
+ * candidates of different beams that lie closer may come in either order.  Mask
+ * tokens with -inf: a finite stand-in as large as fp32's lowest value works beside
+ * other logits, but in a row that holds nothing else it leaves no digits for the
+ * normaliser and the score (c = 0), and a c below fp32's range is never selected.
  * n_beams and n_select 1 .. 64, n_beams * vocab < 2^31, n_groups at most 2^20
  * and n_groups * n_beams * ceil(vocab / 2048) below 2^24.  out_scores may be
  * scores itself where n_select == n_beams or n_groups == 1, since each search

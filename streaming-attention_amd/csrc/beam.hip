@@ -5,14 +5,16 @@
 //
 // Two launches.  The first streams the logits once: every row is cut into
 // segments, and each leaves its largest logit and its sum of exponentials
-// relative to it (fp32, at most 64 VPT values a sum).  The second, a workgroup
+// relative to it (fp32, at most 512 values a sum; longer segments are joined in 64
+// bits).  The second, a workgroup
 // per group, joins the sums in 64 bits and selects.  c is non-decreasing in x,
 // so with tau a value that at least n_select segment maxima reach, only
 // segments whose maximum reaches tau hold candidates, and only their elements
 // that reach tau are candidates: a few dozen, put in order by counting for
 // each how many precede it.  Comparisons with tau are in fp32 (rounding is
-// monotone, so nothing is lost); the order is decided in 64 bits, since
-// candidates of different beams may lie closer than fp32 sums are exact.
+// monotone, so nothing is lost); the order is decided in 64 bits, so that a beam's
+// own candidates keep theirs.  Those of different beams are apart by their
+// normalisers' errors too.
 // Where equal maxima make the lists overflow, the selection goes in n_select
 // rounds over (c, index) instead.
 //
@@ -65,10 +67,33 @@ __device__ __forceinline__ float exp_diff(float d) {
     return __builtin_amdgcn_exp2f(fmaf(d, 1.44269502162933349609f, d * 1.92596299112661746887e-8f));
 }
 
+// The sum over a wave, in 64 bits: lane exchanges inside 16 lanes with DPP
+// (after each step groups are uniform, so the mirrors act as xor 4 and 8), then
+// halves of 32 and of the wave.
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t u = __double_as_longlong(v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
+    return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+__device__ __forceinline__ double wave_sum_f64(double v) {
+    v += dpp_f64<kDppXor1>(v);
+    v += dpp_f64<kDppXor2>(v);
+    v += dpp_f64<kDppHalfMirror>(v);
+    v += dpp_f64<kDppMirror>(v);
+    v += __shfl_xor(v, 16, kWave);
+    v += __shfl_xor(v, 32, kWave);
+    return v;
+}
+
 // A wave takes `steps` steps of kBlock consecutive elements of a row, four
 // neighbouring ones per lane and load (VEC: rows start 16-byte aligned, else
 // four loads).  VPT < 8: the 64 VPT elements of 16 VPT lanes are a segment, so
-// one reduction serves all segments of a load; VPT = 8: the wave's steps are one.
+// one reduction serves all segments of a load; VPT = 8: the wave's steps are one,
+// whose maxima and sums the lanes keep, a step each, until 64 of them are joined
+// in 64 bits (a running fp32 sum, rescaled at each step, would carry an error of
+// its own per step).
 template <int VPT, bool VEC>
 __global__ void __launch_bounds__(256) beam_scan_kernel(BeamArgs a) {
     constexpr int LANES = VPT < 4 ? 16 * VPT : kWave;   // lanes of a segment
@@ -79,7 +104,8 @@ __global__ void __launch_bounds__(256) beam_scan_kernel(BeamArgs a) {
     const long long first = (long long)block * a.steps * kBlock;
     if (first >= a.vocab) return;
     const float* x = a.logits + (long long)row * a.row_stride;
-    float m_run = kNone, l_run = 0.f;
+    float m_run = kNone, m_of = kNone, l_of = 0.f;   // m_of, l_of: this lane's step
+    double l_run = 0.0;
     for (int s = 0; s < a.steps; ++s) {
         const long long at = first + (long long)s * kBlock;
         float v[2][4];
@@ -111,35 +137,28 @@ __global__ void __launch_bounds__(256) beam_scan_kernel(BeamArgs a) {
                 const long long seg = (at + g * 4 * kWave + 4 * lane) / (kWave * VPT);
                 if (lane % LANES == 0 && seg < a.n_seg) a.seg[(long long)row * a.n_seg + seg] = make_float2(m, l);
             } else {
-                const float mn = fmaxf(m_run, m);
-                l_run = (m_run == kNone ? l_run : l_run * exp_diff(m_run - mn)) + (m == kNone ? l : l * exp_diff(m - mn));
-                m_run = mn;
+                if (a.steps == 1) {
+                    m_run = m;
+                    l_run = l;
+                    continue;
+                }
+                if (lane == s % kWave) {
+                    m_of = m;
+                    l_of = l;
+                }
+                if ((s + 1) % kWave && s + 1 < a.steps) continue;
+                const float top = fmaxf(m_run, group_reduce<OpMax, 1, kWave>(m_of));
+                const double sum = wave_sum_f64(m_of == kNone ? (double)l_of : (double)l_of * (double)exp_diff(m_of - top));
+                l_run = (m_run == kNone ? l_run : l_run * (double)exp_diff(m_run - top)) + sum;
+                m_run = top;
+                m_of = kNone;
+                l_of = 0.f;
             }
         }
     }
     if constexpr (VPT == 8) {
-        if (lane == 0) a.seg[(long long)row * a.n_seg + block] = make_float2(m_run, l_run);
+        if (lane == 0) a.seg[(long long)row * a.n_seg + block] = make_float2(m_run, (float)l_run);
     }
-}
-
-// The sum over a wave, in 64 bits: lane exchanges inside 16 lanes with DPP
-// (after each step groups are uniform, so the mirrors act as xor 4 and 8), then
-// halves of 32 and of the wave.
-template <int CTRL>
-__device__ __forceinline__ double dpp_f64(double v) {
-    const uint64_t u = __double_as_longlong(v);
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, false);
-    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
-    return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
-}
-__device__ __forceinline__ double wave_sum_f64(double v) {
-    v += dpp_f64<kDppXor1>(v);
-    v += dpp_f64<kDppXor2>(v);
-    v += dpp_f64<kDppHalfMirror>(v);
-    v += dpp_f64<kDppMirror>(v);
-    v += __shfl_xor(v, 16, kWave);
-    v += __shfl_xor(v, 32, kWave);
-    return v;
 }
 
 // Floats as unsigned integers of the same order (NaN aside), and back.

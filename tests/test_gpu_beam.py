@@ -190,3 +190,41 @@ def test_few_tokens_allowed(sa, B):
     check(sa, masked, s, 8)
     masked[1, B - 1, 40000] = math.nan
     check(sa, masked, s, 8)
+
+
+def test_sums_of_many_steps(sa):
+    """Segments of 128 steps alike, whose sums would round the same way again and
+    again.  Scores that take the normaliser away leave its error: the exponential's
+    argument below 1.5 (half a step, 4.2e-8 of the value) and result (2^-23), sums of
+    eight equal values (the four that are not exact round by at most (3 + 5 + 6 + 7) /
+    8 x 2^-24) and of lanes of which one differs (1 + 1/2 + .. + 1/32 x 2^-24), the
+    segment's sum to fp32 (2^-24) and its factor exp(-0.01) (result 2^-23, product
+    2^-24): 6.8e-7."""
+    B, V = 64, 1 << 23
+    u = torch.linspace(0.3, 1.0, B, dtype=torch.float32)
+    x = torch.empty(1, B, V, device="cuda")
+    x[0] = -u.cuda()[:, None]
+    x[0, :, ::512] = 0
+    x[0, :, 0] = 0.01
+    most = x[0, 0, 0].double().item()
+    lse = torch.log(math.exp(most) + (V // 512 - 1) + (V - V // 512) * torch.exp(-u.double()))
+    scores = lse.float()
+    c, t, b = sa.beam_select(x, scores.cuda()[None], B)
+    assert (t == 0).all() and sorted(b[0].tolist()) == list(range(B))
+    want = (most + scores.double() - lse)[b[0].cpu().long()]
+    assert (c[0].cpu().double() - want).abs().max().item() <= 6.8e-7 + 2.0 ** -24 * 0.02
+
+
+@pytest.mark.parametrize("B,V", [(64, 300001), (64, 4500000), (33, 1000003)])
+def test_steps_that_rise(sa, B, V):
+    """Every step of a segment has a larger maximum than those before it, or a
+    smaller one."""
+    gen = torch.Generator(device="cuda").manual_seed(V)
+    x = torch.randn(1, B, V, device="cuda", generator=gen) * 0.1 + torch.linspace(0, 5, V, device="cuda")
+    s = -torch.rand(1, B, device="cuda", generator=gen)
+    for logits in (x, x.flip(-1).contiguous()):
+        c, t, b = sa.beam_select(logits, s, 16)
+        lp = torch.log_softmax(logits[0].double(), -1) + s[0].double()[:, None]
+        best, at = torch.topk(lp.view(-1), 16)
+        assert torch.equal(b[0].long() * V + t[0].long(), at)
+        assert ((c[0].double() - best).abs() <= 2.4e-7 + 2.0 ** -24 * best.abs()).all()
