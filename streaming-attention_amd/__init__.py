@@ -802,13 +802,22 @@ class Qwen3:
         tokens), best first.  Ends for a prompt when n_beams ended continuations
         score above its running ones.  Up to 64 beams; a step offers min(2 *
         n_beams, 64) continuations, so with more than 32 beams fewer may run on
-        where some end.  The cache holds the last beams afterwards: reset it."""
+        where some end.  A search that the model's rows and positions or a row's
+        pages have no room for is refused (ValueError) before it begins, whether or
+        not eos might end it in time; a pool that runs out of pages ends it with an
+        SaError.  The cache holds the last beams afterwards: reset it."""
         import torch
         if not 1 <= n_beams <= 64 or n_tokens < 1:
             raise ValueError("beam_search takes 1 to 64 beams and at least one token")
         G, L = prompts.shape
         if G * n_beams > cache.desc.max_seqs:
             raise ValueError("the cache needs a row per beam")
+        if G * n_beams > self.max_batch:
+            raise ValueError("the model has fewer rows than there are beams")
+        if L + n_tokens - 1 > self.desc.max_pos:      # the last token is not appended
+            raise ValueError("prompt and tokens need more positions than the model's max_pos")
+        if L + n_tokens - 1 > cache.desc.max_pages_per_seq * PAGE_TOKENS:
+            raise ValueError("prompt and tokens need more pages than a row of the cache can list")
         B, dev = n_beams, prompts.device
         n_select = min(2 * B, 64)
         for g in range(G):

@@ -52,6 +52,32 @@ def test_beam_search_arguments(sa):
             model.beam_search(None, None, beams, tokens)
 
 
+def test_beam_searches_that_cannot_end(sa):
+    """More beams than the model's rows, or more tokens than its positions or the
+    cache's pages: refused with the cache untouched."""
+    import torch
+
+    class Cache:
+        desc = sa.KvDesc(1, 1, 64, 16, 4, 64, sa.SA_DTYPE_F32)
+
+        def __getattr__(self, name):
+            raise RuntimeError(f"the cache was touched: {name}")
+
+    model = sa.Qwen3.__new__(sa.Qwen3)
+    model.handle, model.max_batch = None, 8
+    for max_pos, G, L, B, n, why in ((1000, 2, 10, 5, 3, "rows"), (1000, 3, 10, 6, 3, "row per beam"),
+                                     (50, 1, 30, 4, 22, "positions"), (1000, 1, 200, 4, 58, "pages"),
+                                     (300, 1, 300, 1, 1, "pages")):
+        model.desc = sa.Qwen3Desc(1, 64, 64, 64, 1, 1, 64, max_pos, 1e-6, 1e6)
+        for eos in (None, 3):
+            with pytest.raises(ValueError, match=why):
+                model.beam_search(Cache(), torch.zeros(G, L, dtype=torch.int32), B, n, eos)
+    for max_pos, L, n in ((51, 30, 22), (1000, 200, 57)):       # the last that fit reach the cache
+        model.desc = sa.Qwen3Desc(1, 64, 64, 64, 1, 1, 64, max_pos, 1e-6, 1e6)
+        with pytest.raises(RuntimeError, match="touched"):
+            model.beam_search(Cache(), torch.zeros(1, L, dtype=torch.int32), 4, n)
+
+
 def test_scores_in_place_where_searches_would_meet(sa):
     """Searches run side by side: results of one may not fall on scores that
     another has yet to read.  (A workspace too small is what the calls that may
