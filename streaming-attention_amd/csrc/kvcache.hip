@@ -160,18 +160,25 @@ __global__ void __launch_bounds__(256) update_rows_kernel(RowsArgs a) {
 // The device side of what fork and reorder decided for rows[0, n): `before`
 // holds each row's table entries as they were.  like: the row whose first
 // `alike` entries the one row of a fork has, which the device copies itself.
+// Nothing is allocated: the page table has changed already, and the device's has
+// to follow.
 sa_status publish_rows(sa_kvcache* c, const std::vector<int32_t>& rows,
                        const std::vector<std::vector<int32_t>>& before, const std::vector<PageCopy>& copies,
                        hipStream_t st, int like = 0, int alike = 0) {
-    std::vector<TableEdit> edits;
-    for (size_t i = 0; i < rows.size(); ++i) {
-        const int32_t* now = c->pt.row(rows[i]);
-        const int old_n = (int)before[i].size(), n = std::max(old_n, c->pt.npages(rows[i]));
-        for (int j = alike; j < n; ++j)
-            if (now[j] != (j < old_n ? before[i][j] : -1)) edits.push_back(TableEdit{rows[i], j, now[j]});
-    }
-    size_t e = 0, l = 0, k = 0;   // a changed row has a length to publish: one launch at least
-    while (e < edits.size() || l < rows.size() || k < copies.size()) {
+    // The next entry that changes: column ej of row ei (ei = rows.size(): none).
+    size_t ei = 0;
+    int ej = alike;
+    auto seek = [&]() {
+        for (; ei < rows.size(); ++ei, ej = alike) {
+            const int32_t* now = c->pt.row(rows[ei]);
+            const int old_n = (int)before[ei].size(), n = std::max(old_n, c->pt.npages(rows[ei]));
+            for (; ej < n; ++ej)
+                if (now[ej] != (ej < old_n ? before[ei][ej] : -1)) return;
+        }
+    };
+    seek();
+    size_t l = 0, k = 0;   // a changed row has a length to publish: one launch at least
+    while (ei < rows.size() || l < rows.size() || k < copies.size()) {
         RowsArgs a{};
         a.table = c->d_table; a.lens = c->d_lens; a.pool = c->pool; a.layer_bytes = c->layer_bytes;
         a.max_pages = c->desc.max_pages_per_seq; a.n_kv = c->desc.num_kv_heads;
@@ -180,7 +187,8 @@ sa_status publish_rows(sa_kvcache* c, const std::vector<int32_t>& rows,
         if (l == 0 && alike > 0) {
             a.like_dst = rows[0]; a.like_src = like; a.like_n = alike;
         }
-        for (; a.n_edits < kEdits && e < edits.size(); ++e) a.edit[a.n_edits++] = edits[e];
+        for (; a.n_edits < kEdits && ei < rows.size(); ++ej, seek())
+            a.edit[a.n_edits++] = TableEdit{rows[ei], ej, c->pt.row(rows[ei])[ej]};
         for (; a.n_lens < kRowsPerLaunch && l < rows.size(); ++l) {
             a.len_row[a.n_lens] = rows[l];
             a.len[a.n_lens++] = c->pt.len(rows[l]);
