@@ -129,7 +129,8 @@ sa_status sa_qwen3_prefill(sa_qwen3* model, sa_kvcache* cache, const int32_t* to
  * outside [0, vocab) embed as zeros.  Asynchronous on stream; the first call
  * with a given cache geometry allocates the attention workspace.  Workspaces
  * that are outgrown live until the model is destroyed, so that a graph that
- * captured a step stays valid after a larger one. */
+ * captured a step stays valid after a larger one.  A model has one set of
+ * activations and workspaces: calls and replays that overlap race. */
 sa_status sa_qwen3_decode_step(sa_qwen3* model, sa_kvcache* cache, const int32_t* tokens, int batch,
                                int32_t* next_tokens, float* logits, sa_stream_t stream);
 

@@ -60,6 +60,9 @@ struct PlainRow {
     float m = -INFINITY, l = 0.f;
     float o[E] = {};
 
+    // A NaN among the weights makes one of every column, whatever else there is.
+    __device__ __forceinline__ bool lost() const { return l != l; }
+
     // n keys (1 .. 64), lane i's score is that of key i: c sum_d q[d] key(i)[d].
     // key(i), value(i): where key or value i starts, for i < n.
     template <class T, class Key, class Value>

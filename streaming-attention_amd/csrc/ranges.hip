@@ -549,7 +549,7 @@ __device__ __forceinline__ void attend_plain(const RangeArgs& a, const Item& it,
     const int r = row_of(a, j), head = it.kvh * a.rep + j - r * a.rep;
     const size_t row = ((size_t)(it.row0 + r) * a.n_q + head) * D;
     PlainRow<D> p;
-    for (int u = it.u0; u < it.u1; ++u) {
+    for (int u = it.u0; u < it.u1 && !p.lost(); ++u) {
         const TileSpan sp = tile_span(it.src, u);
         const size_t at = (((size_t)pages[u - it.u0] * a.n_kv + it.kvh) * SA_PAGE_TOKENS + (sp.lo & (SA_PAGE_TOKENS - 1))) * D;
         p.keys(sp.hi - sp.lo, a.q + row, a.sl2,

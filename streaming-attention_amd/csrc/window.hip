@@ -96,7 +96,7 @@ __device__ __forceinline__ void window_plain(int dh, int row) {
     const int from = max(0, row - a.window + 1);
     PlainRow<D> p;
     auto span = [&](int k0, int k1) {
-        for (int k = k0; k < k1; k += kWave)
+        for (int k = k0; k < k1 && !p.lost(); k += kWave)
             p.keys(min(kWave, k1 - k), Q + row * a.qs[2], factor, [&](int i) { return K + (k + i) * a.kvs[2]; },
                    [&](int i) { return V + (k + i) * a.kvs[2]; });
     };
