@@ -8,8 +8,9 @@
 // NaN never leaves them) and computes the rows that are not finite anew here,
 // over the keys that the row sees and no others.  Ordinary rows pay for the look
 // alone, an FMA per accumulator (decode over ranges, 16 / 8 heads of 128: 4 x 4 rows
-// in fp32 20.9 -> 21.0 us, 64 rows behind 32768 shared tokens 74.4 -> 74.6; the
-// latter with NaN in every row 6.4 ms).
+// in fp32 20.7 -> 20.8 us, one row 10.7 -> 10.9, 64 rows behind 32768 shared tokens
+// 75.3 -> 75.4; windowed prefill of 3 x 777 in bf16 10.3 -> 10.4, of 8192 86.5 as
+// before).  Rows computed anew: 64 behind 32768 tokens, all values NaN, 6.4 ms.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -32,7 +32,7 @@
 //
 // Bound, 16 / 8 heads of 128: HBM for many rows (64 rows, window 4096 and 4 sinks,
 // bf16: 992 MB in 157 us, 6.3 TB/s); the products and the softmax between for many
-// rows behind one prefix (64 behind 32768 tokens, bf16: 73 us, MFMA 41 % and VALU
+// rows behind one prefix (64 behind 32768 tokens, bf16: 75 us, MFMA 42 % and VALU
 // 45 % busy; loads alone 55, computing alone 66, of both 15 for launches, queries
 // and partials); the latency of the tiles for few rows (4 x 4 beams, fp32: 19.4 us,
 // 2.65 per tile of a wave; 4 rows behind 512 tokens, bf16: 9.0).

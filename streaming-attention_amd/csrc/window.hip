@@ -26,10 +26,12 @@
 // the keys that they see (plain_row.h).
 //
 // Bound: MFMA, with the softmax between.  16 / 8 heads of 128: 8192 queries,
-// window 1024, 4 sinks, bf16 86.9 us (64.7 GF of visible products, 0.74 PFLOP/s;
-// MFMA alone at a large product's rate 53); 2048 queries, window 512, fp32 54.8
-// us (7.6 GF, six products each: 0.83 PFLOP/s; 37); 3 prompts of 777, window 200,
-// 16 / 4 heads of 64, bf16 10.2 us, a launch and a wave's chain of five tiles.
+// window 1024, 4 sinks, bf16 87 us (64.7 GF of visible products, 0.74 PFLOP/s;
+// at a large product's rate 40): two rounds of a workgroup per CU, whose queries,
+// first tile and stores nothing covers.  2048 queries, window 512, fp32 54.6 us (7.6
+// GF, six products each: 0.83 PFLOP/s; 28): every key is split by each query tile
+// that sees it.  3 prompts of 777, window 200, 16 / 4 heads of 64, bf16 10.4 us: a
+// launch and a wave's chain of five tiles.
 #include <algorithm>
 #include <cmath>
 
@@ -625,9 +627,9 @@ __global__ void __launch_bounds__(W * kWave) window_f32_kernel(WindowArgs a) {
 // ---------------------------------------------------------------- launch
 
 // Waves per workgroup, the heads it serves and its query tile: eight waves where
-// that fills the CUs (8192 queries, bf16, 512 workgroups: 86.9 us against 92.5 in
-// workgroups of four; 2048, fp32, 256: 54.8 against 83.5), else four (3 x 777, bf16,
-// 300 against 156: 10.2 us against 13.1 in eight).
+// that fills the CUs (8192 queries, bf16, 512 workgroups: 87 us against 92.5 in
+// workgroups of four; 2048, fp32, 256: 54.6 against 83.5), else four (3 x 777, bf16,
+// 300 against 156: 10.4 us against 13.1 in eight).
 struct WindowShape {
     int waves, gh, q_tile;
 };
