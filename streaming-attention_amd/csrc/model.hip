@@ -1042,7 +1042,11 @@ sa_status decode_rows(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int
 extern "C" sa_status sa_qwen3_decode_step(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int batch,
                                           int32_t* next_tokens, float* logits, sa_stream_t stream) {
     clear_error();
-    return decode_rows(m, cache, tokens, batch, nullptr, next_tokens, logits, stream);
+    try {
+        return decode_rows(m, cache, tokens, batch, nullptr, next_tokens, logits, stream);
+    } catch (const std::bad_alloc&) {
+        return fail(SA_ENOMEM, "out of host memory");
+    }
 }
 
 extern "C" sa_status sa_qwen3_beam_step(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int n_groups,
