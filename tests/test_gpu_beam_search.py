@@ -287,3 +287,31 @@ def test_head_ratios(sa, Hq, Hkv, P):
     for c in (cache, anew):
         c.close()
     model.close()
+
+
+def test_step_in_place(sa):
+    """A step whose results take the scores' place."""
+    model = make_model(sa, 6, 100, 10)
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    tokens = torch.randint(0, SMALL["vocab"], (2, 3), dtype=torch.int32, device="cuda", generator=gen)
+    got = []
+    for apart in (True, False):
+        cache = make_cache(sa, 6, 64, sa.SA_DTYPE_F32)
+        for r in range(6):
+            cache.reserve(r, 21)
+        model.prefill(cache, torch.arange(120, dtype=torch.int32, device="cuda").view(6, 20))
+        scores = torch.tensor([[-1.0, -2.0, -0.5], [-3.0, -0.1, -2.5]], device="cuda")
+        out = (torch.empty(2, 3, device="cuda") if apart else scores,
+               *(torch.empty(2, 3, dtype=torch.int32, device="cuda") for _ in range(2)))
+        model.beam_step(cache, tokens, scores, 3, out=out)
+        got.append(out)
+        torch.cuda.synchronize()
+        if not apart:
+            with pytest.raises(RuntimeError, match="out_scores"):
+                wide = torch.zeros(12, device="cuda")
+                model.beam_step(cache, tokens, wide[:6].view(2, 3), 6,
+                                out=(wide.view(2, 6), *(torch.empty(2, 6, dtype=torch.int32, device="cuda") for _ in range(2))))
+            assert [cache.length(r) for r in range(6)] == [21] * 6
+        cache.close()
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+    model.close()

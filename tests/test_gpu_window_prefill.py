@@ -211,3 +211,31 @@ def test_not_finite(sa, dtype, B, Hq, Hkv, L, D, window, sink):
         bound = 1e-4 + (0.0 if dtype == "f32" else 2.0 ** -8 * mag + 2.0 ** -9 * want.abs())
         assert ((g - want).abs() <= bound)[fine].all()
     assert all(torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) for a, b in zip((q, k, v), before))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("D", [64, 128])
+def test_not_finite_in_views(sa, dtype, D):
+    """The same through token-major views, a negative scale and a padded output,
+    whose other places stay as they are: every query sees an infinite value, so
+    that all of its columns are computed anew."""
+    B, L, Hq, Hkv, window, sink, scale = 3, 210, 4, 2, 50, 2, -0.1
+    gen = torch.Generator(device="cuda").manual_seed(13)
+    x = torch.randn(B, L, Hq + 2 * Hkv, D, device="cuda", generator=gen).to(DT[dtype])
+    q, k, v = (t.transpose(1, 2) for t in x.split([Hq, Hkv, Hkv], 2))
+    v[:, :, 0, 11] = float("inf")                      # a sink
+    buf = torch.full((B, L, Hq + 1, D + 64), 5.0, device="cuda", dtype=DT[dtype])
+    out = buf[:, :, :Hq, :D].transpose(1, 2)
+    got = sa.prefill_window(q, k, v, scale, window, sink, out=out)
+    assert torch.isposinf(got[..., 11]).all()
+    rest = [c for c in range(D) if c != 11]
+    clean = v.clone()
+    clean[:, :, 0, 11] = 0
+    want, mag = reference(q, k, clean, scale, window, sink)
+    compare(got[..., rest], want[..., rest], mag[..., rest])
+    assert (buf[:, :, Hq] == 5).all() and (buf[:, :, :, D:] == 5).all()
+    k1, v1 = (t[:1].expand(B, -1, -1, -1) for t in (k, v))
+    want, mag = reference(q, k1, clean[:1].expand(B, -1, -1, -1), scale, window, sink)
+    got = sa.prefill_window(q, k1, v1, scale, window, sink)
+    assert torch.isposinf(got[..., 11]).all()
+    compare(got[..., rest], want[..., rest], mag[..., rest])
