@@ -40,7 +40,8 @@ typedef enum sa_status {
 
 typedef enum sa_dtype {
     SA_DTYPE_F32 = 0,
-    SA_DTYPE_BF16 = 1
+    SA_DTYPE_BF16 = 1,
+    SA_DTYPE_FP8 = 2   /* KV caches only: e4m3 codes with a scale per row (sa_kv_desc) */
 } sa_dtype;
 
 typedef void* sa_stream_t;   /* a hipStream_t */
@@ -128,6 +129,19 @@ typedef struct sa_kv_desc {
     sa_dtype kv_dtype;
 } sa_kv_desc;
 
+/* Caches in 8 bits (kv_dtype SA_DTYPE_FP8; no counterpart in the reference),
+ * head_dim 64 or 128.  Every row (the key or value of one token and KV head) is
+ * quantised as it is appended: codes in e4m3 (OCP: 3 mantissa bits, largest
+ * magnitude 448, no infinity) and one scale 2^e, e the smallest from -100 on with
+ * max |x| <= 448 2^e over the row's finite values; an element becomes the code
+ * nearest to x 2^-e, ties to even.  What the row holds from then on is code 2^e,
+ * within 2^-4 of x relative to it, or 2^(e - 10) where |x| < 2^(e - 6); infinities
+ * and NaN become NaN, and magnitudes above 1.9375 2^127 become 1.875 2^127.
+ * Reading back (sa_kvcache_gather) and attending are exact in what is held.
+ * Codes: pools of [num_pages][num_kv_heads][64][head_dim] bytes
+ * (sa_kvcache_k_pool); scales: e + 127, a byte per row,
+ * [num_pages][num_kv_heads][64] (sa_kvcache_k_scales). */
+
 typedef struct sa_kvcache sa_kvcache;
 
 sa_status sa_kvcache_create(const sa_kv_desc* desc, sa_kvcache** out);
@@ -145,6 +159,12 @@ sa_status sa_kvcache_set_pages(sa_kvcache* cache, int seq, const int32_t* pages,
                                int n_pages, sa_stream_t stream);
 /* Set the committed length of seq (host and device), within its reserved pages. */
 sa_status sa_kvcache_set_len(sa_kvcache* cache, int seq, int len, sa_stream_t stream);
+/* The same for rows seqs[0..n) (host ids, each at most once) and lengths lens[0..n)
+ * at once, one launch per 64 rows; refused as a whole.  What is behind a length
+ * that moves back is overwritten by later appends (drafted tokens that were not
+ * accepted). */
+sa_status sa_kvcache_set_lens(sa_kvcache* cache, const int32_t* seqs, const int32_t* lens, int n,
+                              sa_stream_t stream);
 /* Committed length of seq as tracked on the host, or -1. */
 int sa_kvcache_len(const sa_kvcache* cache, int seq);
 /* Tokens the pages assigned to seq can hold (64 per page), or -1.  No
@@ -189,6 +209,9 @@ sa_status sa_kvcache_reorder(sa_kvcache* cache, const int32_t* rows, const int32
 /* Device pointers into the cache, for callers that drive kernels themselves. */
 void* sa_kvcache_k_pool(sa_kvcache* cache, int layer);
 void* sa_kvcache_v_pool(sa_kvcache* cache, int layer);
+/* Scales of a cache in 8 bits (NULL for others): a byte per row. */
+uint8_t* sa_kvcache_k_scales(sa_kvcache* cache, int layer);
+uint8_t* sa_kvcache_v_scales(sa_kvcache* cache, int layer);
 int32_t* sa_kvcache_block_table(sa_kvcache* cache);   /* [max_seqs][max_pages_per_seq] */
 int32_t* sa_kvcache_seq_lens(sa_kvcache* cache);      /* [max_seqs] committed lengths */
 size_t sa_kvcache_bytes(const sa_kvcache* cache);
@@ -228,6 +251,17 @@ sa_status sa_qknorm_rope_append(sa_kvcache* cache, int layer,
                                 const float* q_norm_w, const float* k_norm_w, float eps,
                                 const float* rope_cos, const float* rope_sin, int rope_max_pos,
                                 float* q_out, sa_stream_t stream);
+
+/* The same with counts[i] >= 0 new tokens of sequence i (host array [n_seq];
+ * sequences of 0 are left alone): q, k and v hold the sequences' tokens one behind
+ * the other, [sum counts][heads][D].  No counterpart in the reference, whose
+ * batches have one length. */
+sa_status sa_qknorm_rope_append_ragged(sa_kvcache* cache, int layer,
+                                       const float* q, const float* k, const float* v,
+                                       int n_seq, const int32_t* counts, const int32_t* seq_ids, int n_q_heads,
+                                       const float* q_norm_w, const float* k_norm_w, float eps,
+                                       const float* rope_cos, const float* rope_sin, int rope_max_pos,
+                                       float* q_out, sa_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * Per-row RMSNorm + rotate-half RoPE without a cache.
@@ -320,6 +354,32 @@ sa_status sa_paged_decode_shared(const sa_kvcache* cache, int layer, const float
                                  int n_seq, const int32_t* seq_ids, const int32_t* group_sizes, int n_groups,
                                  int n_q_heads, int n_pending, float scale, float* out,
                                  void* ws, size_t ws_bytes, sa_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Attention of a chunk of new tokens over a paged cache.
+ *
+ * No counterpart in the reference, whose prompts start on an empty cache.
+ * Sequence i has counts[i] >= 0 new tokens (host array [n_seq]) at positions len
+ * .. len + counts[i] - 1, len its committed length; they have been appended and
+ * not committed, so every row has pages for them (SA_ERANGE otherwise).  New
+ * token j attends over what came before it and itself:
+ *   out_ij = softmax(scale q_ij k_t) v_t over t <= len + j.
+ * q and out [sum counts][n_q_heads][D], the sequences' tokens one behind the
+ * other, both in q_dtype: fp32 with any cache, accurate to fp32; bf16 with a bf16
+ * or 8-bit cache, where large chunks take products of bf16 operands (weights
+ * rounded to bf16) with fp32 sums and softmax.  seq_ids: host array [n_seq] of
+ * cache rows or NULL for 0..n_seq-1; a row may be listed more than once.  head_dim 64 or 128, at
+ * most 64 query heads per KV head, at most 2^20 new tokens.  What a token does not see does not reach it,
+ * NaN and infinities included; rows whose tiles hold such values take longer.
+ * q, out and ws 16-byte aligned; out must not overlap q.  ws:
+ * sa_paged_extend_ws_bytes bytes, enough for any lengths of the same counts;
+ * calls that overlap on one workspace race.  The tokens are those of the lengths
+ * at the call, also where a graph that holds the call is replayed.
+ * ------------------------------------------------------------------------ */
+size_t sa_paged_extend_ws_bytes(const sa_kvcache* cache, int n_seq, const int32_t* counts, int n_q_heads);
+sa_status sa_paged_extend(const sa_kvcache* cache, int layer, const void* q, sa_dtype q_dtype,
+                          int n_seq, const int32_t* seq_ids, const int32_t* counts, int n_q_heads,
+                          float scale, void* out, void* ws, size_t ws_bytes, sa_stream_t stream);
 
 /* ------------------------------------------------------------------------
  * One decode step of a layer in one call: sa_qknorm_rope_append with S = 1,

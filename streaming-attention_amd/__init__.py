@@ -29,6 +29,7 @@ SA_ERANGE = -5
 SA_EIO = -6
 SA_DTYPE_F32 = 0
 SA_DTYPE_BF16 = 1
+SA_DTYPE_FP8 = 2       # KV caches: e4m3 codes with a power-of-two scale per row
 PAGE_TOKENS = 64
 
 _STATUS_NAMES = {0: "SA_OK", -1: "SA_EINVAL", -2: "SA_ENOMEM", -3: "SA_EFULL",
@@ -73,6 +74,7 @@ SIGNATURES = {
     "sa_kvcache_reserve": (_I, [_P, _I, _I, _P]),
     "sa_kvcache_set_pages": (_I, [_P, _I, _P, _I, _P]),
     "sa_kvcache_set_len": (_I, [_P, _I, _I, _P]),
+    "sa_kvcache_set_lens": (_I, [_P, _P, _P, _I, _P]),
     "sa_kvcache_len": (_I, [_P, _I]),
     "sa_kvcache_capacity": (_I, [_P, _I]),
     "sa_kvcache_commit": (_I, [_P, _P, _I, _I, _P]),
@@ -80,6 +82,8 @@ SIGNATURES = {
     "sa_kvcache_reorder": (_I, [_P, _P, _P, _I, _P]),
     "sa_kvcache_k_pool": (_P, [_P, _I]),
     "sa_kvcache_v_pool": (_P, [_P, _I]),
+    "sa_kvcache_k_scales": (_P, [_P, _I]),
+    "sa_kvcache_v_scales": (_P, [_P, _I]),
     "sa_kvcache_block_table": (_P, [_P]),
     "sa_kvcache_seq_lens": (_P, [_P]),
     "sa_kvcache_bytes": (_SZ, [_P]),
@@ -87,6 +91,7 @@ SIGNATURES = {
     "sa_rope_table_init": (_I, [_P, _P, _I, _I, _F, _P]),
     "sa_qknorm_rope_append": (_I, [_P, _I, _P, _P, _P, _I, _I, _P, _I, _P, _P, _F, _P, _P, _I,
                                    _P, _P]),
+    "sa_qknorm_rope_append_ragged": (_I, [_P, _I, _P, _P, _P, _I, _P, _P, _I, _P, _P, _F, _P, _P, _I, _P, _P]),
     "sa_qk_norm_rope": (_I, [_P, _I, _I, _P, _P, _F, _P, _P, _I, _P, _P]),
     "sa_qk_norm_rope_ex": (_I, [_P, _I, _I, _P, _P, _F, _I, _P, _P, _I, _P, _P]),
     "sa_linear_f32": (_I, [_P, _I, _I, _P, _I, _P, _P, _P]),
@@ -99,6 +104,8 @@ SIGNATURES = {
     "sa_paged_decode_window": (_I, [_P, _I, _P, _I, _P, _I, _I, _I, _I, _F, _P, _P, _SZ, _P]),
     "sa_paged_decode_shared_ws_bytes": (_SZ, [_P, _I, _I]),
     "sa_paged_decode_shared": (_I, [_P, _I, _P, _I, _P, _P, _I, _I, _I, _F, _P, _P, _SZ, _P]),
+    "sa_paged_extend_ws_bytes": (_SZ, [_P, _I, _P, _I]),
+    "sa_paged_extend": (_I, [_P, _I, _P, _I, _I, _P, _P, _I, _F, _P, _P, _SZ, _P]),
     "sa_append_decode_partials": (_I, [_P, _I, _P, _I, _I, _P, _I, _P, _P, _F, _P, _P, _I, _F, _P, _P, _P,
                                        _SZ, _I, _P]),
     "sa_kvcache_gather": (_I, [_P, _I, _I, _I, _P, _P, _P]),
@@ -269,7 +276,7 @@ def decode_dense(q, k, v, scale: float, out=None, ws=None, stream=None):
 # ---------------------------------------------------------------- KV cache
 
 class KVCache:
-    """Owner of an sa_kvcache handle (64-token pages, fp32 or bf16 storage)."""
+    """Owner of an sa_kvcache handle (64-token pages; fp32, bf16 or 8-bit storage)."""
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, max_seqs: int,
                  max_pages_per_seq: int, num_pages: int, kv_dtype: int = SA_DTYPE_F32):
@@ -302,6 +309,15 @@ class KVCache:
 
     def set_len(self, seq: int, n: int, stream=None) -> None:
         check(lib().sa_kvcache_set_len(self.handle, seq, n, _stream(stream)))
+
+    def set_lens(self, seqs, lens, stream=None) -> None:
+        """Committed lengths of several rows at once (host ints)."""
+        seqs = [int(r) for r in seqs]
+        lens = [int(n) for n in lens]
+        if len(lens) != len(seqs):
+            raise ValueError("set_lens takes a length per row")
+        check(lib().sa_kvcache_set_lens(self.handle, _rows(seqs, len(seqs)), _rows(lens, len(lens)), len(seqs),
+                                        _stream(stream)))
 
     def length(self, seq: int) -> int:
         return lib().sa_kvcache_len(self.handle, seq)
@@ -338,9 +354,13 @@ class KVCache:
         return lib().sa_kvcache_bytes(self.handle)
 
     def append(self, layer: int, q, k, v, q_norm_w=None, k_norm_w=None, eps: float = 1e-6,
-               rope=None, q_out=None, seq_ids=None, stream=None):
+               rope=None, q_out=None, seq_ids=None, stream=None, counts=None):
         """q [n, S, Hq, D] (or None), k/v [n, S, Hkv, D]; rope = (cos, sin) tables;
-        seq_ids: cache rows of the n sequences (host ints), or None for 0..n-1."""
+        seq_ids: cache rows of the n sequences (host ints), or None for 0..n-1.
+        counts: new tokens of each sequence (host ints); q [sum counts, Hq, D], k/v
+        [sum counts, Hkv, D] then hold them one behind the other."""
+        if counts is not None:
+            return self._append_ragged(layer, q, k, v, q_norm_w, k_norm_w, eps, rope, q_out, seq_ids, stream, counts)
         n_seq, S = k.shape[0], k.shape[1]
         Hq = 0 if q is None else q.shape[2]
         cos, sin = (None, None) if rope is None else rope
@@ -353,6 +373,65 @@ class KVCache:
             _rows(seq_ids, n_seq), Hq, _ptr(_f32(q_norm_w, "q_norm_w")), _ptr(_f32(k_norm_w, "k_norm_w")), eps,
             _ptr(cos), _ptr(sin), max_pos, _ptr(q_out), _stream(stream)))
         return q_out
+
+    def _append_ragged(self, layer, q, k, v, q_norm_w, k_norm_w, eps, rope, q_out, seq_ids, stream, counts):
+        counts = [int(n) for n in counts]
+        H, D, T = self.desc.num_kv_heads, self.desc.head_dim, sum(counts)
+        if tuple(k.shape) != (T, H, D) or k.shape != v.shape:
+            raise ValueError("k and v must be [sum counts, Hkv, head_dim]")
+        if q is not None and (q.dim() != 3 or q.shape[0] != T or q.shape[2] != D):
+            raise ValueError("q must be [sum counts, Hq, head_dim]")
+        if q is not None and q_out is None:
+            import torch
+            q_out = _alloc(stream, lambda: torch.empty_like(q))
+        if q is not None and q_out.shape != q.shape:
+            raise ValueError("q_out must have q's shape")
+        cos, sin = (None, None) if rope is None else rope
+        st = _on(stream, *(t for t in (q, k, v, q_norm_w, k_norm_w, cos, sin, q_out) if t is not None))
+        check(lib().sa_qknorm_rope_append_ragged(
+            self.handle, layer, _ptr(_f32(q, "q")), _ptr(_f32(k, "k")), _ptr(_f32(v, "v")), len(counts),
+            _rows(counts, len(counts)), _rows(seq_ids, len(counts)), 0 if q is None else q.shape[1],
+            _ptr(_f32(q_norm_w, "q_norm_w")), _ptr(_f32(k_norm_w, "k_norm_w")), eps, _ptr(_f32(cos, "cos")),
+            _ptr(_f32(sin, "sin")), 0 if rope is None else cos.shape[0], _ptr(_f32(q_out, "q_out")), st))
+        return q_out
+
+    def extend_ws_bytes(self, counts, n_q_heads: int) -> int:
+        counts = [int(n) for n in counts]
+        return lib().sa_paged_extend_ws_bytes(self.handle, len(counts), _rows(counts, len(counts)), n_q_heads)
+
+    def extend(self, layer: int, q, scale: float, counts=None, out=None, ws=None, seq_ids=None, stream=None):
+        """Attention of new tokens that have been appended and not committed, each over
+        what came before it and itself: q [sum counts, Hq, D], counts[i] tokens of
+        sequence i (host ints), or q [n, S, Hq, D] for S tokens of each; fp32, or bf16
+        with a bf16 or 8-bit cache -> out like q."""
+        import torch
+        if counts is None:
+            if q.dim() != 4:
+                raise ValueError("q must be [n, S, Hq, head_dim], or [sum counts, Hq, head_dim] with counts")
+            counts = [q.shape[1]] * q.shape[0]
+        else:
+            counts = [int(n) for n in counts]
+            if q.dim() != 3 or q.shape[0] != sum(counts):
+                raise ValueError("q must be [sum counts, Hq, head_dim]")
+        if q.dtype != torch.float32 and q.dtype != torch.bfloat16:
+            raise ValueError("q must be float32 or bfloat16")
+        if q.shape[-1] != self.desc.head_dim or not q.is_cuda or not q.is_contiguous():
+            raise ValueError("q must be a contiguous CUDA tensor of rows of head_dim")
+        if out is None:
+            out = _alloc(stream, lambda: torch.empty_like(q))
+        elif out.shape != q.shape or out.dtype != q.dtype or not out.is_cuda or not out.is_contiguous():
+            raise ValueError("out must be a contiguous CUDA tensor like q")
+        n, Hq = len(counts), q.shape[-2]
+        c_counts = _rows(counts, n)
+        if ws is None:
+            need = lib().sa_paged_extend_ws_bytes(self.handle, n, c_counts, Hq)
+            ws = _alloc(stream, lambda: torch.empty(max(need, 16), dtype=torch.uint8, device=q.device))
+        st = _on(stream, q, out, ws)
+        check(lib().sa_paged_extend(self.handle, layer, q.data_ptr(),
+                                    SA_DTYPE_F32 if q.dtype == torch.float32 else SA_DTYPE_BF16, n,
+                                    _rows(seq_ids, n), c_counts, Hq, scale, out.data_ptr(), ws.data_ptr(),
+                                    _nbytes(ws), st))
+        return out
 
     def decode_ws_bytes(self, n_seq: int, n_q_heads: int) -> int:
         return lib().sa_paged_decode_ws_bytes(self.handle, n_seq, n_q_heads)
@@ -878,6 +957,8 @@ def _device_view(ptr: int, n: int, dtype):
     if dtype == torch.bfloat16:
         # torch has no bfloat16 typestr: view the bits as int16
         return torch.as_tensor(_CudaArray(ptr, n, "<i2"), device="cuda").view(torch.bfloat16)
+    if dtype == torch.uint8 or dtype == torch.float8_e4m3fn:
+        return torch.as_tensor(_CudaArray(ptr, n, "|u1"), device="cuda").view(dtype)
     return torch.as_tensor(_CudaArray(ptr, n, "<f4"), device="cuda")
 
 
@@ -886,5 +967,16 @@ def kv_pool_views(cache: "KVCache", layer: int):
     import torch
     d = cache.desc
     n = d.num_pages * d.num_kv_heads * PAGE_TOKENS * d.head_dim
-    dt = torch.bfloat16 if d.kv_dtype == SA_DTYPE_BF16 else torch.float32
+    dt = {SA_DTYPE_BF16: torch.bfloat16, SA_DTYPE_FP8: torch.float8_e4m3fn}.get(d.kv_dtype, torch.float32)
     return _device_view(cache.k_pool(layer), n, dt), _device_view(cache.v_pool(layer), n, dt)
+
+
+def kv_scale_views(cache: "KVCache", layer: int):
+    """Flat torch views (uint8: exponent + 127) of an 8-bit cache's K and V scales."""
+    import torch
+    d = cache.desc
+    if d.kv_dtype != SA_DTYPE_FP8:
+        raise ValueError("only 8-bit caches have scales")
+    n = d.num_pages * d.num_kv_heads * PAGE_TOKENS
+    return tuple(_device_view(f(cache.handle, layer), n, torch.uint8)
+                 for f in (lib().sa_kvcache_k_scales, lib().sa_kvcache_v_scales))

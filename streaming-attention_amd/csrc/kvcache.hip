@@ -28,6 +28,8 @@ struct sa_kvcache {
     sa_kv_desc desc{};
     int device = 0;
     char* pool = nullptr;          // [layers][2][num_pages][n_kv][64][D]
+    uint8_t* scales = nullptr;     // 8 bits: [layers][2][num_pages][n_kv][64], else NULL
+    size_t scale_bytes = 0;        // K and V scales of one layer
     size_t elem_bytes = 4;
     size_t page_bytes = 0;         // one page of one of K / V: n_kv * 64 * D * elem
     size_t layer_bytes = 0;        // K pool + V pool of one layer
@@ -66,6 +68,12 @@ __global__ void update_lens_kernel(int32_t* lens, RowList rows, int n, int val, 
     if (i < n) lens[rows.row[i]] = add ? lens[rows.row[i]] + val : val;
 }
 
+// seq_lens[rows[i]] = to[i]
+__global__ void write_lens_kernel(int32_t* lens, RowList rows, RowList to, int n) {
+    const int i = threadIdx.x;
+    if (i < n) lens[rows.row[i]] = to.row[i];
+}
+
 __global__ void add_lens_range_kernel(int32_t* lens, int n, int val) {
     int i = blockIdx.x * blockDim.x + threadIdx.x;
     if (i < n) lens[i] += val;
@@ -102,15 +110,6 @@ sa_status publish_lens(sa_kvcache* c, const int32_t* rows, int n, int val, int a
 
 sa_status refused(const Verdict& v) { return fail(v.status, v.msg); }
 
-// Kernels of a cache run on its own device; a call made while another one is
-// current is refused.
-sa_status on_cache_device(const sa_kvcache* c) {
-    int dev = 0;
-    SA_HIP_TRY(hipGetDevice(&dev));
-    if (dev != c->device) return fail(SA_EINVAL, "the cache lives on another device than the current one");
-    return SA_OK;
-}
-
 // ---------------------------------------------------------------------------
 // Publishing a fork or a reorder: table entries, lengths and page copies of
 // several rows in one launch.  Rows that share their prompt differ in a few
@@ -125,7 +124,8 @@ struct RowsArgs {
     int32_t* table;
     int32_t* lens;
     char* pool;
-    size_t layer_bytes;
+    uint8_t* scales;                              // 8 bits, else NULL
+    size_t layer_bytes, scale_bytes;
     int max_pages, n_kv, head_bytes, row_bytes;   // head_bytes: 64 rows of one head of a page
     int n_edits, n_lens, n_copies;
     int like_dst, like_src, like_n;               // a fork: row dst's first n entries are row src's
@@ -155,6 +155,11 @@ __global__ void __launch_bounds__(256) update_rows_kernel(RowsArgs a) {
     uint4* dst = reinterpret_cast<uint4*>(base + ((size_t)cp.dst * a.n_kv + head) * a.head_bytes);
     const int n = cp.tokens * a.row_bytes / 16;
     for (int i = threadIdx.x; i < n; i += 256) dst[i] = src[i];
+    if (a.scales && (int)threadIdx.x < cp.tokens) {
+        uint8_t* sc = a.scales + (size_t)half * (a.scale_bytes / 2) + (size_t)head * SA_PAGE_TOKENS + threadIdx.x;
+        const size_t page = (size_t)a.n_kv * SA_PAGE_TOKENS;
+        sc[cp.dst * page] = sc[cp.src * page];
+    }
 }
 
 // The device side of what fork and reorder decided for rows[0, n): `before`
@@ -181,6 +186,7 @@ sa_status publish_rows(sa_kvcache* c, const std::vector<int32_t>& rows,
     while (ei < rows.size() || l < rows.size() || k < copies.size()) {
         RowsArgs a{};
         a.table = c->d_table; a.lens = c->d_lens; a.pool = c->pool; a.layer_bytes = c->layer_bytes;
+        a.scales = c->scales; a.scale_bytes = c->scale_bytes;
         a.max_pages = c->desc.max_pages_per_seq; a.n_kv = c->desc.num_kv_heads;
         a.row_bytes = (int)(c->desc.head_dim * c->elem_bytes);
         a.head_bytes = SA_PAGE_TOKENS * a.row_bytes;
@@ -237,9 +243,43 @@ struct AppendArgs {
     const int32_t* seq_lens;
     const int32_t* table;
     char* k_pool; char* v_pool;
-    int n_q, n_kv, S, max_pages, rope_max_pos;
-    int s0, n_s;               // tokens [s0, s0 + n_s) of the S
+    uint8_t* k_scale; uint8_t* v_scale;   // 8 bits
+    int n_q, n_kv, max_pages, rope_max_pos;
+    int s0, n_s;               // tokens [s0, s0 + n_s) of each sequence
     float eps;
+    int32_t first[kRowsPerLaunch + 1];    // sequence i's tokens are first[i] .. first[i + 1] - 1 of q, k and v
+};
+
+// What a row of an 8-bit cache is held by: codes of x 2^-e, ties to even, and the
+// byte e + 127, where 2^e is the smallest power of two, from 2^-100 on, with amax <=
+// 448 2^e.  A scale that is a power of two costs a floating format no accuracy, and
+// products with it are exact: what is held is code 2^e to the last bit, in bf16
+// too, and a row that is read back and appended again holds the same values.
+struct RowScale {
+    uint32_t byte;
+    float up, top;   // 2^-e; the largest code's value
+    __device__ __forceinline__ explicit RowScale(float amax) {
+        const uint32_t u = __float_as_uint(amax);
+        // 448 = 1.75 2^8
+        const int e = max(-100, (int)(u >> 23) - 127 - 8 + ((u & 0x7fffffu) > 0x600000u));
+        byte = (uint32_t)(e + 127);
+        up = __uint_as_float((uint32_t)(127 - e) << 23);
+        // 2^e 256 is beyond fp32's range where e is largest
+        top = e < 120 ? 448.f : 240.f;
+    }
+    // Four codes, the first in the lowest byte.  Infinities and NaN become NaN.
+    __device__ __forceinline__ uint32_t codes(float a, float b, float c, float d) const {
+        const uint32_t lo = __builtin_amdgcn_cvt_pk_fp8_f32(fit(a), fit(b), 0, false);
+        return __builtin_amdgcn_cvt_pk_fp8_f32(fit(c), fit(d), (int)lo, true);
+    }
+    __device__ __forceinline__ float fit(float x) const {
+        const float y = x * up;
+        return fabsf(x) < INFINITY ? __builtin_amdgcn_fmed3f(y, -top, top) : __uint_as_float(0x7fc00000u);
+    }
+    // The larger of m and |x|, where x is finite.
+    static __device__ __forceinline__ float larger(float m, float x) {
+        return fabsf(x) < INFINITY ? fmaxf(m, fabsf(x)) : m;
+    }
 };
 
 template <int D>
@@ -356,10 +396,29 @@ struct LaneRow {
             store_e(y + E * j + kWave * c + H, hi[c]);
         }
     }
-    // A row of the cache pools, 16-byte aligned.
-    template <bool BF16>
-    __device__ __forceinline__ void store_pool(char* pool, size_t row, int j) const {
-        if constexpr (BF16) {
+    // Row `row` of the cache pools (scale: of the scales), 16-byte aligned.
+    template <int KV>
+    __device__ __forceinline__ void store_pool(char* pool, uint8_t* scale, size_t at_row, int j) const {
+        const size_t row = at_row * D;
+        if constexpr (KV == SA_DTYPE_FP8) {
+            float amax = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+#pragma unroll
+                for (int e = 0; e < E; ++e) amax = RowScale::larger(RowScale::larger(amax, lo[c][e]), hi[c][e]);
+            const RowScale rs(group_reduce<OpMax, 1, LANES>(amax));
+            uint8_t* d = reinterpret_cast<uint8_t*>(pool) + row;
+            auto put = [&](int at, const float (&v)[E]) {
+                if constexpr (E == 4) *reinterpret_cast<uint32_t*>(d + at) = rs.codes(v[0], v[1], v[2], v[3]);
+                else d[at] = (uint8_t)rs.codes(v[0], 0.f, 0.f, 0.f);
+            };
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                put(E * j + kWave * c, lo[c]);
+                put(E * j + kWave * c + H, hi[c]);
+            }
+            if (j == 0) scale[at_row] = (uint8_t)rs.byte;
+        } else if constexpr (KV == SA_DTYPE_BF16) {
             uint16_t* d = reinterpret_cast<uint16_t*>(pool) + row;
             auto put = [&](int at, const float (&v)[E]) {
                 if constexpr (E == 4) {
@@ -393,7 +452,7 @@ struct LaneRow {
 };
 
 // VEC: q, k, v, the partials, weights, tables and outputs are 16-byte aligned.
-template <int D, bool BF16, int E, bool VEC>
+template <int D, int KV, int E, bool VEC>
 __global__ void __launch_bounds__(256)
 qknorm_rope_append_kernel(AppendArgs a) {
     using Row = LaneRow<D, E, VEC>;
@@ -403,10 +462,11 @@ qknorm_rope_append_kernel(AppendArgs a) {
     const int s = a.s0 + (int)(idx / per_token);
     const int id = (int)(idx % per_token);   // query heads, key heads, value heads
     const int i_seq = blockIdx.y;
-    if (s >= a.s0 + a.n_s) return;
+    const int first = a.first[i_seq];
+    if (s >= min(a.s0 + a.n_s, a.first[i_seq + 1] - first)) return;
     const bool is_q = id < a.n_q, is_k = !is_q && id < a.n_q + a.n_kv;
     const int head = is_q ? id : is_k ? id - a.n_q : id - a.n_q - a.n_kv;
-    const size_t token = (size_t)i_seq * a.S + s;
+    const size_t token = (size_t)first + s;
     const size_t src = (token * (is_q ? a.n_q : a.n_kv) + head) * D;
     const int cache_row = a.rows.row[i_seq];
     const int pos = a.seq_lens[cache_row] + s;
@@ -430,21 +490,29 @@ qknorm_rope_append_kernel(AppendArgs a) {
     float* copy = is_q ? a.q_out : is_k ? a.k_out : a.v_out;
     if (copy) r.store(copy + src, j);
     if (page < 0) return;
-    r.template store_pool<BF16>(is_k ? a.k_pool : a.v_pool, (((size_t)page * a.n_kv + head) * 64 + (pos & 63)) * D, j);
+    r.template store_pool<KV>(is_k ? a.k_pool : a.v_pool, is_k ? a.k_scale : a.v_scale,
+                              ((size_t)page * a.n_kv + head) * 64 + (pos & 63), j);
 }
 
 // Dense copy [n_kv][len][D] of one sequence (fp32 out).
-template <bool BF16>
-__global__ void gather_kernel(const char* k_pool, const char* v_pool, const int32_t* table_row,
-                              int n_kv, int D, int len, float* k_out, float* v_out) {
+template <int KV>
+__global__ void gather_kernel(const char* k_pool, const char* v_pool, const uint8_t* k_scale, const uint8_t* v_scale,
+                              const int32_t* table_row, int n_kv, int D, int len, float* k_out, float* v_out) {
     const int t = blockIdx.x;
     const int h = blockIdx.y;
     const int page = table_row[t >> 6];
-    const size_t row = (((size_t)page * n_kv + h) * 64 + (t & 63)) * D;
+    const size_t at = ((size_t)page * n_kv + h) * 64 + (t & 63), row = at * D;
     const size_t dst = ((size_t)h * len + t) * D;
     for (int i = threadIdx.x; i < D; i += blockDim.x) {
         float kv, vv;
-        if constexpr (BF16) {
+        if constexpr (KV == SA_DTYPE_FP8) {
+            auto value = [&](const char* pool, const uint8_t* scale) {
+                const uint32_t code = reinterpret_cast<const uint8_t*>(pool)[row + i];
+                return __builtin_amdgcn_cvt_f32_fp8((int)code, 0) * __uint_as_float((uint32_t)scale[at] << 23);
+            };
+            kv = value(k_pool, k_scale);
+            vv = value(v_pool, v_scale);
+        } else if constexpr (KV == SA_DTYPE_BF16) {
             kv = __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(k_pool)[row + i] << 16);
             vv = __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(v_pool)[row + i] << 16);
         } else {
@@ -461,6 +529,33 @@ bool valid_cache(const sa_kvcache* c) { return c && c->pool; }
 char* k_pool_of(const sa_kvcache* c, int layer) { return c->pool + (size_t)layer * c->layer_bytes; }
 char* v_pool_of(const sa_kvcache* c, int layer) {
     return c->pool + (size_t)layer * c->layer_bytes + c->layer_bytes / 2;
+}
+uint8_t* k_scales_of(const sa_kvcache* c, int layer) {
+    return c->scales ? c->scales + (size_t)layer * c->scale_bytes : nullptr;
+}
+uint8_t* v_scales_of(const sa_kvcache* c, int layer) {
+    return c->scales ? c->scales + (size_t)layer * c->scale_bytes + c->scale_bytes / 2 : nullptr;
+}
+
+PagedView view_of(const sa_kvcache* c, int layer) {
+    PagedView pv;
+    pv.k_pool = k_pool_of(c, layer); pv.v_pool = v_pool_of(c, layer);
+    pv.k_scale = k_scales_of(c, layer); pv.v_scale = v_scales_of(c, layer);
+    pv.block_table = c->d_table; pv.seq_lens = c->d_lens;
+    pv.n_kv = c->desc.num_kv_heads; pv.d = c->desc.head_dim;
+    pv.max_pages = c->desc.max_pages_per_seq; pv.num_pages = c->desc.num_pages;
+    pv.kv = c->desc.kv_dtype;
+    pv.bf16 = c->desc.kv_dtype == SA_DTYPE_BF16;
+    return pv;
+}
+
+// Kernels of a cache run on its own device; a call made while another one is
+// current is refused.
+sa_status on_cache_device(const sa_kvcache* c) {
+    int dev = 0;
+    SA_HIP_TRY(hipGetDevice(&dev));
+    if (dev != c->device) return fail(SA_EINVAL, "the cache lives on another device than the current one");
+    return SA_OK;
 }
 
 }  // namespace
@@ -480,18 +575,22 @@ extern "C" sa_status sa_kvcache_create(const sa_kv_desc* d, sa_kvcache** out) {
     if (d->head_dim != 8 && d->head_dim != 16 && d->head_dim != 32 && d->head_dim != 64 && d->head_dim != 128 &&
         d->head_dim != 256)
         return fail(SA_EINVAL, "head_dim must be 8, 16, 32, 64, 128 or 256");
-    if (d->kv_dtype != SA_DTYPE_F32 && d->kv_dtype != SA_DTYPE_BF16)
-        return fail(SA_EINVAL, "kv_dtype must be F32 or BF16");
+    if (d->kv_dtype != SA_DTYPE_F32 && d->kv_dtype != SA_DTYPE_BF16 && d->kv_dtype != SA_DTYPE_FP8)
+        return fail(SA_EINVAL, "kv_dtype must be F32, BF16 or FP8");
+    const bool fp8 = d->kv_dtype == SA_DTYPE_FP8;
+    if (fp8 && !ranges_head_dim(d->head_dim)) return fail(SA_EINVAL, "caches in 8 bits take head_dim 64 or 128");
     int device = 0;
     const hipError_t de = hipGetDevice(&device);
     if (de != hipSuccess) return hip_fail(de, "hipGetDevice");
     auto* c = new sa_kvcache();
     c->desc = *d;
     c->device = device;
-    c->elem_bytes = d->kv_dtype == SA_DTYPE_BF16 ? 2 : 4;
+    c->elem_bytes = fp8 ? 1 : d->kv_dtype == SA_DTYPE_BF16 ? 2 : 4;
     c->page_bytes = (size_t)d->num_kv_heads * 64 * d->head_dim * c->elem_bytes;
     c->layer_bytes = 2 * c->page_bytes * (size_t)d->num_pages;
     c->total_bytes = c->layer_bytes * (size_t)d->num_layers;
+    c->scale_bytes = fp8 ? 2 * (size_t)d->num_kv_heads * SA_PAGE_TOKENS * (size_t)d->num_pages : 0;
+    const size_t all_scales = c->scale_bytes * (size_t)d->num_layers;
     const size_t n_table = (size_t)d->max_seqs * d->max_pages_per_seq;
     hipError_t e = hipMalloc(&c->pool, c->total_bytes);
     if (e != hipSuccess) {
@@ -500,8 +599,10 @@ extern "C" sa_status sa_kvcache_create(const sa_kv_desc* d, sa_kvcache** out) {
     }
     e = hipMalloc(&c->d_table, n_table * sizeof(int32_t));
     if (e == hipSuccess) e = hipMalloc(&c->d_lens, (size_t)d->max_seqs * sizeof(int32_t));
+    if (e == hipSuccess && fp8) e = hipMalloc(&c->scales, all_scales);
     if (e != hipSuccess) {
         (void)hipFree(c->pool);
+        (void)hipFree(c->scales);
         (void)hipFree(c->d_table);
         (void)hipFree(c->d_lens);
         delete c;
@@ -528,6 +629,7 @@ extern "C" sa_status sa_kvcache_destroy(sa_kvcache* c) {
     // memory goes; a failure here leaves nothing else to do.
     (void)hipDeviceSynchronize();
     (void)hipFree(c->pool);
+    (void)hipFree(c->scales);
     (void)hipFree(c->d_table);
     (void)hipFree(c->d_lens);
     delete c;
@@ -550,6 +652,11 @@ extern "C" sa_status sa_kvcache_reset(sa_kvcache* c, sa_stream_t stream) {
     hipLaunchKernelGGL(fill_zero_u128_kernel, dim3(4096), dim3(256), 0, st,
                        reinterpret_cast<uint4*>(c->pool), n16);
     SA_CHECK_LAUNCH();
+    if (c->scales) {
+        hipLaunchKernelGGL(fill_zero_u128_kernel, dim3(256), dim3(256), 0, st, reinterpret_cast<uint4*>(c->scales),
+                           c->scale_bytes * (size_t)c->desc.num_layers / 16);
+        SA_CHECK_LAUNCH();
+    }
     return SA_OK;
 }
 
@@ -588,6 +695,29 @@ extern "C" sa_status sa_kvcache_set_len(sa_kvcache* c, int seq, int len, sa_stre
     if (!v.ok()) return refused(v);
     const int32_t row = seq;
     return publish_lens(c, &row, 1, len, 0, as_stream(stream));
+}
+
+extern "C" sa_status sa_kvcache_set_lens(sa_kvcache* c, const int32_t* seqs, const int32_t* lens, int n,
+                                         sa_stream_t stream) {
+    clear_error();
+    if (!valid_cache(c)) return fail(SA_EINVAL, "invalid cache");
+    if (n < 0) return fail(SA_EINVAL, "negative sequence count");
+    if (n > 0 && (!seqs || !lens)) return fail(SA_EINVAL, "null seqs or lens");
+    return no_throw([&]() -> sa_status {
+        SA_TRY(on_cache_device(c));
+        const Verdict v = c->pt.set_lens(seqs, lens, n);
+        if (!v.ok()) return refused(v);
+        for (int i0 = 0; i0 < n; i0 += kRowsPerLaunch) {
+            const int m = std::min(kRowsPerLaunch, n - i0);
+            RowList rows, to;
+            std::copy(seqs + i0, seqs + i0 + m, rows.row);
+            std::copy(lens + i0, lens + i0 + m, to.row);
+            hipLaunchKernelGGL(write_lens_kernel, dim3(1), dim3(kRowsPerLaunch), 0, as_stream(stream), c->d_lens, rows,
+                               to, m);
+            SA_CHECK_LAUNCH();
+        }
+        return SA_OK;
+    });
 }
 
 extern "C" int sa_kvcache_len(const sa_kvcache* c, int seq) {
@@ -667,9 +797,19 @@ extern "C" void* sa_kvcache_v_pool(sa_kvcache* c, int layer) {
     if (!valid_cache(c) || layer < 0 || layer >= c->desc.num_layers) return nullptr;
     return v_pool_of(c, layer);
 }
+extern "C" uint8_t* sa_kvcache_k_scales(sa_kvcache* c, int layer) {
+    if (!valid_cache(c) || layer < 0 || layer >= c->desc.num_layers) return nullptr;
+    return k_scales_of(c, layer);
+}
+extern "C" uint8_t* sa_kvcache_v_scales(sa_kvcache* c, int layer) {
+    if (!valid_cache(c) || layer < 0 || layer >= c->desc.num_layers) return nullptr;
+    return v_scales_of(c, layer);
+}
 extern "C" int32_t* sa_kvcache_block_table(sa_kvcache* c) { return valid_cache(c) ? c->d_table : nullptr; }
 extern "C" int32_t* sa_kvcache_seq_lens(sa_kvcache* c) { return valid_cache(c) ? c->d_lens : nullptr; }
-extern "C" size_t sa_kvcache_bytes(const sa_kvcache* c) { return valid_cache(c) ? c->total_bytes : 0; }
+extern "C" size_t sa_kvcache_bytes(const sa_kvcache* c) {
+    return valid_cache(c) ? c->total_bytes + c->scale_bytes * (size_t)c->desc.num_layers : 0;
+}
 
 extern "C" sa_status sa_rope_table_init(float* d_cos, float* d_sin, int max_pos, int head_dim,
                                         float theta, sa_stream_t stream) {
@@ -708,73 +848,90 @@ namespace {
 // 2.91, 256 tokens 3.99 / 3.50 / 3.57, 1024 tokens 10.6 / 7.1 / 7.9.
 constexpr long long kAppendNarrow = 3000;
 
+template <int D, int KV>
+void launch_append_kv(bool wide, bool vec, dim3 grid, hipStream_t st, const AppendArgs& a) {
+    if (vec) hipLaunchKernelGGL((qknorm_rope_append_kernel<D, KV, 4, true>), grid, dim3(256), 0, st, a);
+    else if (wide) hipLaunchKernelGGL((qknorm_rope_append_kernel<D, KV, 4, false>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((qknorm_rope_append_kernel<D, KV, 1, false>), grid, dim3(256), 0, st, a);
+}
+template <int D>
+void launch_append(sa_dtype kv, bool wide, bool vec, dim3 grid, hipStream_t st, const AppendArgs& a) {
+    if constexpr (D == 64 || D == 128)   // the head sizes of 8-bit caches
+        if (kv == SA_DTYPE_FP8) return launch_append_kv<D, SA_DTYPE_FP8>(wide, vec, grid, st, a);
+    if (kv == SA_DTYPE_BF16) launch_append_kv<D, SA_DTYPE_BF16>(wide, vec, grid, st, a);
+    else launch_append_kv<D, SA_DTYPE_F32>(wide, vec, grid, st, a);
+}
+
 // Shared by the entry points below: q/k/v given (part == NULL), or summed from
 // the n_part split-K partials of the projection at part (q, k, v NULL).
+// counts: the sequences' new tokens where they differ (host), else NULL and S each.
 sa_status append_impl(sa_kvcache* c, int layer, const float* q, const float* k, const float* v, const float* part,
-                      int n_part, int n_seq, int S, const int32_t* seq_ids, int n_q_heads, const float* q_norm_w,
-                      const float* k_norm_w, float eps, const float* rope_cos, const float* rope_sin,
-                      int rope_max_pos, float* q_out, float* k_out, float* v_out, hipStream_t st) {
+                      int n_part, int n_seq, int S, const int32_t* counts, const int32_t* seq_ids, int n_q_heads,
+                      const float* q_norm_w, const float* k_norm_w, float eps, const float* rope_cos,
+                      const float* rope_sin, int rope_max_pos, float* q_out, float* k_out, float* v_out,
+                      hipStream_t st) {
     if (!valid_cache(c)) return fail(SA_EINVAL, "invalid cache");
     if (layer < 0 || layer >= c->desc.num_layers) return fail(SA_ERANGE, "Layer index out of range");
     if (part ? n_part <= 0 : (!k || !v)) return fail(SA_EINVAL, "null k or v");
     if ((q || part) && (!q_out || n_q_heads <= 0)) return fail(SA_EINVAL, "q needs q_out and n_q_heads > 0");
-    if (n_seq <= 0 || S <= 0) return fail(SA_EINVAL, "n_seq and S must be positive");
+    if (n_seq <= 0 || (!counts && S <= 0)) return fail(SA_EINVAL, "n_seq and S must be positive");
     if ((rope_cos == nullptr) != (rope_sin == nullptr)) return fail(SA_EINVAL, "cos and sin go together");
     if (rope_cos && rope_max_pos <= 0) return fail(SA_EINVAL, "RoPE table needs rope_max_pos > 0");
-    const Verdict vd = c->pt.check_append(seq_ids, n_seq, S, rope_cos ? rope_max_pos : 0);
+    const Verdict vd = counts ? c->pt.check_append(seq_ids, n_seq, counts, rope_cos ? rope_max_pos : 0)
+                              : c->pt.check_append(seq_ids, n_seq, S, rope_cos ? rope_max_pos : 0);
     if (!vd.ok()) return refused(vd);
+    long long tokens = 0;
+    for (int i = 0; i < n_seq; ++i) tokens += counts ? counts[i] : S;
+    if (tokens > 0x7fffffffLL) return fail(SA_EINVAL, "more than 2^31 - 1 new tokens");
     AppendArgs a{};
     a.q_out = q_out;
-    a.part = part; a.part_S = n_part; a.part_M = n_seq * S;
+    a.part = part; a.part_S = n_part; a.part_M = (int)tokens;
     a.wq = q_norm_w; a.wk = k_norm_w; a.cos_t = rope_cos; a.sin_t = rope_sin;
     a.seq_lens = c->d_lens; a.table = c->d_table;
     a.k_pool = k_pool_of(c, layer); a.v_pool = v_pool_of(c, layer);
-    a.n_q = q || part ? n_q_heads : 0; a.n_kv = c->desc.num_kv_heads; a.S = S;
+    a.k_scale = k_scales_of(c, layer); a.v_scale = v_scales_of(c, layer);
+    a.n_q = q || part ? n_q_heads : 0; a.n_kv = c->desc.num_kv_heads;
     a.max_pages = c->desc.max_pages_per_seq; a.rope_max_pos = rope_max_pos; a.eps = eps;
     const int rows = a.n_q + 2 * a.n_kv;
     const int D = c->desc.head_dim;
-    const bool bf = c->desc.kv_dtype == SA_DTYPE_BF16;
+    const sa_dtype kv = c->desc.kv_dtype;
     // Up to kRowsPerLaunch sequences per launch, their cache rows by value.
+    size_t at = 0;   // the launch's first token
     for (int i0 = 0; i0 < n_seq; i0 += kRowsPerLaunch) {
         const int m = std::min(kRowsPerLaunch, n_seq - i0);
-        for (int i = 0; i < m; ++i) a.rows.row[i] = seq_ids ? seq_ids[i0 + i] : i0 + i;
-        a.q = q ? q + (size_t)i0 * S * n_q_heads * D : nullptr;
-        a.q_out = a.n_q ? q_out + (size_t)i0 * S * n_q_heads * D : nullptr;
-        a.k = k ? k + (size_t)i0 * S * a.n_kv * D : nullptr;
-        a.k_out = k_out ? k_out + (size_t)i0 * S * a.n_kv * D : nullptr;
-        a.v = v ? v + (size_t)i0 * S * a.n_kv * D : nullptr;
-        a.v_out = v_out ? v_out + (size_t)i0 * S * a.n_kv * D : nullptr;
-        a.part_row0 = i0 * S;
-        const bool wide = (long long)rows * S * m > kAppendNarrow;
+        int most = 0;
+        a.first[0] = 0;
+        for (int i = 0; i < m; ++i) {
+            const int n = counts ? counts[i0 + i] : S;
+            a.rows.row[i] = seq_ids ? seq_ids[i0 + i] : i0 + i;
+            a.first[i + 1] = a.first[i] + n;
+            most = std::max(most, n);
+        }
+        a.q = q ? q + at * n_q_heads * D : nullptr;
+        a.q_out = a.n_q ? q_out + at * n_q_heads * D : nullptr;
+        a.k = k ? k + at * a.n_kv * D : nullptr;
+        a.k_out = k_out ? k_out + at * a.n_kv * D : nullptr;
+        a.v = v ? v + at * a.n_kv * D : nullptr;
+        a.v_out = v_out ? v_out + at * a.n_kv * D : nullptr;
+        a.part_row0 = (int)at;
+        at += a.first[m];
+        const bool wide = (long long)rows * a.first[m] > kAppendNarrow;
         bool vec = wide;   // the launch's pointers allow 16-byte accesses
         for (const void* p : std::initializer_list<const void*>{a.q, a.k, a.v, a.part, a.q_out, a.k_out, a.v_out, a.wq,
                                                                 a.wk, a.cos_t, a.sin_t})
             vec = vec && aligned16(p);
         const int lanes = std::min(D / 2, kWave) / (wide ? 4 : 1);
         const int step = tokens_per_launch(rows, lanes);
-        for (a.s0 = 0; a.s0 < S; a.s0 += a.n_s) {
-            a.n_s = std::min(step, S - a.s0);
+        for (a.s0 = 0; a.s0 < most; a.s0 += a.n_s) {
+            a.n_s = std::min(step, most - a.s0);
             const dim3 grid((unsigned)(((long long)rows * a.n_s * lanes + 255) / 256), m);
             switch (D) {
-#define SA_APPEND_LAUNCH(DD, BB, EE, VV)                                                                           \
-    hipLaunchKernelGGL((qknorm_rope_append_kernel<DD, BB, EE, VV>), grid, dim3(256), 0, st, a)
-#define SA_APPEND_CASE(DD)                                                                                         \
-    case DD:                                                                                                       \
-        if (bf && vec) SA_APPEND_LAUNCH(DD, true, 4, true);                                                        \
-        else if (bf && wide) SA_APPEND_LAUNCH(DD, true, 4, false);                                                 \
-        else if (bf) SA_APPEND_LAUNCH(DD, true, 1, false);                                                         \
-        else if (vec) SA_APPEND_LAUNCH(DD, false, 4, true);                                                        \
-        else if (wide) SA_APPEND_LAUNCH(DD, false, 4, false);                                                      \
-        else SA_APPEND_LAUNCH(DD, false, 1, false);                                                                \
-        break;
-                SA_APPEND_CASE(8)
-                SA_APPEND_CASE(16)
-                SA_APPEND_CASE(32)
-                SA_APPEND_CASE(64)
-                SA_APPEND_CASE(128)
-                SA_APPEND_CASE(256)
-#undef SA_APPEND_CASE
-#undef SA_APPEND_LAUNCH
+                case 8: launch_append<8>(kv, wide, vec, grid, st, a); break;
+                case 16: launch_append<16>(kv, wide, vec, grid, st, a); break;
+                case 32: launch_append<32>(kv, wide, vec, grid, st, a); break;
+                case 64: launch_append<64>(kv, wide, vec, grid, st, a); break;
+                case 128: launch_append<128>(kv, wide, vec, grid, st, a); break;
+                case 256: launch_append<256>(kv, wide, vec, grid, st, a); break;
                 default: return fail(SA_EINVAL, "head_dim");
             }
             SA_CHECK_LAUNCH();
@@ -789,8 +946,8 @@ sa_status qknorm_rope_append(sa_kvcache* c, int layer, const float* q, const flo
                              int S, const int32_t* seq_ids, int n_q_heads, const float* q_norm_w,
                              const float* k_norm_w, float eps, const float* rope_cos, const float* rope_sin,
                              int rope_max_pos, float* q_out, float* k_out, hipStream_t st) {
-    return append_impl(c, layer, q, k, v, nullptr, 0, n_seq, S, seq_ids, n_q_heads, q_norm_w, k_norm_w, eps, rope_cos,
-                       rope_sin, rope_max_pos, q_out, k_out, nullptr, st);
+    return append_impl(c, layer, q, k, v, nullptr, 0, n_seq, S, nullptr, seq_ids, n_q_heads, q_norm_w, k_norm_w, eps,
+                       rope_cos, rope_sin, rope_max_pos, q_out, k_out, nullptr, st);
 }
 
 sa_status qknorm_rope_append_partials(sa_kvcache* c, int layer, const float* part, int n_part, int n_seq, int S,
@@ -798,8 +955,17 @@ sa_status qknorm_rope_append_partials(sa_kvcache* c, int layer, const float* par
                                       const float* rope_cos, const float* rope_sin, int rope_max_pos, float* q_out,
                                       float* k_out, float* v_out, hipStream_t st) {
     if (!part) return fail(SA_EINVAL, "null partials");
-    return append_impl(c, layer, nullptr, nullptr, nullptr, part, n_part, n_seq, S, nullptr, n_q_heads, q_norm_w,
-                       k_norm_w, eps, rope_cos, rope_sin, rope_max_pos, q_out, k_out, v_out, st);
+    return append_impl(c, layer, nullptr, nullptr, nullptr, part, n_part, n_seq, S, nullptr, nullptr, n_q_heads,
+                       q_norm_w, k_norm_w, eps, rope_cos, rope_sin, rope_max_pos, q_out, k_out, v_out, st);
+}
+
+sa_status append_partials_ragged(sa_kvcache* c, int layer, const float* part, int n_part, int n_seq,
+                                 const int32_t* counts, int n_q_heads, const float* q_norm_w, const float* k_norm_w,
+                                 float eps, const float* rope_cos, const float* rope_sin, int rope_max_pos,
+                                 float* q_out, hipStream_t st) {
+    if (!part) return fail(SA_EINVAL, "null partials");
+    return append_impl(c, layer, nullptr, nullptr, nullptr, part, n_part, n_seq, 0, counts, nullptr, n_q_heads,
+                       q_norm_w, k_norm_w, eps, rope_cos, rope_sin, rope_max_pos, q_out, nullptr, nullptr, st);
 }
 
 }  // namespace sa
@@ -815,8 +981,57 @@ extern "C" sa_status sa_qknorm_rope_append(sa_kvcache* c, int layer, const float
                               rope_sin, rope_max_pos, q_out, nullptr, as_stream(stream));
 }
 
+extern "C" sa_status sa_qknorm_rope_append_ragged(sa_kvcache* c, int layer, const float* q, const float* k,
+                                                  const float* v, int n_seq, const int32_t* counts,
+                                                  const int32_t* seq_ids, int n_q_heads, const float* q_norm_w,
+                                                  const float* k_norm_w, float eps, const float* rope_cos,
+                                                  const float* rope_sin, int rope_max_pos, float* q_out,
+                                                  sa_stream_t stream) {
+    clear_error();
+    if (!counts) return fail(SA_EINVAL, "null counts");
+    return no_throw([&] {
+        return append_impl(c, layer, q, k, v, nullptr, 0, n_seq, 0, counts, seq_ids, n_q_heads, q_norm_w, k_norm_w,
+                           eps, rope_cos, rope_sin, rope_max_pos, q_out, nullptr, nullptr, as_stream(stream));
+    });
+}
+
+namespace sa {
+namespace {
+
+// A step's queries, normed and rotated, before the partials of a decode over an
+// 8-bit cache.
+size_t step_q_bytes(const sa_kvcache* c, int n_seq, int n_q_heads) {
+    return ((size_t)n_seq * n_q_heads * c->desc.head_dim * sizeof(float) + 255) / 256 * 256;
+}
+
+sa_status check_ranges(const sa_kvcache* c, int layer, const void* q, int n_seq, int n_q_heads, const void* out,
+                       const void* ws, size_t ws_bytes, size_t ws_need);
+
+// Decode over an 8-bit cache: every row's tokens as one range.
+sa_status decode_fp8(const sa_kvcache* c, int layer, const float* q, int n_seq, const int32_t* seq_ids, int n_q_heads,
+                     int n_pending, float scale, float* out, void* ws, size_t ws_bytes, hipStream_t st) {
+    const size_t need = ranges_ws(n_seq, n_q_heads, c->desc.head_dim,
+                                  (long long)c->desc.max_pages_per_seq * SA_PAGE_TOKENS, 0);
+    SA_TRY(check_ranges(c, layer, q, n_seq, n_q_heads, out, ws, ws_bytes, need));
+    const Verdict vd = c->pt.check_decode(seq_ids, n_seq, n_pending, nullptr, nullptr);
+    if (!vd.ok()) return refused(vd);
+    std::vector<RangeSource> own(n_seq);
+    for (int i = 0; i < n_seq; ++i) {
+        const int row = seq_ids ? seq_ids[i] : i;
+        own[i] = RangeSource{row, 0, 0, c->pt.len(row) + n_pending};
+    }
+    return decode_ranges(view_of(c, layer), q, n_q_heads, RangePlan{n_seq, own.data(), 0, nullptr, nullptr}, scale, out,
+                         ws, ws_bytes, st);
+}
+
+}  // namespace
+}  // namespace sa
+
 extern "C" size_t sa_paged_decode_ws_bytes(const sa_kvcache* c, int n_seq, int n_q_heads) {
     if (!valid_cache(c) || n_seq <= 0 || n_q_heads <= 0) return 0;
+    if (c->scales)
+        return step_q_bytes(c, n_seq, n_q_heads) +
+               ranges_ws(n_seq, n_q_heads, c->desc.head_dim, (long long)c->desc.max_pages_per_seq * SA_PAGE_TOKENS, 0);
     return paged_ws(n_seq, n_q_heads, c->desc.num_kv_heads, c->desc.head_dim, c->desc.max_pages_per_seq);
 }
 
@@ -827,16 +1042,16 @@ extern "C" sa_status sa_paged_decode(const sa_kvcache* c, int layer, const float
     if (!valid_cache(c)) return fail(SA_EINVAL, "invalid cache");
     if (layer < 0 || layer >= c->desc.num_layers) return fail(SA_ERANGE, "Layer index out of range");
     if (n_seq <= 0) return fail(SA_EINVAL, "n_seq must be positive");
+    if (c->scales)
+        return no_throw([&] {
+            return decode_fp8(c, layer, q, n_seq, seq_ids, n_q_heads, n_pending, scale, out, ws, ws_bytes,
+                              as_stream(stream));
+        });
     int max_len = 0;
     long long total = 0;
     const Verdict vd = c->pt.check_decode(seq_ids, n_seq, n_pending, &max_len, &total);
     if (!vd.ok()) return refused(vd);
-    PagedView pv;
-    pv.k_pool = k_pool_of(c, layer); pv.v_pool = v_pool_of(c, layer);
-    pv.block_table = c->d_table; pv.seq_lens = c->d_lens;
-    pv.n_kv = c->desc.num_kv_heads; pv.d = c->desc.head_dim;
-    pv.max_pages = c->desc.max_pages_per_seq; pv.num_pages = c->desc.num_pages;
-    pv.bf16 = c->desc.kv_dtype == SA_DTYPE_BF16;
+    const PagedView pv = view_of(c, layer);
     std::vector<int32_t> lens(n_seq);
     for (int i = 0; i < n_seq; ++i) lens[i] = c->pt.len(seq_ids ? seq_ids[i] : i);
     return decode_paged(pv, q, n_seq, seq_ids, lens.data(), n_q_heads, n_pending, max_len, total, scale, out, ws,
@@ -846,9 +1061,11 @@ extern "C" sa_status sa_paged_decode(const sa_kvcache* c, int layer, const float
 namespace sa {
 namespace {
 
+constexpr int kMaxNewTokens = 1 << 20;   // of one call
+
 // What the decodes over ranges share: the checks of their arguments and the
 // view of a layer's pools.
-sa_status check_ranges(const sa_kvcache* c, int layer, const float* q, int n_seq, int n_q_heads, const float* out,
+sa_status check_ranges(const sa_kvcache* c, int layer, const void* q, int n_seq, int n_q_heads, const void* out,
                        const void* ws, size_t ws_bytes, size_t ws_need) {
     if (layer < 0 || layer >= c->desc.num_layers) return fail(SA_ERANGE, "Layer index out of range");
     if (!q || !out) return fail(SA_EINVAL, "null pointer");
@@ -863,16 +1080,6 @@ sa_status check_ranges(const sa_kvcache* c, int layer, const float* q, int n_seq
     if (n_seq > kRowsPerLaunch && (!ws || ws_bytes < ws_need))
         return fail(SA_ENOMEM, "workspace too small for the partials");
     return on_cache_device(c);
-}
-
-PagedView view_of(const sa_kvcache* c, int layer) {
-    PagedView pv;
-    pv.k_pool = k_pool_of(c, layer); pv.v_pool = v_pool_of(c, layer);
-    pv.block_table = c->d_table; pv.seq_lens = c->d_lens;
-    pv.n_kv = c->desc.num_kv_heads; pv.d = c->desc.head_dim;
-    pv.max_pages = c->desc.max_pages_per_seq; pv.num_pages = c->desc.num_pages;
-    pv.bf16 = c->desc.kv_dtype == SA_DTYPE_BF16;
-    return pv;
 }
 
 }  // namespace
@@ -969,6 +1176,47 @@ extern "C" sa_status sa_paged_decode_shared(const sa_kvcache* c, int layer, cons
     });
 }
 
+extern "C" size_t sa_paged_extend_ws_bytes(const sa_kvcache* c, int n_seq, const int32_t* counts, int n_q_heads) {
+    if (!valid_cache(c) || n_seq <= 0 || !counts || n_q_heads <= 0 || n_q_heads % c->desc.num_kv_heads ||
+        !ranges_head_dim(c->desc.head_dim) || n_q_heads / c->desc.num_kv_heads > kRangesMaxRep)
+        return 0;
+    for (int i = 0; i < n_seq; ++i)
+        if (counts[i] < 0) return 0;
+    return extend_rows_ws(n_seq, counts, n_q_heads, c->desc.num_kv_heads, c->desc.head_dim,
+                          c->desc.kv_dtype == SA_DTYPE_F32, (long long)c->desc.max_pages_per_seq * SA_PAGE_TOKENS);
+}
+
+extern "C" sa_status sa_paged_extend(const sa_kvcache* c, int layer, const void* q, sa_dtype q_dtype, int n_seq,
+                                     const int32_t* seq_ids, const int32_t* counts, int n_q_heads, float scale,
+                                     void* out, void* ws, size_t ws_bytes, sa_stream_t stream) {
+    clear_error();
+    if (!valid_cache(c)) return fail(SA_EINVAL, "invalid cache");
+    if (q_dtype != SA_DTYPE_F32 && q_dtype != SA_DTYPE_BF16) return fail(SA_EINVAL, "q_dtype must be F32 or BF16");
+    if (q_dtype == SA_DTYPE_BF16 && c->desc.kv_dtype == SA_DTYPE_F32)
+        return fail(SA_EINVAL, "bf16 queries take a bf16 or 8-bit cache");
+    if (!counts) return fail(SA_EINVAL, "null counts");
+    return no_throw([&]() -> sa_status {
+        SA_TRY(check_ranges(c, layer, q, n_seq, n_q_heads, out, ws, ws_bytes,
+                            sa_paged_extend_ws_bytes(c, n_seq, counts, n_q_heads)));
+        const Verdict vd = c->pt.check_rows(seq_ids, n_seq, false);
+        if (!vd.ok()) return refused(vd);
+        std::vector<ChunkSeq> seqs;
+        seqs.reserve(n_seq);
+        long long rows = 0;
+        for (int i = 0; i < n_seq; ++i) {
+            const int row = seq_ids ? seq_ids[i] : i, len = c->pt.len(row);
+            if (counts[i] < 0) return fail(SA_EINVAL, "counts must be >= 0");
+            if (rows + counts[i] > kMaxNewTokens) return fail(SA_EINVAL, "more than 2^20 new tokens");
+            if ((long long)len + counts[i] > c->pt.capacity(row))
+                return fail(SA_ERANGE, "Requested seq_len exceeds cached length");
+            if (counts[i]) seqs.push_back(ChunkSeq{row, len, counts[i], (int)rows});
+            rows += counts[i];
+        }
+        return extend_rows(view_of(c, layer), q, q_dtype == SA_DTYPE_BF16, n_q_heads, seqs.data(), (int)seqs.size(),
+                           scale, out, ws, ws_bytes, as_stream(stream));
+    });
+}
+
 namespace sa {
 namespace {
 
@@ -990,18 +1238,32 @@ sa_status append_decode_impl(sa_kvcache* c, int layer, const float* q, const flo
     if (c->desc.head_dim < 64) return fail(SA_EINVAL, "the fused decode step takes head_dim 64, 128 or 256");
     Verdict vd = c->pt.check_append(seq_ids, n_seq, 1, rope_cos ? rope_max_pos : 0);
     if (!vd.ok()) return refused(vd);
+    if (c->scales) {
+        // The append and the decode as launches of their own, the normed, rotated
+        // queries where the caller wants them or before the partials.
+        const size_t head = q_out ? 0 : step_q_bytes(c, n_seq, n_q_heads);
+        float* q_step = q_out ? q_out : static_cast<float*>(ws);
+        if (!q_out && (!ws || ws_bytes < head)) return fail(SA_ENOMEM, "workspace too small for the queries");
+        if (n_q_heads / c->desc.num_kv_heads > kRangesMaxRep || n_q_heads > 65535)
+            return fail(SA_EINVAL, "at most 64 query heads per KV head");
+        if (!aligned16(out) || !aligned16(q_step) || !aligned16(ws))
+            return fail(SA_EINVAL, "out, q_out and ws must be 16-byte aligned");
+        const size_t need = sa_paged_decode_ws_bytes(c, n_seq, n_q_heads);
+        if (need > 0 && (!ws || ws_bytes < need)) return fail(SA_ENOMEM, "workspace too small for the partials");
+        SA_TRY(on_cache_device(c));
+        SA_TRY(append_impl(c, layer, q, k, v, part, n_part, n_seq, 1, nullptr, seq_ids, n_q_heads, q_norm_w, k_norm_w,
+                           eps, rope_cos, rope_sin, rope_max_pos, q_step, nullptr, nullptr, stream));
+        SA_TRY(decode_fp8(c, layer, q_step, n_seq, seq_ids, n_q_heads, 1, scale, out,
+                          ws ? static_cast<char*>(ws) + head : nullptr, ws_bytes - head, stream));
+        return commit ? sa_kvcache_commit(c, seq_ids, n_seq, 1, stream) : SA_OK;
+    }
     int max_len = 0;
     long long total = 0;
     vd = c->pt.check_decode(seq_ids, n_seq, 1, &max_len, &total);
     if (!vd.ok()) return refused(vd);
     std::vector<int32_t> pos(n_seq);
     for (int i = 0; i < n_seq; ++i) pos[i] = c->pt.len(seq_ids ? seq_ids[i] : i);
-    PagedView pv;
-    pv.k_pool = k_pool_of(c, layer); pv.v_pool = v_pool_of(c, layer);
-    pv.block_table = c->d_table; pv.seq_lens = c->d_lens;
-    pv.n_kv = c->desc.num_kv_heads; pv.d = c->desc.head_dim;
-    pv.max_pages = c->desc.max_pages_per_seq; pv.num_pages = c->desc.num_pages;
-    pv.bf16 = c->desc.kv_dtype == SA_DTYPE_BF16;
+    const PagedView pv = view_of(c, layer);
     FusedAppend f{};
     f.k = k; f.v = v; f.wq = q_norm_w; f.wk = k_norm_w; f.eps = eps;
     f.cos_t = rope_cos; f.sin_t = rope_sin; f.rope_max_pos = rope_max_pos;
@@ -1074,14 +1336,16 @@ extern "C" sa_status sa_kvcache_gather(const sa_kvcache* c, int layer, int seq, 
     dim3 grid(len, c->desc.num_kv_heads);
     const int32_t* row = c->d_table + (size_t)seq * c->desc.max_pages_per_seq;
     hipStream_t st = as_stream(stream);
-    if (c->desc.kv_dtype == SA_DTYPE_BF16)
-        hipLaunchKernelGGL(gather_kernel<true>, grid, dim3(128), 0, st, k_pool_of(c, layer),
-                           v_pool_of(c, layer), row, c->desc.num_kv_heads, c->desc.head_dim, len,
-                           k_out, v_out);
-    else
-        hipLaunchKernelGGL(gather_kernel<false>, grid, dim3(128), 0, st, k_pool_of(c, layer),
-                           v_pool_of(c, layer), row, c->desc.num_kv_heads, c->desc.head_dim, len,
-                           k_out, v_out);
+    const PagedView pv = view_of(c, layer);
+    auto launch = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, grid, dim3(128), 0, st, k_pool_of(c, layer), v_pool_of(c, layer), pv.k_scale,
+                           pv.v_scale, row, c->desc.num_kv_heads, c->desc.head_dim, len, k_out, v_out);
+    };
+    switch (c->desc.kv_dtype) {
+        case SA_DTYPE_FP8: launch(gather_kernel<SA_DTYPE_FP8>); break;
+        case SA_DTYPE_BF16: launch(gather_kernel<SA_DTYPE_BF16>); break;
+        default: launch(gather_kernel<SA_DTYPE_F32>);
+    }
     SA_CHECK_LAUNCH();
     return SA_OK;
 }

@@ -86,6 +86,15 @@ Verdict PageTable::set_len(int seq, int len) {
     return kOk;
 }
 
+Verdict PageTable::set_lens(const int32_t* seqs, const int32_t* lens, int n) {
+    Verdict v = check_rows(seqs, n, true);
+    if (!v.ok()) return v;
+    for (int i = 0; i < n; ++i)
+        if (lens[i] < 0 || lens[i] > capacity(seqs[i])) return refuse(SA_EFULL, "length exceeds reserved pages");
+    for (int i = 0; i < n; ++i) lens_[seqs[i]] = lens[i];
+    return kOk;
+}
+
 Verdict PageTable::check_rows(const int32_t* ids, int n, bool unique) const {
     if (n < 0) return refuse(SA_EINVAL, "negative sequence count");
     if (!ids) {
@@ -107,13 +116,30 @@ Verdict PageTable::check_append(const int32_t* ids, int n, int S, int rope_max_p
     Verdict v = check_rows(ids, n, true);
     if (!v.ok()) return v;
     for (int i = 0; i < n; ++i) {
-        const int s = ids ? ids[i] : i;
-        const long long end = (long long)lens_[s] + S;
-        if (end > capacity(s)) return refuse(SA_EFULL, "KV cache full, cannot append more tokens");
-        if (rope_max_pos > 0 && end > rope_max_pos) return refuse(SA_ERANGE, "position beyond RoPE table");
-        for (long long j = lens_[s] / kPage; j * kPage < end; ++j)
-            if (refs_[row(s)[j]] > 1) return refuse(SA_EINVAL, "append into a page that another sequence shares");
+        v = check_append_row(ids ? ids[i] : i, S, rope_max_pos);
+        if (!v.ok()) return v;
     }
+    return kOk;
+}
+
+Verdict PageTable::check_append(const int32_t* ids, int n, const int32_t* counts, int rope_max_pos) const {
+    Verdict v = check_rows(ids, n, true);
+    if (!v.ok()) return v;
+    for (int i = 0; i < n; ++i) {
+        if (counts[i] < 0) return refuse(SA_EINVAL, "counts must be >= 0");
+        if (counts[i] == 0) continue;
+        v = check_append_row(ids ? ids[i] : i, counts[i], rope_max_pos);
+        if (!v.ok()) return v;
+    }
+    return kOk;
+}
+
+Verdict PageTable::check_append_row(int s, int S, int rope_max_pos) const {
+    const long long end = (long long)lens_[s] + S;
+    if (end > capacity(s)) return refuse(SA_EFULL, "KV cache full, cannot append more tokens");
+    if (rope_max_pos > 0 && end > rope_max_pos) return refuse(SA_ERANGE, "position beyond RoPE table");
+    for (long long j = lens_[s] / kPage; j * kPage < end; ++j)
+        if (refs_[row(s)[j]] > 1) return refuse(SA_EINVAL, "append into a page that another sequence shares");
     return kOk;
 }
 

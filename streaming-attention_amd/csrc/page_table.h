@@ -48,12 +48,16 @@ public:
     // the new capacity is cut to it (*len_cut tells the caller to publish it).
     Verdict set_pages(int seq, const int32_t* pages, int n, bool* len_cut);
     Verdict set_len(int seq, int len);
+    // Lengths lens[0, n) of rows seqs[0, n), each listed once; refused as a whole.
+    Verdict set_lens(const int32_t* seqs, const int32_t* lens, int n);
     // Rows ids[0, n) (NULL: 0 .. n-1) are cache rows; with unique, no row twice.
     Verdict check_rows(const int32_t* ids, int n, bool unique) const;
     // An append of S tokens to each row: every row has pages of its own (none
     // that another row shares) for tokens len .. len + S - 1 and, when
     // rope_max_pos > 0, len + S <= rope_max_pos.
     Verdict check_append(const int32_t* ids, int n, int S, int rope_max_pos) const;
+    // The same of counts[i] >= 0 tokens to row i.
+    Verdict check_append(const int32_t* ids, int n, const int32_t* counts, int rope_max_pos) const;
     // A decode over len + n_pending tokens of each row: every row has pages for
     // them.  Returns the longest such length and their sum.
     Verdict check_decode(const int32_t* ids, int n, int n_pending, int* max_len, long long* total) const;
@@ -100,6 +104,7 @@ private:
     std::vector<int32_t> free_;    // stack of free pages
     std::vector<int32_t> refs_;    // [num_pages]: rows that list the page, 0 = free
 
+    Verdict check_append_row(int seq, int S, int rope_max_pos) const;
     int32_t* row_mut(int seq) { return table_.data() + (size_t)seq * max_pages_; }
 };
 

@@ -23,6 +23,7 @@ namespace sa {
 
 __device__ __forceinline__ float plain_value(float v) { return v; }
 __device__ __forceinline__ float plain_value(uint16_t v) { return bf16_lo(v); }
+__device__ __forceinline__ float plain_value(uint8_t v) { return __builtin_amdgcn_cvt_f32_fp8(v, 0); }   // e4m3
 
 // Eight values from a 16-byte aligned place.
 __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
@@ -41,6 +42,22 @@ __device__ __forceinline__ void load8(const uint16_t* p, float (&v)[8]) {
         v[2 * i + 1] = bf16_hi(x[i]);
     }
 }
+
+// Eight codes in e4m3 from an 8-byte aligned place.
+__device__ __forceinline__ void load8(const uint8_t* p, float (&v)[8]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int x = reinterpret_cast<const int*>(p)[h];
+        v[4 * h] = __builtin_amdgcn_cvt_f32_fp8(x, 0);
+        v[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(x, 1);
+        v[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(x, 2);
+        v[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(x, 3);
+    }
+}
+
+struct NoScale {
+    __device__ __forceinline__ float operator()(int) const { return 1.f; }
+};
 
 // 0 where all values are finite, else NaN.
 template <int N>
@@ -65,9 +82,11 @@ struct PlainRow {
     __device__ __forceinline__ bool lost() const { return l != l; }
 
     // n keys (1 .. 64), lane i's score is that of key i: c sum_d q[d] key(i)[d].
-    // key(i), value(i): where key or value i starts, for i < n.
-    template <class T, class Key, class Value>
-    __device__ __forceinline__ void keys(int n, const T* q, float c, const Key& key, const Value& value) {
+    // key(i), value(i): where key or value i starts, for i < n; ks(i), vs(i): a
+    // power of two that its elements are times.
+    template <class T, class Key, class Value, class KeyScale = NoScale, class ValueScale = NoScale>
+    __device__ __forceinline__ void keys(int n, const T* q, float c, const Key& key, const Value& value,
+                                         const KeyScale& ks = {}, const ValueScale& vs = {}) {
         const int lane = threadIdx.x & (kWave - 1);
         const auto* k = key(min(lane, n - 1));
         float s = 0.f;
@@ -79,7 +98,7 @@ struct PlainRow {
 #pragma unroll
             for (int i = 0; i < 8; ++i) s = fmaf(x[i], y[i], s);
         }
-        s = lane < n ? s * c : -INFINITY;
+        s = lane < n ? s * ks(min(lane, n - 1)) * c : -INFINITY;
         const float top = group_reduce<OpMax, 1, kWave>(s);   // leaves NaN out, which the sums then hold
         const float m_new = fmaxf(m, top);
         const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
@@ -98,7 +117,7 @@ struct PlainRow {
             const float w = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), i));
             const auto* v = value(i) + lane * E;
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[e] = fmaf(w, plain_value(v[e]), o[e]);
+            for (int e = 0; e < E; ++e) o[e] = fmaf(w, plain_value(v[e]) * vs(i), o[e]);
         }
     }
 };

@@ -34,4 +34,16 @@ size_t ranges_ws(int n_rows, int n_q, int d, long long own_tokens, long long gro
 sa_status decode_ranges(const PagedView& c, const float* q, int n_q, const RangePlan& plan, float scale, float* out,
                         void* ws, size_t ws_bytes, hipStream_t st);
 
+// A chunk of n new tokens, appended at positions len .. len + n - 1 of a cache row,
+// each seeing what came before it and itself; first: its first row of q and out.
+struct ChunkSeq {
+    int32_t cache_row, len, n, first;
+};
+
+// Attention of chunks of new tokens: q and out [rows][n_q][D], fp32 or (q16) bf16.
+// extend_rows_ws: enough for any lengths of at most max_tokens.
+size_t extend_rows_ws(int n, const int32_t* counts, int n_q, int n_kv, int d, bool f32, long long max_tokens);
+sa_status extend_rows(const PagedView& c, const void* q, bool q16, int n_q, const ChunkSeq* seqs, int n, float scale,
+                      void* out, void* ws, size_t ws_bytes, hipStream_t st);
+
 }  // namespace sa

@@ -53,6 +53,9 @@ namespace {
 using pf::lds_s16x4_t;
 using pf::lds_u8_t;
 using pf::s16x4_t;
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef int s32x2_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) s32x2_t lds_s32x2_t;
 
 constexpr int kTile = 32;                    // keys per tile; divides a page
 constexpr int kWaves = 4;
@@ -62,21 +65,27 @@ constexpr int kChunkTiles = 1024;            // tiles of one chunk, whose page i
 constexpr int kSources = 2 * kRowsPerLaunch;
 constexpr float kRaiseAt = 65536.f;          // a lane's sum of weights that raises the running max
 
-struct RangeArgs {
-    const float* q;          // [n_rows][n_q][D]
+// What every launch over a cache has.
+struct CacheArgs {
+    const void* q;           // [rows][n_q][D], fp32 or (chunks of tokens) bf16
     const void* k;           // pool [pages][n_kv][64][D]
     const void* v;
+    const uint8_t* k_scale;  // 8 bits: [pages][n_kv][64]
+    const uint8_t* v_scale;
     const int32_t* table;    // [max_seqs][max_pages]
-    float* out;              // [n_rows][n_q][D]
+    void* out;               // like q
     float* part_o;           // [partial rows][n_kv][D]
     float* part_ml;          // [partial rows][n_kv][2]
     int n_kv, n_q, rep, max_pages, num_pages;
+    uint32_t rep_inv;                        // ceil(2^20 / rep): j / rep = j rep_inv >> 20 for query rows j
+    float sl2;                               // scale * log2(e)
+};
+
+struct RangeArgs : CacheArgs {
     int n_groups, n_rows;
     int row_block;                           // query rows of a workgroup
     int chunk_group, chunk_own;              // tiles
-    uint32_t rep_inv;                        // ceil(2^20 / rep): j / rep = j rep_inv >> 20 for query rows j
     uint64_t single;                         // rows with one partial, which is the output
-    float sl2;                               // scale * log2(e)
     // Sources 0 .. n_groups - 1 are the groups', n_groups + i is row i's own.
     RangeSource src[kSources];
     int32_t start[kSources + 1];             // a source's first workgroup in the grid
@@ -113,17 +122,23 @@ __device__ __forceinline__ TileSpan tile_span(const RangeSource& s, int u) {
     return r;
 }
 
-template <int D, bool BF16>
+// The cached values' type, as the cache's sa_dtype.
+constexpr int kF32 = SA_DTYPE_F32, kBf16 = SA_DTYPE_BF16, kFp8 = SA_DTYPE_FP8;
+
+template <int D, int KV>
 struct Geo {
-    static constexpr int ROWB = D * (BF16 ? 2 : 4);   // bytes of one key's row
+    static constexpr bool BF16 = KV == kBf16, FP8 = KV == kFp8;
+    static constexpr int ROWB = D * (FP8 ? 1 : BF16 ? 2 : 4);   // bytes of one key's row
     static constexpr int HALF = kTile * ROWB;         // K or V of a tile
-    static constexpr int TILEB = 2 * HALF;
+    static constexpr int SCALES = 2 * kTile;          // 8 bits: bytes of the tile's scales, K's, then V's
+    static constexpr int TILEB = 2 * HALF + (FP8 ? SCALES : 0);
+    static constexpr int MORE = FP8 ? 1 : 0;          // wave loads of the scales
     static constexpr int CPR = ROWB / 16;             // 16-byte chunks of a row
     static constexpr int RPL = kWave / CPR;           // rows per wave load
     static constexpr int NL = kTile / RPL;            // wave loads per half
     static constexpr int KS = D / 32, DB = D / 16;
-    static constexpr int NT = BF16 ? 1 : kTerms;      // terms of a cached value
-    static constexpr int RT = BF16 ? 1 : 2;           // most tiles of 16 query rows of a wave
+    static constexpr int NT = KV == kF32 ? kTerms : 1;   // terms of a cached value
+    static constexpr int RT = KV == kF32 ? 2 : 1;     // most tiles of 16 query rows of a wave
     static constexpr int ROWS = kWaves * RT * 16;     // query rows of a workgroup
     // LDS: one tile per wave, or the partials of the waves' query rows at the end.
     static constexpr int LDS = kWaves * (TILEB > 16 * RT * D * 4 ? TILEB : 16 * RT * D * 4);
@@ -132,9 +147,12 @@ struct Geo {
     // + b (a, b < 4) of a K fragment read, and the rows of a V^T read (bf16: 8g
     // + 4u + b with b < 4 and g of one half wave; fp32: 8g + e, g < 4), fall on
     // different banks; for fp32 products (F32) 16 neighbouring rows, and 4g + e.
+    // 8 bits: the 16 rows of a K fragment read as above (16 codes a lane), rows 8g + s / 2
+    // (s < 16, 8 codes a lane) of a V^T read.
     template <bool F32>
     static __device__ __forceinline__ int swz(int r) {
         if constexpr (F32) return r & 15;
+        else if constexpr (FP8) return (CPR == 8 ? ((r >> 1) & 1) << 2 : 0) | (((r >> 4) ^ (r >> 2)) & 1) << 1 | ((r >> 3) & 1);
         else if constexpr (!BF16) return (((r >> 3) & 3) << 2) | (r & 3);
         else if constexpr (CPR == 16) return ((r & 3) << 2) | (((r >> 3) & 1) << 1) | ((r >> 4) & 1);
         else return (((r >> 1) & 1) << 2) | (((r >> 3) & 1) << 1) | ((r >> 4) & 1);
@@ -153,6 +171,23 @@ __device__ __forceinline__ void dma16_nt(const void* g, lds_u8_t* dst) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(g), "s"(m) : "memory", "m0");
 }
 
+// The same of 4 bytes per lane.
+__device__ __forceinline__ void dma4_nt(const void* g, lds_u8_t* dst) {
+    const uint32_t m = static_cast<uint32_t>(reinterpret_cast<size_t>(dst));
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off nt" ::"v"(g), "s"(m) : "memory", "m0");
+}
+
+// Eight codes, times a power of two.
+__device__ __forceinline__ bf16x8_t codes_bf16x8(uint32_t lo, uint32_t hi, float scale) {
+    const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+    const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+    const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+    const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+    return __builtin_bit_cast(bf16x8_t, u32x4_t{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b),
+                                                __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)});
+}
+__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
+
 template <int N>
 __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -163,17 +198,18 @@ __device__ __forceinline__ float row_max(float v) { return group_reduce<OpMax, 1
 
 // The state of one wave: 16 RT query rows, lane (g = lane / 16, r16 = lane %
 // 16) holds row r16 of each tile of 16.
-template <int D, bool BF16, int RT>
+template <int D, int KV, int RT>
 struct WaveState {
-    using G = Geo<D, BF16>;
-    static constexpr int PAIRS = BF16 ? 3 : 6;
+    using G = Geo<D, KV>;
+    static constexpr bool BF16 = G::BF16, FP8 = G::FP8;
+    static constexpr int PAIRS = KV == kF32 ? 6 : 3;
     // fp32 values whose split into terms would serve one tile of query rows only:
     // v_mfma_f32_16x16x4_f32 instead.
-    static constexpr bool F32 = !BF16 && RT == 1;
+    static constexpr bool F32 = KV == kF32 && RT == 1;
     static __device__ __forceinline__ int off(int r, int c) { return G::template off<F32>(r, c); }
     // Terms of the cached and of the other operand of a product, largest first.
-    static constexpr int pair_a(int pr) { return BF16 ? 0 : (pr == 2 || pr == 4 ? 1 : pr == 5 ? 2 : 0); }
-    static constexpr int pair_b(int pr) { return BF16 ? pr : (pr == 1 || pr == 4 ? 1 : pr == 3 ? 2 : 0); }
+    static constexpr int pair_a(int pr) { return KV != kF32 ? 0 : (pr == 2 || pr == 4 ? 1 : pr == 5 ? 2 : 0); }
+    static constexpr int pair_b(int pr) { return KV != kF32 ? pr : (pr == 1 || pr == 4 ? 1 : pr == 3 ? 2 : 0); }
 
     bf16x8_t q[RT][G::KS][kTerms];
     f32x4_t qf[D / 16], pf[2];   // F32: q from D / 4 g on, the weights
@@ -198,7 +234,21 @@ struct WaveState {
             cap[rt] = -1.f;
         }
     }
-    __device__ __forceinline__ void load_q(int rt, const float* row, float sl2) {
+    // 8 bits: a lane reads 16 codes of a key at once, which two products take, so
+    // product ks multiplies d = 64 (ks / 2) + 16 g + 8 (ks % 2) ...
+    template <class T>
+    __device__ __forceinline__ void load_q(int rt, const T* row, float sl2) {
+        if constexpr (sizeof(T) == 2) {
+            static_assert(!F32, "bf16 queries of fp32 caches");
+#pragma unroll
+            for (int ks = 0; ks < G::KS; ++ks) {
+                const int d = FP8 ? 64 * (ks / 2) + 16 * g + 8 * (ks % 2) : 32 * ks + 8 * g;
+                const u32x4_t x = *reinterpret_cast<const u32x4_t*>(row + d);
+                split_terms(f32x4_t{bf16_lo(x[0]), bf16_hi(x[0]), bf16_lo(x[1]), bf16_hi(x[1])} * sl2,
+                            f32x4_t{bf16_lo(x[2]), bf16_hi(x[2]), bf16_lo(x[3]), bf16_hi(x[3])} * sl2, q[rt][ks]);
+            }
+            return;
+        } else {
         if constexpr (F32) {
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) qf[i] = *reinterpret_cast<const f32x4_t*>(row + D / 4 * g + 4 * i) * sl2;
@@ -208,16 +258,28 @@ struct WaveState {
 #pragma unroll
         for (int ks = 0; ks < G::KS; ++ks)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) x[ks][i] = *reinterpret_cast<const f32x4_t*>(row + 32 * ks + 8 * g + 4 * i);
+            for (int i = 0; i < 2; ++i) {
+                const int d = FP8 ? 64 * (ks / 2) + 16 * g + 8 * (ks % 2) : 32 * ks + 8 * g;
+                x[ks][i] = *reinterpret_cast<const f32x4_t*>(row + d + 4 * i);
+            }
 #pragma unroll
         for (int ks = 0; ks < G::KS; ++ks) split_terms(x[ks][0] * sl2, x[ks][1] * sl2, q[rt][ks]);
+        }
     }
 
-    // Scores of the tile whose K sits at kb, masked to its tokens [lo, hi), and
+    // Scores of the tile whose K sits at kb, masked to its tokens [lo, hi) and, in a
+    // chunk (CAUSAL), to those before limit[rt], and
     // the weights p = 2^(s - m) as three bf16 terms.  Element 4 h + e of a lane
     // is key 8 g + 4 h + e (F32: 16 h + 4 g + e, the operand of V^T P^T as it is;
     // the products take d in the order that lets a lane read 16 bytes of K).
-    __device__ __forceinline__ void scores(const lds_u8_t* kb, const TileSpan& sp) {
+    template <bool CAUSAL>
+    __device__ __forceinline__ void scores(const lds_u8_t* kb, const TileSpan& sp, const int (&limit)[RT], int first_limit) {
+        float vs[8];   // 8 bits: the scales of V's rows, which the weights take
+        if constexpr (FP8) {
+            const u32x2_t b = *reinterpret_cast<const __attribute__((address_space(3))) u32x2_t*>(kb + 2 * G::HALF + kTile + 8 * g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) vs[j] = scale_of(b[j >> 2] >> (8 * (j & 3)) & 255u);
+        }
         f32x4_t s[RT][2];
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) s[rt][0] = s[rt][1] = f32x4_t{b[rt], b[rt], b[rt], b[rt]};
@@ -240,7 +302,11 @@ struct WaveState {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int r = 8 * (r16 >> 2) + 4 * h + (r16 & 3);
-                if constexpr (BF16) {
+                if constexpr (FP8) {
+                    const u32x4_t x = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(
+                        kb + off(r, 4 * (ks / 2) + g));
+                    kf[h][0] = codes_bf16x8(x[2 * (ks & 1)], x[2 * (ks & 1) + 1], scale_of(kb[2 * G::HALF + r]));
+                } else if constexpr (BF16) {
                     kf[h][0] = *reinterpret_cast<const __attribute__((address_space(3))) bf16x8_t*>(
                         kb + off(r, 4 * ks + g));
                 } else {
@@ -257,14 +323,15 @@ struct WaveState {
                         s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[h][pair_a(pr)], q[rt][ks][pair_b(pr)],
                                                                            s[rt][h], 0, 0, 0);
         }
-        const bool ragged = sp.hi - sp.lo < kTile;
+        const bool ragged = sp.hi - sp.lo < kTile || (CAUSAL && sp.hi > first_limit);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             if (ragged) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int t = sp.t0 + (F32 ? 16 * (j >> 2) + 4 * g + (j & 3) : 8 * g + j);
-                    if (t < sp.lo || t >= sp.hi) s[rt][j >> 2][j & 3] = -INFINITY;
+                    if (t < sp.lo || t >= sp.hi || (CAUSAL && t >= limit[rt])) s[rt][j >> 2][j & 3] = -INFINITY;
+                    if (FP8 && (t < sp.lo || t >= sp.hi)) vs[j] = 0.f;   // a byte that no row has written
                 }
             }
             float w[8];
@@ -290,6 +357,9 @@ struct WaveState {
                 cap[rt] = m_new == -INFINITY ? -1.f : kRaiseAt;
             }
             l[rt] += sum;
+            if constexpr (FP8)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[j] *= vs[j];
             pf[0] = f32x4_t{w[0], w[1], w[2], w[3]};
             pf[1] = f32x4_t{w[4], w[5], w[6], w[7]};
             if constexpr (!F32) split_terms(pf[0], pf[1], p[rt]);
@@ -321,7 +391,13 @@ struct WaveState {
             bf16x8_t vf[ND][G::NT];
 #pragma unroll
             for (int d = 0; d < ND; ++d) {
-                if constexpr (BF16) {
+                if constexpr (FP8) {
+                    // Lane s of a group of 16 reads row 8 g + s / 2, columns 16 db + 8 (s %
+                    // 2) ..; lane r16 receives the codes V[8 g + e][16 db + r16].
+                    const s32x2_t x = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                        (lds_s32x2_t*)(vb + off(8 * g + (r16 >> 1), d0 + d) + (r16 & 1) * 8));
+                    vf[d][0] = codes_bf16x8(x[0], x[1], 1.f);
+                } else if constexpr (BF16) {
                     // Lane s of a group of 16 reads row 8 g + 4 u + s / 4, columns
                     // 16 db + 4 (s % 4) ..; lane r16 receives V[8 g + 4 u + e][16 db + r16].
                     const int c = 2 * (d0 + d) + ((r16 & 3) >> 1), h8 = (r16 & 1) * 8;
@@ -360,13 +436,14 @@ struct Item {
     int q0, q1;        // the workgroup's query rows of those
     int part0;         // the chunk's first partial row
     uint64_t single;   // RangeArgs::single from row0 on
+    int limit0;        // a chunk of new tokens: row r sees tokens before limit0 + r
 };
 
 // Query row j of an item: row row0 + j / rep of the launch, head j % rep of the
 // KV head.  j <= 64 rep and rep <= 64, so j rep < 2^20 and the product's quotient
 // is exact.
 static_assert(kRowsPerLaunch * kRangesMaxRep * kRangesMaxRep < (1 << 20), "query rows divided by a product");
-__device__ __forceinline__ int row_of(const RangeArgs& a, int j) { return (int)(((uint32_t)j * a.rep_inv) >> 20); }
+__device__ __forceinline__ int row_of(const CacheArgs& a, int j) { return (int)(((uint32_t)j * a.rep_inv) >> 20); }
 
 __device__ __forceinline__ int group_chunks(const RangeArgs& a, int g) {
     const int rows = (a.first[g + 1] - a.first[g]) * a.rep;
@@ -376,14 +453,21 @@ __device__ __forceinline__ int own_chunks(const RangeArgs& a, int row) {
     return a.start[a.n_groups + row + 1] - a.start[a.n_groups + row];
 }
 
+__device__ __forceinline__ void store4(float* p, f32x4_t v) { *reinterpret_cast<f32x4_t*>(p) = v; }
+__device__ __forceinline__ void store4(uint16_t* p, f32x4_t v) {
+    const bf16x2_t lo = __builtin_convertvector(f32x2_t{v[0], v[1]}, bf16x2_t);
+    const bf16x2_t hi = __builtin_convertvector(f32x2_t{v[2], v[3]}, bf16x2_t);
+    *reinterpret_cast<u32x2_t*>(p) = u32x2_t{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
+}
+
 // O (unnormalised), m and l of query row j of an item: the output itself if it
 // is the row's only partial.  c: float4 column.
-template <int D>
-__device__ __forceinline__ void put(const RangeArgs& a, const Item& it, int j, int c, f32x4_t o, float m, float l) {
+template <int D, class T>
+__device__ __forceinline__ void put(const CacheArgs& a, const Item& it, int j, int c, f32x4_t o, float m, float l) {
     const int r = row_of(a, j);
     if (it.single >> r & 1) {
         const int head = it.kvh * a.rep + j - r * a.rep;
-        *reinterpret_cast<f32x4_t*>(a.out + ((size_t)(it.row0 + r) * a.n_q + head) * D + 4 * c) = o * (1.0f / l);
+        store4(static_cast<T*>(a.out) + ((size_t)(it.row0 + r) * a.n_q + head) * D + 4 * c, o * (1.0f / l));
         return;
     }
     const size_t at = (size_t)(it.part0 + j) * a.n_kv + it.kvh;
@@ -393,18 +477,24 @@ __device__ __forceinline__ void put(const RangeArgs& a, const Item& it, int j, i
 
 // Returns the query rows, from it.q0 (RG = 4: the wave's first) on a bit each, that
 // the wave has to compute anew: their sums are not finite and nothing was put.
-template <int D, bool BF16, int RG, int RT>
-__device__ __forceinline__ uint64_t attend(const RangeArgs& a, const Item& it, lds_u8_t* smem, const int32_t* pages,
+// T: the queries' and the output's type; CAUSAL: the rows are a chunk of new tokens.
+template <int D, int KV, int RG, int RT, class T, bool CAUSAL>
+__device__ __forceinline__ uint64_t attend(const CacheArgs& a, const Item& it, lds_u8_t* smem, const int32_t* pages,
                                        float (*ml)[2]) {
-    using G = Geo<D, BF16>;
+    using G = Geo<D, KV>;
     constexpr int KG = kWaves / RG;
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int kg = wave / RG, rg = wave % RG;
     const int q_base = it.q0 + rg * 16 * RT;
 
-    WaveState<D, BF16, RT> w;
+    WaveState<D, KV, RT> w;
     w.init(lane);
+    int limit[RT];
+    const int first_limit = CAUSAL ? it.limit0 + row_of(a, it.q0) : 0;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt)
+        limit[rt] = CAUSAL ? it.limit0 + row_of(a, min(q_base + 16 * rt + w.r16, it.q1 - 1)) : 0;
 
     // Wave loads [first, first + N) of the 2 NL of tile u (K's, then V's) into the
     // tile at dst.  Rows outside the source's tokens read the nearest one inside.
@@ -421,11 +511,21 @@ __device__ __forceinline__ uint64_t attend(const RangeArgs& a, const Item& it, l
             dma16_nt(pool + at + (size_t)tok * G::ROWB + col, dst + (first + i) * 1024);
         }
     };
+    // 8 bits: the tile's scales, 8 lanes for K's and 8 for V's, behind its V at dst.
+    auto load_scales = [&](int u, lds_u8_t* dst) {
+        if constexpr (G::FP8) {
+            const size_t at = ((size_t)pages[u - it.u0] * a.n_kv + it.kvh) * SA_PAGE_TOKENS +
+                              (tile_span(it.src, u).t0 & (SA_PAGE_TOKENS - 1));
+            const uint8_t* s = (lane < 8 ? a.k_scale : a.v_scale) + at + 4 * (lane & 7);
+            if (lane < 16) dma4_nt(s, dst);
+        }
+    };
     auto load_queries = [&]() {
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
             const int j = min(q_base + 16 * rt + w.r16, it.q1 - 1), r = row_of(a, j);
-            w.load_q(rt, a.q + ((size_t)(it.row0 + r) * a.n_q + it.kvh * a.rep + j - r * a.rep) * D, a.sl2);
+            w.load_q(rt, static_cast<const T*>(a.q) + ((size_t)(it.row0 + r) * a.n_q + it.kvh * a.rep + j - r * a.rep) * D,
+                     a.sl2);
         }
     };
 
@@ -435,6 +535,7 @@ __device__ __forceinline__ uint64_t attend(const RangeArgs& a, const Item& it, l
         lds_u8_t* const vb = kb + G::HALF;
         int u = it.u0 + kg;
         if (u < it.u1) {
+            load_scales(u, kb + 2 * G::HALF);
             load(u, kb, 0, Half{});
             load(u, kb, G::NL, Half{});
         }
@@ -442,11 +543,12 @@ __device__ __forceinline__ uint64_t attend(const RangeArgs& a, const Item& it, l
         for (; u < it.u1; u += KG) {
             const bool more = u + KG < it.u1;
             wait_loads<G::NL>();                               // K; V may be in flight
-            w.scores(kb, tile_span(it.src, u));
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // K has been read
+            w.template scores<CAUSAL>(kb, tile_span(it.src, u), limit, first_limit);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // K and the scales have been read
             if (more) {
+                load_scales(u + KG, kb + 2 * G::HALF);
                 load(u + KG, kb, 0, Half{});
-                wait_loads<G::NL>();                           // V; the next K may be in flight
+                wait_loads<G::NL + G::MORE>();                 // V; the next K may be in flight
             } else {
                 wait_loads<0>();
             }
@@ -462,19 +564,23 @@ __device__ __forceinline__ uint64_t attend(const RangeArgs& a, const Item& it, l
         lds_u8_t* const ring = smem + kg * RG * G::TILEB;
         const int n_all = (it.u1 - it.u0 + KG - 1) / KG;                  // steps of the workgroup
         const int n = it.u0 + kg < it.u1 ? (it.u1 - it.u0 - kg + KG - 1) / KG : 0;   // of this key group
-        auto load_tile = [&](int t) { load(it.u0 + kg + t * KG, ring + (t % RG) * G::TILEB, rg * MINE, Mine{}); };
+        auto load_tile = [&](int t) {
+            lds_u8_t* dst = ring + (t % RG) * G::TILEB;
+            load_scales(it.u0 + kg + t * KG, dst + 2 * G::HALF);   // every wave, so that all wait for as many loads
+            load(it.u0 + kg + t * KG, dst, rg * MINE, Mine{});
+        };
         for (int t = 0; t < RG - 1; ++t)
             if (t < n) load_tile(t);
         load_queries();
         for (int t = 0; t < n_all; ++t) {
             // tiles t .. t + RG - 2 are in flight where the chunk has them
-            if (t + RG - 1 <= n) wait_loads<(RG - 2) * MINE>();
+            if (t + RG - 1 <= n) wait_loads<(RG - 2) * (MINE + G::MORE)>();
             else wait_loads<0>();
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (t + RG - 1 < n) load_tile(t + RG - 1);
             if (t < n) {
                 const lds_u8_t* kb = ring + (t % RG) * G::TILEB;
-                w.scores(kb, tile_span(it.src, it.u0 + kg + t * KG));
+                w.template scores<CAUSAL>(kb, tile_span(it.src, it.u0 + kg + t * KG), limit, first_limit);
                 w.weigh(kb + G::HALF);
             }
         }
@@ -492,7 +598,7 @@ __device__ __forceinline__ uint64_t attend(const RangeArgs& a, const Item& it, l
             anew |= (__ballot(j < it.q1 && !fine) & 0xffff) << (16 * rt);
             if (j < it.q1 && fine) {
 #pragma unroll
-                for (int db = 0; db < G::DB; ++db) put<D>(a, it, j, 4 * db + w.g, w.acc[rt][db], w.m[rt], l[rt]);
+                for (int db = 0; db < G::DB; ++db) put<D, T>(a, it, j, 4 * db + w.g, w.acc[rt][db], w.m[rt], l[rt]);
             }
         }
     } else {
@@ -532,7 +638,7 @@ __device__ __forceinline__ uint64_t attend(const RangeArgs& a, const Item& it, l
             const uint64_t bad = __ballot(mine && !(L + not_finite<1>(&o) < INFINITY));
             constexpr uint64_t row = (1ull << C) - 1;
             static_assert(ROWS <= 64, "a bit per row");
-            if (mine && !(bad >> (lane / C * C) & row)) put<D>(a, it, it.q0 + j, c, o, M, L);
+            if (mine && !(bad >> (lane / C * C) & row)) put<D, T>(a, it, it.q0 + j, c, o, M, L);
 #pragma unroll
             for (int g = 0; g < kWave / C; ++g)
                 if (bad >> (g * C) & row) anew |= 1ull << (j0 + g);
@@ -542,23 +648,35 @@ __device__ __forceinline__ uint64_t attend(const RangeArgs& a, const Item& it, l
 }
 
 // Query row j of an item without matrix instructions.
-template <int D, bool BF16>
-__device__ __forceinline__ void attend_plain(const RangeArgs& a, const Item& it, const int32_t* pages, int j) {
-    using T = std::conditional_t<BF16, uint16_t, float>;
+template <int D, int KV, class T, bool CAUSAL>
+__device__ __forceinline__ void attend_plain(const CacheArgs& a, const Item& it, const int32_t* pages, int j) {
+    using E = std::conditional_t<KV == kFp8, uint8_t, std::conditional_t<KV == kBf16, uint16_t, float>>;
     const int lane = threadIdx.x & (kWave - 1);
     const int r = row_of(a, j), head = it.kvh * a.rep + j - r * a.rep;
     const size_t row = ((size_t)(it.row0 + r) * a.n_q + head) * D;
     PlainRow<D> p;
     for (int u = it.u0; u < it.u1 && !p.lost(); ++u) {
-        const TileSpan sp = tile_span(it.src, u);
-        const size_t at = (((size_t)pages[u - it.u0] * a.n_kv + it.kvh) * SA_PAGE_TOKENS + (sp.lo & (SA_PAGE_TOKENS - 1))) * D;
-        p.keys(sp.hi - sp.lo, a.q + row, a.sl2,
-               [&](int i) { return static_cast<const T*>(a.k) + at + (size_t)i * D; },
-               [&](int i) { return static_cast<const T*>(a.v) + at + (size_t)i * D; });
+        TileSpan sp = tile_span(it.src, u);
+        if (CAUSAL) sp.hi = min(sp.hi, it.limit0 + r);
+        if (CAUSAL && sp.hi <= sp.lo) break;
+        const size_t key = ((size_t)pages[u - it.u0] * a.n_kv + it.kvh) * SA_PAGE_TOKENS + (sp.lo & (SA_PAGE_TOKENS - 1));
+        const size_t at = key * D;
+        auto value = [&](const void* pool, int i) { return static_cast<const E*>(pool) + at + (size_t)i * D; };
+        auto scale = [&](const uint8_t* s, int i) {
+            if constexpr (KV == kFp8) return scale_of(s[key + i]);
+            else return 1.f;
+        };
+        p.keys(sp.hi - sp.lo, static_cast<const T*>(a.q) + row, a.sl2, [&](int i) { return value(a.k, i); },
+               [&](int i) { return value(a.v, i); }, [&](int i) { return scale(a.k_scale, i); },
+               [&](int i) { return scale(a.v_scale, i); });
     }
     if (it.single >> r & 1) {
 #pragma unroll
-        for (int e = 0; e < p.E; ++e) a.out[row + lane * p.E + e] = p.o[e] / p.l;
+        for (int e = 0; e < p.E; ++e) {
+            const float v = p.o[e] / p.l;
+            if constexpr (sizeof(T) == 2) static_cast<T*>(a.out)[row + lane * p.E + e] = f32_to_bf16_rne(v);
+            else static_cast<T*>(a.out)[row + lane * p.E + e] = v;
+        }
         return;
     }
     const size_t at = (size_t)(it.part0 + j) * a.n_kv + it.kvh;
@@ -570,9 +688,39 @@ __device__ __forceinline__ void attend_plain(const RangeArgs& a, const Item& it,
     }
 }
 
-template <int D, bool BF16>
+// The tiles' pages; an id outside the pool (a table entry that was never set) is
+// clamped so that no load can fault.
+__device__ __forceinline__ void stage_pages(const CacheArgs& a, const Item& it, int32_t* pages) {
+    const int32_t* trow = a.table + (size_t)it.src.cache_row * a.max_pages;
+    for (int i = threadIdx.x; i < it.u1 - it.u0; i += kThreads)
+        pages[i] = min(max(trow[tile_span(it.src, it.u0 + i).t0 / SA_PAGE_TOKENS], 0), a.num_pages - 1);
+    __syncthreads();
+}
+
+// An item's query rows by as many waves as they need.
+template <int D, int KV, class T, bool CAUSAL>
+__device__ __forceinline__ void attend_item(const CacheArgs& a, const Item& it, lds_u8_t* smem, const int32_t* pages,
+                                            float (*ml)[2]) {
+    const int rows = it.q1 - it.q0;
+    uint64_t anew;
+    int first = it.q0;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    if constexpr (KV != kF32) {
+        if (rows <= 16) anew = attend<D, KV, 1, 1, T, CAUSAL>(a, it, smem, pages, ml);
+        else if (rows <= 32) anew = attend<D, KV, 2, 1, T, CAUSAL>(a, it, smem, pages, ml);
+        else anew = attend<D, KV, 4, 1, T, CAUSAL>(a, it, smem, pages, ml), first += 16 * wave;
+    } else {
+        if (rows <= 16) anew = attend<D, KV, 1, 1, T, CAUSAL>(a, it, smem, pages, ml);
+        else if (rows <= 32) anew = attend<D, KV, 1, 2, T, CAUSAL>(a, it, smem, pages, ml);
+        else if (rows <= 64) anew = attend<D, KV, 2, 2, T, CAUSAL>(a, it, smem, pages, ml);
+        else anew = attend<D, KV, 4, 2, T, CAUSAL>(a, it, smem, pages, ml), first += 32 * wave;
+    }
+    for (; anew; anew &= anew - 1) attend_plain<D, KV, T, CAUSAL>(a, it, pages, first + __builtin_ctzll(anew));
+}
+
+template <int D, int KV>
 __global__ void __launch_bounds__(kThreads) range_attn_kernel(RangeArgs a) {
-    using G = Geo<D, BF16>;
+    using G = Geo<D, KV>;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ int32_t pages[kChunkTiles];
     __shared__ float ml[G::ROWS][2];
@@ -601,28 +749,9 @@ __global__ void __launch_bounds__(kThreads) range_attn_kernel(RangeArgs a) {
     it.part0 = a.base[lo] + chunk * it.rows;
     it.single = a.single >> it.row0;
 
-    // The tiles' pages; an id outside the pool (a table entry that was never
-    // set) is clamped so that no load can fault.
-    const int32_t* trow = a.table + (size_t)it.src.cache_row * a.max_pages;
-    for (int i = threadIdx.x; i < it.u1 - it.u0; i += kThreads)
-        pages[i] = min(max(trow[tile_span(it.src, it.u0 + i).t0 / SA_PAGE_TOKENS], 0), a.num_pages - 1);
-    __syncthreads();
-
-    const int rows = it.q1 - it.q0;
-    uint64_t anew;
-    int first = it.q0;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    if constexpr (BF16) {
-        if (rows <= 16) anew = attend<D, BF16, 1, 1>(a, it, smem, pages, ml);
-        else if (rows <= 32) anew = attend<D, BF16, 2, 1>(a, it, smem, pages, ml);
-        else anew = attend<D, BF16, 4, 1>(a, it, smem, pages, ml), first += 16 * wave;
-    } else {
-        if (rows <= 16) anew = attend<D, BF16, 1, 1>(a, it, smem, pages, ml);
-        else if (rows <= 32) anew = attend<D, BF16, 1, 2>(a, it, smem, pages, ml);
-        else if (rows <= 64) anew = attend<D, BF16, 2, 2>(a, it, smem, pages, ml);
-        else anew = attend<D, BF16, 4, 2>(a, it, smem, pages, ml), first += 32 * wave;
-    }
-    for (; anew; anew &= anew - 1) attend_plain<D, BF16>(a, it, pages, first + __builtin_ctzll(anew));
+    it.limit0 = 0;
+    stage_pages(a, it, pages);
+    attend_item<D, KV, float, false>(a, it, smem, pages, ml);
 }
 
 // Joins the partials of row blockIdx.y's query head blockIdx.x: thread (s, c)
@@ -679,16 +808,16 @@ __global__ void __launch_bounds__(256) range_merge_kernel(RangeArgs a) {
         o += so[k][c] * wk;
         L += sm[k][1] * wk;
     }
-    float* dst = a.out + ((size_t)row * a.n_q + head) * D + 4 * c;
+    float* dst = static_cast<float*>(a.out) + ((size_t)row * a.n_q + head) * D + 4 * c;
     *reinterpret_cast<f32x4_t*>(dst) = n ? o * (1.0f / L) : f32x4_t{0.f, 0.f, 0.f, 0.f};
 }
 
-template <int D, bool BF16>
+template <int D, int KV>
 sa_status launch(const RangeArgs& a, bool merge, hipStream_t st) {
     const int n_src = a.n_groups + a.n_rows;
     if (a.start[n_src] > 0) {
-        constexpr int lds = Geo<D, BF16>::LDS;
-        constexpr auto kernel = range_attn_kernel<D, BF16>;
+        constexpr int lds = Geo<D, KV>::LDS;
+        constexpr auto kernel = range_attn_kernel<D, KV>;
         SA_TRY(pf::opt_in_lds<kernel>(lds));
         hipLaunchKernelGGL(kernel, dim3(a.n_kv, a.start[n_src]), dim3(kThreads), lds, st, a);
         SA_CHECK_LAUNCH();
@@ -735,15 +864,24 @@ size_t ranges_ws(int n_rows, int n_q, int d, long long own_tokens, long long gro
     return (size_t)(std::min(n_rows, kRowsPerLaunch) * per_row) * n_q * (d + 2) * sizeof(float);
 }
 
-sa_status decode_ranges(const PagedView& c, const float* q, int n_q, const RangePlan& plan, float scale, float* out,
-                        void* ws, size_t ws_bytes, hipStream_t st) {
-    RangeArgs a{};
-    a.k = c.k_pool; a.v = c.v_pool; a.table = c.block_table;
+namespace {
+
+void set_cache(CacheArgs& a, const PagedView& c, int n_q, float scale) {
+    a.k = c.k_pool; a.v = c.v_pool; a.k_scale = c.k_scale; a.v_scale = c.v_scale; a.table = c.block_table;
     a.n_kv = c.n_kv; a.n_q = n_q; a.rep = n_q / c.n_kv;
     a.max_pages = c.max_pages; a.num_pages = c.num_pages;
     a.sl2 = scale * pf::kLog2eP;
-    a.row_block = c.bf16 ? Geo<128, true>::ROWS : Geo<128, false>::ROWS;
     a.rep_inv = ((1u << 20) + a.rep - 1) / a.rep;
+}
+
+}  // namespace
+
+sa_status decode_ranges(const PagedView& c, const float* q, int n_q, const RangePlan& plan, float scale, float* out,
+                        void* ws, size_t ws_bytes, hipStream_t st) {
+    RangeArgs a{};
+    set_cache(a, c, n_q, scale);
+    const bool f32 = c.kv == SA_DTYPE_F32;
+    a.row_block = f32 ? Geo<128, kF32>::ROWS : Geo<128, kBf16>::ROWS;
     int g = 0, done = 0;   // the group of the launch's first row, and its rows already attended
     for (int i0 = 0; i0 < plan.n_rows; i0 += kRowsPerLaunch) {
         a.n_rows = std::min(kRowsPerLaunch, plan.n_rows - i0);
@@ -785,13 +923,13 @@ sa_status decode_ranges(const PagedView& c, const float* q, int n_q, const Range
                     n += (long long)ceil_div(tiles_of(a.src[s]), tiles) * blocks_of(s) * a.n_kv;
                 return n;
             };
-            int chunk = whole && longest <= (c.bf16 ? 4 : 2) * kWaves ? std::max(1, longest)
+            int chunk = whole && longest <= (f32 ? 2 : 4) * kWaves ? std::max(1, longest)
                                                                       : pick_tiles(round, work, workgroups);
             if (attn_kv_block() > 0) chunk = attn_kv_block() / kTile;
             chunk = std::min(std::max(chunk, ceil_div(longest, kMaxChunks)), kChunkTiles);
             return std::pair<int, long long>(chunk, workgroups(chunk));
         };
-        const long long slots = (c.bf16 ? 2LL : 1LL) * device_cu_count(), round = slots + slots / 4;
+        const long long slots = (f32 ? 1LL : 2LL) * device_cu_count(), round = slots + slots / 4;
         const auto own = pick(a.n_groups, n_src, round, a.n_groups == 0);
         a.chunk_own = own.first;
         a.chunk_group = pick(0, a.n_groups, std::max(round - own.second, round / 2), false).first;
@@ -823,13 +961,222 @@ sa_status decode_ranges(const PagedView& c, const float* q, int n_q, const Range
         }
         a.q = q + (size_t)i0 * n_q * c.d;
         a.out = out + (size_t)i0 * n_q * c.d;
-        if (c.bf16) {
-            if (c.d == 64) SA_TRY((launch<64, true>(a, merge, st)));
-            else SA_TRY((launch<128, true>(a, merge, st)));
-        } else {
-            if (c.d == 64) SA_TRY((launch<64, false>(a, merge, st)));
-            else SA_TRY((launch<128, false>(a, merge, st)));
+        if (c.d == 64) SA_TRY(c.kv == SA_DTYPE_FP8    ? (launch<64, kFp8>(a, merge, st))
+                              : c.kv == SA_DTYPE_BF16 ? (launch<64, kBf16>(a, merge, st))
+                                                      : (launch<64, kF32>(a, merge, st)));
+        else SA_TRY(c.kv == SA_DTYPE_FP8    ? (launch<128, kFp8>(a, merge, st))
+                    : c.kv == SA_DTYPE_BF16 ? (launch<128, kBf16>(a, merge, st))
+                                            : (launch<128, kF32>(a, merge, st)));
+    }
+    return SA_OK;
+}
+
+// ---------------------------------------------------------------- chunks of new tokens
+
+namespace {
+
+// Blocks of consecutive tokens of a sequence (as many query rows as a workgroup
+// takes) whose keys are cut into chunks of tiles; a workgroup takes a chunk of one
+// KV head for a block.
+struct ChunkArgs : CacheArgs {
+    int n_seq;
+    int block;                               // tokens of a block
+    int tiles;                               // of a chunk
+    ChunkSeq seq[kRowsPerLaunch];
+    int32_t start[kRowsPerLaunch + 1];       // a sequence's first item, of blocks x chunks
+    int32_t base[kRowsPerLaunch];            // its first partial row
+    int32_t chunks[kRowsPerLaunch];          // of its last block
+};
+static_assert(sizeof(ChunkArgs) <= 4096, "kernel arguments");
+static_assert(kRowsPerLaunch <= kWave, "a lane per sequence");
+
+// Tiles that the tokens of block b of a sequence see.
+__host__ __device__ inline int block_tiles(const ChunkSeq& s, int b, int block) {
+    return (s.len + (s.n < (b + 1) * block ? s.n : (b + 1) * block) - 1) / kTile + 1;
+}
+
+template <int D, int KV, class T>
+__global__ void __launch_bounds__(kThreads) chunk_attn_kernel(ChunkArgs a) {
+    using G = Geo<D, KV>;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    __shared__ int32_t pages[kChunkTiles];
+    __shared__ float ml[G::ROWS][2];
+    const int lane = threadIdx.x & (kWave - 1);
+    const int item = blockIdx.x / a.n_kv;
+    // The last sequence that starts at or before the item (those without tokens
+    // start where the next one does).
+    const int i = __popcll(__ballot(lane < a.n_seq && a.start[lane] <= item)) - 1;
+    const ChunkSeq sq = a.seq[i];
+    const int chunks = a.chunks[i], local = item - a.start[i];
+    const int b = local / chunks, c = local % chunks;
+    Item it;
+    it.kvh = blockIdx.x % a.n_kv;
+    it.u0 = c * a.tiles;
+    it.u1 = min(it.u0 + a.tiles, block_tiles(sq, b, a.block));
+    if (it.u0 >= it.u1) return;
+    const int t0 = b * a.block, n = min(a.block, sq.n - t0);
+    it.src = RangeSource{sq.cache_row, 0, 0, sq.len + t0 + n};
+    it.row0 = sq.first + t0;
+    it.rows = n * a.rep;
+    it.q0 = 0;
+    it.q1 = it.rows;
+    it.part0 = a.base[i] + (c * sq.n + t0) * a.rep;
+    it.single = chunks == 1 ? ~0ull : 0;
+    it.limit0 = sq.len + t0 + 1;
+    stage_pages(a, it, pages);
+    attend_item<D, KV, T, true>(a, it, (lds_u8_t*)smem_raw, pages, ml);
+}
+
+// Joins the partials of new token blockIdx.x / n_q, head blockIdx.x % n_q.
+template <int D, class T>
+__global__ void __launch_bounds__(D / 4) chunk_merge_kernel(ChunkArgs a) {
+    const int head = blockIdx.x % a.n_q, row = a.seq[0].first + blockIdx.x / a.n_q;
+    int i = a.n_seq - 1;
+    while (a.seq[i].first > row) --i;
+    if (a.chunks[i] == 1) return;
+    const ChunkSeq sq = a.seq[i];
+    const int t = row - sq.first;
+    const int n = (block_tiles(sq, t / a.block, a.block) + a.tiles - 1) / a.tiles;
+    const int kvh = head / a.rep, c = threadIdx.x;
+    float M = -INFINITY, L = 0.f;
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int k = 0; k < n; ++k) {
+        const size_t at = (size_t)(a.base[i] + (k * sq.n + t) * a.rep + head % a.rep) * a.n_kv + kvh;
+        const f32x2_t ml = *reinterpret_cast<const f32x2_t*>(a.part_ml + at * 2);
+        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part_o + at * D + 4 * c);
+        const float m_new = fmaxf(M, ml[0]);
+        const float w0 = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - m_new);
+        const float w1 = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m_new);
+        o = o * w0 + x * w1;
+        L = L * w0 + ml[1] * w1;
+        M = m_new;
+    }
+    store4(static_cast<T*>(a.out) + ((size_t)row * a.n_q + head) * D + 4 * c, o * (1.0f / L));
+}
+
+template <int D, int KV, class T>
+sa_status launch_chunks(const ChunkArgs& a, int rows, bool merge, hipStream_t st) {
+    constexpr int lds = Geo<D, KV>::LDS;
+    constexpr auto kernel = chunk_attn_kernel<D, KV, T>;
+    SA_TRY(pf::opt_in_lds<kernel>(lds));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)a.start[a.n_seq] * a.n_kv), dim3(kThreads), lds, st, a);
+    SA_CHECK_LAUNCH();
+    if (merge) {
+        hipLaunchKernelGGL((chunk_merge_kernel<D, T>), dim3((unsigned)rows * a.n_q), dim3(D / 4), 0, st, a);
+        SA_CHECK_LAUNCH();
+    }
+    return SA_OK;
+}
+
+template <int D>
+sa_status dispatch_chunks(const ChunkArgs& a, sa_dtype kv, bool q16, int rows, bool merge, hipStream_t st) {
+    if (kv == SA_DTYPE_F32) return launch_chunks<D, kF32, float>(a, rows, merge, st);
+    if (kv == SA_DTYPE_BF16)
+        return q16 ? launch_chunks<D, kBf16, uint16_t>(a, rows, merge, st)
+                   : launch_chunks<D, kBf16, float>(a, rows, merge, st);
+    return q16 ? launch_chunks<D, kFp8, uint16_t>(a, rows, merge, st) : launch_chunks<D, kFp8, float>(a, rows, merge, st);
+}
+
+// Tokens of a block: the query rows that a workgroup takes, at most 64 tokens (a
+// bit of Item::single each).
+int block_tokens(bool f32, int rep) {
+    return std::max(1, std::min(64, (f32 ? Geo<128, kF32>::ROWS : Geo<128, kBf16>::ROWS) / rep));
+}
+// Workgroups that a launch of chunks aims at: a round and a quarter of them.
+long long chunk_round(bool f32) {
+    const long long slots = (f32 ? 1LL : 2LL) * device_cu_count();
+    return slots + slots / 4;
+}
+constexpr int kChunkRounds = 4;   // of workgroups that long contexts are cut into
+
+}  // namespace
+
+size_t extend_rows_ws(int n, const int32_t* counts, int n_q, int n_kv, int d, bool f32, long long max_tokens) {
+    const int rep = n_q / n_kv, block = block_tokens(f32, rep);
+    const long long tiles = (max_tokens + kTile - 1) / kTile;
+    const long long most = std::min<long long>(tiles, std::max<long long>(kMaxChunks, ceil_div(tiles, kChunkTiles)));
+    if (most <= 1) return 0;
+    size_t need = 0;
+    for (int i0 = 0; i0 < n; i0 += kRowsPerLaunch) {
+        long long rows = 0, blocks = 0, widest = 0;
+        for (int i = i0; i < std::min(n, i0 + kRowsPerLaunch); ++i) {
+            rows += (long long)counts[i] * n_q;
+            blocks += ceil_div(counts[i], block);
+            widest = std::max<long long>(widest, std::min(counts[i], block) * rep);
         }
+        // By chunks of a sequence, and by workgroups of the launch.
+        const long long by_chunks = rows * most;
+        const long long forced = tiles > kChunkTiles ? blocks * n_kv * ceil_div(tiles, kChunkTiles) : 0;
+        const long long by_groups = std::max(kChunkRounds * chunk_round(f32), forced) * widest;
+        need = std::max(need, (size_t)std::max(rows, std::min(by_chunks, by_groups)) * (d + 2) * sizeof(float));
+    }
+    return need;
+}
+
+sa_status extend_rows(const PagedView& c, const void* q, bool q16, int n_q, const ChunkSeq* seqs, int n, float scale,
+                      void* out, void* ws, size_t ws_bytes, hipStream_t st) {
+    ChunkArgs a{};
+    set_cache(a, c, n_q, scale);
+    a.q = q;
+    a.out = out;
+    const bool f32 = c.kv == SA_DTYPE_F32;
+    a.block = block_tokens(f32, a.rep);
+    for (int i0 = 0; i0 < n; i0 += kRowsPerLaunch) {
+        a.n_seq = std::min(kRowsPerLaunch, n - i0);
+        long long work = 0;
+        int longest = 0;
+        for (int i = 0; i < a.n_seq; ++i) {
+            a.seq[i] = seqs[i0 + i];
+            const int blocks = ceil_div(a.seq[i].n, a.block);
+            for (int b = 0; b < blocks; ++b) work += block_tiles(a.seq[i], b, a.block);
+            if (blocks) longest = std::max(longest, block_tiles(a.seq[i], blocks - 1, a.block));
+        }
+        if (longest == 0) continue;
+        work *= a.n_kv;
+        auto items = [&](int tiles) {
+            long long k = 0;
+            for (int i = 0; i < a.n_seq; ++i) {
+                const int blocks = ceil_div(a.seq[i].n, a.block);
+                if (blocks) k += (long long)blocks * ceil_div(block_tiles(a.seq[i], blocks - 1, a.block), tiles);
+            }
+            return k;
+        };
+        const long long round = chunk_round(f32);
+        int tiles = longest <= (f32 ? 2 : 4) * kWaves
+                        ? longest
+                        : std::max<int>(pick_tiles(round, work, [&](int t) { return items(t) * a.n_kv; }),
+                                        (int)std::min<long long>(longest, work / (kChunkRounds * round)));
+        // no more partials than extend_rows_ws counts on
+        while (tiles < longest && items(tiles) * a.n_kv > kChunkRounds * round) tiles += kWaves;
+        tiles = std::min(std::max(tiles, ceil_div(longest, kMaxChunks)), kChunkTiles);
+        a.tiles = tiles;
+        long long parts = 0, at = 0;
+        bool merge = false;
+        for (int i = 0; i < a.n_seq; ++i) {
+            const int blocks = ceil_div(a.seq[i].n, a.block);
+            a.chunks[i] = blocks ? ceil_div(block_tiles(a.seq[i], blocks - 1, a.block), tiles) : 1;
+            a.start[i] = (int)at;
+            a.base[i] = (int)parts;
+            at += (long long)blocks * a.chunks[i];
+            if (a.chunks[i] > 1) {
+                parts += (long long)a.chunks[i] * a.seq[i].n * a.rep;
+                merge = true;
+            }
+        }
+        a.start[a.n_seq] = (int)at;
+        const int rows = a.seq[a.n_seq - 1].first + a.seq[a.n_seq - 1].n - a.seq[0].first;
+        // a grid has fewer than 2^32 threads
+        if (at * a.n_kv >= (1LL << 32) / kThreads || (long long)rows * n_q >= (1LL << 32) / 64)
+            return fail(SA_EINVAL, "too many tokens for one call");
+        if (merge) {
+            const size_t need = (size_t)parts * a.n_kv * (c.d + 2) * sizeof(float);
+            if (!ws || ws_bytes < need) return fail(SA_ENOMEM, "workspace too small for the partials");
+            a.part_o = static_cast<float*>(ws);
+            a.part_ml = a.part_o + (size_t)parts * a.n_kv * c.d;
+        }
+        SA_TRY(c.d == 64 ? dispatch_chunks<64>(a, c.kv, q16, rows, merge, st)
+                         : dispatch_chunks<128>(a, c.kv, q16, rows, merge, st));
     }
     return SA_OK;
 }

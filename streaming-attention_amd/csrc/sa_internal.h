@@ -246,7 +246,10 @@ struct PagedView {
     const void* v_pool;
     const int32_t* block_table;
     const int32_t* seq_lens;
+    const uint8_t* k_scale;   // 8 bits, else NULL
+    const uint8_t* v_scale;
     int n_kv, d, max_pages, num_pages;
+    sa_dtype kv;
     bool bf16;
 };
 
@@ -264,6 +267,13 @@ sa_status qknorm_rope_append_partials(sa_kvcache* c, int layer, const float* par
                                       int n_q_heads, const float* q_norm_w, const float* k_norm_w, float eps,
                                       const float* rope_cos, const float* rope_sin, int rope_max_pos, float* q_out,
                                       float* k_out, float* v_out, hipStream_t st);
+
+// sa_qknorm_rope_append_ragged of rows 0 .. n_seq - 1 with q, k and v as the sum of
+// n_part split-K partials of a [sum counts][(n_q_heads + 2 n_kv) * D] projection.
+sa_status append_partials_ragged(sa_kvcache* c, int layer, const float* part, int n_part, int n_seq,
+                                 const int32_t* counts, int n_q_heads, const float* q_norm_w, const float* k_norm_w,
+                                 float eps, const float* rope_cos, const float* rope_sin, int rope_max_pos,
+                                 float* q_out, hipStream_t st);
 
 // sa_append_decode with q, k and v read from split-K partials (FusedAppend).
 // parts, if given: a launch of at most parts_limit chunks per sequence leaves
