@@ -579,6 +579,41 @@ sa_status sa_beam_select(const float* logits, int64_t row_stride, const float* s
                          int n_beams, int vocab, int n_select, float* out_scores, int32_t* out_tokens,
                          int32_t* out_beams, void* ws, size_t ws_bytes, sa_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Verification of drafted tokens (speculative decoding), and sampling (no
+ * counterpart in the reference, which decodes greedily).
+ *
+ * Sequence i has counts[i] drafted tokens, 0 to 64 (host array [n_seq], or NULL for
+ * none).  tokens, u_accept [sum counts]: the drafts x, sequence behind sequence, and
+ * uniform numbers in [0, 1); u_sample [n_seq]: one more each.  target: fp32 logits of
+ * the target model, counts[i] + 1 rows for sequence i (the place of each drafted
+ * token and the one behind the last), target_stride floats from row to row; draft:
+ * the draft model's, a row per drafted token, or NULL for drafts without a
+ * distribution (looked up, greedy).  With p = softmax(target / temperature), q =
+ * softmax(draft / temperature) (draft NULL: probability 1 on the drafted token):
+ * x_k is accepted while u_k q_k(x_k) < p_k(x_k); at the first place a where it is not,
+ * or behind the last, one token is drawn with weights max(p_a - q_a, 0) (behind the
+ * last, or where these are all 0: p_a), the first t with sum_{t' <= t} w > u sum w.  The
+ * tokens are then distributed as drawn from the target alone.  temperature 0: x_k is
+ * accepted while it is the largest logit's token (the lowest of equal ones), which
+ * also follows; draft, u_accept and u_sample are not read.
+ * out_accepted [n_seq]: a.  out_tokens [n_seq][out_stride], out_stride > counts[i]: the
+ * accepted tokens, the drawn one at place a, -1 behind it.
+ * Probabilities and their sums are 64-bit, off by some 1e-13.  Mask tokens with -inf.
+ * A target row without a distribution (NaN or +inf among its logits, nothing but
+ * -inf; temperature 0: nothing but NaN and -inf) accepts nothing and draws -1;
+ * a draft row without one rejects its token, whose place is drawn from p.  Drafted
+ * tokens outside [0, vocab) are rejected.
+ * vocab up to 2^30, n_seq up to 2^20; rows may start at any 4-byte address.  Outputs
+ * must not overlap inputs or each other.  ws: 16-byte aligned,
+ * sa_draft_verify_ws_bytes bytes; calls that overlap on one workspace race.
+ * ------------------------------------------------------------------------ */
+size_t sa_draft_verify_ws_bytes(int n_seq, const int32_t* counts, int vocab);
+sa_status sa_draft_verify(const float* target, int64_t target_stride, const float* draft, int64_t draft_stride,
+                          const int32_t* tokens, const float* u_accept, const float* u_sample, int n_seq,
+                          const int32_t* counts, int vocab, float temperature, int32_t* out_accepted,
+                          int32_t* out_tokens, int out_stride, void* ws, size_t ws_bytes, sa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -123,6 +123,8 @@ SIGNATURES = {
     "sa_prefill_query_tile": (_I, [_I, _I, _I, _I, _I, _I]),
     "sa_beam_select_ws_bytes": (_SZ, [_I, _I, _I, _I]),
     "sa_beam_select": (_I, [_P, C.c_int64, _P, _I, _I, _I, _I, _P, _P, _P, _P, _SZ, _P]),
+    "sa_draft_verify_ws_bytes": (_SZ, [_I, _P, _I]),
+    "sa_draft_verify": (_I, [_P, C.c_int64, _P, C.c_int64, _P, _P, _P, _I, _P, _I, _F, _P, _P, _I, _P, _SZ, _P]),
     "sa_qwen3_create": (_I, [C.POINTER(Qwen3Desc), _I, C.POINTER(_P)]),
     "sa_qwen3_destroy": (_I, [_P]),
     "sa_qwen3_get_desc": (_I, [_P, C.POINTER(Qwen3Desc)]),
@@ -672,6 +674,88 @@ def beam_select(logits, scores, n_select: int, out=None, ws=None, stream=None):
     st = _on(stream, logits, _f32(scores, "scores"), o, t, b, ws)
     check(lib().sa_beam_select(logits.data_ptr(), stride, scores.data_ptr(), G, B, V, n_select, o.data_ptr(),
                                t.data_ptr(), b.data_ptr(), ws.data_ptr(), _nbytes(ws), st))
+    return out
+
+
+# ---------------------------------------------------------------- drafted tokens and sampling
+
+def draft_verify_ws_bytes(counts, vocab: int) -> int:
+    counts = [int(n) for n in counts]
+    return lib().sa_draft_verify_ws_bytes(len(counts), _rows(counts, len(counts)), vocab)
+
+
+def _logit_rows(t, rows: int, name: str) -> int:
+    """The row stride of fp32 CUDA logits [rows, vocab]."""
+    if t.dim() != 2 or t.shape[0] != rows or t.dtype != _f32_type() or not t.is_cuda:
+        raise ValueError(f"{name} must be a float32 CUDA tensor [{rows}, vocab]")
+    if t.shape[1] > 1 and t.stride(1) != 1:
+        raise ValueError(f"the rows of {name} must be contiguous")
+    return t.stride(0) if rows > 1 else max(t.stride(0), t.shape[1])
+
+
+def _f32_type():
+    global _float32
+    if _float32 is None:
+        import torch
+        _float32 = torch.float32
+    return _float32
+
+
+def draft_verify(target, tokens, u_accept, u_sample, counts, draft=None, temperature: float = 1.0, out=None, ws=None,
+                 stream=None):
+    """Speculative decoding's verification: counts[i] drafted tokens of sequence i (host
+    ints), tokens int32 [N] and uniform numbers u_accept [N], u_sample [len(counts)]; logits
+    target [N + len(counts), vocab], a row per drafted token and one behind each
+    sequence's last, and draft [N, vocab] (None: drafts without a distribution) ->
+    (accepted int32 [len(counts)], tokens int32 [len(counts), max(counts) + 1]: the
+    accepted ones, the one drawn behind them, then -1)."""
+    import torch
+    counts = [int(n) for n in counts]
+    n_seq, N, width = len(counts), sum(counts), max(counts, default=0) + 1
+    V = target.shape[-1]
+    stride = _logit_rows(target, N + n_seq, "target")
+    if draft is not None and draft.shape[-1] != V:
+        raise ValueError("target and draft must have one vocabulary")
+    d_stride = 0 if draft is None else _logit_rows(draft, N, "draft")
+    if tokens.dtype != torch.int32 or tuple(tokens.shape) != (N,) or not tokens.is_cuda or not tokens.is_contiguous():
+        raise ValueError("tokens must be a contiguous int32 CUDA tensor [sum counts]")
+    if tuple(u_accept.shape) != (N,) or tuple(u_sample.shape) != (n_seq,):
+        raise ValueError("u_accept must be [sum counts] and u_sample [len(counts)]")
+    if out is None:
+        out = _alloc(stream, lambda: (torch.empty(n_seq, dtype=torch.int32, device=target.device),
+                                      torch.empty(n_seq, width, dtype=torch.int32, device=target.device)))
+    accepted, drawn = out
+    if not (tuple(accepted.shape) == (n_seq,) and tuple(drawn.shape) == (n_seq, width) and
+            accepted.dtype == drawn.dtype == torch.int32 and accepted.is_cuda and drawn.is_cuda and
+            accepted.is_contiguous() and drawn.is_contiguous()):
+        raise ValueError("out must be contiguous int32 CUDA tensors [len(counts)] and [len(counts), max(counts) + 1]")
+    c_counts = _rows(counts, n_seq)
+    if ws is None:
+        need = lib().sa_draft_verify_ws_bytes(n_seq, c_counts, V)
+        ws = _alloc(stream, lambda: torch.empty(max(need, 16), dtype=torch.uint8, device=target.device))
+    st = _on(stream, target, tokens, _f32(u_accept, "u_accept"), _f32(u_sample, "u_sample"), accepted, drawn, ws,
+             *(() if draft is None else (draft,)))
+    check(lib().sa_draft_verify(target.data_ptr(), stride, _ptr(draft), d_stride, tokens.data_ptr(),
+                                u_accept.data_ptr(), u_sample.data_ptr(), n_seq, c_counts, V, temperature,
+                                accepted.data_ptr(), drawn.data_ptr(), width, ws.data_ptr(), _nbytes(ws), st))
+    return out
+
+
+def sample(logits, u, temperature: float = 1.0, out=None, ws=None, stream=None):
+    """A token of each row of logits [n, vocab], drawn from softmax(logits / temperature) by
+    uniform numbers u [n]: the first t whose probabilities up to it sum beyond u
+    (temperature 0: the largest logit's) -> int32 [n]; -1 for rows without a distribution."""
+    import torch
+    n = logits.shape[0]
+    none = _alloc(stream, lambda: (torch.empty(0, dtype=torch.int32, device=logits.device),
+                                   torch.empty(0, dtype=torch.float32, device=logits.device)))
+    if out is None:
+        out = _alloc(stream, lambda: torch.empty(n, dtype=torch.int32, device=logits.device))
+    elif tuple(out.shape) != (n,) or out.dtype != torch.int32 or not out.is_contiguous():
+        raise ValueError("out must be a contiguous int32 CUDA tensor [n]")
+    accepted = _alloc(stream, lambda: torch.empty(n, dtype=torch.int32, device=logits.device))
+    draft_verify(logits, none[0], none[1], u, [0] * n, temperature=temperature, out=(accepted, out.view(n, 1)), ws=ws,
+                 stream=stream)
     return out
 
 

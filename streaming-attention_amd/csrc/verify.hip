@@ -1,0 +1,568 @@
+// Verification of drafted tokens against the target model's logits, from given
+// uniform numbers; without drafts, sampling.
+//
+// A sequence has n drafted tokens x_0 .. x_{n-1}, target logits at n + 1 places and,
+// from a draft model, draft logits at n.  With p = softmax(target / T) and q =
+// softmax(draft / T) (without draft logits all of x_i's probability on x_i), x_i is
+// accepted while u_i q(x_i) < p(x_i); one more token is then drawn from w = max(p - q,
+// 0) at the first rejected place, or from w = p behind the last: the first t with
+// sum_{t' <= t} w > u sum w.  T = 0: x_i is accepted while it is the largest logit's,
+// whose token also follows.
+//
+// A sum of probabilities decides which token is drawn, and tokens of a large
+// vocabulary lie as close as 1e-6: sums and exponentials are in 64 bits (fp64 runs
+// at fp32's rate here), off by some 1e-13.
+//
+// Launches: (1) every row is cut into segments of 1024 logits, a wave each, which
+// leave their largest logit and sum of exponentials relative to it; (2) with draft
+// logits, the rejected places' sums of w per segment; (3) a workgroup per sequence
+// finds the segment that the uniform number falls into, then the token.  (2) and
+// (3) decide what is accepted, from the segments of the sequence's rows.
+//
+// Bound: HBM for the first launch, latency for the others.
+#include "sa_internal.h"
+
+#include <algorithm>
+#include <cmath>
+#include <initializer_list>
+#include <new>
+
+namespace sa {
+namespace {
+
+constexpr int kSeg = 1024;          // logits of a segment
+constexpr int kPer = kSeg / kWave;  // of a lane
+constexpr int kMaxDraft = 64;       // drafted tokens of a sequence (a lane each)
+constexpr int kThreads = 256, kWaves = kThreads / kWave;
+
+struct Segment {
+    double sum;     // of exp((x - top) / T)
+    float top;      // the largest logit, -inf if there is none
+    int32_t at;     // T = 0: its token
+};
+
+// What is drawn from.
+enum Source { kTarget, kRest, kRestOfOne, kNothing };
+
+struct VerifyArgs {
+    const float* target;      // rows first[i] + i .. first[i + 1] + i of sequence i
+    const float* draft;       // rows first[i] ..; NULL: none
+    const int32_t* tokens;    // [drafts]
+    const float* u_accept;    // [drafts]
+    const float* u_sample;    // [sequences]
+    long long target_stride, draft_stride;
+    Segment* seg;             // [target rows, then draft rows][n_seg]
+    double* rest;             // [sequences of the launch][n_seg]: sums of w
+    int32_t* out_accepted;    // [sequences]
+    int32_t* out_tokens;      // [sequences][out_stride]
+    int n_target, n_draft;    // rows
+    int vocab, n_seg, n_seq, out_stride;
+    int groups;               // workgroups per sequence of the second launch
+    double factor;            // log2(e) / T
+    int seq0;                 // the launch's first sequence
+    int32_t first[kRowsPerLaunch + 1];   // sequences' first drafts
+};
+static_assert(sizeof(VerifyArgs) <= 4096, "kernel arguments");
+
+// 2^t for t <= 0: 2^f by the series of exp(f ln 2), |f| <= 1/2, whose term of degree 11
+// is below 2.2e-13.
+__device__ __forceinline__ double exp2_64(double t) {
+    t = t < -1100.0 ? -1100.0 : t;   // NaN stays
+    const double n = __builtin_rint(t);
+    const double z = (t - n) * 0.69314718055994530942;
+    double s = 1.0 / 3628800.0;
+    s = fma(s, z, 1.0 / 362880.0);
+    s = fma(s, z, 1.0 / 40320.0);
+    s = fma(s, z, 1.0 / 5040.0);
+    s = fma(s, z, 1.0 / 720.0);
+    s = fma(s, z, 1.0 / 120.0);
+    s = fma(s, z, 1.0 / 24.0);
+    s = fma(s, z, 1.0 / 6.0);
+    s = fma(s, z, 0.5);
+    s = fma(s, z, 1.0);
+    s = fma(s, z, 1.0);
+    return __builtin_ldexp(s, (int)n);
+}
+// exp((x - top) / T); 0 where there is no largest logit.
+__device__ __forceinline__ double weight(float x, float top, double factor) {
+    return exp2_64(((double)x - (double)top) * factor);
+}
+
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double v) {
+    const uint64_t u = __double_as_longlong(v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
+    return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+__device__ __forceinline__ double wave_sum(double v) {
+    v += dpp_f64<kDppXor1>(v);
+    v += dpp_f64<kDppXor2>(v);
+    v += dpp_f64<kDppHalfMirror>(v);
+    v += dpp_f64<kDppMirror>(v);
+    v += __shfl_xor(v, 16, kWave);
+    v += __shfl_xor(v, 32, kWave);
+    return v;
+}
+
+// A row's logits by segments.  Segment s holds tokens kSeg s - off .. of the row, off
+// the row's distance from the 16-byte boundary before it, so that rows of any
+// alignment are read in 16-byte pieces.
+struct Row {
+    const float* x;
+    int off, vocab;
+    __device__ __forceinline__ Row(const float* row, int v)
+        : x(row), off((int)(reinterpret_cast<uintptr_t>(row) >> 2 & 3)), vocab(v) {}
+    // The four tokens from first() on; places outside the row are none.
+    __device__ __forceinline__ long long first(int s, int quad) const { return (long long)kSeg * s + 4 * quad - off; }
+    __device__ __forceinline__ void load(int s, int quad, float none, float (&v)[4]) const {
+        const long long i = first(s, quad);
+        if (i >= 0 && i + 4 <= vocab) {
+            const float4 f = *reinterpret_cast<const float4*>(x + i);
+            v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = i + e >= 0 && i + e < vocab ? x[i + e] : none;
+        }
+    }
+};
+
+__device__ __forceinline__ const float* target_row(const VerifyArgs& a, long long r) { return a.target + r * a.target_stride; }
+__device__ __forceinline__ const float* draft_row(const VerifyArgs& a, long long r) { return a.draft + r * a.draft_stride; }
+
+// A wave per segment of a row.
+template <bool GREEDY>
+__global__ void __launch_bounds__(kThreads) verify_segments_kernel(VerifyArgs a) {
+    const int wgs = (a.n_seg + kWaves - 1) / kWaves;
+    const int row = blockIdx.x / wgs, s = blockIdx.x % wgs * kWaves + threadIdx.x / kWave;
+    const int lane = threadIdx.x & (kWave - 1);
+    if (s >= a.n_seg) return;
+    const Row r(row < a.n_target ? target_row(a, row) : draft_row(a, row - a.n_target), a.vocab);
+    float v[kPer / 4][4];
+#pragma unroll
+    for (int j = 0; j < kPer / 4; ++j) r.load(s, j * kWave + lane, -INFINITY, v[j]);
+    float top = -INFINITY;
+    int at = 0x7fffffff;
+#pragma unroll
+    for (int j = 0; j < kPer / 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if constexpr (GREEDY) {
+                const int t = (int)(r.first(s, j * kWave + lane)) + e;
+                if (v[j][e] > top) top = v[j][e], at = t;   // tokens ascend
+            } else {
+                top = fmaxf(top, v[j][e]);
+            }
+        }
+    Segment out;
+    if constexpr (GREEDY) {
+#pragma unroll
+        for (int mask = 1; mask < kWave; mask *= 2) {
+            const float ot = __shfl_xor(top, mask, kWave);
+            const int oi = __shfl_xor(at, mask, kWave);
+            if (better(ot, oi, top, at)) top = ot, at = oi;
+        }
+        out = Segment{0.0, top, at};
+    } else {
+        top = group_reduce<OpMax, 1, kWave>(top);
+        double sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < kPer / 4; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                // without a largest logit there are -inf, which add 0, and NaN, which stay
+                sum += weight(v[j][e], top == -INFINITY ? 0.f : top, a.factor);
+        out = Segment{wave_sum(sum), top, 0};
+    }
+    if (lane == 0) a.seg[(long long)row * a.n_seg + s] = out;
+}
+
+// A row's largest logit and its sum of exponentials relative to it; a row whose sum
+// is 0 or not finite has no distribution.
+struct Norm {
+    double sum;
+    float top;
+    __device__ __forceinline__ bool ok() const { return sum > 0.0 && sum < INFINITY; }
+};
+__device__ __forceinline__ Norm row_norm(const VerifyArgs& a, long long row) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const Segment* seg = a.seg + row * a.n_seg;
+    float top = -INFINITY;
+    for (int s = lane; s < a.n_seg; s += kWave) top = fmaxf(top, seg[s].top);
+    top = group_reduce<OpMax, 1, kWave>(top);
+    double sum = 0.0;
+    for (int s = lane; s < a.n_seg; s += kWave) {
+        const Segment g = seg[s];
+        // a segment of NaN and -inf alone: its sum is 0 or NaN
+        sum += g.top == -INFINITY ? g.sum : g.sum * weight(g.top, top, a.factor);
+    }
+    return Norm{wave_sum(sum), top};
+}
+
+struct Shared {
+    Norm p[kMaxDraft + 1], q[kMaxDraft];
+};
+// What a sequence's uniform numbers decide.
+struct Decision {
+    int accepted;
+    Source source;
+    Norm p, q;            // of the place that the next token comes from
+    int token;            // kRestOfOne: the rejected token
+    long long row, drow;  // of the target, of the draft
+};
+
+// The same for every thread of the workgroup.
+__device__ __forceinline__ Decision decide(const VerifyArgs& a, int i, Shared& sh, int* box) {
+    const int first = a.first[i], n = a.first[i + 1] - first;
+    const long long row0 = (long long)first + a.seq0 + i;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x & (kWave - 1);
+    const int rows = n + 1 + (a.draft ? n : 0);
+    for (int r = wave; r < rows; r += kWaves) {
+        const Norm m = row_norm(a, r <= n ? row0 + r : (long long)a.n_target + first + r - n - 1);
+        if (lane == 0) (r <= n ? sh.p[r] : sh.q[r - n - 1]) = m;
+    }
+    __syncthreads();
+    if (wave == 0) {
+        bool ok = false;
+        if (lane < n) {
+            const int x = a.tokens[first + lane];
+            const Norm p = sh.p[lane];
+            if (x >= 0 && x < a.vocab && p.ok()) {
+                const double px = weight(target_row(a, row0 + lane)[x], p.top, a.factor) / p.sum;
+                double qx = 1.0;
+                if (a.draft) {
+                    const Norm q = sh.q[lane];
+                    qx = q.ok() ? weight(draft_row(a, first + lane)[x], q.top, a.factor) / q.sum : NAN;
+                }
+                ok = (double)a.u_accept[first + lane] * qx < px;
+            }
+        }
+        const int accepted = __ffsll((long long)~__ballot(ok)) - 1;
+        if (lane == 0) *box = accepted < 0 ? kMaxDraft : accepted;
+    }
+    __syncthreads();
+    Decision d;
+    d.accepted = *box;
+    d.p = sh.p[d.accepted];
+    d.row = row0 + d.accepted;
+    d.drow = first + d.accepted;
+    d.source = kTarget;
+    d.token = -1;
+    d.q = Norm{0.0, 0.f};
+    if (!d.p.ok()) {
+        d.source = kNothing;
+    } else if (d.accepted < n) {
+        if (a.draft) {
+            d.q = sh.q[d.accepted];
+            if (d.q.ok()) d.source = kRest;
+        } else {
+            d.token = a.tokens[d.drow];
+            if (d.token >= 0 && d.token < a.vocab) d.source = kRestOfOne;
+        }
+    }
+    return d;
+}
+
+// w of the four tokens of a place of a segment.
+struct Weigher {
+    const VerifyArgs& a;
+    const Decision& d;
+    Row p, q;
+    double pi, qi;
+    __device__ __forceinline__ Weigher(const VerifyArgs& args, const Decision& dec)
+        : a(args), d(dec), p(target_row(args, dec.row), args.vocab),
+          q(dec.source == kRest ? draft_row(args, dec.drow) : nullptr, args.vocab), pi(1.0 / dec.p.sum),
+          qi(dec.source == kRest ? 1.0 / dec.q.sum : 0.0) {}
+    __device__ __forceinline__ void operator()(int s, int quad, double (&w)[4]) const {
+        float x[4];
+        p.load(s, quad, -INFINITY, x);
+        const long long t = p.first(s, quad);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = weight(x[e], d.p.top, a.factor) * pi;
+        if (d.source == kRest) {
+            // the draft's row may start at another distance from its boundary
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (t + e >= 0 && t + e < a.vocab) w[e] = fmax(0.0, w[e] - weight(q.x[t + e], d.q.top, a.factor) * qi);
+        } else if (d.source == kRestOfOne) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (t + e == d.token) w[e] = 0.0;
+        }
+    }
+};
+
+// Sums of w per segment at the sequences' rejected places.
+__global__ void __launch_bounds__(kThreads) verify_rest_kernel(VerifyArgs a) {
+    __shared__ Shared sh;
+    __shared__ int box;
+    const int i = blockIdx.x / a.groups, g = blockIdx.x % a.groups;
+    if (a.first[i + 1] == a.first[i]) return;
+    const Decision d = decide(a, i, sh, &box);
+    if (d.source != kRest) return;
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+    const Weigher w(a, d);
+    for (int s = g * kWaves + wave; s < a.n_seg; s += a.groups * kWaves) {
+        double sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < kPer / 4; ++j) {
+            double v[4];
+            w(s, j * kWave + lane, v);
+            sum += (v[0] + v[1]) + (v[2] + v[3]);
+        }
+        sum = wave_sum(sum);
+        if (lane == 0) a.rest[(long long)i * a.n_seg + s] = sum;
+    }
+}
+
+// The sum of the threads' values before this one's, and of all.
+__device__ __forceinline__ double scan(double v, double (&part)[kWaves], double* all) {
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+    double sum = v;
+#pragma unroll
+    for (int k = 1; k < kWave; k *= 2) {
+        const double o = __shfl_up(sum, k, kWave);
+        if (lane >= k) sum += o;
+    }
+    __syncthreads();
+    if (lane == kWave - 1) part[wave] = sum;
+    __syncthreads();
+    double before = 0.0;
+    *all = 0.0;
+    for (int k = 0; k < kWaves; ++k) {
+        if (k < wave) before += part[k];
+        *all += part[k];
+    }
+    return before + (sum - v);
+}
+
+// The smallest of the threads' values.
+__device__ __forceinline__ int least(int v, int (&part)[kWaves]) {
+    const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+    for (int k = 1; k < kWave; k *= 2) v = min(v, __shfl_xor(v, k, kWave));
+    __syncthreads();
+    if (lane == 0) part[wave] = v;
+    __syncthreads();
+    for (int k = 0; k < kWaves; ++k) v = min(v, part[k]);
+    return v;
+}
+
+// A workgroup per sequence: the token that u falls on, and the results.
+__global__ void __launch_bounds__(kThreads) verify_draw_kernel(VerifyArgs a) {
+    __shared__ Shared sh;
+    __shared__ int box;
+    __shared__ double part[kWaves];
+    __shared__ int ipart[kWaves];
+    const int i = blockIdx.x, seq = a.seq0 + i, tid = threadIdx.x;
+    Decision d = decide(a, i, sh, &box);
+    constexpr int kNone = 0x7fffffff;
+    int token = -1;
+    if (d.source != kNothing) {
+        const Segment* seg = a.seg + d.row * a.n_seg;
+        const double* rest = a.rest + (long long)i * a.n_seg;
+        // The segment of a rejected token without a distribution is summed anew without
+        // it: a difference would lose the others' digits.
+        int without = -1;
+        double without_sum = 0.0;
+        if (d.source == kRestOfOne) {
+            const Weigher w(a, d);
+            without = (d.token + w.p.off) / kSeg;
+            double v[4];
+            w(without, tid, v);
+            scan((v[0] + v[1]) + (v[2] + v[3]), part, &without_sum);
+        }
+        auto sum_of = [&](int s) -> double {
+            if (d.source == kRest) return rest[s];
+            if (d.source == kRestOfOne && s == without) return without_sum;
+            const Segment g = seg[s];
+            return g.top == -INFINITY ? 0.0 : g.sum * weight(g.top, d.p.top, a.factor) / d.p.sum;
+        };
+        const int per = (a.n_seg + kThreads - 1) / kThreads;
+        double mine = 0.0, all, before;
+        auto sums = [&]() {
+            mine = 0.0;
+            for (int s = tid * per; s < min(a.n_seg, (tid + 1) * per); ++s) mine += sum_of(s);
+            before = scan(mine, part, &all);
+        };
+        sums();
+        if (!(all > 0.0)) {   // p is nowhere above q
+            d.source = kTarget;
+            sums();
+        }
+        const double goal = (double)a.u_sample[seq] * all;
+        // The first segment whose sums reach beyond the goal, else the last that has any.
+        int found = kNone, last = -1;
+        double sum = before;
+        double start = 0.0;
+        for (int s = tid * per; s < min(a.n_seg, (tid + 1) * per); ++s) {
+            const double v = sum_of(s);
+            if (v > 0.0) {
+                last = s;
+                if (found == kNone && sum + v > goal) found = s, start = sum;
+            }
+            sum += v;
+        }
+        int s = least(found, ipart);
+        if (s == kNone) {
+            s = -least(-last, ipart);
+            if (s == last) found = s, start = sum - sum_of(s);
+        }
+        __shared__ double s_start;
+        if (found == s) s_start = start;
+        __syncthreads();
+        const Weigher w(a, d);
+        double v[4];
+        w(s, tid, v);
+        const double four = (v[0] + v[1]) + (v[2] + v[3]);
+        double whole;
+        double c = s_start + scan(four, part, &whole);
+        found = kNone;
+        last = -1;
+        const long long t0 = w.p.first(s, tid);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            c += v[e];
+            if (v[e] > 0.0) {
+                last = (int)(t0 + e);
+                if (found == kNone && c > goal) found = last;
+            }
+        }
+        token = least(found, ipart);
+        if (token == kNone) token = -least(-last, ipart);
+    }
+    const int n = a.first[i + 1] - a.first[i];
+    if (tid == 0) a.out_accepted[seq] = d.accepted;
+    for (int k = tid; k < a.out_stride; k += kThreads)
+        a.out_tokens[(long long)seq * a.out_stride + k] =
+            k < d.accepted && k < n ? a.tokens[a.first[i] + k] : k == d.accepted ? token : -1;
+}
+
+// T = 0, a wave per sequence.
+__global__ void __launch_bounds__(kWave) verify_greedy_kernel(VerifyArgs a) {
+    const int i = blockIdx.x, seq = a.seq0 + i, lane = threadIdx.x;
+    const int first = a.first[i], n = a.first[i + 1] - first;
+    int accepted = 0, token = -1;
+    for (;; ++accepted) {
+        const Segment* seg = a.seg + ((long long)first + seq + accepted) * a.n_seg;
+        float top = -INFINITY;
+        int at = 0x7fffffff;
+        for (int s = lane; s < a.n_seg; s += kWave) {
+            const Segment g = seg[s];
+            if (g.top > top) top = g.top, at = g.at;   // segments ascend
+        }
+#pragma unroll
+        for (int mask = 1; mask < kWave; mask *= 2) {
+            const float ot = __shfl_xor(top, mask, kWave);
+            const int oi = __shfl_xor(at, mask, kWave);
+            if (better(ot, oi, top, at)) top = ot, at = oi;
+        }
+        token = at == 0x7fffffff ? -1 : at;
+        if (accepted == n || token < 0 || a.tokens[first + accepted] != token) break;
+    }
+    if (lane == 0) a.out_accepted[seq] = accepted;
+    for (int k = lane; k < a.out_stride; k += kWave)
+        a.out_tokens[(long long)seq * a.out_stride + k] =
+            k < accepted ? a.tokens[first + k] : k == accepted ? token : -1;
+}
+
+bool verify_sizes_ok(int n_seq, const int32_t* counts, int vocab, long long* drafts) {
+    *drafts = 0;
+    if (n_seq <= 0 || n_seq > (1 << 20) || vocab <= 0 || vocab > (1 << 30)) return false;
+    for (int i = 0; counts && i < n_seq; ++i) {
+        if (counts[i] < 0 || counts[i] > kMaxDraft) return false;
+        *drafts += counts[i];
+    }
+    return true;
+}
+
+int segments_of(int vocab) { return (vocab + 3 + kSeg - 1) / kSeg; }   // rows start up to 3 logits into the first
+
+bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && na && nb && x < y + nb && y < x + na;
+}
+
+}  // namespace
+}  // namespace sa
+
+using namespace sa;
+
+extern "C" size_t sa_draft_verify_ws_bytes(int n_seq, const int32_t* counts, int vocab) {
+    long long n;
+    if (!verify_sizes_ok(n_seq, counts, vocab, &n)) return 0;
+    const size_t segs = segments_of(vocab);
+    return (size_t)(2 * n + n_seq) * segs * sizeof(Segment) + (size_t)std::min(n_seq, kRowsPerLaunch) * segs * sizeof(double);
+}
+
+extern "C" sa_status sa_draft_verify(const float* target, int64_t target_stride, const float* draft,
+                                     int64_t draft_stride, const int32_t* tokens, const float* u_accept,
+                                     const float* u_sample, int n_seq, const int32_t* counts, int vocab,
+                                     float temperature, int32_t* out_accepted, int32_t* out_tokens, int out_stride,
+                                     void* ws, size_t ws_bytes, sa_stream_t stream) {
+    clear_error();
+    long long n;
+    if (!verify_sizes_ok(n_seq, counts, vocab, &n))
+        return fail(SA_EINVAL, "verification takes 1 to 2^20 sequences, 0 to 64 drafted tokens each, vocab 1 to 2^30");
+    if (!(temperature >= 0.f) || !(temperature < INFINITY)) return fail(SA_EINVAL, "temperature must be >= 0 and finite");
+    const bool greedy = temperature == 0.f;
+    if (greedy) draft = nullptr;   // unused
+    if (!target || !out_accepted || !out_tokens || (n > 0 && !tokens)) return fail(SA_EINVAL, "null pointer");
+    if (!greedy && (!u_sample || (n > 0 && !u_accept))) return fail(SA_EINVAL, "null uniform numbers");
+    if (target_stride < vocab || (draft && draft_stride < vocab)) return fail(SA_EINVAL, "row strides must be at least vocab");
+    int most = 0;
+    for (int i = 0; counts && i < n_seq; ++i) most = std::max(most, counts[i]);
+    if (out_stride < most + 1) return fail(SA_EINVAL, "out_stride must be above the most drafted tokens");
+    const size_t out_n = (size_t)n_seq * out_stride * sizeof(int32_t), acc_n = (size_t)n_seq * sizeof(int32_t);
+    const size_t target_n = ((size_t)(n + n_seq - 1) * target_stride + vocab) * sizeof(float);
+    const size_t draft_n = n ? ((size_t)(n - 1) * draft_stride + vocab) * sizeof(float) : 0;
+    struct { const void* p; size_t n; } in[] = {{target, target_n}, {draft, draft_n}, {tokens, (size_t)n * 4},
+                                                {greedy ? nullptr : u_accept, (size_t)n * 4},
+                                                {greedy ? nullptr : u_sample, (size_t)n_seq * 4}};
+    for (const auto& x : in)
+        if (overlap(out_tokens, out_n, x.p, x.n) || overlap(out_accepted, acc_n, x.p, x.n))
+            return fail(SA_EINVAL, "outputs must not overlap inputs");
+    if (overlap(out_tokens, out_n, out_accepted, acc_n)) return fail(SA_EINVAL, "outputs must not overlap each other");
+    if (!draft) draft_stride = 0;
+    VerifyArgs a{};
+    a.n_target = (int)(n + n_seq);
+    a.n_draft = draft ? (int)n : 0;
+    a.n_seg = segments_of(vocab);
+    const long long wgs = (long long)(a.n_target + a.n_draft) * ((a.n_seg + kWaves - 1) / kWaves);
+    // a grid has fewer than 2^32 threads
+    if (wgs >= (1LL << 32) / kThreads) return fail(SA_EINVAL, "too many logits for one call");
+    if (!ws || ws_bytes < sa_draft_verify_ws_bytes(n_seq, counts, vocab))
+        return fail(SA_ENOMEM, "workspace too small for the segments");
+    if (!aligned16(ws)) return fail(SA_EINVAL, "ws must be 16-byte aligned");
+    a.target = target; a.draft = draft; a.tokens = tokens; a.u_accept = u_accept; a.u_sample = u_sample;
+    a.target_stride = target_stride; a.draft_stride = draft_stride;
+    a.seg = static_cast<Segment*>(ws);
+    a.rest = reinterpret_cast<double*>(a.seg + (size_t)(2 * n + n_seq) * a.n_seg);
+    a.out_accepted = out_accepted; a.out_tokens = out_tokens; a.out_stride = out_stride;
+    a.vocab = vocab;
+    a.factor = greedy ? 0.0 : 1.4426950408889634074 / (double)temperature;
+    hipStream_t st = as_stream(stream);
+    if (greedy) hipLaunchKernelGGL(verify_segments_kernel<true>, dim3((unsigned)wgs), dim3(kThreads), 0, st, a);
+    else hipLaunchKernelGGL(verify_segments_kernel<false>, dim3((unsigned)wgs), dim3(kThreads), 0, st, a);
+    SA_CHECK_LAUNCH();
+    int at = 0;
+    for (a.seq0 = 0; a.seq0 < n_seq; a.seq0 += kRowsPerLaunch) {
+        a.n_seq = std::min(kRowsPerLaunch, n_seq - a.seq0);
+        a.first[0] = at;
+        for (int i = 0; i < a.n_seq; ++i) a.first[i + 1] = a.first[i] + (counts ? counts[a.seq0 + i] : 0);
+        at = a.first[a.n_seq];
+        if (greedy) {
+            hipLaunchKernelGGL(verify_greedy_kernel, dim3(a.n_seq), dim3(kWave), 0, st, a);
+            SA_CHECK_LAUNCH();
+            continue;
+        }
+        if (draft && at > a.first[0]) {
+            a.groups = std::max(1, std::min((a.n_seg + kWaves - 1) / kWaves, 2 * device_cu_count() / a.n_seq));
+            hipLaunchKernelGGL(verify_rest_kernel, dim3(a.n_seq * a.groups), dim3(kThreads), 0, st, a);
+            SA_CHECK_LAUNCH();
+        }
+        hipLaunchKernelGGL(verify_draw_kernel, dim3(a.n_seq), dim3(kThreads), 0, st, a);
+        SA_CHECK_LAUNCH();
+    }
+    return SA_OK;
+}
