@@ -157,6 +157,25 @@ sa_status sa_qwen3_beam_step(sa_qwen3* model, sa_kvcache* cache, const int32_t* 
                              const float* scores, int n_select, float* out_scores, int32_t* out_tokens,
                              int32_t* out_beams, sa_stream_t stream);
 
+/* A forward over chunks of new tokens behind what the cache holds (no counterpart
+ * in the reference, whose forward over a cache takes one token or an empty cache): counts[i] tokens
+ * for sequence i = 0 .. n_seq - 1 (host array), tokens: device int32 [sum counts],
+ * sequence behind sequence.  Every layer appends them behind sequence i's committed
+ * tokens (sa_qknorm_rope_append_ragged) and attends (sa_paged_extend).  For prompts
+ * taken in chunks, turns of a chat, and verification of drafted tokens.
+ * all_rows != 0: next_tokens [sum counts] and logits [sum counts][vocab] of every new
+ * token, sum counts <= max_batch, counts >= 0; else next_tokens [n_seq] and logits
+ * [n_seq][vocab] of each sequence's last, n_seq <= max_batch, counts >= 1.  logits may
+ * be NULL.  commit != 0: lengths grow by counts; else they stay, and what was
+ * appended is committed by sa_kvcache_set_lens as far as it is accepted
+ * (sa_draft_verify), or overwritten by the next append.  The caller must have
+ * reserved pages of every row's own for the new tokens; at most 2^20 of them.
+ * Asynchronous on stream; a graph that holds a call repeats it for the lengths at
+ * the call, also after larger calls.  Refused calls enqueue nothing. */
+sa_status sa_qwen3_extend(sa_qwen3* model, sa_kvcache* cache, const int32_t* tokens, int n_seq,
+                          const int32_t* counts, int all_rows, int32_t* next_tokens, float* logits, int commit,
+                          sa_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

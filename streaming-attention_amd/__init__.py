@@ -134,6 +134,7 @@ SIGNATURES = {
     "sa_qwen3_init_random": (_I, [_P, C.c_uint64, _F, _P]),
     "sa_qwen3_decode_step": (_I, [_P, _P, _P, _I, _P, _P, _P]),
     "sa_qwen3_prefill": (_I, [_P, _P, _P, _I, _I, _P, _P, _P]),
+    "sa_qwen3_extend": (_I, [_P, _P, _P, _I, _P, _I, _P, _P, _I, _P]),
     "sa_qwen3_beam_step": (_I, [_P, _P, _P, _I, _I, _P, _I, _P, _P, _P, _P]),
 }
 
@@ -937,6 +938,149 @@ class Qwen3:
                                          _ptr(logits), _stream(stream)))
         return next_tokens
 
+    def extend(self, cache: "KVCache", tokens, counts=None, all_rows: bool = False, next_tokens=None, logits=None,
+               commit: bool = True, stream=None):
+        """A forward over new tokens behind what the cache holds: tokens int32 CUDA [sum
+        counts], counts[i] of sequence i (host ints), or [n_seq, S] for S of each -> next
+        tokens int32 CUDA of each sequence's last token (and its logits [n_seq, vocab] if
+        given), or with all_rows of every new token ([sum counts], [sum counts, vocab]).
+        commit=False leaves the lengths for KVCache.set_lens."""
+        import torch
+        if counts is None:
+            if tokens.dim() != 2:
+                raise ValueError("tokens must be [n_seq, S], or [sum counts] with counts")
+            counts = [tokens.shape[1]] * tokens.shape[0]
+        counts = [int(n) for n in counts]
+        T = sum(counts)
+        if tokens.dtype != torch.int32 or not tokens.is_cuda or not tokens.is_contiguous() or tokens.numel() != T:
+            raise ValueError("tokens must be a contiguous int32 CUDA tensor of sum counts")
+        rows = T if all_rows else len(counts)
+        if next_tokens is None:
+            next_tokens = _alloc(stream, lambda: torch.empty(rows, dtype=torch.int32, device=tokens.device))
+        elif next_tokens.numel() != rows or next_tokens.dtype != torch.int32 or not next_tokens.is_contiguous():
+            raise ValueError("next_tokens must be a contiguous int32 CUDA tensor, a token per row of logits")
+        if logits is not None and tuple(logits.shape) != (rows, self.desc.vocab):
+            raise ValueError("logits must be [rows, vocab]")
+        st = _on(stream, tokens, next_tokens, *(() if logits is None else (_f32(logits, "logits"),)))
+        check(lib().sa_qwen3_extend(self.handle, cache.handle, tokens.data_ptr(), len(counts), _rows(counts, len(counts)),
+                                    int(bool(all_rows)), next_tokens.data_ptr(), _ptr(logits), int(bool(commit)), st))
+        return next_tokens
+
+    def speculative(self, cache: "KVCache", prompts, n_tokens: int, draft: "Qwen3 | None" = None,
+                    draft_cache: "KVCache | None" = None, n_draft: int = 4, temperature: float = 1.0,
+                    eos: int | None = None, generator=None):
+        """Generation with drafted tokens: prompts int32 CUDA [G, L] over empty caches -> a list
+        of up to n_tokens tokens per prompt (host ints), ended by eos, distributed as sampled
+        from this model alone at the temperature (0: greedy).  A round drafts up to n_draft
+        tokens per sequence, from the draft model (of this model's vocabulary, over
+        draft_cache) or, without one, what followed the last two tokens where they stood
+        before; one forward of this model verifies them (extend, draft_verify).  generator: a
+        CUDA torch.Generator of the uniform numbers.  Rounds need G * (n_draft + 1) <=
+        max_batch; a generation that positions or a row's pages have no room for is refused
+        (ValueError) before it begins.  The caches hold the sequences afterwards: reset them."""
+        import torch
+        G, L = prompts.shape
+        if n_tokens < 1 or not 0 <= n_draft <= 64:
+            raise ValueError("speculative takes at least one token and 0 to 64 drafts")
+        if not temperature >= 0.0 or temperature == float("inf"):
+            raise ValueError("temperature must be >= 0 and finite")
+        if draft is not None and (draft_cache is None or draft.desc.vocab != self.desc.vocab):
+            raise ValueError("a draft model takes a cache and this model's vocabulary")
+        for m, c in ((self, cache), (draft, draft_cache)):
+            if m is None:
+                continue
+            if G > c.desc.max_seqs or G * (n_draft + 1) > m.max_batch:
+                raise ValueError("the cache and the model need a row per sequence and drafted token")
+            if L + n_tokens - 1 > m.desc.max_pos or L + n_tokens - 1 > c.desc.max_pages_per_seq * PAGE_TOKENS:
+                raise ValueError("prompt and tokens need more positions or pages than there are")
+            for g in range(G):
+                c.reserve(g, L + n_tokens - 1)
+        dev, V = prompts.device, self.desc.vocab
+
+        def uniform(n):
+            return torch.rand(n, device=dev, generator=generator)
+
+        def ids(x):
+            return torch.tensor(x, dtype=torch.int64, device=dev)
+
+        logits = torch.empty(G, V, dtype=torch.float32, device=dev)
+        self.prefill(cache, prompts, logits=logits)
+        if draft is not None:
+            draft.prefill(draft_cache, prompts)
+        text = prompts.tolist()
+        for t, new in zip(text, sample(logits, uniform(G), temperature).tolist()):
+            t.append(new)
+        done = [False] * G
+        while True:
+            for g in range(G):
+                new = text[g][L:]
+                if eos is not None and eos in new:
+                    text[g] = text[g][:L + new.index(eos) + 1]
+                    done[g] = True
+                done[g] = done[g] or len(text[g]) >= L + n_tokens
+            if all(done):
+                return [t[L:L + n_tokens] for t in text]
+            # the last token of each sequence is in neither cache
+            room = [0 if done[g] else min(n_draft, L + n_tokens - 1 - len(text[g])) for g in range(G)]
+            if draft is None:
+                looked = [_looked_up(text[g], room[g]) for g in range(G)]
+                counts = [len(x) for x in looked]
+                drafts, q = torch.tensor(sum(looked, []), dtype=torch.int32, device=dev), None
+            else:
+                counts = room
+                drafts, q = draft._drafts(draft_cache, text, counts, temperature, uniform, ids)
+            # this model over the last token and the drafts of every sequence that goes on
+            going = [g for g in range(G) if not done[g]]
+            rows = [0 if done[g] else counts[g] + 1 for g in range(G)]
+            at, tokens = [], torch.empty(sum(rows), dtype=torch.int32, device=dev)
+            starts = [sum(rows[:g]) for g in range(G)]
+            for g in going:
+                at += range(starts[g] + 1, starts[g] + rows[g])
+            tokens[ids([starts[g] for g in going])] = ids([text[g][-1] for g in going]).int()
+            if at:
+                tokens[ids(at)] = drafts
+            target = torch.empty(sum(rows), V, dtype=torch.float32, device=dev)
+            self.extend(cache, tokens, rows, all_rows=True, logits=target, commit=False)
+            kept = [counts[g] for g in going]
+            accepted, new = draft_verify(target, drafts, uniform(sum(kept)), uniform(len(going)), kept, draft=q,
+                                         temperature=temperature)
+            for g, a, new_tokens in zip(going, accepted.tolist(), new.tolist()):
+                text[g] += new_tokens[:a + 1]
+                if new_tokens[a] < 0:
+                    raise ValueError("logits without a distribution (NaN or infinities)")
+            cache.set_lens(going, [len(text[g]) - 1 for g in going])
+
+    def _drafts(self, cache, text, counts, temperature, uniform, ids):
+        """counts[g] tokens behind each text, drawn from this model: (tokens int32 [sum counts],
+        their logits [sum counts, vocab]), sequence behind sequence.  The cache holds a
+        prefix of each text; it is left with no more than that and the drafts but the last."""
+        import torch
+        G, V = len(text), self.desc.vocab
+        N = sum(counts)
+        first = [sum(counts[:g]) for g in range(G)]
+        drafts = torch.empty(N, dtype=torch.int32, device=torch.cuda.current_device())
+        q = torch.empty(N, V, dtype=torch.float32, device=drafts.device)
+        held = [min(cache.length(g), len(text[g]) - 1) for g in range(G)]
+        cache.set_lens(range(G), held)
+        last = None
+        for k in range(max(counts, default=0)):
+            on = [g for g in range(G) if counts[g] > k]
+            if k == 0:
+                new = [text[g][held[g]:] if counts[g] else [] for g in range(G)]
+                tokens = torch.tensor(sum(new, []), dtype=torch.int32, device=drafts.device)
+                rows = [len(x) for x in new]
+            else:
+                tokens = last[ids([i for i, g in enumerate(was) if counts[g] > k])]
+                rows = [1 if counts[g] > k else 0 for g in range(G)]
+            logits = torch.empty(sum(rows), V, dtype=torch.float32, device=drafts.device)
+            self.extend(cache, tokens, rows, all_rows=True, logits=logits)
+            ends = ids([sum(rows[:g + 1]) - 1 for g in on])
+            logits = logits[ends].contiguous()
+            last = sample(logits, uniform(len(on)), temperature)
+            to = ids([first[g] + k for g in on])
+            drafts[to], q[to] = last, logits
+            was = on
+        return drafts, q
 
     def beam_step(self, cache: "KVCache", tokens, scores, n_select: int, out=None, stream=None):
         """One beam search step: tokens int32 CUDA [G, B] (row g * B + b of the
@@ -1026,6 +1170,14 @@ class Qwen3:
             last = [(s, p) for s, p in zip(scores[g], paths[g]) if s > float("-inf")]
             out.append(sorted(done[g] + last, key=lambda x: -x[0])[:B])
         return out
+
+
+def _looked_up(text, n: int):
+    """Up to n tokens that followed the last two of text where they stood before, latest first."""
+    for at in range(len(text) - 3, -1, -1) if n else ():
+        if text[at:at + 2] == text[-2:]:
+            return text[at + 2:at + 2 + n]
+    return []
 
 
 class _CudaArray:

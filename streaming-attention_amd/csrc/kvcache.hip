@@ -872,8 +872,9 @@ sa_status append_impl(sa_kvcache* c, int layer, const float* q, const float* k, 
                       hipStream_t st) {
     if (!valid_cache(c)) return fail(SA_EINVAL, "invalid cache");
     if (layer < 0 || layer >= c->desc.num_layers) return fail(SA_ERANGE, "Layer index out of range");
-    if (part ? n_part <= 0 : (!k || !v)) return fail(SA_EINVAL, "null k or v");
-    if ((q || part) && (!q_out || n_q_heads <= 0)) return fail(SA_EINVAL, "q needs q_out and n_q_heads > 0");
+    const bool none = counts && n_seq > 0 && std::all_of(counts, counts + n_seq, [](int32_t m) { return m == 0; });
+    if (part ? n_part <= 0 : (!k || !v) && !none) return fail(SA_EINVAL, "null k or v");
+    if ((q || part) && ((!q_out && !none) || n_q_heads <= 0)) return fail(SA_EINVAL, "q needs q_out and n_q_heads > 0");
     if (n_seq <= 0 || (!counts && S <= 0)) return fail(SA_EINVAL, "n_seq and S must be positive");
     if ((rope_cos == nullptr) != (rope_sin == nullptr)) return fail(SA_EINVAL, "cos and sin go together");
     if (rope_cos && rope_max_pos <= 0) return fail(SA_EINVAL, "RoPE table needs rope_max_pos > 0");
@@ -1061,8 +1062,6 @@ extern "C" sa_status sa_paged_decode(const sa_kvcache* c, int layer, const float
 namespace sa {
 namespace {
 
-constexpr int kMaxNewTokens = 1 << 20;   // of one call
-
 // What the decodes over ranges share: the checks of their arguments and the
 // view of a layer's pools.
 sa_status check_ranges(const sa_kvcache* c, int layer, const void* q, int n_seq, int n_q_heads, const void* out,
@@ -1077,7 +1076,7 @@ sa_status check_ranges(const sa_kvcache* c, int layer, const void* q, int n_seq,
     if (!aligned16(q) || !aligned16(out) || !aligned16(ws))
         return fail(SA_EINVAL, "q, out and ws must be 16-byte aligned");
     // A call of one launch is refused by that launch, which may need less.
-    if (n_seq > kRowsPerLaunch && (!ws || ws_bytes < ws_need))
+    if (n_seq > kRowsPerLaunch && ws_need > 0 && (!ws || ws_bytes < ws_need))
         return fail(SA_ENOMEM, "workspace too small for the partials");
     return on_cache_device(c);
 }
@@ -1087,6 +1086,11 @@ sa_status check_ranges(const sa_kvcache* c, int layer, const void* q, int n_seq,
 
 sa_status sa::check_append(const sa_kvcache* c, int n, int S, int max_pos) {
     const Verdict v = c->pt.check_append(nullptr, n, S, max_pos);
+    return v.ok() ? SA_OK : refused(v);
+}
+
+sa_status sa::check_append_ragged(const sa_kvcache* c, int n, const int32_t* counts, int max_pos) {
+    const Verdict v = c->pt.check_append(nullptr, n, counts, max_pos);
     return v.ok() ? SA_OK : refused(v);
 }
 
@@ -1196,10 +1200,12 @@ extern "C" sa_status sa_paged_extend(const sa_kvcache* c, int layer, const void*
         return fail(SA_EINVAL, "bf16 queries take a bf16 or 8-bit cache");
     if (!counts) return fail(SA_EINVAL, "null counts");
     return no_throw([&]() -> sa_status {
-        SA_TRY(check_ranges(c, layer, q, n_seq, n_q_heads, out, ws, ws_bytes,
-                            sa_paged_extend_ws_bytes(c, n_seq, counts, n_q_heads)));
         const Verdict vd = c->pt.check_rows(seq_ids, n_seq, false);
         if (!vd.ok()) return refused(vd);
+        // nothing to do needs no tensors
+        if (n_seq > 0 && std::all_of(counts, counts + n_seq, [](int32_t k) { return k == 0; })) return SA_OK;
+        SA_TRY(check_ranges(c, layer, q, n_seq, n_q_heads, out, ws, ws_bytes,
+                            sa_paged_extend_ws_bytes(c, n_seq, counts, n_q_heads)));
         std::vector<ChunkSeq> seqs;
         seqs.reserve(n_seq);
         long long rows = 0;

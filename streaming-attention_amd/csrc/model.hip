@@ -72,6 +72,8 @@ struct sa_qwen3 {
     float* part2 = nullptr;
     void* ws2 = nullptr;
     size_t ws2_bytes = 0;
+    void* ext = nullptr;       // chunks of new tokens: attention workspace or activations (see grow)
+    size_t ext_bytes = 0;
     void* beam_ws = nullptr;   // a beam step's greedy tokens, selection and shared attention (see grow)
     size_t beam_ws_bytes = 0;
     hipStream_t side = nullptr;
@@ -517,6 +519,8 @@ void release(sa_qwen3* m) {
     m->ws = nullptr;
     if (m->ws2) (void)hipFree(m->ws2);
     m->ws2 = nullptr;
+    if (m->ext) (void)hipFree(m->ext);
+    m->ext = nullptr;
     if (m->beam_ws) (void)hipFree(m->beam_ws);
     m->beam_ws = nullptr;
     if (m->pf) (void)hipFree(m->pf);
@@ -707,6 +711,67 @@ extern "C" sa_status sa_qwen3_init_random(sa_qwen3* m, uint64_t seed, float stde
     return SA_OK;
 }
 
+namespace sa {
+namespace {
+
+// A forward over M token rows of prompts: activations carved from one buffer, n
+// rows for the head, ws_attn bytes for the attention.
+struct PromptSizes {
+    size_t part, floats, bytes;
+    PromptSizes(const Shapes& s, long long M, int n, size_t ws_attn) {
+        part = part_floats(s, (size_t)M);
+        const size_t f_x = M * s.H, f_q = M * s.Nq, f_k = M * s.Nk, f_act = M * s.I;
+        floats = (2 * f_x + 2 * f_q + 2 * f_k + f_act + part + (size_t)n * s.H + 63) / 64 * 64;
+        bytes = (floats + (ws_attn + 255) / 256 * 64) * sizeof(float);
+    }
+};
+struct PromptRows {
+    float *x, *h, *q, *attn, *k, *v, *act, *part, *h_last, *ws;
+    Projections g;
+    PromptRows(const Shapes& s, long long M, const PromptSizes& sz, void* buf)
+        : x(static_cast<float*>(buf)), h(x + M * s.H), q(h + M * s.H), attn(q + M * s.Nq), k(attn + M * s.Nq),
+          v(k + M * s.Nk), act(v + M * s.Nk), part(act + M * s.I), h_last(part + sz.part),
+          ws(sz.bytes > sz.floats * sizeof(float) ? x + sz.floats : nullptr), g(plan_layer(s, M, sz.part)) {}
+};
+
+sa_status check_prompt_rows(const Shapes& s, long long M) {
+    if (M > 0x7fffffffLL / std::max({s.Nqkv, 2 * s.I, s.H})) return fail(SA_ERANGE, "batch * prompt too large");
+    return SA_OK;
+}
+
+// The layers of M token rows, up to the final norm's output in r.h.  attention(l,
+// split): r.attn from the qkv projection's `split` partials in r.part.
+template <class Attention>
+sa_status prompt_layers(sa_qwen3* m, const Shapes& s, long long M, const int32_t* tokens, const PromptRows& r,
+                        hipStream_t st, const Attention& attention) {
+    const sa_qwen3_desc& d = m->d;
+    const float eps = d.rms_eps;
+    hipLaunchKernelGGL(embed_norm_kernel, dim3((unsigned)M), dim3(256), 0, st, m->embed, tokens, s.V, s.H,
+                       m->layers[0].in_norm, eps, r.x, r.h);
+    SA_CHECK_LAUNCH();
+    for (int l = 0; l < d.num_layers; ++l) {
+        const sa_qwen3::Layer& Ly = m->layers[l];
+        // ---- attention block ----
+        SA_TRY(project(r.h, (int)M, Ly.qkv, r.g.qkv, r.part, st));
+        SA_TRY(attention(l, r.g.qkv.split));
+        SA_TRY(project(r.attn, (int)M, Ly.o, r.g.o, r.part, st));
+        hipLaunchKernelGGL(residual_norm_kernel, dim3((unsigned)M), dim3(256), 0, st, r.part, r.g.o.split, (int)M, s.H,
+                           r.x, Ly.post_norm, eps, r.h);
+        SA_CHECK_LAUNCH();
+        // ---- MLP ----
+        SA_TRY(project(r.h, (int)M, Ly.gate_up, r.g.gate_up, r.act, st));
+        SA_TRY(project(r.act, (int)M, Ly.down, r.g.down, r.part, st));
+        const float* next_norm = l + 1 < d.num_layers ? m->layers[l + 1].in_norm : m->final_norm;
+        hipLaunchKernelGGL(residual_norm_kernel, dim3((unsigned)M), dim3(256), 0, st, r.part, r.g.down.split, (int)M,
+                           s.H, r.x, next_norm, eps, r.h);
+        SA_CHECK_LAUNCH();
+    }
+    return SA_OK;
+}
+
+}  // namespace
+}  // namespace sa
+
 // A prompt of L tokens for each of sequences 0 .. batch-1 (all empty), run
 // as one causal prefill: the activations are batch * L token rows, the
 // projections GEMMs over row tiles (proj.hip; split-K where the tiles are few), the attention
@@ -738,73 +803,37 @@ extern "C" sa_status sa_qwen3_prefill(sa_qwen3* m, sa_kvcache* cache, const int3
     hipStream_t st = as_stream(stream);
     const Shapes s = shapes_of(d);
     const long long M = (long long)batch * L;
-    if (M > 0x7fffffffLL / std::max({s.Nqkv, 2 * s.I, s.H}))
-        return fail(SA_ERANGE, "batch * prompt too large");
-    const size_t f_part = part_floats(s, (size_t)M);
-    const Projections g = plan_layer(s, M, f_part);
-
-    // activations of the M token rows, carved from one grow-only buffer
-    const size_t f_x = M * s.H, f_q = M * s.Nq, f_k = M * s.Nk, f_act = M * s.I;
+    SA_TRY(check_prompt_rows(s, M));
     // the attention's workspace (paired key ranges of short prompts) after
     // the activations, at a 256-byte boundary
     const size_t ws_attn = sa_prefill_causal_ws_bytes(SA_DTYPE_F32, batch, s.Hq, s.Hkv, L, s.D);
-    const size_t f_act_all = (2 * f_x + 2 * f_q + 2 * f_k + f_act + f_part + (size_t)batch * s.H + 63) / 64 * 64;
-    const size_t floats = f_act_all + (ws_attn + 255) / 256 * 64;
-    const size_t need = floats * sizeof(float);
-    if (need > m->pf_bytes) {
+    const PromptSizes sz(s, M, batch, ws_attn);
+    if (sz.bytes > m->pf_bytes) {
         if (m->pf) SA_HIP_TRY(hipFree(m->pf));
         m->pf = nullptr;
         m->pf_bytes = 0;
-        if (hipMalloc(&m->pf, need) != hipSuccess) return fail(SA_ENOMEM, "prefill activations");
-        m->pf_bytes = need;
+        if (hipMalloc(&m->pf, sz.bytes) != hipSuccess) return fail(SA_ENOMEM, "prefill activations");
+        m->pf_bytes = sz.bytes;
     }
-    float* x = static_cast<float*>(m->pf);
-    float* h = x + f_x;
-    float* q = h + f_x;
-    float* attn = q + f_q;
-    float* k = attn + f_q;
-    float* v = k + f_k;
-    float* act = v + f_k;
-    float* part = act + f_act;
-    float* h_last = part + f_part;
-    float* attn_ws = ws_attn ? static_cast<float*>(m->pf) + f_act_all : nullptr;
-    const float eps = d.rms_eps;
     const float scale = 1.0f / sqrtf((float)d.head_dim);
-    float* out_logits = logits ? logits : m->logits;
-
-    hipLaunchKernelGGL(embed_norm_kernel, dim3((unsigned)M), dim3(256), 0, st, m->embed, tokens, s.V, s.H,
-                       m->layers[0].in_norm, eps, x, h);
-    SA_CHECK_LAUNCH();
+    const PromptRows r(s, M, sz, m->pf);
     const int64_t q_str[3] = {(int64_t)L * s.Nq, s.D, s.Nq};
     const int64_t kv_str[3] = {(int64_t)L * s.Nk, s.D, s.Nk};
-    for (int l = 0; l < d.num_layers; ++l) {
+    SA_TRY(prompt_layers(m, s, M, tokens, r, st, [&](int l, int split) -> sa_status {
         const sa_qwen3::Layer& Ly = m->layers[l];
-        // ---- attention block ----
-        SA_TRY(project(h, (int)M, Ly.qkv, g.qkv, part, st));
         // q, k, v summed from the projection's split-K partials, q and k
         // normed and rotated (positions 0 .. L-1: the cache is empty), K and V
         // appended to the cache, q, k, v written for the attention: one launch.
-        SA_TRY(qknorm_rope_append_partials(cache, l, part, g.qkv.split, batch, L, s.Hq, Ly.q_norm, Ly.k_norm, eps,
-                                           m->rope_cos, m->rope_sin, d.max_pos, q, k, v, st));
-        SA_TRY(sa_prefill_causal_strided_ws(q, k, v, SA_DTYPE_F32, batch, s.Hq, s.Hkv, L, s.D, q_str, kv_str, q_str,
-                                            scale, attn, attn_ws, ws_attn, stream));
-        SA_TRY(project(attn, (int)M, Ly.o, g.o, part, st));
-        hipLaunchKernelGGL(residual_norm_kernel, dim3((unsigned)M), dim3(256), 0, st, part, g.o.split, (int)M, s.H, x,
-                           Ly.post_norm, eps, h);
-        SA_CHECK_LAUNCH();
-        // ---- MLP ----
-        SA_TRY(project(h, (int)M, Ly.gate_up, g.gate_up, act, st));
-        SA_TRY(project(act, (int)M, Ly.down, g.down, part, st));
-        const float* next_norm = l + 1 < d.num_layers ? m->layers[l + 1].in_norm : m->final_norm;
-        hipLaunchKernelGGL(residual_norm_kernel, dim3((unsigned)M), dim3(256), 0, st, part, g.down.split, (int)M, s.H,
-                           x, next_norm, eps, h);
-        SA_CHECK_LAUNCH();
-    }
+        SA_TRY(qknorm_rope_append_partials(cache, l, r.part, split, batch, L, s.Hq, Ly.q_norm, Ly.k_norm, d.rms_eps,
+                                           m->rope_cos, m->rope_sin, d.max_pos, r.q, r.k, r.v, st));
+        return sa_prefill_causal_strided_ws(r.q, r.k, r.v, SA_DTYPE_F32, batch, s.Hq, s.Hkv, L, s.D, q_str, kv_str,
+                                            q_str, scale, r.attn, r.ws, ws_attn, stream);
+    }));
     // ---- the last position of each sequence: lm_head, greedy argmax ----
-    SA_HIP_TRY(hipMemcpy2DAsync(h_last, (size_t)s.H * sizeof(float), h + (size_t)(L - 1) * s.H,
+    SA_HIP_TRY(hipMemcpy2DAsync(r.h_last, (size_t)s.H * sizeof(float), r.h + (size_t)(L - 1) * s.H,
                                 (size_t)L * s.H * sizeof(float), (size_t)s.H * sizeof(float), batch,
                                 hipMemcpyDeviceToDevice, st));
-    SA_TRY(head(m, s, {h_last, nullptr, 0, nullptr, 0.f, nullptr}, batch, out_logits, next_tokens, st));
+    SA_TRY(head(m, s, {r.h_last, nullptr, 0, nullptr, 0.f, nullptr}, batch, logits ? logits : m->logits, next_tokens, st));
     return sa_kvcache_commit(cache, nullptr, batch, L, stream);
 }
 
@@ -827,9 +856,42 @@ struct RowGroups {
     size_t ws_bytes;
 };
 
-// One step of rows 0 .. batch-1, in groups or (NULL) not.
+// Chunks of new tokens instead of one per row: counts[i] tokens of cache row i, the
+// workspace of their attention, and whether the head takes each sequence's last
+// token only.
+struct Chunks {
+    const int32_t* counts;
+    int n_seq;
+    bool last_only;
+    void* ws;
+    size_t ws_bytes;
+};
+
+// The last token's row of each sequence.
+struct LastRows {
+    int32_t row[kRowsPerLaunch];
+};
+__global__ void __launch_bounds__(256) last_rows_kernel(const float* h, LastRows rows, int H, float* out) {
+    const float4* src = reinterpret_cast<const float4*>(h + (size_t)rows.row[blockIdx.x] * H);
+    float4* dst = reinterpret_cast<float4*>(out + (size_t)blockIdx.x * H);
+    for (int i = threadIdx.x; i < H / 4; i += 256) dst[i] = src[i];
+}
+sa_status last_rows(const float* h, int H, int n_seq, const int32_t* counts, float* out, hipStream_t st) {
+    int row = -1;
+    for (int i0 = 0; i0 < n_seq; i0 += kRowsPerLaunch) {
+        LastRows lr{};
+        const int n = std::min(kRowsPerLaunch, n_seq - i0);
+        for (int i = 0; i < n; ++i) lr.row[i] = row += counts[i0 + i];
+        hipLaunchKernelGGL(last_rows_kernel, dim3(n), dim3(256), 0, st, h, lr, H, out + (size_t)i0 * H);
+        SA_CHECK_LAUNCH();
+    }
+    return SA_OK;
+}
+
+// One step of rows 0 .. batch-1, in groups or (NULL) not; with chunks, of their batch
+// tokens, which stay uncommitted (the caller has checked positions and pages).
 sa_status decode_rows(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int batch, const RowGroups* groups,
-                      int32_t* next_tokens, float* logits, sa_stream_t stream) {
+                      int32_t* next_tokens, float* logits, sa_stream_t stream, const Chunks* chunks = nullptr) {
     if (!m || !cache || !tokens || !next_tokens) return fail(SA_EINVAL, "null argument");
     if (batch < 1 || batch > m->max_batch) return fail(SA_ERANGE, "batch outside [1, max_batch]");
     sa_kv_desc kd;
@@ -837,23 +899,25 @@ sa_status decode_rows(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int
     const sa_qwen3_desc& d = m->d;
     if (kd.num_layers != d.num_layers || kd.num_kv_heads != d.n_kv_heads || kd.head_dim != d.head_dim)
         return fail(SA_EINVAL, "cache geometry does not match the model");
-    if (batch > kd.max_seqs) return fail(SA_ERANGE, "batch exceeds the cache's sequences");
-    for (int i = 0; i < batch; ++i) {
-        const int len = sa_kvcache_len(cache, i);
-        if (len < 0 || len >= d.max_pos) return fail(SA_ERANGE, "position outside the RoPE table");
-        if (len + 1 > sa_kvcache_capacity(cache, i)) return fail(SA_EFULL, "KV cache full, cannot append more tokens");
+    if (!chunks) {
+        if (batch > kd.max_seqs) return fail(SA_ERANGE, "batch exceeds the cache's sequences");
+        for (int i = 0; i < batch; ++i) {
+            const int len = sa_kvcache_len(cache, i);
+            if (len < 0 || len >= d.max_pos) return fail(SA_ERANGE, "position outside the RoPE table");
+            if (len + 1 > sa_kvcache_capacity(cache, i)) return fail(SA_EFULL, "KV cache full, cannot append more tokens");
+        }
+        SA_TRY(check_append(cache, batch, 1, d.max_pos));
     }
-    SA_TRY(check_append(cache, batch, 1, d.max_pos));
     // The row-by-row form is made for some head ratios; the shared one takes
     // rows that share nothing too.
     const int rep = d.n_q_heads / d.n_kv_heads;
     const bool by_rows = decode_rep_ok(rep);
-    if (!by_rows && !groups) return fail(SA_EINVAL, "n_q_heads / n_kv_heads must be 1, 2, 4 or 8");
+    if (!by_rows && !groups && !chunks) return fail(SA_EINVAL, "n_q_heads / n_kv_heads must be 1, 2, 4 or 8");
     if (!by_rows && rep > kRangesMaxRep) return fail(SA_EINVAL, "at most 64 query heads per KV head");
     hipStream_t st = as_stream(stream);
     const bool shared =
         groups && (!by_rows || shared_tokens_saved(cache, groups->sizes, groups->n) >= kSharedTokens);
-    const size_t need = sa_paged_decode_ws_bytes(cache, batch, d.n_q_heads);
+    const size_t need = chunks ? 0 : sa_paged_decode_ws_bytes(cache, batch, d.n_q_heads);
     SA_TRY(grow(m, &m->ws, &m->ws_bytes, need));
     const Shapes s = shapes_of(d);
     const int M = batch;
@@ -874,12 +938,13 @@ sa_status decode_rows(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int
     // has a tail of its own.
     long long total = 0;
     std::vector<long long> prefix(M + 1, 0);
-    for (int i = 0; i < M; ++i) prefix[i + 1] = prefix[i] + sa_kvcache_len(cache, i) + 1;
+    if (!chunks)
+        for (int i = 0; i < M; ++i) prefix[i + 1] = prefix[i] + sa_kvcache_len(cache, i) + 1;
     total = prefix[M];
-    const int kv_elem = kd.kv_dtype == SA_DTYPE_BF16 ? 2 : 4;
+    const int kv_elem = kd.kv_dtype == SA_DTYPE_FP8 ? 1 : kd.kv_dtype == SA_DTYPE_BF16 ? 2 : 4;
     const long long attn_bytes = total * d.n_kv_heads * d.head_dim * 2LL * kv_elem;
     const char* fenv = std::getenv("SA_DECODE_INTERLEAVE");
-    const bool interleave = !shared && M >= 2 && (fenv ? std::atoi(fenv) != 0 : attn_bytes >= kInterleaveBytes);
+    const bool interleave = !shared && !chunks && M >= 2 && (fenv ? std::atoi(fenv) != 0 : attn_bytes >= kInterleaveBytes);
     const bool long_attn = !shared && attn_bytes >= kBesideBytes;
     bool few_head_rows = false;   // the head takes the last layer's residual sum of all rows
 
@@ -929,6 +994,12 @@ sa_status decode_rows(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int
     auto attention = [&](Rows& r, int l) -> sa_status {
         const sa_qwen3::Layer& L = m->layers[l];
         const int n_part = r.few ? 1 : r.beside ? r.gb.qkv.S : r.g.qkv.split;
+        if (chunks) {
+            SA_TRY(append_partials_ragged(cache, l, r.part, n_part, chunks->n_seq, chunks->counts, s.Hq, L.q_norm,
+                                          L.k_norm, eps, m->rope_cos, m->rope_sin, d.max_pos, m->q_rope, r.st));
+            return sa_paged_extend(cache, l, m->q_rope, SA_DTYPE_F32, chunks->n_seq, nullptr, chunks->counts, s.Hq, scale,
+                                   m->attn, chunks->ws, chunks->ws_bytes, r.st);
+        }
         if (shared) {
             SA_TRY(qknorm_rope_append_partials(cache, l, r.part, n_part, r.n, 1, s.Hq, L.q_norm, L.k_norm, eps,
                                                m->rope_cos, m->rope_sin, d.max_pos, m->q_rope, nullptr, nullptr, r.st));
@@ -990,7 +1061,7 @@ sa_status decode_rows(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int
                        m->layers[0].in_norm, eps, m->x, m->h);
     SA_CHECK_LAUNCH();
     Rows all = make_rows(0, M, m->part, m->ws, m->ws_bytes, st, false);
-    few_head_rows = all.few && !interleave;
+    few_head_rows = all.few && !interleave && !(chunks && chunks->last_only);
     if (!interleave) {
         for (int l = 0; l < d.num_layers; ++l) {
             SA_TRY(qkv(all, l));
@@ -1032,7 +1103,14 @@ sa_status decode_rows(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int
     // ---- final norm, lm_head, greedy argmax ----
     FewInput last{m->h, nullptr, 0, nullptr, 0.f, nullptr};   // normed by the last layer's residual launch
     if (few_head_rows) last = {all.x, all.down_part, kFewSplit, m->final_norm, eps, nullptr};
-    SA_TRY(head(m, s, last, M, out_logits, next_tokens, st));
+    int head_rows = M;
+    if (chunks && chunks->last_only) {
+        float* rows = all.x == m->x ? m->x2 : m->x;   // the residual stream has been read
+        SA_TRY(last_rows(m->h, s.H, chunks->n_seq, chunks->counts, rows, st));
+        last.x = rows;
+        head_rows = chunks->n_seq;
+    }
+    SA_TRY(head(m, s, last, head_rows, out_logits, next_tokens, st));
     return SA_OK;   // the last layer's attention committed the token
 }
 
@@ -1076,4 +1154,70 @@ extern "C" sa_status sa_qwen3_beam_step(sa_qwen3* m, sa_kvcache* cache, const in
     }
     return sa_beam_select(m->logits, m->d.vocab, scores, n_groups, n_beams, m->d.vocab, n_select, out_scores, out_tokens,
                           out_beams, static_cast<char*>(m->beam_ws) + next, select, stream);
+}
+
+// Every check is made before anything is enqueued.  Up to max_batch new tokens take
+// the decoder step's launches (few rows their streaming projections), more the
+// prompt's, with activations in a buffer of their own.
+extern "C" sa_status sa_qwen3_extend(sa_qwen3* m, sa_kvcache* cache, const int32_t* tokens, int n_seq,
+                                     const int32_t* counts, int all_rows, int32_t* next_tokens, float* logits,
+                                     int commit, sa_stream_t stream) {
+    clear_error();
+    if (!m || !cache || !counts) return fail(SA_EINVAL, "null argument");
+    const sa_qwen3_desc& d = m->d;
+    sa_kv_desc kd;
+    SA_TRY(sa_kvcache_get_desc(cache, &kd));
+    if (kd.num_layers != d.num_layers || kd.num_kv_heads != d.n_kv_heads || kd.head_dim != d.head_dim)
+        return fail(SA_EINVAL, "cache geometry does not match the model");
+    if (n_seq < 1 || n_seq > kd.max_seqs) return fail(SA_ERANGE, "n_seq outside [1, the cache's sequences]");
+    if (d.n_q_heads / d.n_kv_heads > kRangesMaxRep) return fail(SA_EINVAL, "at most 64 query heads per KV head");
+    long long M = 0;
+    for (int i = 0; i < n_seq; ++i) {
+        if (counts[i] < 0 || (counts[i] == 0 && !all_rows))
+            return fail(SA_EINVAL, "every sequence takes a new token, or with every token's logits none or more");
+        const long long end = (long long)sa_kvcache_len(cache, i) + counts[i];
+        if (end > d.max_pos) return fail(SA_ERANGE, "position outside the RoPE table");
+        if (end > sa_kvcache_capacity(cache, i)) return fail(SA_EFULL, "KV cache full, cannot append more tokens");
+        M += counts[i];
+    }
+    if (M == 0) return SA_OK;
+    if (!tokens || !next_tokens) return fail(SA_EINVAL, "null argument");
+    const Shapes s = shapes_of(d);
+    if (M > kMaxNewTokens) return fail(SA_ERANGE, "more than 2^20 new tokens");
+    SA_TRY(check_prompt_rows(s, M));
+    const int head_rows = all_rows ? (int)M : n_seq;
+    if (head_rows > m->max_batch) return fail(SA_ERANGE, "more rows of logits than max_batch");
+    SA_TRY(check_append_ragged(cache, n_seq, counts, d.max_pos));
+    const size_t attn = (sa_paged_extend_ws_bytes(cache, n_seq, counts, d.n_q_heads) + 255) / 256 * 256;
+    hipStream_t st = as_stream(stream);
+    try {
+        std::vector<int32_t> rows(n_seq), lens(n_seq);
+        for (int i = 0; i < n_seq; ++i) {
+            rows[i] = i;
+            lens[i] = sa_kvcache_len(cache, i) + counts[i];
+        }
+        if (M <= m->max_batch) {
+            SA_TRY(grow(m, &m->ext, &m->ext_bytes, std::max<size_t>(attn, 256)));
+            const Chunks chunks{counts, n_seq, !all_rows, m->ext, m->ext_bytes};
+            SA_TRY(decode_rows(m, cache, tokens, (int)M, nullptr, next_tokens, logits, stream, &chunks));
+        } else {
+            const PromptSizes sz(s, M, head_rows, attn);
+            SA_TRY(grow(m, &m->ext, &m->ext_bytes, sz.bytes));
+            const PromptRows r(s, M, sz, m->ext);
+            const float scale = 1.0f / sqrtf((float)d.head_dim);
+            SA_TRY(prompt_layers(m, s, M, tokens, r, st, [&](int l, int split) -> sa_status {
+                const sa_qwen3::Layer& L = m->layers[l];
+                SA_TRY(append_partials_ragged(cache, l, r.part, split, n_seq, counts, s.Hq, L.q_norm, L.k_norm,
+                                              d.rms_eps, m->rope_cos, m->rope_sin, d.max_pos, r.q, st));
+                return sa_paged_extend(cache, l, r.q, SA_DTYPE_F32, n_seq, nullptr, counts, s.Hq, scale, r.attn, r.ws,
+                                       attn, stream);
+            }));
+            SA_TRY(last_rows(r.h, s.H, n_seq, counts, r.h_last, st));
+            SA_TRY(head(m, s, {r.h_last, nullptr, 0, nullptr, 0.f, nullptr}, n_seq, logits ? logits : m->logits,
+                        next_tokens, st));
+        }
+        return commit ? sa_kvcache_set_lens(cache, rows.data(), lens.data(), n_seq, stream) : SA_OK;
+    } catch (const std::bad_alloc&) {
+        return fail(SA_ENOMEM, "out of host memory");
+    }
 }

@@ -287,6 +287,10 @@ sa_status append_decode_partials(sa_kvcache* c, int layer, const float* part, in
 // Whether the next S tokens of rows 0 .. n - 1 can be appended: pages of their
 // own for them, and positions below max_pos.
 sa_status check_append(const sa_kvcache* c, int n, int S, int max_pos);
+// The same of counts[i] tokens of row i.
+sa_status check_append_ragged(const sa_kvcache* c, int n, const int32_t* counts, int max_pos);
+
+constexpr int kMaxNewTokens = 1 << 20;   // of one call over chunks of new tokens
 
 // Tokens that a shared decode of rows 0 .. in groups of sizes[0, n_groups)
 // reads once instead of once per row, with one token pending in each row.

@@ -304,12 +304,18 @@ def test_refusals(sa):
 
 
 def test_no_tokens_is_nothing_to_do(sa):
-    rows = Rows(sa, "f32", 1, 64, [10], seed=22)
+    rows = Rows(sa, "f32", 1, 64, [10, 0], seed=22)
     x = torch.empty(0, 2, 64, device="cuda")
-    buf = torch.zeros(1, 2, 64, device="cuda")
-    lib = sa.lib()
-    zero = (C.c_int32 * 1)(0)
-    assert lib.sa_paged_extend(rows.cache.handle, 0, buf.data_ptr(), 0, 1, None, C.cast(zero, C.c_void_p), 2, 1.0,
-                               buf.data_ptr(), None, 0, None) == sa.SA_OK
-    assert x.numel() == 0 and (buf == 0).all()
+    assert rows.cache.extend(0, x, 1.0, [0, 0]).shape == x.shape
+    rows.cache.append(0, x, x[:, :1].contiguous(), x[:, :1].contiguous(), counts=[0, 0])
+    assert rows.cache.length(0) == 10
     assert code(sa, "fp8") == sa.SA_DTYPE_FP8
+
+
+def test_short_rows_of_many_sequences_take_no_workspace(sa):
+    """Pages of one tile's tokens hold no more than one partial per row."""
+    rows = Rows(sa, "bf16", 1, 64, [5] * 66, seed=23, room=2)
+    rows.append([2] * 66)
+    x = rows.normal(132, 1, 64)
+    got = rows.cache.extend(0, x, 0.125, [2] * 66)
+    check_all(rows, got, x, [2] * 66, [5] * 66, 0.125)
