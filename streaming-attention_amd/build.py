@@ -44,6 +44,7 @@ DEVICE = [
 # VGPRs (their softmax rescales them with VALU ops); the register-staged bf16
 # kernel parks Q in AGPRs.
 EXTRA = {
+    "extend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "ranges.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "window.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],

@@ -1,0 +1,520 @@
+// Attention of chunks of many new tokens over a paged cache, on bf16 MFMA.
+//
+// A chunk's query rows (new tokens x query heads of a KV head, in that order) are cut
+// into blocks of 32 per wave; token j of a sequence of len committed tokens sees keys
+// 0 .. len + j.  A workgroup takes a block of one KV head and a range of its key
+// tiles, a tile being a page's 64 keys, and leaves its rows' output, or where a
+// block's tiles are cut a partial (m, l, O) per row for a second launch to join.
+//
+// bf16 queries (and output) over a bf16 or 8-bit cache: v_mfma_f32_32x32x16_bf16 and
+// the softmax of bf16_wave.h; the roundings are P to bf16 (2^-8 of each weight, the
+// sums taken of the rounded ones) and the output's.  A bf16 page is loaded straight
+// into LDS; codes of an 8-bit page are widened on the way, times their row's scale,
+// which is exact, once per workgroup rather than once per wave.
+//
+// Rows whose sums are not finite are computed anew over what they see (plain_row.h).
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "bf16_terms.h"
+#include "bf16_wave.h"
+#include "plain_row.h"
+#include "ranges.h"
+
+namespace sa {
+namespace {
+
+struct BlockArgs {
+    const void* q;
+    const void* k;
+    const void* v;
+    const uint8_t* k_scale;
+    const uint8_t* v_scale;
+    const int32_t* table;
+    void* out;
+    float* part_o;
+    float* part_ml;
+    int n_kv, n_q, rep, max_pages, num_pages;
+    int n_seq;
+    int rows;                                // query rows of a block
+    int tiles;                               // key tiles of a workgroup
+    float sl2;                               // |scale| log2(e)
+    float factor;                            // scale log2(e)
+    uint32_t q_sign;                         // 0x80008000 for a negative scale
+    ChunkSeq seq[kRowsPerLaunch];
+    int32_t start[kRowsPerLaunch + 1];       // a sequence's first item, of blocks x parts
+    int32_t base[kRowsPerLaunch];            // its first partial row
+    int32_t parts[kRowsPerLaunch];           // of its last block
+};
+static_assert(sizeof(BlockArgs) <= 4096, "kernel arguments");
+
+// Key tiles that block b of a sequence sees.
+__host__ __device__ inline int block_key_tiles(const ChunkSeq& s, int b, int rows, int rep) {
+    const long long end = (long long)(b + 1) * rows, all = (long long)s.n * rep;
+    return (int)((s.len + ((end < all ? end : all) - 1) / rep) / kBfTile) + 1;
+}
+
+// A workgroup's place.
+struct Block {
+    ChunkSeq sq;
+    int kvh, r0, row_end;   // query rows [r0, row_end) of the sequence
+    int u0, u1;             // key tiles
+    bool whole;             // the output itself
+    long long part0;        // partial row of query row 0
+    const __attribute__((address_space(4))) int32_t* pages;
+};
+__device__ __forceinline__ bool place(const BlockArgs& a, Block& w) {
+    const int lane = threadIdx.x & (kWave - 1);
+    const int item = blockIdx.x / a.n_kv;   // the KV head varies fastest: with 8 of them each XCD has one
+    const int i = __popcll(__ballot(lane < a.n_seq && a.start[lane] <= item)) - 1;
+    w.sq = a.seq[i];
+    w.kvh = blockIdx.x % a.n_kv;
+    const int parts = a.parts[i], local = item - a.start[i], all = w.sq.n * a.rep;
+    const int b = (all + a.rows - 1) / a.rows - 1 - local / parts, c = local % parts;   // the longest first
+    w.r0 = b * a.rows;
+    w.row_end = min(all, w.r0 + a.rows);
+    w.u0 = c * a.tiles;
+    w.u1 = min(w.u0 + a.tiles, block_key_tiles(w.sq, b, a.rows, a.rep));
+    w.whole = parts == 1;
+    w.part0 = a.base[i] + (long long)c * all;
+    // read with scalar loads
+    w.pages = (const __attribute__((address_space(4))) int32_t*)(a.table + (size_t)w.sq.cache_row * a.max_pages);
+    return w.u0 < w.u1;
+}
+// An id outside the pool (an entry that was never set) is clamped so that no load
+// can fault.
+__device__ __forceinline__ int page_of(const BlockArgs& a, const Block& w, int u) {
+    return min(max(w.pages[u], 0), a.num_pages - 1);
+}
+__device__ __forceinline__ size_t out_row(const BlockArgs& a, const Block& w, int row) {
+    const int t = row / a.rep;
+    return ((size_t)(w.sq.first + t) * a.n_q + w.kvh * a.rep + row - t * a.rep);
+}
+
+// Query row `row` over the workgroup's keys without matrix instructions, one wave.
+template <int D, int KV, class T>
+__device__ __forceinline__ void block_plain(const BlockArgs& a, const Block& w, int row) {
+    using E = std::conditional_t<KV == SA_DTYPE_FP8, uint8_t, std::conditional_t<KV == SA_DTYPE_BF16, uint16_t, float>>;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int end = w.sq.len + row / a.rep + 1;   // keys that it sees
+    const size_t o = out_row(a, w, row) * D;
+    PlainRow<D> p;
+    for (int u = w.u0; u < w.u1 && u * kBfTile < end && !p.lost(); ++u) {
+        const size_t key = ((size_t)page_of(a, w, u) * a.n_kv + w.kvh) * kBfTile;
+        auto value = [&](const void* pool, int i) { return static_cast<const E*>(pool) + (key + i) * D; };
+        auto scale = [&](const uint8_t* s, int i) {
+            if constexpr (KV == SA_DTYPE_FP8) return __uint_as_float((uint32_t)s[key + i] << 23);
+            else return 1.f;
+        };
+        p.keys(min(kBfTile, end - u * kBfTile), static_cast<const T*>(a.q) + o, a.factor,
+               [&](int i) { return value(a.k, i); }, [&](int i) { return value(a.v, i); },
+               [&](int i) { return scale(a.k_scale, i); }, [&](int i) { return scale(a.v_scale, i); });
+    }
+    const size_t at = (size_t)(w.part0 + row) * a.n_kv + w.kvh;
+#pragma unroll
+    for (int e = 0; e < p.E; ++e) {
+        const int d = lane * p.E + e;
+        if (!w.whole) a.part_o[at * D + d] = p.o[e];
+        else if constexpr (sizeof(T) == 2) static_cast<T*>(a.out)[o + d] = f32_to_bf16_rne(p.o[e] / p.l);
+        else static_cast<T*>(a.out)[o + d] = p.o[e] / p.l;
+    }
+    if (!w.whole && lane == 0) {
+        a.part_ml[at * 2] = p.m;
+        a.part_ml[at * 2 + 1] = p.l;
+    }
+}
+
+// ---------------------------------------------------------------- bf16
+
+// Sixteen codes of a row as two chunks of LDS.
+__device__ __forceinline__ bf16x8_t widen8(uint32_t lo, uint32_t hi, float scale) {
+    const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
+    const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
+    const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
+    const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
+    return __builtin_bit_cast(bf16x8_t, u32x4_t{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b),
+                                                __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)});
+}
+
+template <int D, int W, bool FP8>
+__global__ void __launch_bounds__(W * kWave, W == 8 && D == 64 ? 4 : 1) extend_bf16_kernel(BlockArgs a) {
+    using G = BfGeo<D>;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    lds_u8_t* const smem = (lds_u8_t*)smem_raw;
+    const uint32_t lds_at = static_cast<uint32_t>(reinterpret_cast<size_t>(smem));
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    Block b;
+    if (!place(a, b)) return;
+    const int last_key = b.sq.len + b.sq.n - 1;   // of the sequence: keys behind it are not read
+
+    // ---- a bf16 tile straight into LDS, two tiles ahead ----
+    // Load i of a wave copies RPL rows, this lane's 16 bytes of them at off[i] from
+    // the page's first row; rows behind the sequence repeat its last.
+    constexpr int NI = G::NL / W > 0 ? G::NL / W : 1;
+    int row[NI], col[NI];
+    uint32_t off[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        row[i] = (wave * NI + i) * G::RPL + lane / G::CPR;
+        col[i] = 16 * ((lane % G::CPR) ^ G::swz(row[i] & 15));
+        off[i] = row[i] * G::ROWB + col[i];
+    }
+    auto load_bf16 = [&](int u, int page) {
+        if (G::NL < W && wave >= G::NL) return;
+        const size_t at = ((size_t)page * a.n_kv + b.kvh) * G::HALF;
+        const char* kt = static_cast<const char*>(a.k) + at;
+        const char* vt = static_cast<const char*>(a.v) + at;
+        lds_u8_t* dst = smem + (u & 1) * G::STAGE;
+        const int most = last_key - u * kBfTile;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            uint32_t o = off[i];
+            if (most < kBfTile - 1) o = min(row[i], most) * G::ROWB + col[i];
+            dma16_from(kt, o, dst + (wave * NI + i) * 1024);
+            dma16_from(vt, o, dst + G::HALF + (wave * NI + i) * 1024);
+        }
+    };
+    // ---- an 8-bit tile through registers, one tile ahead ----
+    constexpr int PIECES = kBfTile * D / 16;             // of 16 codes
+    constexpr int NP = PIECES / (W * kWave) > 0 ? PIECES / (W * kWave) : 1;
+    const bool loads = PIECES >= W * kWave || threadIdx.x < PIECES;
+    u32x4_t rk[NP], rv[NP];
+    uint32_t sk[NP], sv[NP];
+    auto load_fp8 = [&](int u, int page) {
+        if (!loads) return;
+        const size_t at = ((size_t)page * a.n_kv + b.kvh) * kBfTile;
+        const int most = last_key - u * kBfTile;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int idx = threadIdx.x + i * W * kWave;
+            const size_t r = at + min(idx / (D / 16), most);
+            rk[i] = *reinterpret_cast<const u32x4_t*>(static_cast<const char*>(a.k) + r * D + 16 * (idx % (D / 16)));
+            rv[i] = *reinterpret_cast<const u32x4_t*>(static_cast<const char*>(a.v) + r * D + 16 * (idx % (D / 16)));
+            sk[i] = a.k_scale[r];
+            sv[i] = a.v_scale[r];
+        }
+    };
+    auto store_fp8 = [&](int u) {
+        if (!loads) return;
+        lds_u8_t* dst = smem + (u & 1) * G::STAGE;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int idx = threadIdx.x + i * W * kWave;
+            const int r = idx / (D / 16), c = 2 * (idx % (D / 16));
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                lds_u8_t* at = dst + r * G::ROWB + (((c + h) ^ G::swz(r & 15)) << 4);
+                *reinterpret_cast<__attribute__((address_space(3))) bf16x8_t*>(at) =
+                    widen8(rk[i][2 * h], rk[i][2 * h + 1], __uint_as_float(sk[i] << 23));
+                *reinterpret_cast<__attribute__((address_space(3))) bf16x8_t*>(at + G::HALF) =
+                    widen8(rv[i][2 * h], rv[i][2 * h + 1], __uint_as_float(sv[i] << 23));
+            }
+        }
+    };
+
+    int page = page_of(a, b, b.u0), next = b.u0 + 1 < b.u1 ? page_of(a, b, b.u0 + 1) : 0;
+    if constexpr (FP8) load_fp8(b.u0, page);
+    else load_bf16(b.u0, page);
+    // This wave's 32 query rows, and the tokens that they belong to.
+    const int w0 = b.r0 + wave * 32;
+    const int my_row = min(w0 + (lane & 31), b.row_end - 1);
+    const bool active = w0 < b.row_end;
+    const int q_lo = b.sq.len + min(w0, b.row_end - 1) / a.rep, q_hi = b.sq.len + min(w0 + 31, b.row_end - 1) / a.rep;
+    const int q_mine = b.sq.len + my_row / a.rep;   // the last key that this lane's row sees
+    BfWave<D> w;
+    w.init(static_cast<const uint16_t*>(a.q) + out_row(a, b, my_row) * D, a.sl2, a.q_sign, w0, lane);
+    if constexpr (FP8) {
+        store_fp8(b.u0);
+        if (b.u0 + 1 < b.u1) load_fp8(b.u0 + 1, next);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    } else if (b.u0 + 1 < b.u1) {
+        load_bf16(b.u0 + 1, next);
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(2 * NI) : "memory");   // the first tile
+    } else {
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    }
+    next = b.u0 + 2 < b.u1 ? page_of(a, b, b.u0 + 2) : 0;
+    // Tile u has been computed by this wave.
+    auto end_tile = [&](int u) {
+        if constexpr (FP8) {
+            if (u + 1 < b.u1) store_fp8(u + 1);           // where tile u - 1 was
+            if (u + 2 < b.u1) load_fp8(u + 2, next);
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (u + 2 < b.u1) load_bf16(u + 2, next);
+        }
+        if (u + 3 < b.u1) next = page_of(a, b, u + 3);
+    };
+    auto edge_tile = [&](int u) {
+        const uint32_t sb = lds_at + (u & 1) * G::STAGE;
+        if (active) {
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                const int k = u * kBfTile + 32 * kb;
+                if (k + 31 <= q_lo) w.template half<false>(sb + kb * 32 * G::ROWB, [](f32x16_t&) {});
+                else if (k <= q_hi)
+                    w.template half<true>(sb + kb * 32 * G::ROWB, [&](f32x16_t& s) {
+                        const int last = q_mine - k - 8 * w.hh;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) s[j] = 16 * (j / 8) + j % 8 > last ? -INFINITY : s[j] * w.c;
+                    });
+            }
+        }
+        end_tile(u);
+    };
+    int u = b.u0;
+    if constexpr (W == 8) {
+        // The tiles that every row of the workgroup sees whole, in ping-pong: waves w and
+        // w + 4 share a SIMD, and each half tile is a block of MFMAs (the half before's P
+        // V, this half's scores) and a softmax.  Waves 4 - 7 take the half's barrier
+        // between the two, waves 0 - 3 behind both, so that on every SIMD one wave's
+        // softmax runs under the other's MFMAs.
+        const int hi = min(b.u1, (b.sq.len + b.r0 / a.rep + 1) / kBfTile);
+        if (u < hi) {
+            const bool late = wave >= W / 2;
+            if (!late) __builtin_amdgcn_s_setprio(1);
+            bf16x8_t vf[G::NDB][2], pb[2];
+#pragma unroll
+            for (int db = 0; db < G::NDB; ++db) vf[db][0] = vf[db][1] = bf16x8_t{};
+            pb[0] = pb[1] = bf16x8_t{};
+            auto pv = [&]() {
+#pragma unroll
+                for (int db = 0; db < G::NDB; ++db)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+                        w.acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[db][t], pb[t], w.acc[db], 0, 0, 0);
+            };
+            for (; u < hi; ++u) {
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb) {
+                    const uint32_t hb = lds_at + (u & 1) * G::STAGE + kb * 32 * G::ROWB;
+                    bf16x8_t kf[G::NKS];
+#pragma unroll
+                    for (int ks = 0; ks < G::NKS; ++ks) kf[ks] = w.k_frag(hb, ks);
+                    pv();
+#pragma unroll
+                    for (int db = 0; db < G::NDB; ++db)
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) vf[db][t] = w.v_frag(hb, db, t);
+                    f32x16_t s = {};
+#pragma unroll
+                    for (int ks = 0; ks < G::NKS; ++ks)
+                        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[ks], w.qf[ks], s, 0, 0, 0);
+                    auto sync = [&]() {
+                        __builtin_amdgcn_sched_barrier(0);
+                        if (kb == 0) asm volatile("s_barrier" ::: "memory");
+                        else end_tile(u);
+                        __builtin_amdgcn_sched_barrier(0);
+                    };
+                    if (late) sync();
+                    w.template softmax<false>(s, pb);
+                    if (!late) sync();
+                }
+            }
+            pv();
+            __builtin_amdgcn_s_setprio(0);
+        }
+    }
+    for (; u < b.u1; ++u) edge_tile(u);
+
+    const int rows = b.row_end - w0;   // of the wave, where positive
+    uint32_t anew;
+    if (b.whole) {
+        // The output through LDS, 32 rows per wave, so that stores are whole rows.
+        anew = w.store(rows, [&](int r) { return static_cast<uint16_t*>(a.out) + out_row(a, b, w0 + r) * D; },
+                       smem + wave * 32 * G::ROWB, lane);
+    } else {
+        const float l = w.l + xor32(w.l);
+        float zero = 0.f;   // NaN where an accumulator is not finite
+#pragma unroll
+        for (int db = 0; db < G::NDB; ++db)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) zero = fmaf(w.acc[db][j], 0.f, zero);
+        const uint64_t bad = __ballot(w.n < rows && !(l + zero < INFINITY));
+        anew = (uint32_t)bad | (uint32_t)(bad >> 32);
+        if (w.n < rows && !(anew >> w.n & 1)) {
+            const size_t at = (size_t)(b.part0 + w0 + w.n) * a.n_kv + b.kvh;
+            float* o = a.part_o + at * D + 4 * w.hh;
+#pragma unroll
+            for (int db = 0; db < G::NDB; ++db)
+#pragma unroll
+                for (int jj = 0; jj < 4; ++jj)
+                    *reinterpret_cast<f32x4_t*>(o + 32 * db + 8 * jj) =
+                        f32x4_t{w.acc[db][4 * jj], w.acc[db][4 * jj + 1], w.acc[db][4 * jj + 2], w.acc[db][4 * jj + 3]};
+            if (w.hh == 0) *reinterpret_cast<f32x2_t*>(a.part_ml + at * 2) = f32x2_t{w.m, l};
+        }
+    }
+    for (; anew; anew &= anew - 1)
+        block_plain<D, FP8 ? SA_DTYPE_FP8 : SA_DTYPE_BF16, uint16_t>(a, b, w0 + __builtin_ctz(anew));
+}
+
+// ---------------------------------------------------------------- partials
+
+__device__ __forceinline__ void put4(float* p, f32x4_t v) { *reinterpret_cast<f32x4_t*>(p) = v; }
+__device__ __forceinline__ void put4(uint16_t* p, f32x4_t v) {
+    const bf16x2_t lo = __builtin_convertvector(f32x2_t{v[0], v[1]}, bf16x2_t);
+    const bf16x2_t hi = __builtin_convertvector(f32x2_t{v[2], v[3]}, bf16x2_t);
+    *reinterpret_cast<uint2*>(p) = make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
+}
+
+// O = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c, D / 4 lanes per row of 256 D / 4
+// consecutive (token, head) rows from the launch's first token on.
+template <int D, class T>
+__global__ void __launch_bounds__(256) block_merge_kernel(BlockArgs a, long long n) {
+    constexpr int C = D / 4, ROWS = 256 / C;
+    const long long r = (long long)blockIdx.x * ROWS + threadIdx.x / C;
+    if (r >= n) return;
+    const int token = a.seq[0].first + (int)(r / a.n_q), head = (int)(r % a.n_q), c = threadIdx.x % C;
+    int i = a.n_seq - 1;
+    while (a.seq[i].first > token) --i;
+    const ChunkSeq sq = a.seq[i];
+    const int t = token - sq.first;
+    if (a.parts[i] == 1 || t >= sq.n) return;   // written already, or a row of another launch
+    const int kvh = head / a.rep, row = t * a.rep + head % a.rep;
+    const int parts = (block_key_tiles(sq, row / a.rows, a.rows, a.rep) + a.tiles - 1) / a.tiles;
+    const long long step = (long long)sq.n * a.rep;
+    float M = -INFINITY, L = 0.f;
+    f32x4_t o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int p = 0; p < parts; ++p) {
+        const size_t at = (size_t)(a.base[i] + p * step + row) * a.n_kv + kvh;
+        const f32x2_t ml = *reinterpret_cast<const f32x2_t*>(a.part_ml + at * 2);
+        const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part_o + at * D + 4 * c);
+        const float m_new = fmaxf(M, ml[0]);
+        const float w0 = M == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(M - m_new);
+        const float w1 = ml[0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[0] - m_new);
+        o = o * w0 + x * w1;
+        L = L * w0 + ml[1] * w1;
+        M = m_new;
+    }
+    put4(static_cast<T*>(a.out) + ((size_t)token * a.n_q + head) * D + 4 * c, o * (1.0f / L));
+}
+
+// ---------------------------------------------------------------- launch
+
+// Query rows of a sequence and KV head from which blocks are taken.
+constexpr int kBlockRows = 65;
+constexpr int kMaxRounds = 4;    // of workgroups that a launch's tiles are cut into
+constexpr int kPartTiles = 3;    // what a workgroup costs besides its tiles
+
+template <int D, int W, bool FP8>
+sa_status launch_bf16(const BlockArgs& a, hipStream_t st) {
+    constexpr int lds = 2 * BfGeo<D>::STAGE;
+    constexpr auto kernel = extend_bf16_kernel<D, W, FP8>;
+    SA_TRY(pf::opt_in_lds<kernel>(lds));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)a.start[a.n_seq] * a.n_kv), dim3(W * kWave), lds, st, a);
+    SA_CHECK_LAUNCH();
+    return SA_OK;
+}
+template <int D>
+sa_status dispatch_blocks(const BlockArgs& a, bool fp8, hipStream_t st) {
+    if (fp8) return a.rows == 256 ? launch_bf16<D, 8, true>(a, st) : launch_bf16<D, 4, true>(a, st);
+    return a.rows == 256 ? launch_bf16<D, 8, false>(a, st) : launch_bf16<D, 4, false>(a, st);
+}
+
+long long blocks_of(long long rows, int block) { return (rows + block - 1) / block; }
+
+}  // namespace
+
+bool extend_is_block(sa_dtype kv, bool q16, int rep, int n) {
+    return q16 && kv != SA_DTYPE_F32 && (long long)n * rep >= kBlockRows;
+}
+
+size_t extend_blocks_ws(int n, const int32_t* counts, int n_q, int n_kv, int d, long long max_tokens) {
+    const long long tiles = (max_tokens + kBfTile - 1) / kBfTile;
+    if (tiles <= 1) return 0;
+    const long long round = device_cu_count();
+    size_t need = 0;
+    for (int i0 = 0; i0 < n; i0 += kRowsPerLaunch) {
+        long long rows = 0;
+        for (int i = i0; i < std::min(n, i0 + kRowsPerLaunch); ++i) rows += (long long)counts[i] * n_q;
+        // at most as many workgroups of 256 rows as extend_blocks cuts into
+        need = std::max(need, (size_t)std::min(rows * tiles, kMaxRounds * round * 256) * (d + 2) * sizeof(float));
+    }
+    return need;
+}
+
+sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, const ChunkSeq* seqs, int n, float scale,
+                        void* out, void* ws, size_t ws_bytes, hipStream_t st) {
+    BlockArgs a{};
+    a.q = q; a.out = out;
+    a.k = c.k_pool; a.v = c.v_pool; a.k_scale = c.k_scale; a.v_scale = c.v_scale; a.table = c.block_table;
+    a.n_kv = c.n_kv; a.n_q = n_q; a.rep = n_q / c.n_kv;
+    a.max_pages = c.max_pages; a.num_pages = c.num_pages;
+    a.factor = scale * pf::kLog2eP;
+    a.sl2 = std::fabs(a.factor);
+    a.q_sign = scale < 0 ? 0x80008000u : 0u;
+    for (int i0 = 0; i0 < n; i0 += kRowsPerLaunch) {
+        a.n_seq = std::min(kRowsPerLaunch, n - i0);
+        long long most = 0;
+        for (int i = 0; i < a.n_seq; ++i) {
+            a.seq[i] = seqs[i0 + i];
+            most = std::max(most, (long long)a.seq[i].n * a.rep);
+        }
+        a.rows = most > 128 ? 256 : 128;
+        int longest = 1;
+        for (int i = 0; i < a.n_seq; ++i)
+            longest = std::max(longest, block_key_tiles(a.seq[i], (int)blocks_of((long long)a.seq[i].n * a.rep, a.rows) - 1,
+                                                        a.rows, a.rep));
+        auto parts_of = [&](int i, int tiles) {
+            const int last = (int)blocks_of((long long)a.seq[i].n * a.rep, a.rows) - 1;
+            return (block_key_tiles(a.seq[i], last, a.rows, a.rep) + tiles - 1) / tiles;
+        };
+        auto workgroups = [&](int tiles) {
+            long long k = 0;
+            for (int i = 0; i < a.n_seq; ++i) k += blocks_of((long long)a.seq[i].n * a.rep, a.rows) * parts_of(i, tiles);
+            return k * a.n_kv;
+        };
+        // For 1 .. kMaxRounds rounds of a workgroup per CU (two of four waves): the fewest
+        // tiles per workgroup that give no more of them; the cheapest of these.
+        const long long round = (a.rows == 256 ? 1LL : 2LL) * device_cu_count();
+        a.tiles = longest;
+        long long best = ((workgroups(longest) + round - 1) / round) * (longest + kPartTiles);
+        for (int k = 1; k <= kMaxRounds; ++k) {
+            if (workgroups(longest) > k * round) continue;
+            int lo = 1, hi = longest;   // workgroups(tiles) falls
+            while (lo < hi) {
+                const int mid = (lo + hi) / 2;
+                if (workgroups(mid) <= k * round) hi = mid;
+                else lo = mid + 1;
+            }
+            const long long cost = (long long)k * (lo + kPartTiles);
+            if (cost < best) best = cost, a.tiles = lo;
+        }
+        long long at = 0, parts = 0;
+        for (int i = 0; i < a.n_seq; ++i) {
+            a.parts[i] = parts_of(i, a.tiles);
+            a.start[i] = (int)at;
+            a.base[i] = (int)parts;
+            at += blocks_of((long long)a.seq[i].n * a.rep, a.rows) * a.parts[i];
+            if (a.parts[i] > 1) parts += (long long)a.parts[i] * a.seq[i].n * a.rep;
+        }
+        a.start[a.n_seq] = (int)at;
+        const long long tokens = a.seq[a.n_seq - 1].first + a.seq[a.n_seq - 1].n - a.seq[0].first;
+        // a grid has fewer than 2^32 threads
+        if (at * a.n_kv >= (1LL << 32) / (a.rows * 2) || parts > 0x7fffffffLL || tokens * n_q >= (1LL << 32) / 64)
+            return fail(SA_EINVAL, "too many tokens for one call");
+        if (parts) {
+            const size_t need = (size_t)parts * a.n_kv * (c.d + 2) * sizeof(float);
+            if (!ws || ws_bytes < need) return fail(SA_ENOMEM, "workspace too small for the partials");
+            a.part_o = static_cast<float*>(ws);
+            a.part_ml = a.part_o + (size_t)parts * a.n_kv * c.d;
+        }
+        const bool fp8 = c.kv == SA_DTYPE_FP8;
+        SA_TRY(c.d == 64 ? dispatch_blocks<64>(a, fp8, st) : dispatch_blocks<128>(a, fp8, st));
+        if (parts) {
+            const long long n_rows = tokens * n_q;
+            const int per = 256 / (c.d / 4);
+            const dim3 grid((unsigned)((n_rows + per - 1) / per));
+            if (c.d == 64) hipLaunchKernelGGL((block_merge_kernel<64, uint16_t>), grid, dim3(256), 0, st, a, n_rows);
+            else hipLaunchKernelGGL((block_merge_kernel<128, uint16_t>), grid, dim3(256), 0, st, a, n_rows);
+            SA_CHECK_LAUNCH();
+        }
+    }
+    return SA_OK;
+}
+
+}  // namespace sa

@@ -1186,8 +1186,11 @@ extern "C" size_t sa_paged_extend_ws_bytes(const sa_kvcache* c, int n_seq, const
         return 0;
     for (int i = 0; i < n_seq; ++i)
         if (counts[i] < 0) return 0;
-    return extend_rows_ws(n_seq, counts, n_q_heads, c->desc.num_kv_heads, c->desc.head_dim,
-                          c->desc.kv_dtype == SA_DTYPE_F32, (long long)c->desc.max_pages_per_seq * SA_PAGE_TOKENS);
+    const long long tokens = (long long)c->desc.max_pages_per_seq * SA_PAGE_TOKENS;
+    const bool f32 = c->desc.kv_dtype == SA_DTYPE_F32;
+    // whichever way the sequences go
+    return std::max(extend_rows_ws(n_seq, counts, n_q_heads, c->desc.num_kv_heads, c->desc.head_dim, f32, tokens),
+                    extend_blocks_ws(n_seq, counts, n_q_heads, c->desc.num_kv_heads, c->desc.head_dim, tokens));
 }
 
 extern "C" sa_status sa_paged_extend(const sa_kvcache* c, int layer, const void* q, sa_dtype q_dtype, int n_seq,
@@ -1206,8 +1209,13 @@ extern "C" sa_status sa_paged_extend(const sa_kvcache* c, int layer, const void*
         if (n_seq > 0 && std::all_of(counts, counts + n_seq, [](int32_t k) { return k == 0; })) return SA_OK;
         SA_TRY(check_ranges(c, layer, q, n_seq, n_q_heads, out, ws, ws_bytes,
                             sa_paged_extend_ws_bytes(c, n_seq, counts, n_q_heads)));
-        std::vector<ChunkSeq> seqs;
-        seqs.reserve(n_seq);
+        // Sequences of few and of many query rows go their own ways, one behind the
+        // other, in the same workspace.
+        const PagedView view = view_of(c, layer);
+        const bool q16 = q_dtype == SA_DTYPE_BF16;
+        std::vector<ChunkSeq> few, many;
+        few.reserve(n_seq);
+        many.reserve(n_seq);
         long long rows = 0;
         for (int i = 0; i < n_seq; ++i) {
             const int row = seq_ids ? seq_ids[i] : i, len = c->pt.len(row);
@@ -1215,11 +1223,17 @@ extern "C" sa_status sa_paged_extend(const sa_kvcache* c, int layer, const void*
             if (rows + counts[i] > kMaxNewTokens) return fail(SA_EINVAL, "more than 2^20 new tokens");
             if ((long long)len + counts[i] > c->pt.capacity(row))
                 return fail(SA_ERANGE, "Requested seq_len exceeds cached length");
-            if (counts[i]) seqs.push_back(ChunkSeq{row, len, counts[i], (int)rows});
+            if (counts[i])
+                (extend_is_block(view.kv, q16, n_q_heads / view.n_kv, counts[i]) ? many : few)
+                    .push_back(ChunkSeq{row, len, counts[i], (int)rows});
             rows += counts[i];
         }
-        return extend_rows(view_of(c, layer), q, q_dtype == SA_DTYPE_BF16, n_q_heads, seqs.data(), (int)seqs.size(),
-                           scale, out, ws, ws_bytes, as_stream(stream));
+        if (!many.empty())
+            SA_TRY(extend_blocks(view, q, q16, n_q_heads, many.data(), (int)many.size(), scale, out, ws, ws_bytes,
+                                 as_stream(stream)));
+        if (few.empty()) return SA_OK;
+        return extend_rows(view, q, q16, n_q_heads, few.data(), (int)few.size(), scale, out, ws, ws_bytes,
+                           as_stream(stream));
     });
 }
 

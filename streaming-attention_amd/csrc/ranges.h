@@ -46,4 +46,11 @@ size_t extend_rows_ws(int n, const int32_t* counts, int n_q, int n_kv, int d, bo
 sa_status extend_rows(const PagedView& c, const void* q, bool q16, int n_q, const ChunkSeq* seqs, int n, float scale,
                       void* out, void* ws, size_t ws_bytes, hipStream_t st);
 
+// The same for chunks of many query rows (extend.hip): whether a chunk of n tokens
+// takes it, and its workspace and launch for chunks that all do.
+bool extend_is_block(sa_dtype kv, bool q16, int rep, int n);
+size_t extend_blocks_ws(int n, const int32_t* counts, int n_q, int n_kv, int d, long long max_tokens);
+sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, const ChunkSeq* seqs, int n, float scale,
+                        void* out, void* ws, size_t ws_bytes, hipStream_t st);
+
 }  // namespace sa

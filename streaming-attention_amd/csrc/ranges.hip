@@ -1033,9 +1033,9 @@ __global__ void __launch_bounds__(D / 4) chunk_merge_kernel(ChunkArgs a) {
     const int head = blockIdx.x % a.n_q, row = a.seq[0].first + blockIdx.x / a.n_q;
     int i = a.n_seq - 1;
     while (a.seq[i].first > row) --i;
-    if (a.chunks[i] == 1) return;
     const ChunkSeq sq = a.seq[i];
     const int t = row - sq.first;
+    if (a.chunks[i] == 1 || t >= sq.n) return;   // written already, or a row of another launch
     const int n = (block_tiles(sq, t / a.block, a.block) + a.tiles - 1) / a.tiles;
     const int kvh = head / a.rep, c = threadIdx.x;
     float M = -INFINITY, L = 0.f;
