@@ -431,8 +431,8 @@ size_t extend_blocks_ws(int n, const int32_t* counts, int n_q, int n_kv, int d, 
     for (int i0 = 0; i0 < n; i0 += kRowsPerLaunch) {
         long long rows = 0;
         for (int i = i0; i < std::min(n, i0 + kRowsPerLaunch); ++i) rows += (long long)counts[i] * n_q;
-        // at most as many workgroups of 256 rows as extend_blocks cuts into
-        need = std::max(need, (size_t)std::min(rows * tiles, kMaxRounds * round * 256) * (d + 2) * sizeof(float));
+        // at most as many workgroups as extend_blocks cuts into
+        need = std::max(need, (size_t)std::min(rows * tiles, kMaxRounds * round * (d == 64 ? 512 : 256)) * (d + 2) * sizeof(float));
     }
     return need;
 }
@@ -470,7 +470,7 @@ sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, co
         };
         // For 1 .. kMaxRounds rounds of a workgroup per CU (two of four waves): the fewest
         // tiles per workgroup that give no more of them; the cheapest of these.
-        const long long round = (a.rows == 256 ? 1LL : 2LL) * device_cu_count();
+        const long long round = (a.rows == 256 && c.d == 128 ? 1LL : 2LL) * device_cu_count();
         a.tiles = longest;
         long long best = ((workgroups(longest) + round - 1) / round) * (longest + kPartTiles);
         for (int k = 1; k <= kMaxRounds; ++k) {

@@ -10,34 +10,39 @@
 // whose token also follows.
 //
 // A sum of probabilities decides which token is drawn, and tokens of a large
-// vocabulary lie as close as 1e-6: sums and exponentials are in 64 bits (fp64 runs
+// vocabulary lie as close as 1e-6: sums and exponentials are in 64 bits (fp64 FMA runs
 // at fp32's rate here), off by some 1e-13.
 //
-// Launches: (1) every row is cut into segments of 1024 logits, a wave each, which
+// Launches: (1) every row is cut into segments of 4096 logits, a workgroup each, which
 // leave their largest logit and sum of exponentials relative to it; (2) with draft
-// logits, the rejected places' sums of w per segment; (3) a workgroup per sequence
-// finds the segment that the uniform number falls into, then the token.  (2) and
-// (3) decide what is accepted, from the segments of the sequence's rows.
+// logits, what is accepted, and the rejected places' sums of w per segment; (3) a
+// workgroup per sequence finds the segment that the uniform number falls into, then
+// the token (without (2), after deciding what is accepted).
 //
-// Bound: HBM for the first launch, latency for the others.
+// Bound: HBM and fp64 arithmetic alike for the first launch, latency for the others.
 #include "sa_internal.h"
 
 #include <algorithm>
 #include <cmath>
 #include <initializer_list>
 #include <new>
+#include <type_traits>
 
 namespace sa {
 namespace {
 
-constexpr int kSeg = 1024;          // logits of a segment
-constexpr int kPer = kSeg / kWave;  // of a lane
-constexpr int kMaxDraft = 64;       // drafted tokens of a sequence (a lane each)
 constexpr int kThreads = 256, kWaves = kThreads / kWave;
+constexpr int kQuads = 2;                        // 16-byte pieces of a lane in a step
+constexpr int kStep = 4 * kQuads * kWave;        // logits that a wave takes at once
+constexpr int kSteps = 4;                        // of a segment
+constexpr int kSeg = kSteps * kStep;             // logits of a segment
+constexpr int kDraw = 512;                       // threads that look for a token, four logits each
+static_assert(kSeg == 4 * kDraw, "a piece per thread");
+constexpr int kMaxDraft = 64;                    // drafted tokens of a sequence (a lane each)
 
 struct Segment {
     double sum;     // of exp((x - top) / T)
-    float top;      // the largest logit, -inf if there is none
+    float top;      // a logit that no other exceeds by far (T = 0: the largest); -inf if there is none
     int32_t at;     // T = 0: its token
 };
 
@@ -53,6 +58,7 @@ struct VerifyArgs {
     long long target_stride, draft_stride;
     Segment* seg;             // [target rows, then draft rows][n_seg]
     double* rest;             // [sequences of the launch][n_seg]: sums of w
+    struct Decision* decided; // [sequences of the launch], with draft logits
     int32_t* out_accepted;    // [sequences]
     int32_t* out_tokens;      // [sequences][out_stride]
     int n_target, n_draft;    // rows
@@ -64,29 +70,48 @@ struct VerifyArgs {
 };
 static_assert(sizeof(VerifyArgs) <= 4096, "kernel arguments");
 
-// 2^t for t <= 0: 2^f by the series of exp(f ln 2), |f| <= 1/2, whose term of degree 11
-// is below 2.2e-13.
-__device__ __forceinline__ double exp2_64(double t) {
-    t = t < -1100.0 ? -1100.0 : t;   // NaN stays
-    const double n = __builtin_rint(t);
-    const double z = (t - n) * 0.69314718055994530942;
-    double s = 1.0 / 3628800.0;
-    s = fma(s, z, 1.0 / 362880.0);
-    s = fma(s, z, 1.0 / 40320.0);
-    s = fma(s, z, 1.0 / 5040.0);
-    s = fma(s, z, 1.0 / 720.0);
-    s = fma(s, z, 1.0 / 120.0);
-    s = fma(s, z, 1.0 / 24.0);
-    s = fma(s, z, 1.0 / 6.0);
-    s = fma(s, z, 0.5);
-    s = fma(s, z, 1.0);
-    s = fma(s, z, 1.0);
-    return __builtin_ldexp(s, (int)n);
+// 2^f, |f| <= 1/2, within 3.7e-14 of it: 1 + f times the polynomial of degree 8 that
+// equals (2^f - 1) / f at the nine Chebyshev nodes of the interval.
+__device__ __forceinline__ double exp2_half(double f) {
+    double s = 1.0203121294865924e-07;
+    s = fma(s, f, 1.3255224885529674e-06);
+    s = fma(s, f, 1.525268684524423e-05);
+    s = fma(s, f, 1.540345585242065e-04);
+    s = fma(s, f, 1.3333558179044404e-03);
+    s = fma(s, f, 9.618129159402609e-03);
+    s = fma(s, f, 5.550410866476042e-02);
+    s = fma(s, f, 0.2402265069581299);
+    s = fma(s, f, 0.6931471805599453);
+    return fma(s, f, 1.0);
 }
-// exp((x - top) / T); 0 where there is no largest logit.
+// exp((x - top) / T); 0 for a logit of -inf, NaN for one of NaN.
 __device__ __forceinline__ double weight(float x, float top, double factor) {
-    return exp2_64(((double)x - (double)top) * factor);
+    double t = ((double)x - (double)top) * factor;
+    t = t < -1100.0 ? -1100.0 : t;   // 2^-1100 is 0; t is below 1000
+    const double n = __builtin_rint(t);
+    return __builtin_ldexp(exp2_half(t - n), (int)n);
 }
+// The same for sums, in fewer instructions: logits of 2^-1000 of the reference's weight
+// and less, and NaN, count as much.  The argument is a single FMA, off by 2^-53 of
+// ref / T log2(e), so that has to be small (fine).
+constexpr double kFineRef = 1024.0;
+struct SumWeight {
+    double factor, shift;
+    float least;
+    bool fine;
+    __device__ __forceinline__ SumWeight(float ref, double f) : factor(f), shift(-(double)ref * f) {
+        least = (float)((double)ref - 1000.0 / f);
+        fine = fabs(shift) <= kFineRef && least > -3e38f;
+    }
+    __device__ __forceinline__ double operator()(float x) const {
+        constexpr double kRound = 6755399441055744.0;   // 1.5 2^52: a sum's low word is t rounded
+        const double t = fma((double)fmaxf(x, least), factor, shift);
+        const double r = t + kRound;
+        const double s = exp2_half(t - (r - kRound));
+        return __hiloint2double(__double2hiint(s) + (__double2loint(r) << 20), __double2loint(s));
+    }
+};
+constexpr double kNothingLeft = 1e-280;   // sums of weights that are all about 2^-1000 or 0 stay below it
 
 template <int CTRL>
 __device__ __forceinline__ double dpp_f64(double v) {
@@ -116,8 +141,19 @@ struct Row {
     // The four tokens from first() on; places outside the row are none.
     __device__ __forceinline__ long long first(int s, int quad) const { return (long long)kSeg * s + 4 * quad - off; }
     __device__ __forceinline__ void load(int s, int quad, float none, float (&v)[4]) const {
-        const long long i = first(s, quad);
-        if (i >= 0 && i + 4 <= vocab) {
+        load_at(first(s, quad), none, v);
+    }
+    // Whether segment s lies inside the row, and its pieces then.
+    __device__ __forceinline__ bool inside(int s) const {
+        return (s > 0 || off == 0) && (long long)kSeg * (s + 1) - off <= vocab;
+    }
+    __device__ __forceinline__ void load_inside(int s, int quad, float (&v)[4]) const {
+        const float4 f = *reinterpret_cast<const float4*>(x + first(s, quad));
+        v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+    }
+    // Tokens i .. i + 3, wherever another row's pieces start.
+    __device__ __forceinline__ void load_at(long long i, float none, float (&v)[4]) const {
+        if (i >= 0 && i + 4 <= vocab && (i + off) % 4 == 0) {
             const float4 f = *reinterpret_cast<const float4*>(x + i);
             v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
         } else {
@@ -130,51 +166,143 @@ struct Row {
 __device__ __forceinline__ const float* target_row(const VerifyArgs& a, long long r) { return a.target + r * a.target_stride; }
 __device__ __forceinline__ const float* draft_row(const VerifyArgs& a, long long r) { return a.draft + r * a.draft_stride; }
 
-// A wave per segment of a row.
-template <bool GREEDY>
-__global__ void __launch_bounds__(kThreads) verify_segments_kernel(VerifyArgs a) {
-    const int wgs = (a.n_seg + kWaves - 1) / kWaves;
-    const int row = blockIdx.x / wgs, s = blockIdx.x % wgs * kWaves + threadIdx.x / kWave;
-    const int lane = threadIdx.x & (kWave - 1);
-    if (s >= a.n_seg) return;
-    const Row r(row < a.n_target ? target_row(a, row) : draft_row(a, row - a.n_target), a.vocab);
-    float v[kPer / 4][4];
+// A part's sum relative to the largest logit of the whole.
+__device__ __forceinline__ double joined(const Segment& g, float top, double factor) {
+    return g.top == -INFINITY ? g.sum : g.sum * weight(g.top, top, factor);   // 0 or NaN without a largest logit
+}
+
+// Sums of exponentials of a wave's logits, a step at a time, relative to one of the
+// first step's logits: 64 bits hold what exceeds it by 2^kFar, and only then is
+// another one taken.
+constexpr double kFar = 600.0;
+struct WaveSum {
+    double sum = 0.0;
+    float ref = -INFINITY, top = -INFINITY;   // top: this lane's largest
+    bool lost = false;                        // a NaN or +inf
+    __device__ __forceinline__ void add(const float (&v)[kQuads][4], double factor) {
+        float m = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < kPer / 4; ++j) r.load(s, j * kWave + lane, -INFINITY, v[j]);
-    float top = -INFINITY;
-    int at = 0x7fffffff;
+        for (int j = 0; j < kQuads; ++j)
 #pragma unroll
-    for (int j = 0; j < kPer / 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if constexpr (GREEDY) {
-                const int t = (int)(r.first(s, j * kWave + lane)) + e;
-                if (v[j][e] > top) top = v[j][e], at = t;   // tokens ascend
-            } else {
-                top = fmaxf(top, v[j][e]);
+            for (int e = 0; e < 4; ++e) {
+                m = fmaxf(m, v[j][e]);
+                lost = lost || !(v[j][e] < INFINITY);
+            }
+        top = fmaxf(top, m);
+        if (ref == -INFINITY || __any(((double)m - (double)ref) * factor > kFar)) {
+            const float now = group_reduce<OpMax, 1, kWave>(top);
+            if (now < INFINITY) {
+                if (ref != -INFINITY) sum *= weight(ref, now, factor);
+                ref = now;
             }
         }
-    Segment out;
-    if constexpr (GREEDY) {
+        if (ref == -INFINITY) return;
+        const SumWeight w(ref, factor);
+        if (w.fine) {
+#pragma unroll
+            for (int j = 0; j < kQuads; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum += w(v[j][e]);
+        } else {
+            for (int j = 0; j < kQuads; ++j)
+                for (int e = 0; e < 4; ++e) sum += weight(v[j][e], ref, factor);
+        }
+    }
+    __device__ __forceinline__ Segment done() {
+        Segment g{wave_sum(sum), ref, 0};
+        if (__any(lost)) g.sum = NAN;
+        return g;
+    }
+};
+struct WaveTop {
+    float top = -INFINITY;
+    int at = 0x7fffffff;
+    __device__ __forceinline__ void add(const float (&v)[kQuads][4], const int (&t)[kQuads]) {
+#pragma unroll
+        for (int j = 0; j < kQuads; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (v[j][e] > top) top = v[j][e], at = t[j] + e;   // tokens ascend
+    }
+    __device__ __forceinline__ Segment done() {
 #pragma unroll
         for (int mask = 1; mask < kWave; mask *= 2) {
             const float ot = __shfl_xor(top, mask, kWave);
             const int oi = __shfl_xor(at, mask, kWave);
             if (better(ot, oi, top, at)) top = ot, at = oi;
         }
-        out = Segment{0.0, top, at};
-    } else {
-        top = group_reduce<OpMax, 1, kWave>(top);
-        double sum = 0.0;
-#pragma unroll
-        for (int j = 0; j < kPer / 4; ++j)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                // without a largest logit there are -inf, which add 0, and NaN, which stay
-                sum += weight(v[j][e], top == -INFINITY ? 0.f : top, a.factor);
-        out = Segment{wave_sum(sum), top, 0};
+        return Segment{0.0, top, at};
     }
-    if (lane == 0) a.seg[(long long)row * a.n_seg + s] = out;
+};
+
+// A wave per segment of a row, or (SPLIT) a workgroup, a step per wave: few rows.
+template <bool GREEDY, bool SPLIT>
+__global__ void __launch_bounds__(kThreads) verify_segments_kernel(VerifyArgs a) {
+    __shared__ Segment part[kWaves];
+    const int lane = threadIdx.x & (kWave - 1), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const long long item = SPLIT ? (long long)blockIdx.x : (long long)blockIdx.x * kWaves + wave;
+    const int row = (int)(item / a.n_seg), s = (int)(item % a.n_seg);
+    if (row >= a.n_target + a.n_draft) return;
+    const Row r(row < a.n_target ? target_row(a, row) : draft_row(a, row - a.n_target), a.vocab);
+    std::conditional_t<GREEDY, WaveTop, WaveSum> w;
+    auto load = [&](int k, float (&v)[kQuads][4]) {
+#pragma unroll
+        for (int j = 0; j < kQuads; ++j) r.load(s, (k * kQuads + j) * kWave + lane, -INFINITY, v[j]);
+    };
+    auto load_inside = [&](int k, float (&v)[kQuads][4]) {
+#pragma unroll
+        for (int j = 0; j < kQuads; ++j) r.load_inside(s, (k * kQuads + j) * kWave + lane, v[j]);
+    };
+    auto add = [&](int k, const float (&v)[kQuads][4]) {
+        if constexpr (GREEDY) {
+            int t[kQuads];
+#pragma unroll
+            for (int j = 0; j < kQuads; ++j) t[j] = (int)r.first(s, (k * kQuads + j) * kWave + lane);
+            w.add(v, t);
+        } else {
+            w.add(v, a.factor);
+        }
+    };
+    float v[2][kQuads][4];
+    if constexpr (SPLIT) {
+        load(wave, v[0]);
+        add(wave, v[0]);
+    } else if (r.inside(s)) {
+        load_inside(0, v[0]);
+        for (int k = 0; k < kSteps; k += 2) {   // the next step's loads in flight under a step's sums
+            load_inside(k + 1, v[1]);
+            add(k, v[0]);
+            if (k + 2 < kSteps) load_inside(k + 2, v[0]);
+            add(k + 1, v[1]);
+        }
+    } else {
+        for (int k = 0; k < kSteps; ++k) {
+            load(k, v[0]);
+            add(k, v[0]);
+        }
+    }
+    Segment out = w.done();
+    if constexpr (SPLIT) {
+        if (lane == 0) part[wave] = out;
+        __syncthreads();
+        if (wave) return;
+        out = part[lane & 3];
+        if constexpr (GREEDY) {
+#pragma unroll
+            for (int mask = 1; mask < kWaves; mask *= 2) {
+                const float ot = __shfl_xor(out.top, mask, kWave);
+                const int oi = __shfl_xor(out.at, mask, kWave);
+                if (better(ot, oi, out.top, out.at)) out.top = ot, out.at = oi;
+            }
+        } else {
+            const float top = group_reduce<OpMax, 1, kWaves>(out.top);
+            double sum = joined(out, top, a.factor);
+            sum += dpp_f64<kDppXor1>(sum);
+            sum += dpp_f64<kDppXor2>(sum);
+            out = Segment{sum, top, 0};
+        }
+    }
+    if (lane == 0) a.seg[item] = out;
 }
 
 // A row's largest logit and its sum of exponentials relative to it; a row whose sum
@@ -184,65 +312,84 @@ struct Norm {
     float top;
     __device__ __forceinline__ bool ok() const { return sum > 0.0 && sum < INFINITY; }
 };
-__device__ __forceinline__ Norm row_norm(const VerifyArgs& a, long long row) {
+// Lanes' segments of a row, loaded ahead of their use; rows of more segments than
+// lanes are read again.
+__device__ __forceinline__ Segment load_segment(const VerifyArgs& a, long long row) {
+    const int lane = threadIdx.x & (kWave - 1);
+    return lane < a.n_seg ? a.seg[row * a.n_seg + lane] : Segment{0.0, -INFINITY, 0};
+}
+__device__ __forceinline__ Norm row_norm(const VerifyArgs& a, long long row, const Segment& mine) {
     const int lane = threadIdx.x & (kWave - 1);
     const Segment* seg = a.seg + row * a.n_seg;
-    float top = -INFINITY;
-    for (int s = lane; s < a.n_seg; s += kWave) top = fmaxf(top, seg[s].top);
+    float top = mine.top;
+    for (int s = lane + kWave; s < a.n_seg; s += kWave) top = fmaxf(top, seg[s].top);
     top = group_reduce<OpMax, 1, kWave>(top);
-    double sum = 0.0;
-    for (int s = lane; s < a.n_seg; s += kWave) {
-        const Segment g = seg[s];
-        // a segment of NaN and -inf alone: its sum is 0 or NaN
-        sum += g.top == -INFINITY ? g.sum : g.sum * weight(g.top, top, a.factor);
-    }
+    double sum = joined(mine, top, a.factor);
+    for (int s = lane + kWave; s < a.n_seg; s += kWave) sum += joined(seg[s], top, a.factor);
     return Norm{wave_sum(sum), top};
 }
 
-struct Shared {
-    Norm p[kMaxDraft + 1], q[kMaxDraft];
-};
 // What a sequence's uniform numbers decide.
 struct Decision {
+    Norm p, q;            // of the place that the next token comes from
+    long long row, drow;  // of the target, of the draft
     int accepted;
     Source source;
-    Norm p, q;            // of the place that the next token comes from
     int token;            // kRestOfOne: the rejected token
-    long long row, drow;  // of the target, of the draft
+};
+struct Shared {
+    Norm p[kMaxDraft + 1], q[kMaxDraft];
+    int accepted;
 };
 
 // The same for every thread of the workgroup.
-__device__ __forceinline__ Decision decide(const VerifyArgs& a, int i, Shared& sh, int* box) {
+template <int WAVES>
+__device__ __forceinline__ Decision decide(const VerifyArgs& a, int i, Shared& sh) {
     const int first = a.first[i], n = a.first[i + 1] - first;
     const long long row0 = (long long)first + a.seq0 + i;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x & (kWave - 1);
     const int rows = n + 1 + (a.draft ? n : 0);
-    for (int r = wave; r < rows; r += kWaves) {
-        const Norm m = row_norm(a, r <= n ? row0 + r : (long long)a.n_target + first + r - n - 1);
-        if (lane == 0) (r <= n ? sh.p[r] : sh.q[r - n - 1]) = m;
+    auto row_of = [&](int r) { return r <= n ? row0 + r : (long long)a.n_target + first + r - n - 1; };
+    // The drafted tokens' logits, beside the rows' segments.
+    int x = -1;
+    float u = 0.f, tx = 0.f, dx = 0.f;
+    bool drafted = false;
+    if (wave == 0 && lane < n) {
+        x = a.tokens[first + lane];
+        u = a.u_accept[first + lane];
+        drafted = x >= 0 && x < a.vocab;
+        if (drafted) {
+            tx = target_row(a, row0 + lane)[x];
+            if (a.draft) dx = draft_row(a, first + lane)[x];
+        }
+    }
+    constexpr int kAhead = 3;
+    for (int r0 = wave; r0 < rows; r0 += kAhead * WAVES) {
+        Segment g[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) g[k] = load_segment(a, row_of(min(r0 + k * WAVES, rows - 1)));
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            const int r = r0 + k * WAVES;
+            if (r >= rows) break;
+            const Norm m = row_norm(a, row_of(r), g[k]);
+            if (lane == 0) (r <= n ? sh.p[r] : sh.q[r - n - 1]) = m;
+        }
     }
     __syncthreads();
     if (wave == 0) {
         bool ok = false;
-        if (lane < n) {
-            const int x = a.tokens[first + lane];
-            const Norm p = sh.p[lane];
-            if (x >= 0 && x < a.vocab && p.ok()) {
-                const double px = weight(target_row(a, row0 + lane)[x], p.top, a.factor) / p.sum;
-                double qx = 1.0;
-                if (a.draft) {
-                    const Norm q = sh.q[lane];
-                    qx = q.ok() ? weight(draft_row(a, first + lane)[x], q.top, a.factor) / q.sum : NAN;
-                }
-                ok = (double)a.u_accept[first + lane] * qx < px;
-            }
+        if (drafted && sh.p[lane].ok()) {
+            double qx = 1.0;
+            if (a.draft) qx = sh.q[lane].ok() ? weight(dx, sh.q[lane].top, a.factor) / sh.q[lane].sum : NAN;
+            ok = (double)u * qx < weight(tx, sh.p[lane].top, a.factor) / sh.p[lane].sum;
         }
         const int accepted = __ffsll((long long)~__ballot(ok)) - 1;
-        if (lane == 0) *box = accepted < 0 ? kMaxDraft : accepted;
+        if (lane == 0) sh.accepted = accepted < 0 ? kMaxDraft : accepted;
     }
     __syncthreads();
     Decision d;
-    d.accepted = *box;
+    d.accepted = sh.accepted;
     d.p = sh.p[d.accepted];
     d.row = row0 + d.accepted;
     d.drow = first + d.accepted;
@@ -280,10 +427,10 @@ struct Weigher {
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] = weight(x[e], d.p.top, a.factor) * pi;
         if (d.source == kRest) {
-            // the draft's row may start at another distance from its boundary
+            float y[4];
+            q.load_at(t, -INFINITY, y);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (t + e >= 0 && t + e < a.vocab) w[e] = fmax(0.0, w[e] - weight(q.x[t + e], d.q.top, a.factor) * qi);
+            for (int e = 0; e < 4; ++e) w[e] = fmax(0.0, w[e] - weight(y[e], d.q.top, a.factor) * qi);
         } else if (d.source == kRestOfOne) {
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -292,31 +439,53 @@ struct Weigher {
     }
 };
 
-// Sums of w per segment at the sequences' rejected places.
-__global__ void __launch_bounds__(kThreads) verify_rest_kernel(VerifyArgs a) {
+// What is accepted: a workgroup per sequence.
+__global__ void __launch_bounds__(kDraw) verify_decide_kernel(VerifyArgs a) {
     __shared__ Shared sh;
-    __shared__ int box;
+    const Decision d = decide<kDraw / kWave>(a, blockIdx.x, sh);
+    if (threadIdx.x == 0) a.decided[blockIdx.x] = d;
+}
+
+// The sums of w per segment at the rejected places.
+__global__ void __launch_bounds__(kThreads) verify_rest_kernel(VerifyArgs a) {
+    __shared__ double part[kWaves];
     const int i = blockIdx.x / a.groups, g = blockIdx.x % a.groups;
-    if (a.first[i + 1] == a.first[i]) return;
-    const Decision d = decide(a, i, sh, &box);
+    const Decision d = a.decided[i];
     if (d.source != kRest) return;
-    const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
-    const Weigher w(a, d);
-    for (int s = g * kWaves + wave; s < a.n_seg; s += a.groups * kWaves) {
-        double sum = 0.0;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = threadIdx.x & (kWave - 1);
+    const Row p(target_row(a, d.row), a.vocab), q(draft_row(a, d.drow), a.vocab);
+    const double pi = 1.0 / d.p.sum, qi = 1.0 / d.q.sum;
+    const SumWeight pw(d.p.top, a.factor), qw(d.q.top, a.factor);
+    for (int s = g; s < a.n_seg; s += a.groups) {
+        float x[kQuads][4], y[kQuads][4];
 #pragma unroll
-        for (int j = 0; j < kPer / 4; ++j) {
-            double v[4];
-            w(s, j * kWave + lane, v);
-            sum += (v[0] + v[1]) + (v[2] + v[3]);
+        for (int j = 0; j < kQuads; ++j) {
+            const int quad = (wave * kQuads + j) * kWave + lane;
+            p.load(s, quad, -INFINITY, x[j]);
+            q.load_at(p.first(s, quad), -INFINITY, y[j]);
+        }
+        double sum = 0.0;
+        if (pw.fine && qw.fine) {
+#pragma unroll
+            for (int j = 0; j < kQuads; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum += fmax(0.0, pw(x[j][e]) * pi - qw(y[j][e]) * qi);
+        } else {
+            for (int j = 0; j < kQuads; ++j)
+                for (int e = 0; e < 4; ++e)
+                    sum += fmax(0.0, weight(x[j][e], d.p.top, a.factor) * pi - weight(y[j][e], d.q.top, a.factor) * qi);
         }
         sum = wave_sum(sum);
-        if (lane == 0) a.rest[(long long)i * a.n_seg + s] = sum;
+        __syncthreads();
+        if (lane == 0) part[wave] = sum;
+        __syncthreads();
+        if (threadIdx.x == 0) a.rest[(long long)i * a.n_seg + s] = (part[0] + part[1]) + (part[2] + part[3]);
     }
 }
 
 // The sum of the threads' values before this one's, and of all.
-__device__ __forceinline__ double scan(double v, double (&part)[kWaves], double* all) {
+template <int N>
+__device__ __forceinline__ double scan(double v, double (&part)[N], double* all) {
     const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
     double sum = v;
 #pragma unroll
@@ -329,7 +498,7 @@ __device__ __forceinline__ double scan(double v, double (&part)[kWaves], double*
     __syncthreads();
     double before = 0.0;
     *all = 0.0;
-    for (int k = 0; k < kWaves; ++k) {
+    for (int k = 0; k < N; ++k) {
         if (k < wave) before += part[k];
         *all += part[k];
     }
@@ -337,25 +506,25 @@ __device__ __forceinline__ double scan(double v, double (&part)[kWaves], double*
 }
 
 // The smallest of the threads' values.
-__device__ __forceinline__ int least(int v, int (&part)[kWaves]) {
+template <int N>
+__device__ __forceinline__ int least(int v, int (&part)[N]) {
     const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
 #pragma unroll
     for (int k = 1; k < kWave; k *= 2) v = min(v, __shfl_xor(v, k, kWave));
     __syncthreads();
     if (lane == 0) part[wave] = v;
     __syncthreads();
-    for (int k = 0; k < kWaves; ++k) v = min(v, part[k]);
+    for (int k = 0; k < N; ++k) v = min(v, part[k]);
     return v;
 }
 
 // A workgroup per sequence: the token that u falls on, and the results.
-__global__ void __launch_bounds__(kThreads) verify_draw_kernel(VerifyArgs a) {
+__global__ void __launch_bounds__(kDraw) verify_draw_kernel(VerifyArgs a) {
     __shared__ Shared sh;
-    __shared__ int box;
-    __shared__ double part[kWaves];
-    __shared__ int ipart[kWaves];
+    __shared__ double part[kDraw / kWave];
+    __shared__ int ipart[kDraw / kWave];
     const int i = blockIdx.x, seq = a.seq0 + i, tid = threadIdx.x;
-    Decision d = decide(a, i, sh, &box);
+    Decision d = a.decided ? a.decided[i] : decide<kDraw / kWave>(a, i, sh);
     constexpr int kNone = 0x7fffffff;
     int token = -1;
     if (d.source != kNothing) {
@@ -378,7 +547,7 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(VerifyArgs a) {
             const Segment g = seg[s];
             return g.top == -INFINITY ? 0.0 : g.sum * weight(g.top, d.p.top, a.factor) / d.p.sum;
         };
-        const int per = (a.n_seg + kThreads - 1) / kThreads;
+        const int per = (a.n_seg + kDraw - 1) / kDraw;
         double mine = 0.0, all, before;
         auto sums = [&]() {
             mine = 0.0;
@@ -386,7 +555,7 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(VerifyArgs a) {
             before = scan(mine, part, &all);
         };
         sums();
-        if (!(all > 0.0)) {   // p is nowhere above q
+        if (!(all > kNothingLeft)) {   // p is nowhere above q
             d.source = kTarget;
             sums();
         }
@@ -397,7 +566,7 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(VerifyArgs a) {
         double start = 0.0;
         for (int s = tid * per; s < min(a.n_seg, (tid + 1) * per); ++s) {
             const double v = sum_of(s);
-            if (v > 0.0) {
+            if (v > kNothingLeft) {
                 last = s;
                 if (found == kNone && sum + v > goal) found = s, start = sum;
             }
@@ -412,19 +581,16 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(VerifyArgs a) {
         if (found == s) s_start = start;
         __syncthreads();
         const Weigher w(a, d);
-        double v[4];
+        double v[4], whole;
         w(s, tid, v);
-        const double four = (v[0] + v[1]) + (v[2] + v[3]);
-        double whole;
-        double c = s_start + scan(four, part, &whole);
+        double c = s_start + scan((v[0] + v[1]) + (v[2] + v[3]), part, &whole);
         found = kNone;
         last = -1;
-        const long long t0 = w.p.first(s, tid);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             c += v[e];
             if (v[e] > 0.0) {
-                last = (int)(t0 + e);
+                last = (int)w.p.first(s, tid) + e;
                 if (found == kNone && c > goal) found = last;
             }
         }
@@ -433,7 +599,7 @@ __global__ void __launch_bounds__(kThreads) verify_draw_kernel(VerifyArgs a) {
     }
     const int n = a.first[i + 1] - a.first[i];
     if (tid == 0) a.out_accepted[seq] = d.accepted;
-    for (int k = tid; k < a.out_stride; k += kThreads)
+    for (int k = tid; k < a.out_stride; k += kDraw)
         a.out_tokens[(long long)seq * a.out_stride + k] =
             k < d.accepted && k < n ? a.tokens[a.first[i] + k] : k == d.accepted ? token : -1;
 }
@@ -492,7 +658,8 @@ extern "C" size_t sa_draft_verify_ws_bytes(int n_seq, const int32_t* counts, int
     long long n;
     if (!verify_sizes_ok(n_seq, counts, vocab, &n)) return 0;
     const size_t segs = segments_of(vocab);
-    return (size_t)(2 * n + n_seq) * segs * sizeof(Segment) + (size_t)std::min(n_seq, kRowsPerLaunch) * segs * sizeof(double);
+    return (size_t)(2 * n + n_seq) * segs * sizeof(Segment) +
+           (size_t)std::min(n_seq, kRowsPerLaunch) * (segs * sizeof(double) + sizeof(Decision));
 }
 
 extern "C" sa_status sa_draft_verify(const float* target, int64_t target_stride, const float* draft,
@@ -505,6 +672,7 @@ extern "C" sa_status sa_draft_verify(const float* target, int64_t target_stride,
     if (!verify_sizes_ok(n_seq, counts, vocab, &n))
         return fail(SA_EINVAL, "verification takes 1 to 2^20 sequences, 0 to 64 drafted tokens each, vocab 1 to 2^30");
     if (!(temperature >= 0.f) || !(temperature < INFINITY)) return fail(SA_EINVAL, "temperature must be >= 0 and finite");
+    static_assert(sizeof(Segment) == 16 && sizeof(Decision) % 8 == 0, "the workspace's parts are aligned");
     const bool greedy = temperature == 0.f;
     if (greedy) draft = nullptr;   // unused
     if (!target || !out_accepted || !out_tokens || (n > 0 && !tokens)) return fail(SA_EINVAL, "null pointer");
@@ -528,7 +696,10 @@ extern "C" sa_status sa_draft_verify(const float* target, int64_t target_stride,
     a.n_target = (int)(n + n_seq);
     a.n_draft = draft ? (int)n : 0;
     a.n_seg = segments_of(vocab);
-    const long long wgs = (long long)(a.n_target + a.n_draft) * ((a.n_seg + kWaves - 1) / kWaves);
+    const long long segs = (long long)(a.n_target + a.n_draft) * a.n_seg;
+    // a workgroup per segment while that leaves CUs without one
+    const bool split = segs < 4LL * kWaves * 256;
+    const long long wgs = split ? segs : (segs + kWaves - 1) / kWaves;
     // a grid has fewer than 2^32 threads
     if (wgs >= (1LL << 32) / kThreads) return fail(SA_EINVAL, "too many logits for one call");
     if (!ws || ws_bytes < sa_draft_verify_ws_bytes(n_seq, counts, vocab))
@@ -542,8 +713,9 @@ extern "C" sa_status sa_draft_verify(const float* target, int64_t target_stride,
     a.vocab = vocab;
     a.factor = greedy ? 0.0 : 1.4426950408889634074 / (double)temperature;
     hipStream_t st = as_stream(stream);
-    if (greedy) hipLaunchKernelGGL(verify_segments_kernel<true>, dim3((unsigned)wgs), dim3(kThreads), 0, st, a);
-    else hipLaunchKernelGGL(verify_segments_kernel<false>, dim3((unsigned)wgs), dim3(kThreads), 0, st, a);
+    const auto kernel = greedy ? (split ? verify_segments_kernel<true, true> : verify_segments_kernel<true, false>)
+                               : (split ? verify_segments_kernel<false, true> : verify_segments_kernel<false, false>);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)wgs), dim3(kThreads), 0, st, a);
     SA_CHECK_LAUNCH();
     int at = 0;
     for (a.seq0 = 0; a.seq0 < n_seq; a.seq0 += kRowsPerLaunch) {
@@ -556,12 +728,16 @@ extern "C" sa_status sa_draft_verify(const float* target, int64_t target_stride,
             SA_CHECK_LAUNCH();
             continue;
         }
+        a.decided = nullptr;
         if (draft && at > a.first[0]) {
-            a.groups = std::max(1, std::min((a.n_seg + kWaves - 1) / kWaves, 2 * device_cu_count() / a.n_seq));
+            a.decided = reinterpret_cast<Decision*>(a.rest + (size_t)std::min(n_seq, kRowsPerLaunch) * a.n_seg);
+            a.groups = std::max(1, std::min(a.n_seg, 8 * device_cu_count() / a.n_seq));
+            hipLaunchKernelGGL(verify_decide_kernel, dim3(a.n_seq), dim3(kDraw), 0, st, a);
+            SA_CHECK_LAUNCH();
             hipLaunchKernelGGL(verify_rest_kernel, dim3(a.n_seq * a.groups), dim3(kThreads), 0, st, a);
             SA_CHECK_LAUNCH();
         }
-        hipLaunchKernelGGL(verify_draw_kernel, dim3(a.n_seq), dim3(kThreads), 0, st, a);
+        hipLaunchKernelGGL(verify_draw_kernel, dim3(a.n_seq), dim3(kDraw), 0, st, a);
         SA_CHECK_LAUNCH();
     }
     return SA_OK;
