@@ -12,6 +12,12 @@
 // into LDS; codes of an 8-bit page are widened on the way, times their row's scale,
 // which is exact, once per workgroup rather than once per wave.
 //
+// fp32 queries (and output): every operand as the exact sum of bf16 terms, three for
+// fp32 values, one for what bf16 and 8-bit caches hold; of the products of three by
+// three terms the six largest are taken (what is left out is below 2^-24 of the
+// product), of one by three all; v_mfma_f32_16x16x32_bf16, a wave owns 16 rows,
+// tiles of 32 keys become terms on their way into LDS.
+//
 // Rows whose sums are not finite are computed anew over what they see (plain_row.h).
 #include <algorithm>
 #include <cmath>
@@ -38,6 +44,7 @@ struct BlockArgs {
     int n_kv, n_q, rep, max_pages, num_pages;
     int n_seq;
     int rows;                                // query rows of a block
+    int tile;                                // keys of a tile
     int tiles;                               // key tiles of a workgroup
     float sl2;                               // |scale| log2(e)
     float factor;                            // scale log2(e)
@@ -50,9 +57,9 @@ struct BlockArgs {
 static_assert(sizeof(BlockArgs) <= 4096, "kernel arguments");
 
 // Key tiles that block b of a sequence sees.
-__host__ __device__ inline int block_key_tiles(const ChunkSeq& s, int b, int rows, int rep) {
+__host__ __device__ inline int block_key_tiles(const ChunkSeq& s, int b, int rows, int rep, int tile) {
     const long long end = (long long)(b + 1) * rows, all = (long long)s.n * rep;
-    return (int)((s.len + ((end < all ? end : all) - 1) / rep) / kBfTile) + 1;
+    return (int)((s.len + ((end < all ? end : all) - 1) / rep) / tile) + 1;
 }
 
 // A workgroup's place.
@@ -64,6 +71,7 @@ struct Block {
     long long part0;        // partial row of query row 0
     const __attribute__((address_space(4))) int32_t* pages;
 };
+template <int TILE>
 __device__ __forceinline__ bool place(const BlockArgs& a, Block& w) {
     const int lane = threadIdx.x & (kWave - 1);
     const int item = blockIdx.x / a.n_kv;   // the KV head varies fastest: with 8 of them each XCD has one
@@ -75,17 +83,17 @@ __device__ __forceinline__ bool place(const BlockArgs& a, Block& w) {
     w.r0 = b * a.rows;
     w.row_end = min(all, w.r0 + a.rows);
     w.u0 = c * a.tiles;
-    w.u1 = min(w.u0 + a.tiles, block_key_tiles(w.sq, b, a.rows, a.rep));
+    w.u1 = min(w.u0 + a.tiles, block_key_tiles(w.sq, b, a.rows, a.rep, TILE));
     w.whole = parts == 1;
     w.part0 = a.base[i] + (long long)c * all;
     // read with scalar loads
     w.pages = (const __attribute__((address_space(4))) int32_t*)(a.table + (size_t)w.sq.cache_row * a.max_pages);
     return w.u0 < w.u1;
 }
-// An id outside the pool (an entry that was never set) is clamped so that no load
-// can fault.
-__device__ __forceinline__ int page_of(const BlockArgs& a, const Block& w, int u) {
-    return min(max(w.pages[u], 0), a.num_pages - 1);
+// The page of a sequence's 64 keys from 64 j on; an id outside the pool (an entry
+// that was never set) is clamped so that no load can fault.
+__device__ __forceinline__ int page_of(const BlockArgs& a, const Block& w, int j) {
+    return min(max(w.pages[j], 0), a.num_pages - 1);
 }
 __device__ __forceinline__ size_t out_row(const BlockArgs& a, const Block& w, int row) {
     const int t = row / a.rep;
@@ -93,21 +101,23 @@ __device__ __forceinline__ size_t out_row(const BlockArgs& a, const Block& w, in
 }
 
 // Query row `row` over the workgroup's keys without matrix instructions, one wave.
-template <int D, int KV, class T>
+template <int D, int KV, int TILE, class T>
 __device__ __forceinline__ void block_plain(const BlockArgs& a, const Block& w, int row) {
     using E = std::conditional_t<KV == SA_DTYPE_FP8, uint8_t, std::conditional_t<KV == SA_DTYPE_BF16, uint16_t, float>>;
     const int lane = threadIdx.x & (kWave - 1);
     const int end = w.sq.len + row / a.rep + 1;   // keys that it sees
     const size_t o = out_row(a, w, row) * D;
     PlainRow<D> p;
-    for (int u = w.u0; u < w.u1 && u * kBfTile < end && !p.lost(); ++u) {
-        const size_t key = ((size_t)page_of(a, w, u) * a.n_kv + w.kvh) * kBfTile;
+    for (int u = w.u0; u < w.u1 && u * TILE < end && !p.lost(); ++u) {
+        const int k0 = u * TILE;
+        const size_t key = ((size_t)page_of(a, w, k0 / SA_PAGE_TOKENS) * a.n_kv + w.kvh) * SA_PAGE_TOKENS +
+                           k0 % SA_PAGE_TOKENS;
         auto value = [&](const void* pool, int i) { return static_cast<const E*>(pool) + (key + i) * D; };
         auto scale = [&](const uint8_t* s, int i) {
             if constexpr (KV == SA_DTYPE_FP8) return __uint_as_float((uint32_t)s[key + i] << 23);
             else return 1.f;
         };
-        p.keys(min(kBfTile, end - u * kBfTile), static_cast<const T*>(a.q) + o, a.factor,
+        p.keys(min(TILE, end - k0), static_cast<const T*>(a.q) + o, a.factor,
                [&](int i) { return value(a.k, i); }, [&](int i) { return value(a.v, i); },
                [&](int i) { return scale(a.k_scale, i); }, [&](int i) { return scale(a.v_scale, i); });
     }
@@ -146,7 +156,7 @@ __global__ void __launch_bounds__(W * kWave, W == 8 && D == 64 ? 4 : 1) extend_b
     const int lane = threadIdx.x & (kWave - 1);
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     Block b;
-    if (!place(a, b)) return;
+    if (!place<kBfTile>(a, b)) return;
     const int last_key = b.sq.len + b.sq.n - 1;   // of the sequence: keys behind it are not read
 
     // ---- a bf16 tile straight into LDS, two tiles ahead ----
@@ -348,7 +358,229 @@ __global__ void __launch_bounds__(W * kWave, W == 8 && D == 64 ? 4 : 1) extend_b
         }
     }
     for (; anew; anew &= anew - 1)
-        block_plain<D, FP8 ? SA_DTYPE_FP8 : SA_DTYPE_BF16, uint16_t>(a, b, w0 + __builtin_ctz(anew));
+        block_plain<D, FP8 ? SA_DTYPE_FP8 : SA_DTYPE_BF16, kBfTile, uint16_t>(a, b, w0 + __builtin_ctz(anew));
+}
+
+// ---------------------------------------------------------------- fp32
+
+constexpr int kTermTile = 32;
+
+template <int D, int KV>
+struct TermGeo {
+    static constexpr int NT = KV == SA_DTYPE_F32 ? kTerms : 1;   // terms of a cached value
+    static constexpr int PAIRS = KV == SA_DTYPE_F32 ? 6 : 3;
+    static constexpr int ROWB = 2 * D;                  // a row of one term
+    static constexpr int TERM = kTermTile * ROWB;       // one term of K or V
+    static constexpr int STAGE = 2 * NT * TERM;         // K's terms, then V's
+    static constexpr int CPR = ROWB / 16;
+    static constexpr int KS = D / 32, DB = D / 16;
+    // Terms of the cached and of the other operand of a product, largest first.
+    static constexpr int pair_a(int pr) { return NT == 1 ? 0 : (pr == 2 || pr == 4 ? 1 : pr == 5 ? 2 : 0); }
+    static constexpr int pair_b(int pr) { return NT == 1 ? pr : (pr == 1 || pr == 4 ? 1 : pr == 3 ? 2 : 0); }
+    // Chunk c of row r at c ^ swz(r): rows 8a + 4kb + b of a K fragment read and rows
+    // 8g + 4u + b of a half wave's V^T read on different banks.
+    static __device__ __forceinline__ int swz(int r) {
+        if constexpr (CPR == 16) return ((r & 3) << 2) | (((r >> 3) & 1) << 1) | ((r >> 4) & 1);
+        else return (((r >> 1) & 1) << 2) | (((r >> 3) & 1) << 1) | ((r >> 4) & 1);
+    }
+    static __device__ __forceinline__ int off(int r, int c) { return r * ROWB + ((c ^ swz(r)) << 4); }
+};
+
+// Eight cached values on their way into LDS.
+template <int KV>
+struct Staged {
+    u32x4_t x[KV == SA_DTYPE_F32 ? 2 : 1];
+    uint32_t scale;
+    __device__ __forceinline__ void load(const void* pool, const uint8_t* scales, size_t row, size_t at) {
+        if constexpr (KV == SA_DTYPE_F32) {
+            x[0] = *reinterpret_cast<const u32x4_t*>(static_cast<const float*>(pool) + at);
+            x[1] = *reinterpret_cast<const u32x4_t*>(static_cast<const float*>(pool) + at + 4);
+        } else if constexpr (KV == SA_DTYPE_BF16) {
+            x[0] = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(pool) + at);
+        } else {
+            const uint2 c = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(pool) + at);
+            x[0][0] = c.x;
+            x[0][1] = c.y;
+            scale = scales[row];
+        }
+    }
+    template <int N>
+    __device__ __forceinline__ void terms(bf16x8_t (&t)[N]) const {
+        if constexpr (KV == SA_DTYPE_F32)
+            split_terms(__builtin_bit_cast(f32x4_t, x[0]), __builtin_bit_cast(f32x4_t, x[1]), t);
+        else if constexpr (KV == SA_DTYPE_BF16) t[0] = __builtin_bit_cast(bf16x8_t, x[0]);
+        else t[0] = widen8(x[0][0], x[0][1], __uint_as_float(scale << 23));
+    }
+};
+
+template <int D, int W, int KV>
+__global__ void __launch_bounds__(W * kWave) extend_f32_kernel(BlockArgs a) {
+    using G = TermGeo<D, KV>;
+    constexpr int THREADS = W * kWave;
+    constexpr int C8 = D / 8;                           // 8-element pieces of a row
+    constexpr int NC = kTermTile * C8 / THREADS > 0 ? kTermTile * C8 / THREADS : 1;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    lds_u8_t* const smem = (lds_u8_t*)smem_raw;
+    const int lane = threadIdx.x & (kWave - 1);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int r16 = lane & 15, g = lane >> 4;
+    Block b;
+    if (!place<kTermTile>(a, b)) return;
+    const int last_key = b.sq.len + b.sq.n - 1;   // of the sequence: keys behind it are not read
+
+    // ---- tiles: as cached in registers one tile ahead, bf16 terms in LDS ----
+    const bool loads = kTermTile * C8 >= THREADS || threadIdx.x < kTermTile * C8;
+    Staged<KV> sk[NC], sv[NC];
+    auto load = [&](int u, int page) {
+        if (!loads) return;
+        const int k0 = u * kTermTile;
+        const size_t first = ((size_t)page * a.n_kv + b.kvh) * SA_PAGE_TOKENS + k0 % SA_PAGE_TOKENS;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int idx = threadIdx.x + i * THREADS;
+            const size_t row = first + min(idx / C8, last_key - k0), at = row * D + 8 * (idx % C8);
+            sk[i].load(a.k, a.k_scale, row, at);
+            sv[i].load(a.v, a.v_scale, row, at);
+        }
+    };
+    auto store_tile = [&](int u) {
+        if (!loads) return;
+        lds_u8_t* base = smem + (u & 1) * G::STAGE;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            const int idx = threadIdx.x + i * THREADS;
+            const int off = G::off(idx / C8, idx % C8);
+            bf16x8_t t[G::NT];
+            sk[i].terms(t);
+#pragma unroll
+            for (int x = 0; x < G::NT; ++x)
+                *reinterpret_cast<__attribute__((address_space(3))) bf16x8_t*>(base + x * G::TERM + off) = t[x];
+            sv[i].terms(t);
+#pragma unroll
+            for (int x = 0; x < G::NT; ++x)
+                *reinterpret_cast<__attribute__((address_space(3))) bf16x8_t*>(base + (G::NT + x) * G::TERM + off) = t[x];
+        }
+    };
+    auto page_at = [&](int u) { return page_of(a, b, u * kTermTile / SA_PAGE_TOKENS); };
+    load(b.u0, page_at(b.u0));
+    int next = b.u0 + 1 < b.u1 ? page_at(b.u0 + 1) : 0;
+
+    const int w0 = b.r0 + wave * 16;
+    const int my_row = min(w0 + r16, b.row_end - 1);
+    const bool active = w0 < b.row_end;
+    const int q_lo = b.sq.len + min(w0, b.row_end - 1) / a.rep, q_hi = b.sq.len + min(w0 + 15, b.row_end - 1) / a.rep;
+    const int q_mine = b.sq.len + my_row / a.rep;   // the last key that this lane's row sees
+    bf16x8_t qf[G::KS][kTerms];
+    {
+        const float* row = static_cast<const float*>(a.q) + out_row(a, b, my_row) * D + 8 * g;
+#pragma unroll
+        for (int ks = 0; ks < G::KS; ++ks)
+            split_terms(*reinterpret_cast<const f32x4_t*>(row + 32 * ks) * a.factor,
+                        *reinterpret_cast<const f32x4_t*>(row + 32 * ks + 4) * a.factor, qf[ks]);
+    }
+    f32x4_t acc[G::DB];
+#pragma unroll
+    for (int db = 0; db < G::DB; ++db) acc[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, bias = 0.f, l = 0.f, cap = -1.f;
+
+    auto compute = [&](int k0, const lds_u8_t* sb, bool mask) {
+        // element 4 kb + e of a lane: key 8 g + 4 kb + e
+        f32x4_t s[2] = {f32x4_t{bias, bias, bias, bias}, f32x4_t{bias, bias, bias, bias}};
+#pragma unroll
+        for (int ks = 0; ks < G::KS; ++ks) {
+            bf16x8_t kf[2][G::NT];
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int t = 0; t < G::NT; ++t)
+                    kf[kb][t] = *reinterpret_cast<const __attribute__((address_space(3))) bf16x8_t*>(
+                        sb + t * G::TERM + G::off(8 * (r16 >> 2) + 4 * kb + (r16 & 3), 4 * ks + g));
+#pragma unroll
+            for (int pr = 0; pr < G::PAIRS; ++pr)
+#pragma unroll
+                for (int kb = 0; kb < 2; ++kb)
+                    s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kb][G::pair_a(pr)], qf[ks][G::pair_b(pr)], s[kb],
+                                                                    0, 0, 0);
+        }
+        if (mask) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (k0 + 8 * g + j > q_mine) s[j >> 2][j & 3] = -INFINITY;
+        }
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(s[j >> 2][j & 3]);
+        float sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        if (__any(!(sum <= cap))) {
+            float mt = s[0][0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) mt = fmaxf(mt, s[j >> 2][j & 3]);
+            const float m_new = fmaxf(m, group_reduce<OpMax, 16, kWave>(mt) - bias);
+            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+#pragma unroll
+            for (int db = 0; db < G::DB; ++db) acc[db] *= alpha;
+            l *= alpha;
+            const float b_new = m_new == -INFINITY ? 0.f : -m_new;
+            const float delta = b_new - bias;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(s[j >> 2][j & 3] + delta);
+            sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            m = m_new;
+            bias = b_new;
+            cap = m_new == -INFINITY ? -1.f : kBfRaiseAt;
+        }
+        l += sum;
+        bf16x8_t pt[kTerms];
+        split_terms(f32x4_t{p[0], p[1], p[2], p[3]}, f32x4_t{p[4], p[5], p[6], p[7]}, pt);
+#pragma unroll
+        for (int db = 0; db < G::DB; ++db) {
+            bf16x8_t vf[G::NT];
+            const int c = 2 * db + ((r16 & 3) >> 1), r = 8 * g + (r16 >> 2), h8 = (r16 & 1) * 8;
+#pragma unroll
+            for (int t = 0; t < G::NT; ++t) {
+                const lds_u8_t* vb = sb + (G::NT + t) * G::TERM + h8;
+                const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vb + G::off(r, c)));
+                const s16x4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vb + G::off(r + 4, c)));
+                vf[t] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+            }
+#pragma unroll
+            for (int pr = 0; pr < G::PAIRS; ++pr)
+                acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[G::pair_a(pr)], pt[G::pair_b(pr)], acc[db], 0, 0, 0);
+        }
+    };
+
+    store_tile(b.u0);
+    if (b.u0 + 1 < b.u1) load(b.u0 + 1, next);
+    next = b.u0 + 2 < b.u1 ? page_at(b.u0 + 2) : 0;
+    lds_barrier();
+    for (int u = b.u0; u < b.u1; ++u) {
+        const int k0 = u * kTermTile;
+        if (active && k0 <= q_hi) compute(k0, smem + (u & 1) * G::STAGE, k0 + kTermTile - 1 > q_lo);
+        if (u + 1 < b.u1) {
+            store_tile(u + 1);   // where tile u - 1 was
+            if (u + 2 < b.u1) load(u + 2, next);
+            if (u + 3 < b.u1) next = page_at(u + 3);
+        }
+        lds_barrier();
+    }
+
+    const float sum = group_reduce<OpSum, 16, kWave>(l), fine = sum + group_reduce<OpSum, 16, kWave>(not_finite<G::DB>(acc));
+    const bool mine = w0 + r16 < b.row_end, ok = fine < INFINITY;
+    if (mine && ok) {
+        if (b.whole) {
+            const float inv = 1.0f / sum;
+            float* o = static_cast<float*>(a.out) + out_row(a, b, my_row) * D + 4 * g;
+#pragma unroll
+            for (int db = 0; db < G::DB; ++db) *reinterpret_cast<f32x4_t*>(o + 16 * db) = acc[db] * inv;
+        } else {
+            const size_t at = (size_t)(b.part0 + my_row) * a.n_kv + b.kvh;
+#pragma unroll
+            for (int db = 0; db < G::DB; ++db) *reinterpret_cast<f32x4_t*>(a.part_o + at * D + 16 * db + 4 * g) = acc[db];
+            if (g == 0) *reinterpret_cast<f32x2_t*>(a.part_ml + at * 2) = f32x2_t{m, sum};
+        }
+    }
+    for (uint32_t anew = __ballot(mine && !ok) & 0xffff; anew; anew &= anew - 1)
+        block_plain<D, KV, kTermTile, float>(a, b, w0 + __builtin_ctz(anew));
 }
 
 // ---------------------------------------------------------------- partials
@@ -374,7 +606,7 @@ __global__ void __launch_bounds__(256) block_merge_kernel(BlockArgs a, long long
     const int t = token - sq.first;
     if (a.parts[i] == 1 || t >= sq.n) return;   // written already, or a row of another launch
     const int kvh = head / a.rep, row = t * a.rep + head % a.rep;
-    const int parts = (block_key_tiles(sq, row / a.rows, a.rows, a.rep) + a.tiles - 1) / a.tiles;
+    const int parts = (block_key_tiles(sq, row / a.rows, a.rows, a.rep, a.tile) + a.tiles - 1) / a.tiles;
     const long long step = (long long)sq.n * a.rep;
     float M = -INFINITY, L = 0.f;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
@@ -400,19 +632,39 @@ constexpr int kBlockRows = 65;
 constexpr int kMaxRounds = 4;    // of workgroups that a launch's tiles are cut into
 constexpr int kPartTiles = 3;    // what a workgroup costs besides its tiles
 
-template <int D, int W, bool FP8>
-sa_status launch_bf16(const BlockArgs& a, hipStream_t st) {
-    constexpr int lds = 2 * BfGeo<D>::STAGE;
-    constexpr auto kernel = extend_bf16_kernel<D, W, FP8>;
-    SA_TRY(pf::opt_in_lds<kernel>(lds));
-    hipLaunchKernelGGL(kernel, dim3((unsigned)a.start[a.n_seq] * a.n_kv), dim3(W * kWave), lds, st, a);
+template <auto KERNEL>
+sa_status launch_blocks(const BlockArgs& a, int waves, int lds, hipStream_t st) {
+    SA_TRY(pf::opt_in_lds<KERNEL>(lds));
+    hipLaunchKernelGGL(KERNEL, dim3((unsigned)a.start[a.n_seq] * a.n_kv), dim3(waves * kWave), lds, st, a);
     SA_CHECK_LAUNCH();
     return SA_OK;
 }
+template <int D, int KV>
+sa_status launch_f32(const BlockArgs& a, int waves, hipStream_t st) {
+    constexpr int lds = 2 * TermGeo<D, KV>::STAGE;
+    return waves == 8 ? launch_blocks<extend_f32_kernel<D, 8, KV>>(a, 8, lds, st)
+                      : launch_blocks<extend_f32_kernel<D, 4, KV>>(a, 4, lds, st);
+}
+template <int D, bool FP8>
+sa_status launch_bf16(const BlockArgs& a, int waves, hipStream_t st) {
+    constexpr int lds = 2 * BfGeo<D>::STAGE;
+    return waves == 8 ? launch_blocks<extend_bf16_kernel<D, 8, FP8>>(a, 8, lds, st)
+                      : launch_blocks<extend_bf16_kernel<D, 4, FP8>>(a, 4, lds, st);
+}
 template <int D>
-sa_status dispatch_blocks(const BlockArgs& a, bool fp8, hipStream_t st) {
-    if (fp8) return a.rows == 256 ? launch_bf16<D, 8, true>(a, st) : launch_bf16<D, 4, true>(a, st);
-    return a.rows == 256 ? launch_bf16<D, 8, false>(a, st) : launch_bf16<D, 4, false>(a, st);
+sa_status dispatch_blocks(const BlockArgs& a, sa_dtype kv, bool q16, int waves, bool merge, long long rows,
+                          hipStream_t st) {
+    if (q16) SA_TRY(kv == SA_DTYPE_FP8 ? (launch_bf16<D, true>(a, waves, st)) : (launch_bf16<D, false>(a, waves, st)));
+    else SA_TRY(kv == SA_DTYPE_F32    ? (launch_f32<D, SA_DTYPE_F32>(a, waves, st))
+                : kv == SA_DTYPE_BF16 ? (launch_f32<D, SA_DTYPE_BF16>(a, waves, st))
+                                      : (launch_f32<D, SA_DTYPE_FP8>(a, waves, st)));
+    if (!merge) return SA_OK;
+    const int per = 256 / (D / 4);
+    const dim3 grid((unsigned)((rows + per - 1) / per));
+    if (q16) hipLaunchKernelGGL((block_merge_kernel<D, uint16_t>), grid, dim3(256), 0, st, a, rows);
+    else hipLaunchKernelGGL((block_merge_kernel<D, float>), grid, dim3(256), 0, st, a, rows);
+    SA_CHECK_LAUNCH();
+    return SA_OK;
 }
 
 long long blocks_of(long long rows, int block) { return (rows + block - 1) / block; }
@@ -420,7 +672,7 @@ long long blocks_of(long long rows, int block) { return (rows + block - 1) / blo
 }  // namespace
 
 bool extend_is_block(sa_dtype kv, bool q16, int rep, int n) {
-    return q16 && kv != SA_DTYPE_F32 && (long long)n * rep >= kBlockRows;
+    return (long long)n * rep >= kBlockRows;
 }
 
 size_t extend_blocks_ws(int n, const int32_t* counts, int n_q, int n_kv, int d, long long max_tokens) {
@@ -454,23 +706,25 @@ sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, co
             a.seq[i] = seqs[i0 + i];
             most = std::max(most, (long long)a.seq[i].n * a.rep);
         }
-        a.rows = most > 128 ? 256 : 128;
-        int longest = 1;
-        for (int i = 0; i < a.n_seq; ++i)
-            longest = std::max(longest, block_key_tiles(a.seq[i], (int)blocks_of((long long)a.seq[i].n * a.rep, a.rows) - 1,
-                                                        a.rows, a.rep));
-        auto parts_of = [&](int i, int tiles) {
+        const int per_wave = q16 ? 32 : 16, waves = most > 4 * per_wave ? 8 : 4;
+        a.rows = waves * per_wave;
+        a.tile = q16 ? kBfTile : kTermTile;
+        auto last_tiles = [&](int i) {
             const int last = (int)blocks_of((long long)a.seq[i].n * a.rep, a.rows) - 1;
-            return (block_key_tiles(a.seq[i], last, a.rows, a.rep) + tiles - 1) / tiles;
+            return block_key_tiles(a.seq[i], last, a.rows, a.rep, a.tile);
         };
+        int longest = 1;
+        for (int i = 0; i < a.n_seq; ++i) longest = std::max(longest, last_tiles(i));
+        auto parts_of = [&](int i, int tiles) { return (last_tiles(i) + tiles - 1) / tiles; };
         auto workgroups = [&](int tiles) {
             long long k = 0;
             for (int i = 0; i < a.n_seq; ++i) k += blocks_of((long long)a.seq[i].n * a.rep, a.rows) * parts_of(i, tiles);
             return k * a.n_kv;
         };
-        // For 1 .. kMaxRounds rounds of a workgroup per CU (two of four waves): the fewest
+        // For 1 .. kMaxRounds rounds of a workgroup per CU (two of four waves, and of bf16 at
+        // D = 64): the fewest
         // tiles per workgroup that give no more of them; the cheapest of these.
-        const long long round = (a.rows == 256 && c.d == 128 ? 1LL : 2LL) * device_cu_count();
+        const long long round = (waves == 8 && !(q16 && c.d == 64) ? 1LL : 2LL) * device_cu_count();
         a.tiles = longest;
         long long best = ((workgroups(longest) + round - 1) / round) * (longest + kPartTiles);
         for (int k = 1; k <= kMaxRounds; ++k) {
@@ -495,7 +749,7 @@ sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, co
         a.start[a.n_seq] = (int)at;
         const long long tokens = a.seq[a.n_seq - 1].first + a.seq[a.n_seq - 1].n - a.seq[0].first;
         // a grid has fewer than 2^32 threads
-        if (at * a.n_kv >= (1LL << 32) / (a.rows * 2) || parts > 0x7fffffffLL || tokens * n_q >= (1LL << 32) / 64)
+        if (at * a.n_kv >= (1LL << 32) / (waves * kWave) || parts > 0x7fffffffLL || tokens * n_q >= (1LL << 32) / 64)
             return fail(SA_EINVAL, "too many tokens for one call");
         if (parts) {
             const size_t need = (size_t)parts * a.n_kv * (c.d + 2) * sizeof(float);
@@ -503,16 +757,8 @@ sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, co
             a.part_o = static_cast<float*>(ws);
             a.part_ml = a.part_o + (size_t)parts * a.n_kv * c.d;
         }
-        const bool fp8 = c.kv == SA_DTYPE_FP8;
-        SA_TRY(c.d == 64 ? dispatch_blocks<64>(a, fp8, st) : dispatch_blocks<128>(a, fp8, st));
-        if (parts) {
-            const long long n_rows = tokens * n_q;
-            const int per = 256 / (c.d / 4);
-            const dim3 grid((unsigned)((n_rows + per - 1) / per));
-            if (c.d == 64) hipLaunchKernelGGL((block_merge_kernel<64, uint16_t>), grid, dim3(256), 0, st, a, n_rows);
-            else hipLaunchKernelGGL((block_merge_kernel<128, uint16_t>), grid, dim3(256), 0, st, a, n_rows);
-            SA_CHECK_LAUNCH();
-        }
+        SA_TRY(c.d == 64 ? dispatch_blocks<64>(a, c.kv, q16, waves, parts > 0, tokens * n_q, st)
+                         : dispatch_blocks<128>(a, c.kv, q16, waves, parts > 0, tokens * n_q, st));
     }
     return SA_OK;
 }
