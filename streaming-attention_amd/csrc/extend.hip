@@ -627,10 +627,11 @@ __global__ void __launch_bounds__(256) block_merge_kernel(BlockArgs a, long long
 
 // ---------------------------------------------------------------- launch
 
-// Query rows of a sequence and KV head from which blocks are taken.
-constexpr int kBlockRows = 65;
 constexpr int kMaxRounds = 4;    // of workgroups that a launch's tiles are cut into
-constexpr int kPartTiles = 3;    // what a workgroup costs besides its tiles
+// What a workgroup costs besides its tiles, in tiles: its beginning and its output, or
+// where a block is cut a partial written and read again.
+constexpr int kWholeTiles = 2, kCutBf16 = 6, kCutF32 = 4, kCutTerms = 7;
+constexpr double kFourWaves = 0.6;   // a tile of a workgroup of four waves alone on its CU
 
 template <auto KERNEL>
 sa_status launch_blocks(const BlockArgs& a, int waves, int lds, hipStream_t st) {
@@ -671,12 +672,29 @@ long long blocks_of(long long rows, int block) { return (rows + block - 1) / blo
 
 }  // namespace
 
-bool extend_is_block(sa_dtype kv, bool q16, int rep, int n) {
-    return (long long)n * rep >= kBlockRows;
+// Blocks for sequences of kBlockRows query rows of a KV head, where a call has enough
+// of them: below it the rows' launch with its smaller pieces is quicker.  us, rows /
+// blocks, 16 / 8 heads of 128, queries and cache bf16: 256 rows over 1128 keys 19.6 / 20.7,
+// 512 over 1256 31.6 / 24.7, 64 over 8032 36.1 / 29.8, 768 over 384 15.0 / 17.3; fp32 (always
+// blocks): 64 over 32 13.2 / 6.8, over 1032 22.0 / 19.0; 32 sequences of 32 rows over 2016
+// 116 / 146.  Other sequences join the blocks where they cost an eighth of them at most,
+// which saves their launches.
+void split_chunks(sa_dtype kv, int rep, int n_kv, const ChunkSeq* seqs, int n, std::vector<ChunkSeq>* many,
+                  std::vector<ChunkSeq>* few) {
+    constexpr long long kBlockRows = 64, kBlockWork = 3000000, kJoinRows = 256 / 8;
+    long long work = 0, others = 0;   // query rows x keys; keys
+    for (int i = 0; i < n; ++i) {
+        const long long rows = (long long)seqs[i].n * rep, keys = (long long)seqs[i].len + seqs[i].n;
+        if (rows >= kBlockRows) work += rows * keys;
+        else others += keys;
+    }
+    const bool blocks = work > 0 && (kv == SA_DTYPE_F32 || work * n_kv >= kBlockWork), join = others * kJoinRows <= work;
+    for (int i = 0; i < n; ++i)
+        (blocks && (join || (long long)seqs[i].n * rep >= kBlockRows) ? many : few)->push_back(seqs[i]);
 }
 
 size_t extend_blocks_ws(int n, const int32_t* counts, int n_q, int n_kv, int d, long long max_tokens) {
-    const long long tiles = (max_tokens + kBfTile - 1) / kBfTile;
+    const long long tiles = (max_tokens + kTermTile - 1) / kTermTile;
     if (tiles <= 1) return 0;
     const long long round = device_cu_count();
     size_t need = 0;
@@ -684,7 +702,7 @@ size_t extend_blocks_ws(int n, const int32_t* counts, int n_q, int n_kv, int d, 
         long long rows = 0;
         for (int i = i0; i < std::min(n, i0 + kRowsPerLaunch); ++i) rows += (long long)counts[i] * n_q;
         // at most as many workgroups as extend_blocks cuts into
-        need = std::max(need, (size_t)std::min(rows * tiles, kMaxRounds * round * (d == 64 ? 512 : 256)) * (d + 2) * sizeof(float));
+        need = std::max(need, (size_t)std::min(rows * tiles, kMaxRounds * round * 256) * (d + 2) * sizeof(float));
     }
     return need;
 }
@@ -706,38 +724,50 @@ sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, co
             a.seq[i] = seqs[i0 + i];
             most = std::max(most, (long long)a.seq[i].n * a.rep);
         }
-        const int per_wave = q16 ? 32 : 16, waves = most > 4 * per_wave ? 8 : 4;
-        a.rows = waves * per_wave;
         a.tile = q16 ? kBfTile : kTermTile;
+        const int per_wave = q16 ? 32 : 16;
+        int longest = 1;
         auto last_tiles = [&](int i) {
             const int last = (int)blocks_of((long long)a.seq[i].n * a.rep, a.rows) - 1;
             return block_key_tiles(a.seq[i], last, a.rows, a.rep, a.tile);
         };
-        int longest = 1;
-        for (int i = 0; i < a.n_seq; ++i) longest = std::max(longest, last_tiles(i));
         auto parts_of = [&](int i, int tiles) { return (last_tiles(i) + tiles - 1) / tiles; };
         auto workgroups = [&](int tiles) {
             long long k = 0;
             for (int i = 0; i < a.n_seq; ++i) k += blocks_of((long long)a.seq[i].n * a.rep, a.rows) * parts_of(i, tiles);
             return k * a.n_kv;
         };
-        // For 1 .. kMaxRounds rounds of a workgroup per CU (two of four waves, and of bf16 at
-        // D = 64): the fewest
-        // tiles per workgroup that give no more of them; the cheapest of these.
-        const long long round = (waves == 8 && !(q16 && c.d == 64) ? 1LL : 2LL) * device_cu_count();
-        a.tiles = longest;
-        long long best = ((workgroups(longest) + round - 1) / round) * (longest + kPartTiles);
-        for (int k = 1; k <= kMaxRounds; ++k) {
-            if (workgroups(longest) > k * round) continue;
-            int lo = 1, hi = longest;   // workgroups(tiles) falls
-            while (lo < hi) {
-                const int mid = (lo + hi) / 2;
-                if (workgroups(mid) <= k * round) hi = mid;
-                else lo = mid + 1;
+        // Eight or four waves, and the tiles that give no more than 1 .. kMaxRounds times as
+        // many workgroups as there are CUs, or all: what is estimated cheapest, in tiles of a
+        // workgroup of eight waves.
+        const long long cus = device_cu_count();
+        const int cut = q16 ? kCutBf16 : c.kv == SA_DTYPE_F32 ? kCutF32 : kCutTerms;
+        const bool pairs = q16 && c.d == 64;   // two workgroups of eight waves per CU
+        int waves = 8;
+        double best = INFINITY;
+        for (int w = 8; w >= 4; w -= 4) {
+            if (w == 8 && most <= 4 * per_wave) continue;
+            a.rows = w * per_wave;
+            longest = 1;
+            for (int i = 0; i < a.n_seq; ++i) longest = std::max(longest, last_tiles(i));
+            for (int k = 0; k <= kMaxRounds; ++k) {
+                int lo = longest;
+                if (k) {
+                    if (workgroups(longest) > k * cus) continue;
+                    lo = 1;
+                    for (int hi = longest; lo < hi;) {   // workgroups(tiles) falls
+                        const int mid = (lo + hi) / 2;
+                        if (workgroups(mid) <= k * cus) hi = mid;
+                        else lo = mid + 1;
+                    }
+                }
+                const long long wgs = workgroups(lo), slots = w == 4 || pairs ? 2 * cus : cus;
+                const double speed = wgs > cus ? (w == 8 && pairs ? 2.0 : 1.0) : w == 8 ? 1.0 : kFourWaves;
+                const double cost = (double)((wgs + slots - 1) / slots) * (lo + (lo < longest ? cut : kWholeTiles)) * speed;
+                if (cost < best) best = cost, waves = w, a.tiles = lo;
             }
-            const long long cost = (long long)k * (lo + kPartTiles);
-            if (cost < best) best = cost, a.tiles = lo;
         }
+        a.rows = waves * per_wave;
         long long at = 0, parts = 0;
         for (int i = 0; i < a.n_seq; ++i) {
             a.parts[i] = parts_of(i, a.tiles);

@@ -1213,9 +1213,8 @@ extern "C" sa_status sa_paged_extend(const sa_kvcache* c, int layer, const void*
         // other, in the same workspace.
         const PagedView view = view_of(c, layer);
         const bool q16 = q_dtype == SA_DTYPE_BF16;
-        std::vector<ChunkSeq> few, many;
-        few.reserve(n_seq);
-        many.reserve(n_seq);
+        std::vector<ChunkSeq> seqs, few, many;
+        seqs.reserve(n_seq);
         long long rows = 0;
         for (int i = 0; i < n_seq; ++i) {
             const int row = seq_ids ? seq_ids[i] : i, len = c->pt.len(row);
@@ -1223,11 +1222,10 @@ extern "C" sa_status sa_paged_extend(const sa_kvcache* c, int layer, const void*
             if (rows + counts[i] > kMaxNewTokens) return fail(SA_EINVAL, "more than 2^20 new tokens");
             if ((long long)len + counts[i] > c->pt.capacity(row))
                 return fail(SA_ERANGE, "Requested seq_len exceeds cached length");
-            if (counts[i])
-                (extend_is_block(view.kv, q16, n_q_heads / view.n_kv, counts[i]) ? many : few)
-                    .push_back(ChunkSeq{row, len, counts[i], (int)rows});
+            if (counts[i]) seqs.push_back(ChunkSeq{row, len, counts[i], (int)rows});
             rows += counts[i];
         }
+        split_chunks(view.kv, n_q_heads / view.n_kv, view.n_kv, seqs.data(), (int)seqs.size(), &many, &few);
         if (!many.empty())
             SA_TRY(extend_blocks(view, q, q16, n_q_heads, many.data(), (int)many.size(), scale, out, ws, ws_bytes,
                                  as_stream(stream)));

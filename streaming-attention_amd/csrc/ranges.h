@@ -2,6 +2,8 @@
 // windowed decode and the decode of sequences that share their leading pages.
 #pragma once
 
+#include <vector>
+
 #include "sa_internal.h"
 
 namespace sa {
@@ -46,9 +48,10 @@ size_t extend_rows_ws(int n, const int32_t* counts, int n_q, int n_kv, int d, bo
 sa_status extend_rows(const PagedView& c, const void* q, bool q16, int n_q, const ChunkSeq* seqs, int n, float scale,
                       void* out, void* ws, size_t ws_bytes, hipStream_t st);
 
-// The same for chunks of many query rows (extend.hip): whether a chunk of n tokens
-// takes it, and its workspace and launch for chunks that all do.
-bool extend_is_block(sa_dtype kv, bool q16, int rep, int n);
+// The same for chunks of many query rows (extend.hip), and which of a call's chunks
+// (none of them empty) go which way.
+void split_chunks(sa_dtype kv, int rep, int n_kv, const ChunkSeq* seqs, int n, std::vector<ChunkSeq>* many,
+                  std::vector<ChunkSeq>* few);
 size_t extend_blocks_ws(int n, const int32_t* counts, int n_q, int n_kv, int d, long long max_tokens);
 sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, const ChunkSeq* seqs, int n, float scale,
                         void* out, void* ws, size_t ws_bytes, hipStream_t st);
