@@ -75,17 +75,26 @@ template <int TILE>
 __device__ __forceinline__ bool place(const BlockArgs& a, Block& w) {
     const int lane = threadIdx.x & (kWave - 1);
     const int item = blockIdx.x / a.n_kv;   // the KV head varies fastest: with 8 of them each XCD has one
-    const int i = __popcll(__ballot(lane < a.n_seq && a.start[lane] <= item)) - 1;
-    w.sq = a.seq[i];
+    // One sequence: its arguments with the others', not behind a search (arguments may be
+    // a trip to host memory away).
+    int parts = a.parts[0], local = item, base = 0;
+    w.sq = a.seq[0];
+    if (a.n_seq > 1) {
+        const int i = __popcll(__ballot(lane < a.n_seq && a.start[lane] <= item)) - 1;
+        w.sq = a.seq[i];
+        parts = a.parts[i];
+        local = item - a.start[i];
+        base = a.base[i];
+    }
     w.kvh = blockIdx.x % a.n_kv;
-    const int parts = a.parts[i], local = item - a.start[i], all = w.sq.n * a.rep;
+    const int all = w.sq.n * a.rep;
     const int b = (all + a.rows - 1) / a.rows - 1 - local / parts, c = local % parts;   // the longest first
     w.r0 = b * a.rows;
     w.row_end = min(all, w.r0 + a.rows);
     w.u0 = c * a.tiles;
     w.u1 = min(w.u0 + a.tiles, block_key_tiles(w.sq, b, a.rows, a.rep, TILE));
     w.whole = parts == 1;
-    w.part0 = a.base[i] + (long long)c * all;
+    w.part0 = base + (long long)c * all;
     // read with scalar loads
     w.pages = (const __attribute__((address_space(4))) int32_t*)(a.table + (size_t)w.sq.cache_row * a.max_pages);
     return w.u0 < w.u1;

@@ -1005,9 +1005,16 @@ __global__ void __launch_bounds__(kThreads) chunk_attn_kernel(ChunkArgs a) {
     const int item = blockIdx.x / a.n_kv;
     // The last sequence that starts at or before the item (those without tokens
     // start where the next one does).
-    const int i = __popcll(__ballot(lane < a.n_seq && a.start[lane] <= item)) - 1;
-    const ChunkSeq sq = a.seq[i];
-    const int chunks = a.chunks[i], local = item - a.start[i];
+    // One sequence's arguments come with the others, not behind a search.
+    ChunkSeq sq = a.seq[0];
+    int chunks = a.chunks[0], local = item, base = 0;
+    if (a.n_seq > 1) {
+        const int i = __popcll(__ballot(lane < a.n_seq && a.start[lane] <= item)) - 1;
+        sq = a.seq[i];
+        chunks = a.chunks[i];
+        local = item - a.start[i];
+        base = a.base[i];
+    }
     const int b = local / chunks, c = local % chunks;
     Item it;
     it.kvh = blockIdx.x % a.n_kv;
@@ -1020,7 +1027,7 @@ __global__ void __launch_bounds__(kThreads) chunk_attn_kernel(ChunkArgs a) {
     it.rows = n * a.rep;
     it.q0 = 0;
     it.q1 = it.rows;
-    it.part0 = a.base[i] + (c * sq.n + t0) * a.rep;
+    it.part0 = base + (c * sq.n + t0) * a.rep;
     it.single = chunks == 1 ? ~0ull : 0;
     it.limit0 = sq.len + t0 + 1;
     stage_pages(a, it, pages);
