@@ -719,7 +719,7 @@ __device__ __forceinline__ void attend_item(const CacheArgs& a, const Item& it, 
 }
 
 template <int D, int KV>
-__global__ void __launch_bounds__(kThreads) range_attn_kernel(RangeArgs a) {
+__global__ void __launch_bounds__(kThreads, KV == kFp8 ? 3 : 1) range_attn_kernel(RangeArgs a) {
     using G = Geo<D, KV>;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     __shared__ int32_t pages[kChunkTiles];
@@ -929,7 +929,7 @@ sa_status decode_ranges(const PagedView& c, const float* q, int n_q, const Range
             chunk = std::min(std::max(chunk, ceil_div(longest, kMaxChunks)), kChunkTiles);
             return std::pair<int, long long>(chunk, workgroups(chunk));
         };
-        const long long slots = (f32 ? 1LL : 2LL) * device_cu_count(), round = slots + slots / 4;
+        const long long slots = (f32 ? 1LL : c.kv == SA_DTYPE_FP8 ? 3LL : 2LL) * device_cu_count(), round = slots + slots / 4;
         const auto own = pick(a.n_groups, n_src, round, a.n_groups == 0);
         a.chunk_own = own.first;
         a.chunk_group = pick(0, a.n_groups, std::max(round - own.second, round / 2), false).first;
