@@ -607,10 +607,11 @@ template <int D, class T>
 __global__ void __launch_bounds__(256) block_merge_kernel(BlockArgs a, long long n) {
     constexpr int C = D / 4, ROWS = 256 / C;
     const long long r = (long long)blockIdx.x * ROWS + threadIdx.x / C;
+    const int i0 = chunk_of(a.seq, a.n_seq, a.seq[0].first + (int)((long long)blockIdx.x * ROWS / a.n_q));
     if (r >= n) return;
     const int token = a.seq[0].first + (int)(r / a.n_q), head = (int)(r % a.n_q), c = threadIdx.x % C;
-    int i = a.n_seq - 1;
-    while (a.seq[i].first > token) --i;
+    int i = i0;
+    while (i + 1 < a.n_seq && a.seq[i + 1].first <= token) ++i;
     const ChunkSeq sq = a.seq[i];
     const int t = token - sq.first;
     if (a.parts[i] == 1 || t >= sq.n) return;   // written already, or a row of another launch

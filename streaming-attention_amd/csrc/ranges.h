@@ -42,6 +42,14 @@ struct ChunkSeq {
     int32_t cache_row, len, n, first;
 };
 
+// The last of n (1 .. 64) chunks whose rows begin at or before row, for all lanes of a
+// wave alike; row is at or behind the first chunk's.
+__device__ __forceinline__ int chunk_of(const ChunkSeq* seqs, int n, int row) {
+    if (n == 1) return 0;
+    const int lane = threadIdx.x & (kWave - 1);
+    return __popcll(__ballot(lane < n && seqs[lane].first <= row)) - 1;
+}
+
 // Attention of chunks of new tokens: q and out [rows][n_q][D], fp32 or (q16) bf16.
 // extend_rows_ws: enough for any lengths of at most max_tokens.
 size_t extend_rows_ws(int n, const int32_t* counts, int n_q, int n_kv, int d, bool f32, long long max_tokens);

@@ -843,12 +843,15 @@ int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 // bf16, d = 64: 6.7 against 7.8 us in four chunks; 16 query rows of 512 tokens,
 // d = 128: a second, third and fourth tile per wave cost 0.8, 1.7 and 2.7 us, the
 // second launch 3.5), in fp32 two (a tile per wave costs 2.65 us).
-constexpr int kLongChunk = 32;
+// Tiles of an 8-bit cache are half as long: kLongChunk8 (64 rows of 512 - 32768 tokens:
+// 32 tiles 352 us, 48 343, 64 340), and so are the longest of chunks of new tokens (5 of each
+// of 64 sequences of 512 - 16384, bf16: 32 tiles 373 us, 64 368).
+constexpr int kLongChunk = 32, kLongChunk8 = 64;
 template <class F>
-int pick_tiles(long long round, long long work, const F& workgroups) {
-    for (int t = kWaves; t < kLongChunk; t += kWaves)
+int pick_tiles(long long round, long long work, const F& workgroups, int longest) {
+    for (int t = kWaves; t < longest; t += kWaves)
         if (work <= round * t && workgroups(t) <= round) return t;
-    return kLongChunk;
+    return longest;
 }
 
 }  // namespace
@@ -881,6 +884,7 @@ sa_status decode_ranges(const PagedView& c, const float* q, int n_q, const Range
     RangeArgs a{};
     set_cache(a, c, n_q, scale);
     const bool f32 = c.kv == SA_DTYPE_F32;
+    const int long_chunk = c.kv == SA_DTYPE_FP8 ? kLongChunk8 : kLongChunk;
     a.row_block = f32 ? Geo<128, kF32>::ROWS : Geo<128, kBf16>::ROWS;
     int g = 0, done = 0;   // the group of the launch's first row, and its rows already attended
     for (int i0 = 0; i0 < plan.n_rows; i0 += kRowsPerLaunch) {
@@ -924,7 +928,7 @@ sa_status decode_ranges(const PagedView& c, const float* q, int n_q, const Range
                 return n;
             };
             int chunk = whole && longest <= (f32 ? 2 : 4) * kWaves ? std::max(1, longest)
-                                                                      : pick_tiles(round, work, workgroups);
+                                                                      : pick_tiles(round, work, workgroups, long_chunk);
             if (attn_kv_block() > 0) chunk = attn_kv_block() / kTile;
             chunk = std::min(std::max(chunk, ceil_div(longest, kMaxChunks)), kChunkTiles);
             return std::pair<int, long long>(chunk, workgroups(chunk));
@@ -1034,17 +1038,22 @@ __global__ void __launch_bounds__(kThreads) chunk_attn_kernel(ChunkArgs a) {
     attend_item<D, KV, T, true>(a, it, (lds_u8_t*)smem_raw, pages, ml);
 }
 
-// Joins the partials of new token blockIdx.x / n_q, head blockIdx.x % n_q.
+// Joins the partials of (token, head) rows from the launch's first token on, D / 4
+// lanes each.
 template <int D, class T>
-__global__ void __launch_bounds__(D / 4) chunk_merge_kernel(ChunkArgs a) {
-    const int head = blockIdx.x % a.n_q, row = a.seq[0].first + blockIdx.x / a.n_q;
-    int i = a.n_seq - 1;
-    while (a.seq[i].first > row) --i;
+__global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs a, long long rows) {
+    constexpr int C = D / 4;
+    const long long at_row = (long long)blockIdx.x * (256 / C) + threadIdx.x / C;
+    const int i0 = chunk_of(a.seq, a.n_seq, a.seq[0].first + (int)((long long)blockIdx.x * (256 / C) / a.n_q));
+    if (at_row >= rows) return;
+    const int head = (int)(at_row % a.n_q), row = a.seq[0].first + (int)(at_row / a.n_q);
+    int i = i0;
+    while (i + 1 < a.n_seq && a.seq[i + 1].first <= row) ++i;
     const ChunkSeq sq = a.seq[i];
     const int t = row - sq.first;
     if (a.chunks[i] == 1 || t >= sq.n) return;   // written already, or a row of another launch
     const int n = (block_tiles(sq, t / a.block, a.block) + a.tiles - 1) / a.tiles;
-    const int kvh = head / a.rep, c = threadIdx.x;
+    const int kvh = head / a.rep, c = threadIdx.x % C;
     float M = -INFINITY, L = 0.f;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
@@ -1070,7 +1079,9 @@ sa_status launch_chunks(const ChunkArgs& a, int rows, bool merge, hipStream_t st
     hipLaunchKernelGGL(kernel, dim3((unsigned)a.start[a.n_seq] * a.n_kv), dim3(kThreads), lds, st, a);
     SA_CHECK_LAUNCH();
     if (merge) {
-        hipLaunchKernelGGL((chunk_merge_kernel<D, T>), dim3((unsigned)rows * a.n_q), dim3(D / 4), 0, st, a);
+        const long long n = (long long)rows * a.n_q;
+        constexpr int per = 256 / (D / 4);
+        hipLaunchKernelGGL((chunk_merge_kernel<D, T>), dim3((unsigned)((n + per - 1) / per)), dim3(256), 0, st, a, n);
         SA_CHECK_LAUNCH();
     }
     return SA_OK;
@@ -1152,7 +1163,7 @@ sa_status extend_rows(const PagedView& c, const void* q, bool q16, int n_q, cons
         const long long round = chunk_round(f32);
         int tiles = longest <= (f32 ? 2 : 4) * kWaves
                         ? longest
-                        : std::max<int>(pick_tiles(round, work, [&](int t) { return items(t) * a.n_kv; }),
+                        : std::max<int>(pick_tiles(round, work, [&](int t) { return items(t) * a.n_kv; }, kLongChunk8),
                                         (int)std::min<long long>(longest, work / (kChunkRounds * round)));
         // no more partials than extend_rows_ws counts on
         while (tiles < longest && items(tiles) * a.n_kv > kChunkRounds * round) tiles += kWaves;
