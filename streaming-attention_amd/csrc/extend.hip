@@ -88,7 +88,8 @@ __device__ __forceinline__ bool place(const BlockArgs& a, Block& w) {
     }
     w.kvh = blockIdx.x % a.n_kv;
     const int all = w.sq.n * a.rep;
-    const int b = (all + a.rows - 1) / a.rows - 1 - local / parts, c = local % parts;   // the longest first
+    // the longest blocks first
+    const int blocks = (all + a.rows - 1) / a.rows, b = blocks - 1 - local / parts, c = local % parts;
     w.r0 = b * a.rows;
     w.row_end = min(all, w.r0 + a.rows);
     w.u0 = c * a.tiles;
@@ -641,7 +642,24 @@ constexpr int kMaxRounds = 4;    // of workgroups that a launch's tiles are cut 
 // What a workgroup costs besides its tiles, in tiles: its beginning and its output, or
 // where a block is cut a partial written and read again.
 constexpr int kWholeTiles = 2, kCutBf16 = 6, kCutF32 = 4, kCutTerms = 7;
-constexpr double kFourWaves = 0.6;   // a tile of a workgroup of four waves alone on its CU
+
+// Workgroups of a kind that share a CU (by registers, and for fp32 caches by LDS: 96 KiB
+// at D = 128, 48 at 64), and what a tile of one takes of a full CU's time, in those of
+// eight waves (measured, 2048 tokens behind 8192, 16 / 8 heads, us in workgroups of eight
+// and four waves: bf16, D = 128 188 / 333, 64 119 / 174; fp32 cache 803 / 1178, 410 / 469; fp32
+// over a bf16 cache 413 / 402, 273 / 218, so in four waves always), and where no CU has
+// more than one.
+struct Kind {
+    int per_cu;
+    double tile, alone;
+};
+Kind kind_of(bool q16, sa_dtype kv, int d, int waves) {
+    if (q16 && d == 64) return waves == 8 ? Kind{2, 1.0, 1.2} : Kind{2, 0.72, 0.86};
+    if (q16) return waves == 8 ? Kind{1, 1.0, 1.0} : Kind{1, 0.88, 0.6};
+    if (kv != SA_DTYPE_F32) return d == 64 ? Kind{3, 0.5, 0.9} : Kind{2, 0.5, 0.6};
+    if (d == 64) return waves == 8 ? Kind{2, 1.0, 1.2} : Kind{3, 0.57, 1.0};
+    return waves == 8 ? Kind{1, 1.0, 1.0} : Kind{1, 0.73, 0.73};
+}
 
 template <auto KERNEL>
 sa_status launch_blocks(const BlockArgs& a, int waves, int lds, hipStream_t st) {
@@ -653,8 +671,9 @@ sa_status launch_blocks(const BlockArgs& a, int waves, int lds, hipStream_t st) 
 template <int D, int KV>
 sa_status launch_f32(const BlockArgs& a, int waves, hipStream_t st) {
     constexpr int lds = 2 * TermGeo<D, KV>::STAGE;
-    return waves == 8 ? launch_blocks<extend_f32_kernel<D, 8, KV>>(a, 8, lds, st)
-                      : launch_blocks<extend_f32_kernel<D, 4, KV>>(a, 4, lds, st);
+    if constexpr (KV == SA_DTYPE_F32)
+        if (waves == 8) return launch_blocks<extend_f32_kernel<D, 8, KV>>(a, 8, lds, st);
+    return launch_blocks<extend_f32_kernel<D, 4, KV>>(a, 4, lds, st);
 }
 template <int D, bool FP8>
 sa_status launch_bf16(const BlockArgs& a, int waves, hipStream_t st) {
@@ -747,34 +766,51 @@ sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, co
             for (int i = 0; i < a.n_seq; ++i) k += blocks_of((long long)a.seq[i].n * a.rep, a.rows) * parts_of(i, tiles);
             return k * a.n_kv;
         };
-        // Eight or four waves, and the tiles that give no more than 1 .. kMaxRounds times as
-        // many workgroups as there are CUs, or all: what is estimated cheapest, in tiles of a
-        // workgroup of eight waves.
+        // Eight or four waves, and the tiles of a workgroup: what is estimated cheapest, in
+        // tiles of a workgroup of eight waves on a CU of its own.
         const long long cus = device_cu_count();
         const int cut = q16 ? kCutBf16 : c.kv == SA_DTYPE_F32 ? kCutF32 : kCutTerms;
-        const bool pairs = q16 && c.d == 64;   // two workgroups of eight waves per CU
+        const bool terms = !q16 && c.kv != SA_DTYPE_F32;   // in four waves always
         int waves = 8;
         double best = INFINITY;
         for (int w = 8; w >= 4; w -= 4) {
-            if (w == 8 && most <= 4 * per_wave) continue;
+            if (w == 8 && (most <= 4 * per_wave || terms)) continue;
             a.rows = w * per_wave;
             longest = 1;
-            for (int i = 0; i < a.n_seq; ++i) longest = std::max(longest, last_tiles(i));
-            for (int k = 0; k <= kMaxRounds; ++k) {
-                int lo = longest;
-                if (k) {
-                    if (workgroups(longest) > k * cus) continue;
-                    lo = 1;
-                    for (int hi = longest; lo < hi;) {   // workgroups(tiles) falls
-                        const int mid = (lo + hi) / 2;
-                        if (workgroups(mid) <= k * cus) hi = mid;
-                        else lo = mid + 1;
-                    }
+            const Kind kind = kind_of(q16, c.kv, c.d, w);
+            // a sequence's blocks by four of them
+            struct Some { double blocks; int tiles; } some[4 * kRowsPerLaunch];
+            int n_some = 0;
+            double work = 0.0;
+            for (int i = 0; i < a.n_seq; ++i) {
+                longest = std::max(longest, last_tiles(i));
+                const int blocks = (int)blocks_of((long long)a.seq[i].n * a.rep, a.rows), k = std::min(blocks, 4);
+                for (int j = 0; j < k; ++j) {
+                    const int b = (int)((2LL * j + 1) * blocks / (2 * k));
+                    some[n_some] = {(double)blocks / k * a.n_kv, block_key_tiles(a.seq[i], b, a.rows, a.rep, a.tile)};
+                    work += some[n_some].blocks * some[n_some].tiles;
+                    ++n_some;
                 }
-                const long long wgs = workgroups(lo), slots = w == 4 || pairs ? 2 * cus : cus;
-                const double speed = wgs > cus ? (w == 8 && pairs ? 2.0 : 1.0) : w == 8 ? 1.0 : kFourWaves;
-                const double cost = (double)((wgs + slots - 1) / slots) * (lo + (lo < longest ? cut : kWholeTiles)) * speed;
-                if (cost < best) best = cost, waves = w, a.tiles = lo;
+            }
+            for (int p = 1, t = 0; p <= longest; ++p) {
+                if (t == (longest + p - 1) / p) continue;
+                t = (longest + p - 1) / p;
+                const double wgs = (double)workgroups(t), slots = (double)(kind.per_cu * cus);
+                if (p > 1 && wgs > kMaxRounds * cus) break;
+                // Parts of more than half of t in rounds (no two in one's time), or all of the work
+                // evenly, whichever is longer.
+                double big = 0.0, big_tiles = 0.0;
+                for (int j = 0; j < n_some; ++j) {
+                    const int whole = some[j].tiles / t, rest = some[j].tiles % t;
+                    const bool more = 2 * rest > t;
+                    big += some[j].blocks * (whole + more);
+                    big_tiles += some[j].blocks * ((double)whole * t + (more ? rest : 0));
+                }
+                const double rounds = big > 0.0 ? std::ceil(big / slots) * (big_tiles / big) : 0.0;
+                const double tile = wgs > cus ? kind.per_cu * kind.tile : kind.alone;
+                const double cost = (std::max({rounds, work / slots, (double)t}) +
+                                     (p > 1 ? cut : kWholeTiles) * std::max(1.0, wgs / slots)) * tile;
+                if (cost < best) best = cost, waves = w, a.tiles = t;
             }
         }
         a.rows = waves * per_wave;
