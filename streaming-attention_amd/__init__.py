@@ -542,8 +542,9 @@ class KVCache:
 
     def gather(self, layer: int, seq: int, length: int, stream=None):
         import torch
-        k, v = _alloc(stream, lambda: torch.empty((2, self.desc.num_kv_heads, length, self.desc.head_dim),
-                                                  dtype=torch.float32, device="cuda").unbind())
+        H, D = self.desc.num_kv_heads, self.desc.head_dim
+        k = _alloc(stream, lambda: torch.empty(H, length, D, dtype=torch.float32, device="cuda"))
+        v = _alloc(stream, lambda: torch.empty_like(k))
         check(lib().sa_kvcache_gather(self.handle, layer, seq, length, k.data_ptr(), v.data_ptr(), _stream(stream)))
         return k, v
 
