@@ -131,15 +131,20 @@ struct BfWave {
         l += sum;
     }
 
-    // 32 keys whose K rows are at hb.  MASK: hide(s) scales the scores by c (first: -inf
-    // times a factor of 0 would be NaN) and makes those that are not seen -inf; element
-    // j is key 16 (j / 8) + 8 hh + j % 8.
-    template <bool MASK, class Hide>
-    __device__ __forceinline__ void half(uint32_t hb, const Hide& hide) {
+    // The scores of 32 keys whose K rows are at hb: element j is key 16 (j / 8) + 8 hh + j % 8.
+    __device__ __forceinline__ f32x16_t scores(uint32_t hb) const {
         f32x16_t s = {};
 #pragma unroll
         for (int ks = 0; ks < G::NKS; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k_frag(hb, ks), qf[ks], s, 0, 0, 0);
-        if constexpr (MASK) hide(s);
+        return s;
+    }
+
+    // The values of those keys by the scores' weights.  MASK: the caller has scaled the
+    // scores by c (first: -inf times a factor of 0 would be NaN) and made those that are
+    // not seen -inf.  Masks are the callers' own code between the two calls: as a
+    // function passed in here they cost the windowed prefill 15 registers and 2 % of its time.
+    template <bool MASK>
+    __device__ __forceinline__ void weigh(f32x16_t& s, uint32_t hb) {
         bf16x8_t pb[2];
         softmax<MASK>(s, pb);
 #pragma unroll
@@ -150,10 +155,10 @@ struct BfWave {
     }
 
     // O / l: every lane's columns into the wave's part of LDS (chunks of a row
-    // permuted as the tiles' are), then rows of 16-byte pieces to memory, row r < rows
-    // to dst(r).  Returns the rows, a bit each, that are not finite and not written.
+    // permuted as the tiles' are), then rows of 16-byte pieces to memory, row q0 + r < L
+    // to dst(q0 + r).  Returns the rows r, a bit each, that are not finite and not written.
     template <class Dst>
-    __device__ __forceinline__ uint32_t store(int rows, const Dst& dst, lds_u8_t* buf, int lane) const {
+    __device__ __forceinline__ uint32_t store(int L, const Dst& dst, lds_u8_t* buf, int lane) const {
         const float inv = 1.0f / (l + xor32(l));
         const bf16x2_t one = {(__bf16)1.0f, (__bf16)1.0f};
         float sum[4] = {};   // of the outputs: finite where they are
@@ -170,7 +175,7 @@ struct BfWave {
                     buf + n * G::ROWB + (((4 * db + jj) ^ G::swz(n & 15)) << 4) + 8 * hh) =
                     (uint64_t)__builtin_bit_cast(uint32_t, by) << 32 | __builtin_bit_cast(uint32_t, bx);
             }
-        const uint64_t bad = __ballot(n < rows && !(fabsf((sum[0] + sum[1]) + (sum[2] + sum[3])) < INFINITY));
+        const uint64_t bad = __ballot(q0 + n < L && !(fabsf((sum[0] + sum[1]) + (sum[2] + sum[3])) < INFINITY));
         const uint32_t anew = (uint32_t)bad | (uint32_t)(bad >> 32);
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // a wave's own part: no barrier
 #pragma unroll
@@ -178,7 +183,7 @@ struct BfWave {
             const int r = i * G::RPL + lane / G::CPR, ch = lane % G::CPR;
             const u32x4_t v = *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t*>(
                 buf + r * G::ROWB + ((ch ^ G::swz(r & 15)) << 4));
-            if (r < rows && !(anew >> r & 1)) *reinterpret_cast<u32x4_t*>(dst(r) + 8 * ch) = v;
+            if (q0 + r < L && !(anew >> r & 1)) *reinterpret_cast<u32x4_t*>(dst(q0 + r) + 8 * ch) = v;
         }
         return anew;
     }

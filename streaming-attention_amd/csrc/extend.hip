@@ -274,13 +274,20 @@ __global__ void __launch_bounds__(W * kWave, W == 8 && D == 64 ? 4 : 1) extend_b
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
                 const int k = u * kBfTile + 32 * kb;
-                if (k + 31 <= q_lo) w.template half<false>(sb + kb * 32 * G::ROWB, [](f32x16_t&) {});
-                else if (k <= q_hi)
-                    w.template half<true>(sb + kb * 32 * G::ROWB, [&](f32x16_t& s) {
-                        const int last = q_mine - k - 8 * w.hh;
+                const uint32_t hb = sb + kb * 32 * G::ROWB;
+                if (k > q_hi) continue;
+                // Eight waves come here only with the tiles at the diagonal: one form, with
+                // the mask, is enough, and without the other its registers spill no more
+                // (2048 tokens behind none 71 -> 45 us).
+                f32x16_t s = w.scores(hb);
+                if (W == 4 && k + 31 <= q_lo) {
+                    w.template weigh<false>(s, hb);
+                } else {
+                    const int last = q_mine - k - 8 * w.hh;
 #pragma unroll
-                        for (int j = 0; j < 16; ++j) s[j] = 16 * (j / 8) + j % 8 > last ? -INFINITY : s[j] * w.c;
-                    });
+                    for (int j = 0; j < 16; ++j) s[j] = 16 * (j / 8) + j % 8 > last ? -INFINITY : s[j] * w.c;
+                    w.template weigh<true>(s, hb);
+                }
             }
         }
         end_tile(u);
@@ -344,7 +351,7 @@ __global__ void __launch_bounds__(W * kWave, W == 8 && D == 64 ? 4 : 1) extend_b
     uint32_t anew;
     if (b.whole) {
         // The output through LDS, 32 rows per wave, so that stores are whole rows.
-        anew = w.store(rows, [&](int r) { return static_cast<uint16_t*>(a.out) + out_row(a, b, w0 + r) * D; },
+        anew = w.store(b.row_end, [&](int r) { return static_cast<uint16_t*>(a.out) + out_row(a, b, r) * D; },
                        smem + wave * 32 * G::ROWB, lane);
     } else {
         const float l = w.l + xor32(w.l);

@@ -202,8 +202,16 @@ __global__ void __launch_bounds__(W * kWave, W == 8 && D == 64 ? 4 : 1) window_b
             for (int kb = 0; kb < 2; ++kb) {
                 const int k = k0 + 32 * kb;
                 const Seen sn = seen(a, w.q0, q1, k, k + 31);
-                if (sn == kAll) w.template half<false>(sb + kb * 32 * G::ROWB, [](f32x16_t&) {});
-                else if (sn == kSome) w.template half<true>(sb + kb * 32 * G::ROWB, [&](f32x16_t& x) { hide<D>(a, w, k, q1, x); });
+                const uint32_t hb = sb + kb * 32 * G::ROWB;
+                // Both branches with scores of their own: shared, they cost 20 registers.
+                if (sn == kAll) {
+                    f32x16_t s = w.scores(hb);
+                    w.template weigh<false>(s, hb);
+                } else if (sn == kSome) {
+                    f32x16_t s = w.scores(hb);
+                    hide<D>(a, w, k, q1, s);
+                    w.template weigh<true>(s, hb);
+                }
             }
         }
         end_tile(it);
@@ -268,7 +276,7 @@ __global__ void __launch_bounds__(W * kWave, W == 8 && D == 64 ? 4 : 1) window_b
     for (; it < tiles.n; ++it) edge_tile(it);
     // The output through LDS, 32 rows per wave, so that stores are whole rows.
     uint16_t* const head = static_cast<uint16_t*>(a.dst) + wk.b * a.os[0] + h * a.os[1];
-    uint32_t anew = w.store(a.L - w.q0, [&](int r) { return head + (w.q0 + r) * a.os[2]; }, smem + wave * 32 * G::ROWB, lane);
+    uint32_t anew = w.store(a.L, [&](int q) { return head + q * a.os[2]; }, smem + wave * 32 * G::ROWB, lane);
     for (; anew; anew &= anew - 1)
         window_plain<D, uint16_t>(wave / wph, w.q0 + __builtin_ctz(anew));
 }
