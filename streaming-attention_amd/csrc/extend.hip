@@ -653,7 +653,7 @@ constexpr int kWholeTiles = 2, kCutBf16 = 6, kCutF32 = 4, kCutTerms = 7;
 // Workgroups of a kind that share a CU (by registers, and for fp32 caches by LDS: 96 KiB
 // at D = 128, 48 at 64), and what a tile of one takes of a full CU's time, in those of
 // eight waves (measured, 2048 tokens behind 8192, 16 / 8 heads, us in workgroups of eight
-// and four waves: bf16, D = 128 188 / 333, 64 119 / 174; fp32 cache 803 / 1178, 410 / 469; fp32
+// and four waves: bf16, D = 128 169 / 276, 64 100 / 132; fp32 cache 803 / 1178, 410 / 469; fp32
 // over a bf16 cache 413 / 402, 273 / 218, so in four waves always), and where no CU has
 // more than one.
 struct Kind {
@@ -661,8 +661,8 @@ struct Kind {
     double tile, alone;
 };
 Kind kind_of(bool q16, sa_dtype kv, int d, int waves) {
-    if (q16 && d == 64) return waves == 8 ? Kind{2, 1.0, 1.2} : Kind{2, 0.72, 0.86};
-    if (q16) return waves == 8 ? Kind{1, 1.0, 1.0} : Kind{1, 0.88, 0.6};
+    if (q16 && d == 64) return waves == 8 ? Kind{2, 1.0, 1.2} : Kind{2, 0.66, 0.78};
+    if (q16) return waves == 8 ? Kind{1, 1.0, 1.0} : Kind{2, 0.82, 0.7};
     if (kv != SA_DTYPE_F32) return d == 64 ? Kind{3, 0.5, 0.9} : Kind{2, 0.5, 0.6};
     if (d == 64) return waves == 8 ? Kind{2, 1.0, 1.2} : Kind{3, 0.57, 1.0};
     return waves == 8 ? Kind{1, 1.0, 1.0} : Kind{1, 0.73, 0.73};
