@@ -612,10 +612,10 @@ __device__ __forceinline__ void put4(uint16_t* p, f32x4_t v) {
 // O = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c, D / 4 lanes per row of 256 D / 4
 // consecutive (token, head) rows from the launch's first token on.
 template <int D, class T>
-__global__ void __launch_bounds__(256) block_merge_kernel(BlockArgs a, long long n) {
+__global__ void __launch_bounds__(256) block_merge_kernel(BlockArgs a, long long row0, long long n) {
     constexpr int C = D / 4, ROWS = 256 / C;
-    const long long r = (long long)blockIdx.x * ROWS + threadIdx.x / C;
-    const int i0 = chunk_of(a.seq, a.n_seq, a.seq[0].first + (int)((long long)blockIdx.x * ROWS / a.n_q));
+    const long long first = row0 + (long long)blockIdx.x * ROWS, r = first + threadIdx.x / C;
+    const int i0 = chunk_of(a.seq, a.n_seq, a.seq[0].first + (int)(first / a.n_q));
     if (r >= n) return;
     const int token = a.seq[0].first + (int)(r / a.n_q), head = (int)(r % a.n_q), c = threadIdx.x % C;
     int i = i0;
@@ -696,12 +696,10 @@ sa_status dispatch_blocks(const BlockArgs& a, sa_dtype kv, bool q16, int waves, 
                 : kv == SA_DTYPE_BF16 ? (launch_f32<D, SA_DTYPE_BF16>(a, waves, st))
                                       : (launch_f32<D, SA_DTYPE_FP8>(a, waves, st)));
     if (!merge) return SA_OK;
-    const int per = 256 / (D / 4);
-    const dim3 grid((unsigned)((rows + per - 1) / per));
-    if (q16) hipLaunchKernelGGL((block_merge_kernel<D, uint16_t>), grid, dim3(256), 0, st, a, rows);
-    else hipLaunchKernelGGL((block_merge_kernel<D, float>), grid, dim3(256), 0, st, a, rows);
-    SA_CHECK_LAUNCH();
-    return SA_OK;
+    return merge_rows<D>(rows, [&](dim3 grid, long long row0) {
+        if (q16) hipLaunchKernelGGL((block_merge_kernel<D, uint16_t>), grid, dim3(256), 0, st, a, row0, rows);
+        else hipLaunchKernelGGL((block_merge_kernel<D, float>), grid, dim3(256), 0, st, a, row0, rows);
+    });
 }
 
 long long blocks_of(long long rows, int block) { return (rows + block - 1) / block; }
@@ -732,15 +730,10 @@ void split_chunks(sa_dtype kv, int rep, int n_kv, const ChunkSeq* seqs, int n, s
 size_t extend_blocks_ws(int n, const int32_t* counts, int n_q, int n_kv, int d, long long max_tokens) {
     const long long tiles = (max_tokens + kTermTile - 1) / kTermTile;
     if (tiles <= 1) return 0;
-    const long long round = device_cu_count();
-    size_t need = 0;
-    for (int i0 = 0; i0 < n; i0 += kRowsPerLaunch) {
-        long long rows = 0;
-        for (int i = i0; i < std::min(n, i0 + kRowsPerLaunch); ++i) rows += (long long)counts[i] * n_q;
-        // at most as many workgroups as extend_blocks cuts into
-        need = std::max(need, (size_t)std::min(rows * tiles, kMaxRounds * round * 256) * (d + 2) * sizeof(float));
-    }
-    return need;
+    long long rows = 0;
+    for (int i = 0; i < n; ++i) rows += (long long)counts[i] * n_q;
+    // at most as many workgroups as extend_blocks cuts into
+    return (size_t)std::min(rows * tiles, kMaxRounds * device_cu_count() * 256LL) * (d + 2) * sizeof(float);
 }
 
 sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, const ChunkSeq* seqs, int n, float scale,
@@ -832,7 +825,7 @@ sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, co
         a.start[a.n_seq] = (int)at;
         const long long tokens = a.seq[a.n_seq - 1].first + a.seq[a.n_seq - 1].n - a.seq[0].first;
         // a grid has fewer than 2^32 threads
-        if (at * a.n_kv >= (1LL << 32) / (waves * kWave) || parts > 0x7fffffffLL || tokens * n_q >= (1LL << 32) / 64)
+        if (at * a.n_kv >= (1LL << 32) / (waves * kWave) || parts > 0x7fffffffLL)
             return fail(SA_EINVAL, "too many tokens for one call");
         if (parts) {
             const size_t need = (size_t)parts * a.n_kv * (c.d + 2) * sizeof(float);

@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <functional>
 #include <initializer_list>
 #include <new>
 #include <vector>
@@ -1207,7 +1208,14 @@ extern "C" size_t sa_paged_extend_ws_bytes(const sa_kvcache* c, int n_seq, const
         if (counts[i] < 0) return 0;
     const long long tokens = (long long)c->desc.max_pages_per_seq * SA_PAGE_TOKENS;
     const bool f32 = c->desc.kv_dtype == SA_DTYPE_F32;
-    // whichever way the sequences go
+    // Whichever way the sequences go: a launch of either takes up to kRowsPerLaunch of
+    // them, which need no more than the largest.
+    int32_t most[kRowsPerLaunch];
+    if (n_seq > kRowsPerLaunch) {
+        std::partial_sort_copy(counts, counts + n_seq, most, most + kRowsPerLaunch, std::greater<int32_t>());
+        counts = most;
+        n_seq = kRowsPerLaunch;
+    }
     return std::max(extend_rows_ws(n_seq, counts, n_q_heads, c->desc.num_kv_heads, c->desc.head_dim, f32, tokens),
                     extend_blocks_ws(n_seq, counts, n_q_heads, c->desc.num_kv_heads, c->desc.head_dim, tokens));
 }

@@ -2,6 +2,7 @@
 // windowed decode and the decode of sequences that share their leading pages.
 #pragma once
 
+#include <algorithm>
 #include <vector>
 
 #include "sa_internal.h"
@@ -50,8 +51,21 @@ __device__ __forceinline__ int chunk_of(const ChunkSeq* seqs, int n, int row) {
     return __popcll(__ballot(lane < n && seqs[lane].first <= row)) - 1;
 }
 
+// Launches launch(grid, first row) over the partials of rows query rows, 256 / (D / 4) of them
+// per workgroup of 256; a grid has fewer than 2^32 threads.
+template <int D, class Launch>
+sa_status merge_rows(long long rows, const Launch& launch) {
+    constexpr long long per = 256 / (D / 4), most = per << 23;
+    for (long long row = 0; row < rows; row += most) {
+        launch(dim3((unsigned)((std::min(most, rows - row) + per - 1) / per)), row);
+        SA_CHECK_LAUNCH();
+    }
+    return SA_OK;
+}
+
 // Attention of chunks of new tokens: q and out [rows][n_q][D], fp32 or (q16) bf16.
-// extend_rows_ws: enough for any lengths of at most max_tokens.
+// extend_rows_ws: for n <= kRowsPerLaunch of them, enough for any lengths of at most
+// max_tokens.
 size_t extend_rows_ws(int n, const int32_t* counts, int n_q, int n_kv, int d, bool f32, long long max_tokens);
 sa_status extend_rows(const PagedView& c, const void* q, bool q16, int n_q, const ChunkSeq* seqs, int n, float scale,
                       void* out, void* ws, size_t ws_bytes, hipStream_t st);

@@ -1041,10 +1041,10 @@ __global__ void __launch_bounds__(kThreads) chunk_attn_kernel(ChunkArgs a) {
 // Joins the partials of (token, head) rows from the launch's first token on, D / 4
 // lanes each.
 template <int D, class T>
-__global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs a, long long rows) {
+__global__ void __launch_bounds__(256) chunk_merge_kernel(ChunkArgs a, long long row0, long long rows) {
     constexpr int C = D / 4;
-    const long long at_row = (long long)blockIdx.x * (256 / C) + threadIdx.x / C;
-    const int i0 = chunk_of(a.seq, a.n_seq, a.seq[0].first + (int)((long long)blockIdx.x * (256 / C) / a.n_q));
+    const long long first = row0 + (long long)blockIdx.x * (256 / C), at_row = first + threadIdx.x / C;
+    const int i0 = chunk_of(a.seq, a.n_seq, a.seq[0].first + (int)(first / a.n_q));
     if (at_row >= rows) return;
     const int head = (int)(at_row % a.n_q), row = a.seq[0].first + (int)(at_row / a.n_q);
     int i = i0;
@@ -1078,13 +1078,11 @@ sa_status launch_chunks(const ChunkArgs& a, int rows, bool merge, hipStream_t st
     SA_TRY(pf::opt_in_lds<kernel>(lds));
     hipLaunchKernelGGL(kernel, dim3((unsigned)a.start[a.n_seq] * a.n_kv), dim3(kThreads), lds, st, a);
     SA_CHECK_LAUNCH();
-    if (merge) {
-        const long long n = (long long)rows * a.n_q;
-        constexpr int per = 256 / (D / 4);
-        hipLaunchKernelGGL((chunk_merge_kernel<D, T>), dim3((unsigned)((n + per - 1) / per)), dim3(256), 0, st, a, n);
-        SA_CHECK_LAUNCH();
-    }
-    return SA_OK;
+    if (!merge) return SA_OK;
+    const long long n = (long long)rows * a.n_q;
+    return merge_rows<D>(n, [&](dim3 grid, long long row0) {
+        hipLaunchKernelGGL((chunk_merge_kernel<D, T>), grid, dim3(256), 0, st, a, row0, n);
+    });
 }
 
 template <int D>
@@ -1115,21 +1113,17 @@ size_t extend_rows_ws(int n, const int32_t* counts, int n_q, int n_kv, int d, bo
     const long long tiles = (max_tokens + kTile - 1) / kTile;
     const long long most = std::min<long long>(tiles, std::max<long long>(kMaxChunks, ceil_div(tiles, kChunkTiles)));
     if (most <= 1) return 0;
-    size_t need = 0;
-    for (int i0 = 0; i0 < n; i0 += kRowsPerLaunch) {
-        long long rows = 0, blocks = 0, widest = 0;
-        for (int i = i0; i < std::min(n, i0 + kRowsPerLaunch); ++i) {
-            rows += (long long)counts[i] * n_q;
-            blocks += ceil_div(counts[i], block);
-            widest = std::max<long long>(widest, std::min(counts[i], block) * rep);
-        }
-        // By chunks of a sequence, and by workgroups of the launch.
-        const long long by_chunks = rows * most;
-        const long long forced = tiles > kChunkTiles ? blocks * n_kv * ceil_div(tiles, kChunkTiles) : 0;
-        const long long by_groups = std::max(kChunkRounds * chunk_round(f32), forced) * widest;
-        need = std::max(need, (size_t)std::max(rows, std::min(by_chunks, by_groups)) * (d + 2) * sizeof(float));
+    long long rows = 0, blocks = 0, widest = 0;
+    for (int i = 0; i < n; ++i) {
+        rows += (long long)counts[i] * n_q;
+        blocks += ceil_div(counts[i], block);
+        widest = std::max<long long>(widest, std::min(counts[i], block) * rep);
     }
-    return need;
+    // By chunks of a sequence, and by workgroups of the launch.
+    const long long by_chunks = rows * most;
+    const long long forced = tiles > kChunkTiles ? blocks * n_kv * ceil_div(tiles, kChunkTiles) : 0;
+    const long long by_groups = std::max(kChunkRounds * chunk_round(f32), forced) * widest;
+    return (size_t)std::max(rows, std::min(by_chunks, by_groups)) * (d + 2) * sizeof(float);
 }
 
 sa_status extend_rows(const PagedView& c, const void* q, bool q16, int n_q, const ChunkSeq* seqs, int n, float scale,
@@ -1185,7 +1179,7 @@ sa_status extend_rows(const PagedView& c, const void* q, bool q16, int n_q, cons
         a.start[a.n_seq] = (int)at;
         const int rows = a.seq[a.n_seq - 1].first + a.seq[a.n_seq - 1].n - a.seq[0].first;
         // a grid has fewer than 2^32 threads
-        if (at * a.n_kv >= (1LL << 32) / kThreads || (long long)rows * n_q >= (1LL << 32) / 64)
+        if (at * a.n_kv >= (1LL << 32) / kThreads)
             return fail(SA_EINVAL, "too many tokens for one call");
         if (merge) {
             const size_t need = (size_t)parts * a.n_kv * (c.d + 2) * sizeof(float);
