@@ -976,6 +976,8 @@ class Qwen3:
         max_batch; a generation that positions or a row's pages have no room for is refused
         (ValueError) before it begins.  The caches hold the sequences afterwards: reset them."""
         import torch
+        if prompts.dtype != torch.int32 or not prompts.is_cuda or prompts.dim() != 2:
+            raise ValueError("prompts must be an int32 CUDA tensor [G, L]")
         G, L = prompts.shape
         if n_tokens < 1 or not 0 <= n_draft <= 64:
             raise ValueError("speculative takes at least one token and 0 to 64 drafts")
@@ -983,6 +985,8 @@ class Qwen3:
             raise ValueError("temperature must be >= 0 and finite")
         if draft is not None and (draft_cache is None or draft.desc.vocab != self.desc.vocab):
             raise ValueError("a draft model takes a cache and this model's vocabulary")
+        if draft is not None and draft_cache is cache:
+            raise ValueError("the draft model takes a cache of its own")
         for m, c in ((self, cache), (draft, draft_cache)):
             if m is None:
                 continue

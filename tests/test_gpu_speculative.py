@@ -249,3 +249,15 @@ def test_refusals(sa):
     fork2.set_lens([0, 1], [10, 10])          # back into a shared page
     with pytest.raises(sa.SaError, match="shares"):
         model.extend(fork2, x[:2].contiguous(), [1, 1])
+
+
+def test_speculative_refuses_one_cache_for_both_models(sa):
+    model = make_model(sa, 4, 100)
+    cache = make_cache(sa, "f32", 2, 64)
+    p = tokens_of(8, 1).view(2, 4).contiguous()
+    with pytest.raises(ValueError, match="of its own"):
+        model.speculative(cache, p, 5, draft=model, draft_cache=cache, n_draft=1)
+    for bad in (p.long(), p[0], p.cpu()):
+        with pytest.raises(ValueError, match="prompts"):
+            model.speculative(cache, bad, 5, n_draft=1)
+    assert [cache.length(r) for r in range(2)] == [0, 0]
