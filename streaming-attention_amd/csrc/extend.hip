@@ -18,6 +18,13 @@
 // product), of one by three all; v_mfma_f32_16x16x32_bf16, a wave owns 16 rows,
 // tiles of 32 keys become terms on their way into LDS.
 //
+// Whole blocks, or blocks cut into parts of equal lengths, keep the CUs evenly busy where they
+// make many rounds or fit them; for fp32 queries there is a third way, all blocks'
+// tiles in a row cut into as many equal lengths as workgroups run at a time, each
+// going from block to block (700 fp32 tokens behind 4000, 16 / 8 heads of 128: 200 -> 137
+// us).  bf16 queries gain nothing by it: what a further block costs to begin, 8 us with
+// eight waves, is more than they lose by rounds.
+//
 // Rows whose sums are not finite are computed anew over what they see (plain_row.h).
 #include <algorithm>
 #include <cmath>
@@ -30,6 +37,8 @@
 
 namespace sa {
 namespace {
+
+constexpr int kEvenBlocks = 128;
 
 struct BlockArgs {
     const void* q;
@@ -51,8 +60,16 @@ struct BlockArgs {
     uint32_t q_sign;                         // 0x80008000 for a negative scale
     ChunkSeq seq[kRowsPerLaunch];
     int32_t start[kRowsPerLaunch + 1];       // a sequence's first item, of blocks x parts
-    int32_t base[kRowsPerLaunch];            // its first partial row
-    int32_t parts[kRowsPerLaunch];           // of its last block
+    // Tiles cut evenly: even > 0 tiles per workgroup of the blocks' tiles in a row,
+    // block_at[k] before block k; start[i] is then sequence i's first block.
+    int even, n_blocks;
+    union {
+        struct {
+            int32_t base[kRowsPerLaunch];    // its first partial row
+            int32_t parts[kRowsPerLaunch];   // of its last block
+        };
+        int32_t block_at[kEvenBlocks + 1];
+    };
 };
 static_assert(sizeof(BlockArgs) <= 4096, "kernel arguments");
 
@@ -71,6 +88,34 @@ struct Block {
     long long part0;        // partial row of query row 0
     const __attribute__((address_space(4))) int32_t* pages;
 };
+// Where workgroup `item` leaves its partial of a block whose tiles begin at from: of the
+// blocks that it has a part of only its first and its last may be others' too.
+__device__ __forceinline__ long long even_part(int item, int from, int even) {
+    return 2LL * item + (from > item * even);
+}
+// The next block of a workgroup where tiles are cut evenly, while there is one; at: -1, then
+// where it begins.
+__device__ __forceinline__ bool place_even(const BlockArgs& a, Block& w, int& at) {
+    const int lane = threadIdx.x & (kWave - 1), item = blockIdx.x / a.n_kv;
+    const int first = item * a.even, end = min(first + a.even, a.block_at[a.n_blocks]);
+    if (at < 0) at = first;
+    if (at >= end) return false;
+    int k = -1, i = 0;
+    for (int j = lane; j - lane < a.n_blocks; j += kWave) k += __popcll(__ballot(j < a.n_blocks && a.block_at[j] <= at));
+    if (a.n_seq > 1) i = __popcll(__ballot(lane < a.n_seq && a.start[lane] <= k)) - 1;
+    w.sq = a.seq[i];
+    w.kvh = blockIdx.x % a.n_kv;
+    const int all = w.sq.n * a.rep, from = a.block_at[k], to = a.block_at[k + 1];
+    w.r0 = ((all + a.rows - 1) / a.rows - 1 - (k - a.start[i])) * a.rows;
+    w.row_end = min(all, w.r0 + a.rows);
+    w.u0 = at - from;
+    w.u1 = min(to, end) - from;
+    w.whole = w.u0 == 0 && to <= end;
+    w.part0 = even_part(item, from, a.even) * a.rows - w.r0;
+    w.pages = (const __attribute__((address_space(4))) int32_t*)(a.table + (size_t)w.sq.cache_row * a.max_pages);
+    at = from + w.u1;
+    return true;
+}
 template <int TILE>
 __device__ __forceinline__ bool place(const BlockArgs& a, Block& w) {
     const int lane = threadIdx.x & (kWave - 1);
@@ -430,7 +475,7 @@ struct Staged {
     }
 };
 
-template <int D, int W, int KV>
+template <int D, int W, int KV, bool EVEN>
 __global__ void __launch_bounds__(W * kWave) extend_f32_kernel(BlockArgs a) {
     using G = TermGeo<D, KV>;
     constexpr int THREADS = W * kWave;
@@ -438,166 +483,174 @@ __global__ void __launch_bounds__(W * kWave) extend_f32_kernel(BlockArgs a) {
     constexpr int NC = kTermTile * C8 / THREADS > 0 ? kTermTile * C8 / THREADS : 1;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     lds_u8_t* const smem = (lds_u8_t*)smem_raw;
-    const int lane = threadIdx.x & (kWave - 1);
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int r16 = lane & 15, g = lane >> 4;
     Block b;
-    if (!place<kTermTile>(a, b)) return;
-    const int last_key = b.sq.len + b.sq.n - 1;   // of the sequence: keys behind it are not read
+    auto block = [&]() {
+        uint32_t tid = threadIdx.x;
+        if constexpr (EVEN) asm volatile("" : "+v"(tid));   // nothing of a block stays in registers for the next
+        const int lane = tid & (kWave - 1);
+        const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+        const int r16 = lane & 15, g = lane >> 4;
+        const int last_key = b.sq.len + b.sq.n - 1;   // of the sequence: keys behind it are not read
 
-    // ---- tiles: as cached in registers one tile ahead, bf16 terms in LDS ----
-    const bool loads = kTermTile * C8 >= THREADS || threadIdx.x < kTermTile * C8;
-    Staged<KV> sk[NC], sv[NC];
-    auto load = [&](int u, int page) {
-        if (!loads) return;
-        const int k0 = u * kTermTile;
-        const size_t first = ((size_t)page * a.n_kv + b.kvh) * SA_PAGE_TOKENS + k0 % SA_PAGE_TOKENS;
+        // ---- tiles: as cached in registers one tile ahead, bf16 terms in LDS ----
+        const bool loads = kTermTile * C8 >= THREADS || (int)tid < kTermTile * C8;
+        Staged<KV> sk[NC], sv[NC];
+        auto load = [&](int u, int page) {
+            if (!loads) return;
+            const int k0 = u * kTermTile;
+            const size_t first = ((size_t)page * a.n_kv + b.kvh) * SA_PAGE_TOKENS + k0 % SA_PAGE_TOKENS;
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int idx = threadIdx.x + i * THREADS;
-            const size_t row = first + min(idx / C8, last_key - k0), at = row * D + 8 * (idx % C8);
-            sk[i].load(a.k, a.k_scale, row, at);
-            sv[i].load(a.v, a.v_scale, row, at);
+            for (int i = 0; i < NC; ++i) {
+                const int idx = tid + i * THREADS;
+                const size_t row = first + min(idx / C8, last_key - k0), at = row * D + 8 * (idx % C8);
+                sk[i].load(a.k, a.k_scale, row, at);
+                sv[i].load(a.v, a.v_scale, row, at);
+            }
+        };
+        auto store_tile = [&](int u) {
+            if (!loads) return;
+            lds_u8_t* base = smem + (u & 1) * G::STAGE;
+#pragma unroll
+            for (int i = 0; i < NC; ++i) {
+                const int idx = tid + i * THREADS;
+                const int off = G::off(idx / C8, idx % C8);
+                bf16x8_t t[G::NT];
+                sk[i].terms(t);
+#pragma unroll
+                for (int x = 0; x < G::NT; ++x)
+                    *reinterpret_cast<__attribute__((address_space(3))) bf16x8_t*>(base + x * G::TERM + off) = t[x];
+                sv[i].terms(t);
+#pragma unroll
+                for (int x = 0; x < G::NT; ++x)
+                    *reinterpret_cast<__attribute__((address_space(3))) bf16x8_t*>(base + (G::NT + x) * G::TERM + off) = t[x];
+            }
+        };
+        auto page_at = [&](int u) { return page_of(a, b, u * kTermTile / SA_PAGE_TOKENS); };
+        load(b.u0, page_at(b.u0));
+        int next = b.u0 + 1 < b.u1 ? page_at(b.u0 + 1) : 0;
+
+        const int w0 = b.r0 + wave * 16;
+        const int my_row = min(w0 + r16, b.row_end - 1);
+        const bool active = w0 < b.row_end;
+        const int q_lo = b.sq.len + min(w0, b.row_end - 1) / a.rep, q_hi = b.sq.len + min(w0 + 15, b.row_end - 1) / a.rep;
+        const int q_mine = b.sq.len + my_row / a.rep;   // the last key that this lane's row sees
+        bf16x8_t qf[G::KS][kTerms];
+        {
+            const float* row = static_cast<const float*>(a.q) + out_row(a, b, my_row) * D + 8 * g;
+#pragma unroll
+            for (int ks = 0; ks < G::KS; ++ks)
+                split_terms(*reinterpret_cast<const f32x4_t*>(row + 32 * ks) * a.factor,
+                            *reinterpret_cast<const f32x4_t*>(row + 32 * ks + 4) * a.factor, qf[ks]);
         }
-    };
-    auto store_tile = [&](int u) {
-        if (!loads) return;
-        lds_u8_t* base = smem + (u & 1) * G::STAGE;
+        f32x4_t acc[G::DB];
 #pragma unroll
-        for (int i = 0; i < NC; ++i) {
-            const int idx = threadIdx.x + i * THREADS;
-            const int off = G::off(idx / C8, idx % C8);
-            bf16x8_t t[G::NT];
-            sk[i].terms(t);
-#pragma unroll
-            for (int x = 0; x < G::NT; ++x)
-                *reinterpret_cast<__attribute__((address_space(3))) bf16x8_t*>(base + x * G::TERM + off) = t[x];
-            sv[i].terms(t);
-#pragma unroll
-            for (int x = 0; x < G::NT; ++x)
-                *reinterpret_cast<__attribute__((address_space(3))) bf16x8_t*>(base + (G::NT + x) * G::TERM + off) = t[x];
-        }
-    };
-    auto page_at = [&](int u) { return page_of(a, b, u * kTermTile / SA_PAGE_TOKENS); };
-    load(b.u0, page_at(b.u0));
-    int next = b.u0 + 1 < b.u1 ? page_at(b.u0 + 1) : 0;
+        for (int db = 0; db < G::DB; ++db) acc[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        float m = -INFINITY, bias = 0.f, l = 0.f, cap = -1.f;
 
-    const int w0 = b.r0 + wave * 16;
-    const int my_row = min(w0 + r16, b.row_end - 1);
-    const bool active = w0 < b.row_end;
-    const int q_lo = b.sq.len + min(w0, b.row_end - 1) / a.rep, q_hi = b.sq.len + min(w0 + 15, b.row_end - 1) / a.rep;
-    const int q_mine = b.sq.len + my_row / a.rep;   // the last key that this lane's row sees
-    bf16x8_t qf[G::KS][kTerms];
-    {
-        const float* row = static_cast<const float*>(a.q) + out_row(a, b, my_row) * D + 8 * g;
+        auto compute = [&](int k0, const lds_u8_t* sb, bool mask) {
+            // element 4 kb + e of a lane: key 8 g + 4 kb + e
+            f32x4_t s[2] = {f32x4_t{bias, bias, bias, bias}, f32x4_t{bias, bias, bias, bias}};
 #pragma unroll
-        for (int ks = 0; ks < G::KS; ++ks)
-            split_terms(*reinterpret_cast<const f32x4_t*>(row + 32 * ks) * a.factor,
-                        *reinterpret_cast<const f32x4_t*>(row + 32 * ks + 4) * a.factor, qf[ks]);
-    }
-    f32x4_t acc[G::DB];
-#pragma unroll
-    for (int db = 0; db < G::DB; ++db) acc[db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, bias = 0.f, l = 0.f, cap = -1.f;
-
-    auto compute = [&](int k0, const lds_u8_t* sb, bool mask) {
-        // element 4 kb + e of a lane: key 8 g + 4 kb + e
-        f32x4_t s[2] = {f32x4_t{bias, bias, bias, bias}, f32x4_t{bias, bias, bias, bias}};
-#pragma unroll
-        for (int ks = 0; ks < G::KS; ++ks) {
-            bf16x8_t kf[2][G::NT];
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int t = 0; t < G::NT; ++t)
-                    kf[kb][t] = *reinterpret_cast<const __attribute__((address_space(3))) bf16x8_t*>(
-                        sb + t * G::TERM + G::off(8 * (r16 >> 2) + 4 * kb + (r16 & 3), 4 * ks + g));
-#pragma unroll
-            for (int pr = 0; pr < G::PAIRS; ++pr)
+            for (int ks = 0; ks < G::KS; ++ks) {
+                bf16x8_t kf[2][G::NT];
 #pragma unroll
                 for (int kb = 0; kb < 2; ++kb)
-                    s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kb][G::pair_a(pr)], qf[ks][G::pair_b(pr)], s[kb],
-                                                                    0, 0, 0);
-        }
-        if (mask) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (k0 + 8 * g + j > q_mine) s[j >> 2][j & 3] = -INFINITY;
-        }
-        float p[8];
+                    for (int t = 0; t < G::NT; ++t)
+                        kf[kb][t] = *reinterpret_cast<const __attribute__((address_space(3))) bf16x8_t*>(
+                            sb + t * G::TERM + G::off(8 * (r16 >> 2) + 4 * kb + (r16 & 3), 4 * ks + g));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(s[j >> 2][j & 3]);
-        float sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-        if (__any(!(sum <= cap))) {
-            float mt = s[0][0];
+                for (int pr = 0; pr < G::PAIRS; ++pr)
 #pragma unroll
-            for (int j = 1; j < 8; ++j) mt = fmaxf(mt, s[j >> 2][j & 3]);
-            const float m_new = fmaxf(m, group_reduce<OpMax, 16, kWave>(mt) - bias);
-            const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
-#pragma unroll
-            for (int db = 0; db < G::DB; ++db) acc[db] *= alpha;
-            l *= alpha;
-            const float b_new = m_new == -INFINITY ? 0.f : -m_new;
-            const float delta = b_new - bias;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(s[j >> 2][j & 3] + delta);
-            sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-            m = m_new;
-            bias = b_new;
-            cap = m_new == -INFINITY ? -1.f : kBfRaiseAt;
-        }
-        l += sum;
-        bf16x8_t pt[kTerms];
-        split_terms(f32x4_t{p[0], p[1], p[2], p[3]}, f32x4_t{p[4], p[5], p[6], p[7]}, pt);
-#pragma unroll
-        for (int db = 0; db < G::DB; ++db) {
-            bf16x8_t vf[G::NT];
-            const int c = 2 * db + ((r16 & 3) >> 1), r = 8 * g + (r16 >> 2), h8 = (r16 & 1) * 8;
-#pragma unroll
-            for (int t = 0; t < G::NT; ++t) {
-                const lds_u8_t* vb = sb + (G::NT + t) * G::TERM + h8;
-                const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vb + G::off(r, c)));
-                const s16x4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vb + G::off(r + 4, c)));
-                vf[t] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+                    for (int kb = 0; kb < 2; ++kb)
+                        s[kb] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[kb][G::pair_a(pr)], qf[ks][G::pair_b(pr)], s[kb],
+                                                                        0, 0, 0);
             }
+            if (mask) {
 #pragma unroll
-            for (int pr = 0; pr < G::PAIRS; ++pr)
-                acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[G::pair_a(pr)], pt[G::pair_b(pr)], acc[db], 0, 0, 0);
-        }
-    };
+                for (int j = 0; j < 8; ++j)
+                    if (k0 + 8 * g + j > q_mine) s[j >> 2][j & 3] = -INFINITY;
+            }
+            float p[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(s[j >> 2][j & 3]);
+            float sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+            if (__any(!(sum <= cap))) {
+                float mt = s[0][0];
+#pragma unroll
+                for (int j = 1; j < 8; ++j) mt = fmaxf(mt, s[j >> 2][j & 3]);
+                const float m_new = fmaxf(m, group_reduce<OpMax, 16, kWave>(mt) - bias);
+                const float alpha = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - m_new);
+#pragma unroll
+                for (int db = 0; db < G::DB; ++db) acc[db] *= alpha;
+                l *= alpha;
+                const float b_new = m_new == -INFINITY ? 0.f : -m_new;
+                const float delta = b_new - bias;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(s[j >> 2][j & 3] + delta);
+                sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                m = m_new;
+                bias = b_new;
+                cap = m_new == -INFINITY ? -1.f : kBfRaiseAt;
+            }
+            l += sum;
+            bf16x8_t pt[kTerms];
+            split_terms(f32x4_t{p[0], p[1], p[2], p[3]}, f32x4_t{p[4], p[5], p[6], p[7]}, pt);
+#pragma unroll
+            for (int db = 0; db < G::DB; ++db) {
+                bf16x8_t vf[G::NT];
+                const int c = 2 * db + ((r16 & 3) >> 1), r = 8 * g + (r16 >> 2), h8 = (r16 & 1) * 8;
+#pragma unroll
+                for (int t = 0; t < G::NT; ++t) {
+                    const lds_u8_t* vb = sb + (G::NT + t) * G::TERM + h8;
+                    const s16x4_t x = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vb + G::off(r, c)));
+                    const s16x4_t y = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vb + G::off(r + 4, c)));
+                    vf[t] = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7));
+                }
+#pragma unroll
+                for (int pr = 0; pr < G::PAIRS; ++pr)
+                    acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[G::pair_a(pr)], pt[G::pair_b(pr)], acc[db], 0, 0, 0);
+            }
+        };
 
-    store_tile(b.u0);
-    if (b.u0 + 1 < b.u1) load(b.u0 + 1, next);
-    next = b.u0 + 2 < b.u1 ? page_at(b.u0 + 2) : 0;
-    lds_barrier();
-    for (int u = b.u0; u < b.u1; ++u) {
-        const int k0 = u * kTermTile;
-        if (active && k0 <= q_hi) compute(k0, smem + (u & 1) * G::STAGE, k0 + kTermTile - 1 > q_lo);
-        if (u + 1 < b.u1) {
-            store_tile(u + 1);   // where tile u - 1 was
-            if (u + 2 < b.u1) load(u + 2, next);
-            if (u + 3 < b.u1) next = page_at(u + 3);
-        }
+        store_tile(b.u0);
+        if (b.u0 + 1 < b.u1) load(b.u0 + 1, next);
+        next = b.u0 + 2 < b.u1 ? page_at(b.u0 + 2) : 0;
         lds_barrier();
-    }
-
-    const float sum = group_reduce<OpSum, 16, kWave>(l), fine = sum + group_reduce<OpSum, 16, kWave>(not_finite<G::DB>(acc));
-    const bool mine = w0 + r16 < b.row_end, ok = fine < INFINITY;
-    if (mine && ok) {
-        if (b.whole) {
-            const float inv = 1.0f / sum;
-            float* o = static_cast<float*>(a.out) + out_row(a, b, my_row) * D + 4 * g;
-#pragma unroll
-            for (int db = 0; db < G::DB; ++db) *reinterpret_cast<f32x4_t*>(o + 16 * db) = acc[db] * inv;
-        } else {
-            const size_t at = (size_t)(b.part0 + my_row) * a.n_kv + b.kvh;
-#pragma unroll
-            for (int db = 0; db < G::DB; ++db) *reinterpret_cast<f32x4_t*>(a.part_o + at * D + 16 * db + 4 * g) = acc[db];
-            if (g == 0) *reinterpret_cast<f32x2_t*>(a.part_ml + at * 2) = f32x2_t{m, sum};
+        for (int u = b.u0; u < b.u1; ++u) {
+            const int k0 = u * kTermTile;
+            if (active && k0 <= q_hi) compute(k0, smem + (u & 1) * G::STAGE, k0 + kTermTile - 1 > q_lo);
+            if (u + 1 < b.u1) {
+                store_tile(u + 1);   // where tile u - 1 was
+                if (u + 2 < b.u1) load(u + 2, next);
+                if (u + 3 < b.u1) next = page_at(u + 3);
+            }
+            lds_barrier();
         }
+
+        const float sum = group_reduce<OpSum, 16, kWave>(l), fine = sum + group_reduce<OpSum, 16, kWave>(not_finite<G::DB>(acc));
+        const bool mine = w0 + r16 < b.row_end, ok = fine < INFINITY;
+        if (mine && ok) {
+            if (b.whole) {
+                const float inv = 1.0f / sum;
+                float* o = static_cast<float*>(a.out) + out_row(a, b, my_row) * D + 4 * g;
+#pragma unroll
+                for (int db = 0; db < G::DB; ++db) *reinterpret_cast<f32x4_t*>(o + 16 * db) = acc[db] * inv;
+            } else {
+                const size_t at = (size_t)(b.part0 + my_row) * a.n_kv + b.kvh;
+#pragma unroll
+                for (int db = 0; db < G::DB; ++db) *reinterpret_cast<f32x4_t*>(a.part_o + at * D + 16 * db + 4 * g) = acc[db];
+                if (g == 0) *reinterpret_cast<f32x2_t*>(a.part_ml + at * 2) = f32x2_t{m, sum};
+            }
+        }
+        for (uint32_t anew = __ballot(mine && !ok) & 0xffff; anew; anew &= anew - 1)
+            block_plain<D, KV, kTermTile, float>(a, b, w0 + __builtin_ctz(anew));
+    };
+    if constexpr (EVEN) {
+        for (int at = -1; place_even(a, b, at);) block();
+    } else {
+        if (place<kTermTile>(a, b)) block();
     }
-    for (uint32_t anew = __ballot(mine && !ok) & 0xffff; anew; anew &= anew - 1)
-        block_plain<D, KV, kTermTile, float>(a, b, w0 + __builtin_ctz(anew));
 }
 
 // ---------------------------------------------------------------- partials
@@ -611,7 +664,7 @@ __device__ __forceinline__ void put4(uint16_t* p, f32x4_t v) {
 
 // O = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c, D / 4 lanes per row of 256 D / 4
 // consecutive (token, head) rows from the launch's first token on.
-template <int D, class T>
+template <int D, class T, bool EVEN>
 __global__ void __launch_bounds__(256) block_merge_kernel(BlockArgs a, long long row0, long long n) {
     constexpr int C = D / 4, ROWS = 256 / C;
     const long long first = row0 + (long long)blockIdx.x * ROWS, r = first + threadIdx.x / C;
@@ -622,15 +675,30 @@ __global__ void __launch_bounds__(256) block_merge_kernel(BlockArgs a, long long
     while (i + 1 < a.n_seq && a.seq[i + 1].first <= token) ++i;
     const ChunkSeq sq = a.seq[i];
     const int t = token - sq.first;
-    if (a.parts[i] == 1 || t >= sq.n) return;   // written already, or a row of another launch
+    if (t >= sq.n) return;                      // a row of another launch
     const int kvh = head / a.rep, row = t * a.rep + head % a.rep;
-    const int parts = (block_key_tiles(sq, row / a.rows, a.rows, a.rep, a.tile) + a.tiles - 1) / a.tiles;
-    const long long step = (long long)sq.n * a.rep;
+    const int b = row / a.rows;
+    int parts;
+    long long first_part, others, step;   // part p's row: first_part or, where p > 0, others + p step
+    if constexpr (EVEN) {
+        const int k = a.start[i] + (sq.n * a.rep + a.rows - 1) / a.rows - 1 - b;
+        const int from = a.block_at[k], item = from / a.even;
+        parts = (a.block_at[k + 1] - 1) / a.even - item + 1;
+        if (parts == 1) return;                 // written already
+        first_part = even_part(item, from, a.even) * a.rows + row - b * a.rows;
+        others = even_part(item, item * a.even, a.even) * a.rows + row - b * a.rows;
+        step = 2 * a.rows;
+    } else {
+        if (a.parts[i] == 1) return;
+        parts = (block_key_tiles(sq, b, a.rows, a.rep, a.tile) + a.tiles - 1) / a.tiles;
+        first_part = others = a.base[i] + row;
+        step = (long long)sq.n * a.rep;
+    }
     float M = -INFINITY, L = 0.f;
     f32x4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
     for (int p = 0; p < parts; ++p) {
-        const size_t at = (size_t)(a.base[i] + p * step + row) * a.n_kv + kvh;
+        const size_t at = (size_t)(EVEN && p == 0 ? first_part : others + p * step) * a.n_kv + kvh;
         const f32x2_t ml = *reinterpret_cast<const f32x2_t*>(a.part_ml + at * 2);
         const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.part_o + at * D + 4 * c);
         const float m_new = fmaxf(M, ml[0]);
@@ -649,6 +717,8 @@ constexpr int kMaxRounds = 4;    // of workgroups that a launch's tiles are cut 
 // What a workgroup costs besides its tiles, in tiles: its beginning and its output, or
 // where a block is cut a partial written and read again.
 constexpr int kWholeTiles = 2, kCutBf16 = 6, kCutF32 = 4, kCutTerms = 7;
+// And a workgroup's further blocks where tiles are cut evenly.
+constexpr int kNextF32 = 4, kNextTerms = 14;
 
 // Workgroups of a kind that share a CU (by registers, and for fp32 caches by LDS: 96 KiB
 // at D = 128, 48 at 64), and what a tile of one takes of a full CU's time, in those of
@@ -669,36 +739,40 @@ Kind kind_of(bool q16, sa_dtype kv, int d, int waves) {
 }
 
 template <auto KERNEL>
-sa_status launch_blocks(const BlockArgs& a, int waves, int lds, hipStream_t st) {
+sa_status launch_blocks(const BlockArgs& a, int waves, int items, int lds, hipStream_t st) {
     SA_TRY(pf::opt_in_lds<KERNEL>(lds));
-    hipLaunchKernelGGL(KERNEL, dim3((unsigned)a.start[a.n_seq] * a.n_kv), dim3(waves * kWave), lds, st, a);
+    hipLaunchKernelGGL(KERNEL, dim3((unsigned)items * a.n_kv), dim3(waves * kWave), lds, st, a);
     SA_CHECK_LAUNCH();
     return SA_OK;
 }
 template <int D, int KV>
-sa_status launch_f32(const BlockArgs& a, int waves, hipStream_t st) {
+sa_status launch_f32(const BlockArgs& a, int waves, int items, hipStream_t st) {
     constexpr int lds = 2 * TermGeo<D, KV>::STAGE;
     if constexpr (KV == SA_DTYPE_F32)
-        if (waves == 8) return launch_blocks<extend_f32_kernel<D, 8, KV>>(a, 8, lds, st);
-    return launch_blocks<extend_f32_kernel<D, 4, KV>>(a, 4, lds, st);
+        if (waves == 8)
+            return a.even ? launch_blocks<extend_f32_kernel<D, 8, KV, true>>(a, 8, items, lds, st)
+                          : launch_blocks<extend_f32_kernel<D, 8, KV, false>>(a, 8, items, lds, st);
+    return a.even ? launch_blocks<extend_f32_kernel<D, 4, KV, true>>(a, 4, items, lds, st)
+                  : launch_blocks<extend_f32_kernel<D, 4, KV, false>>(a, 4, items, lds, st);
 }
 template <int D, bool FP8>
-sa_status launch_bf16(const BlockArgs& a, int waves, hipStream_t st) {
+sa_status launch_bf16(const BlockArgs& a, int waves, int items, hipStream_t st) {
     constexpr int lds = 2 * BfGeo<D>::STAGE;
-    return waves == 8 ? launch_blocks<extend_bf16_kernel<D, 8, FP8>>(a, 8, lds, st)
-                      : launch_blocks<extend_bf16_kernel<D, 4, FP8>>(a, 4, lds, st);
+    return waves == 8 ? launch_blocks<extend_bf16_kernel<D, 8, FP8>>(a, 8, items, lds, st)
+                      : launch_blocks<extend_bf16_kernel<D, 4, FP8>>(a, 4, items, lds, st);
 }
 template <int D>
-sa_status dispatch_blocks(const BlockArgs& a, sa_dtype kv, bool q16, int waves, bool merge, long long rows,
+sa_status dispatch_blocks(const BlockArgs& a, sa_dtype kv, bool q16, int waves, int items, bool merge, long long rows,
                           hipStream_t st) {
-    if (q16) SA_TRY(kv == SA_DTYPE_FP8 ? (launch_bf16<D, true>(a, waves, st)) : (launch_bf16<D, false>(a, waves, st)));
-    else SA_TRY(kv == SA_DTYPE_F32    ? (launch_f32<D, SA_DTYPE_F32>(a, waves, st))
-                : kv == SA_DTYPE_BF16 ? (launch_f32<D, SA_DTYPE_BF16>(a, waves, st))
-                                      : (launch_f32<D, SA_DTYPE_FP8>(a, waves, st)));
+    if (q16) SA_TRY(kv == SA_DTYPE_FP8 ? (launch_bf16<D, true>(a, waves, items, st)) : (launch_bf16<D, false>(a, waves, items, st)));
+    else SA_TRY(kv == SA_DTYPE_F32    ? (launch_f32<D, SA_DTYPE_F32>(a, waves, items, st))
+                : kv == SA_DTYPE_BF16 ? (launch_f32<D, SA_DTYPE_BF16>(a, waves, items, st))
+                                      : (launch_f32<D, SA_DTYPE_FP8>(a, waves, items, st)));
     if (!merge) return SA_OK;
     return merge_rows<D>(rows, [&](dim3 grid, long long row0) {
-        if (q16) hipLaunchKernelGGL((block_merge_kernel<D, uint16_t>), grid, dim3(256), 0, st, a, row0, rows);
-        else hipLaunchKernelGGL((block_merge_kernel<D, float>), grid, dim3(256), 0, st, a, row0, rows);
+        if (q16) hipLaunchKernelGGL((block_merge_kernel<D, uint16_t, false>), grid, dim3(256), 0, st, a, row0, rows);
+        else if (a.even) hipLaunchKernelGGL((block_merge_kernel<D, float, true>), grid, dim3(256), 0, st, a, row0, rows);
+        else hipLaunchKernelGGL((block_merge_kernel<D, float, false>), grid, dim3(256), 0, st, a, row0, rows);
     });
 }
 
@@ -773,6 +847,15 @@ sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, co
         const bool terms = !q16 && c.kv != SA_DTYPE_F32;   // in four waves always
         int waves = 8;
         double best = INFINITY;
+        a.even = 0;
+        long long rows_all = 0;
+        int keys = 0;
+        for (int i = 0; i < a.n_seq; ++i) {
+            rows_all += (long long)a.seq[i].n * n_q;
+            keys = std::max(keys, a.seq[i].len + a.seq[i].n);
+        }
+        // extend_blocks_ws's rows
+        const long long room = std::min(rows_all * ((keys + kTermTile - 1) / kTermTile), kMaxRounds * cus * 256);
         for (int w = 8; w >= 4; w -= 4) {
             if (w == 8 && (most <= 4 * per_wave || terms)) continue;
             a.rows = w * per_wave;
@@ -810,19 +893,50 @@ sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, co
                 const double tile = wgs > cus ? kind.per_cu * kind.tile : kind.alone;
                 const double cost = (std::max({rounds, work / slots, (double)t}) +
                                      (p > 1 ? cut : kWholeTiles) * std::max(1.0, wgs / slots)) * tile;
-                if (cost < best) best = cost, waves = w, a.tiles = t;
+                if (cost < best) best = cost, waves = w, a.tiles = t, a.even = 0;
+            }
+            // All blocks' tiles in a row, cut evenly.
+            long long blocks = 0, total = 0;
+            for (int i = 0; i < a.n_seq; ++i) blocks += blocks_of((long long)a.seq[i].n * a.rep, a.rows);
+            if (q16 || blocks > kEvenBlocks || (w == 8 && c.d == 64)) continue;
+            for (int i = 0; i < a.n_seq; ++i)
+                for (int b = 0, k = (int)blocks_of((long long)a.seq[i].n * a.rep, a.rows); b < k; ++b)
+                    total += block_key_tiles(a.seq[i], b, a.rows, a.rep, a.tile);
+            for (int per : {kind.per_cu, 1}) {
+                const long long most_wgs = std::min(total, per * cus / a.n_kv);
+                if (most_wgs < 1) continue;
+                const int t = (int)((total + most_wgs - 1) / most_wgs);
+                const long long wgs = (total + t - 1) / t;
+                if (2 * wgs * a.rows * a.n_kv > room) continue;
+                const double cost = (t + cut + (terms ? kNextTerms : kNextF32) * (double)blocks / wgs) *
+                                    (wgs * a.n_kv > cus ? kind.per_cu * kind.tile : kind.alone);
+                if (cost < best) best = cost, waves = w, a.even = t;
             }
         }
         a.rows = waves * per_wave;
         long long at = 0, parts = 0;
-        for (int i = 0; i < a.n_seq; ++i) {
+        if (a.even) {
+            int k = 0, sum = 0;
+            for (int i = 0; i < a.n_seq; ++i) {
+                a.start[i] = k;
+                for (int b = (int)blocks_of((long long)a.seq[i].n * a.rep, a.rows) - 1; b >= 0; --b) {
+                    a.block_at[k++] = sum;
+                    sum += block_key_tiles(a.seq[i], b, a.rows, a.rep, a.tile);
+                }
+            }
+            a.start[a.n_seq] = a.n_blocks = k;
+            a.block_at[k] = sum;
+            at = (sum + a.even - 1) / a.even;
+            parts = 2 * at * a.rows;
+        }
+        for (int i = 0; i < a.n_seq && !a.even; ++i) {
             a.parts[i] = parts_of(i, a.tiles);
             a.start[i] = (int)at;
             a.base[i] = (int)parts;
             at += blocks_of((long long)a.seq[i].n * a.rep, a.rows) * a.parts[i];
             if (a.parts[i] > 1) parts += (long long)a.parts[i] * a.seq[i].n * a.rep;
         }
-        a.start[a.n_seq] = (int)at;
+        if (!a.even) a.start[a.n_seq] = (int)at;
         const long long tokens = a.seq[a.n_seq - 1].first + a.seq[a.n_seq - 1].n - a.seq[0].first;
         // a grid has fewer than 2^32 threads
         if (at * a.n_kv >= (1LL << 32) / (waves * kWave) || parts > 0x7fffffffLL)
@@ -833,8 +947,8 @@ sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, co
             a.part_o = static_cast<float*>(ws);
             a.part_ml = a.part_o + (size_t)parts * a.n_kv * c.d;
         }
-        SA_TRY(c.d == 64 ? dispatch_blocks<64>(a, c.kv, q16, waves, parts > 0, tokens * n_q, st)
-                         : dispatch_blocks<128>(a, c.kv, q16, waves, parts > 0, tokens * n_q, st));
+        SA_TRY(c.d == 64 ? dispatch_blocks<64>(a, c.kv, q16, waves, (int)at, parts > 0, tokens * n_q, st)
+                         : dispatch_blocks<128>(a, c.kv, q16, waves, (int)at, parts > 0, tokens * n_q, st));
     }
     return SA_OK;
 }
