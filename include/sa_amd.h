@@ -13,7 +13,8 @@
  * Head sizes (head_dim, d, D): 8, 16, 32, 64, 128 or 256 for single-query
  * attention, decode, the KV cache and QK-norm/RoPE; the fused decode step
  * (sa_append_decode) takes 64, 128 or 256; causal prefill 16, 32, 64 or 128
- * in fp32 and 64 or 128 in bf16.  Other sizes return SA_EINVAL.
+ * in fp32 and 64 or 128 in bf16; caches in 8 bits and chunks of new tokens 64 or
+ * 128.  Other sizes return SA_EINVAL.
  */
 #ifndef SA_AMD_H
 #define SA_AMD_H
@@ -99,7 +100,7 @@ sa_status sa_decode_dense_f32(const float* q, const float* k, const float* v,
                               sa_stream_t stream);
 
 /* ------------------------------------------------------------------------
- * Paged KV cache (64-token pages, int32 block tables, fp32 or bf16 storage).
+ * Paged KV cache (64-token pages, int32 block tables; fp32, bf16 or 8-bit storage).
  *
  * Replaces tensor_cpp::qwen3::KVCache (reference
  * tensor_cpp/include/tensor_cpp/kv_cache.h:27-238).  Storage per layer:

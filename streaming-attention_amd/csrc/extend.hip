@@ -26,6 +26,13 @@
 // eight waves, is more than they lose by rounds.
 //
 // Rows whose sums are not finite are computed anew over what they see (plain_row.h).
+//
+// Bound, 16 / 8 heads of 128: MFMA and the softmax's VALU work beside it.  2048 bf16 tokens
+// behind 30720, 533 GF: 505 us, 1.06 PFLOP/s, MFMA 53 % and VALU 44 % busy, the second
+// launch 17 of them.  512 fp32 tokens behind 3584, 16.1 GF x 6: 92 us, 1.05 PFLOP/s of
+// products, MFMA 51 %, VALU 39 %.  Seven chunks of 1 - 700 tokens over 8 bits, 32 / 8 heads of
+// 64, 82.9 GF: 140 us; at 64 the softmax is as long as the products (VALU 63 %, MFMA 40 %),
+// and rounds of workgroups of unequal lengths cost a fifth.
 #include <algorithm>
 #include <cmath>
 #include <vector>
@@ -522,7 +529,8 @@ __global__ void __launch_bounds__(W * kWave) extend_f32_kernel(BlockArgs a) {
                 sv[i].terms(t);
 #pragma unroll
                 for (int x = 0; x < G::NT; ++x)
-                    *reinterpret_cast<__attribute__((address_space(3))) bf16x8_t*>(base + (G::NT + x) * G::TERM + off) = t[x];
+                    *reinterpret_cast<__attribute__((address_space(3))) bf16x8_t*>(base + (G::NT + x) * G::TERM + off) =
+                        t[x];
             }
         };
         auto page_at = [&](int u) { return page_of(a, b, u * kTermTile / SA_PAGE_TOKENS); };
@@ -609,7 +617,8 @@ __global__ void __launch_bounds__(W * kWave) extend_f32_kernel(BlockArgs a) {
                 }
 #pragma unroll
                 for (int pr = 0; pr < G::PAIRS; ++pr)
-                    acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[G::pair_a(pr)], pt[G::pair_b(pr)], acc[db], 0, 0, 0);
+                    acc[db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[G::pair_a(pr)], pt[G::pair_b(pr)], acc[db], 0, 0,
+                                                                      0);
             }
         };
 
@@ -628,7 +637,8 @@ __global__ void __launch_bounds__(W * kWave) extend_f32_kernel(BlockArgs a) {
             lds_barrier();
         }
 
-        const float sum = group_reduce<OpSum, 16, kWave>(l), fine = sum + group_reduce<OpSum, 16, kWave>(not_finite<G::DB>(acc));
+        const float sum = group_reduce<OpSum, 16, kWave>(l);
+        const float fine = sum + group_reduce<OpSum, 16, kWave>(not_finite<G::DB>(acc));
         const bool mine = w0 + r16 < b.row_end, ok = fine < INFINITY;
         if (mine && ok) {
             if (b.whole) {
@@ -639,7 +649,8 @@ __global__ void __launch_bounds__(W * kWave) extend_f32_kernel(BlockArgs a) {
             } else {
                 const size_t at = (size_t)(b.part0 + my_row) * a.n_kv + b.kvh;
 #pragma unroll
-                for (int db = 0; db < G::DB; ++db) *reinterpret_cast<f32x4_t*>(a.part_o + at * D + 16 * db + 4 * g) = acc[db];
+                for (int db = 0; db < G::DB; ++db)
+                    *reinterpret_cast<f32x4_t*>(a.part_o + at * D + 16 * db + 4 * g) = acc[db];
                 if (g == 0) *reinterpret_cast<f32x2_t*>(a.part_ml + at * 2) = f32x2_t{m, sum};
             }
         }
@@ -764,7 +775,8 @@ sa_status launch_bf16(const BlockArgs& a, int waves, int items, hipStream_t st) 
 template <int D>
 sa_status dispatch_blocks(const BlockArgs& a, sa_dtype kv, bool q16, int waves, int items, bool merge, long long rows,
                           hipStream_t st) {
-    if (q16) SA_TRY(kv == SA_DTYPE_FP8 ? (launch_bf16<D, true>(a, waves, items, st)) : (launch_bf16<D, false>(a, waves, items, st)));
+    if (q16) SA_TRY(kv == SA_DTYPE_FP8 ? (launch_bf16<D, true>(a, waves, items, st))
+                                       : (launch_bf16<D, false>(a, waves, items, st)));
     else SA_TRY(kv == SA_DTYPE_F32    ? (launch_f32<D, SA_DTYPE_F32>(a, waves, items, st))
                 : kv == SA_DTYPE_BF16 ? (launch_f32<D, SA_DTYPE_BF16>(a, waves, items, st))
                                       : (launch_f32<D, SA_DTYPE_FP8>(a, waves, items, st)));

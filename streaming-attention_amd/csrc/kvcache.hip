@@ -1,7 +1,8 @@
 // Paged KV cache for gfx950 and the fused q/k RMSNorm + RoPE + K/V append.
 //
 // Storage: one device allocation holding, per layer, a K pool and a V pool of
-// [num_pages][n_kv_heads][64][head_dim] elements (fp32 or bf16).  A page of one
+// [num_pages][n_kv_heads][64][head_dim] elements (fp32, bf16 or 8-bit codes, the
+// codes' scales in pools of their own).  A page of one
 // head is 64 consecutive rows, so the decode kernel streams 8-32 KiB of
 // contiguous memory per page.  Pages are handed out from a host free list;
 // block_table[seq][j] names the page holding tokens 64j..64j+63 (-1: none).
@@ -226,14 +227,15 @@ sa_status no_throw(F&& body) {
 //
 // Bound: HBM for prompts: the 29.4 MB of 1024 tokens (16 query and 8 KV heads of
 // 128, bf16 cache) take 4.7 us at 6.3 TB/s; the launch takes 7.1 us, 4096 tokens
-// 22.5 (rows of 64 lanes with 4-byte loads, two per wave of keys: 7.9 and 25.1).
+// 22.5 (rows of 64 lanes with 4-byte loads, two per wave of keys: 7.9 and 25.1).  K and V
+// of 8192 tokens into an 8-bit cache, 84 MB: 16.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
     const float* q; const float* k; const float* v;
     float* q_out;
     float* k_out;              // optional: K normed and rotated, as q_out
     // Optional: q, k and v are the sum of part_S split-K partials of rows
-    // [part_row0 + i_seq * S + s] of a [part_M][(n_q + 2 n_kv) * D] projection;
+    // part_row0 + a token's place in q, k and v, of a [part_M][(n_q + 2 n_kv) * D] projection;
     // v also goes to v_out.
     const float* part;
     int part_S, part_M, part_row0;

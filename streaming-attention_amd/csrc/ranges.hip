@@ -1,4 +1,5 @@
-// Attention of single tokens over ranges of a paged cache, on bf16 MFMA.
+// Attention of single tokens, and of few new tokens in a row, over ranges of a paged
+// cache, on bf16 MFMA.
 //
 // A row (sequence) of a launch sees the tokens of up to two sources: its
 // group's (a prefix whose pages several rows list, read once for all of them)
@@ -21,6 +22,14 @@
 // (plain_row.h), so that infinities and values near fp32's limit come out as in
 // the paged decode that does not split.
 //
+// An 8-bit cache's codes are one bf16 term each, 2^e times the code: widened with their
+// row's scale on the way from LDS into registers, exactly (K read as rows, V
+// transposed as bytes, ds_read_tr8_b64).
+//
+// Chunks of new tokens (at most some dozen query rows each; extend.hip takes longer ones):
+// the query rows of a source are then the new tokens x query heads of the KV head,
+// and a token's own place is its mask's last key, so only tiles at the end are masked.
+//
 // Layout: v_mfma_f32_16x16x32_bf16 with S^T = K Q^T (rows: keys, columns: query
 // rows), so that a lane's eight scores of a 32-key tile are the operand that
 // O^T += V^T P^T takes.  Four waves: RG of them take 16 RT query
@@ -35,7 +44,10 @@
 // rows behind one prefix (64 behind 32768 tokens, bf16: 75 us, MFMA 42 % and VALU
 // 45 % busy; loads alone 55, computing alone 66, of both 15 for launches, queries
 // and partials); the latency of the tiles for few rows (4 x 4 beams, fp32: 19.4 us,
-// 2.65 per tile of a wave; 4 rows behind 512 tokens, bf16: 9.0).
+// 2.65 per tile of a wave; 4 rows behind 512 tokens, bf16: 9.0).  Over 8 bits 64 rows of
+// 512 - 32768 tokens, 2.12 GB, take 341 us (6.2 TB/s; MFMA 31 % and VALU 52 % busy), one row
+// of 5000 14.1; chunks of 5 tokens of each of 64 sequences of 512 - 16384, bf16, 2.18 GB, 363
+// (6.0 TB/s), 5 tokens behind 1000, fp32, 12.6 (9.2 and 4.4 in two launches).
 #include "ranges.h"
 
 #include <algorithm>
