@@ -31,8 +31,8 @@
 // behind 30720, 533 GF: 505 us, 1.06 PFLOP/s, MFMA 53 % and VALU 44 % busy, the second
 // launch 17 of them.  512 fp32 tokens behind 3584, 16.1 GF x 6: 92 us, 1.05 PFLOP/s of
 // products, MFMA 51 %, VALU 39 %.  Seven chunks of 1 - 700 tokens over 8 bits, 32 / 8 heads of
-// 64, 82.9 GF: 140 us; at 64 the softmax is as long as the products (VALU 63 %, MFMA 40 %),
-// and rounds of workgroups of unequal lengths cost a fifth.
+// 64, 82.9 GF: 130 us; at 64 the softmax is as long as the products (VALU 63 %, MFMA 40 %),
+// and rounds of workgroups of unequal lengths cost a tenth.
 #include <algorithm>
 #include <cmath>
 #include <vector>
@@ -45,7 +45,7 @@
 namespace sa {
 namespace {
 
-constexpr int kEvenBlocks = 128;
+constexpr int kSortedBlocks = 128;   // of a launch whose parts have an order or equal lengths
 
 struct BlockArgs {
     const void* q;
@@ -67,15 +67,22 @@ struct BlockArgs {
     uint32_t q_sign;                         // 0x80008000 for a negative scale
     ChunkSeq seq[kRowsPerLaunch];
     int32_t start[kRowsPerLaunch + 1];       // a sequence's first item, of blocks x parts
+    // Several sequences' parts in the order of their lengths: first the `full` ones of
+    // a.tiles, block k's from full_at[k] on, then rest[..], the blocks that leave a shorter
+    // one, longest first; start[i] is then sequence i's first block.  n_blocks 0: sequence
+    // behind sequence.
+    int n_blocks, full;
+    uint16_t full_at[kSortedBlocks + 1];
+    uint8_t rest[kSortedBlocks];
     // Tiles cut evenly: even > 0 tiles per workgroup of the blocks' tiles in a row,
     // block_at[k] before block k; start[i] is then sequence i's first block.
-    int even, n_blocks;
+    int even;
     union {
         struct {
             int32_t base[kRowsPerLaunch];    // its first partial row
             int32_t parts[kRowsPerLaunch];   // of its last block
         };
-        int32_t block_at[kEvenBlocks + 1];
+        int32_t block_at[kSortedBlocks + 1];
     };
 };
 static_assert(sizeof(BlockArgs) <= 4096, "kernel arguments");
@@ -131,7 +138,20 @@ __device__ __forceinline__ bool place(const BlockArgs& a, Block& w) {
     // a trip to host memory away).
     int parts = a.parts[0], local = item, base = 0;
     w.sq = a.seq[0];
-    if (a.n_seq > 1) {
+    if (a.n_blocks) {
+        int k = -1;
+        if (item < a.full)
+            for (int j = lane; j - lane < a.n_blocks; j += kWave)
+                k += __popcll(__ballot(j < a.n_blocks && a.full_at[j] <= item));
+        else
+            k = __builtin_amdgcn_readfirstlane(a.rest[item - a.full]);
+        const int c = item < a.full ? item - a.full_at[k] : a.full_at[k + 1] - a.full_at[k];
+        const int i = __popcll(__ballot(lane < a.n_seq && a.start[lane] <= k)) - 1;
+        w.sq = a.seq[i];
+        parts = a.parts[i];
+        local = (k - a.start[i]) * parts + c;
+        base = a.base[i];
+    } else if (a.n_seq > 1) {
         const int i = __popcll(__ballot(lane < a.n_seq && a.start[lane] <= item)) - 1;
         w.sq = a.seq[i];
         parts = a.parts[i];
@@ -813,6 +833,41 @@ void split_chunks(sa_dtype kv, int rep, int n_kv, const ChunkSeq* seqs, int n, s
         (blocks && (join || (long long)seqs[i].n * rep >= kBlockRows) ? many : few)->push_back(seqs[i]);
 }
 
+namespace {
+
+// The parts of several sequences by their lengths, so that the last to begin are the
+// shortest: seven chunks of 1 - 700 tokens over 8 bits 137 -> 130 us, eight of 100 - 1000
+// behind up to 16000, bf16, 16 / 8 heads of 64 393 -> 285.  The search costs 0.6 us.
+void sort_parts(BlockArgs& a, long long* items) {
+    struct Rest { int tiles, block; } rest[kSortedBlocks];
+    int k = 0, n_rest = 0;
+    long long full = 0, blocks = 0;
+    for (int i = 0; i < a.n_seq; ++i) blocks += blocks_of((long long)a.seq[i].n * a.rep, a.rows);
+    if (blocks > kSortedBlocks) return;
+    int32_t start[kRowsPerLaunch];
+    for (int i = 0; i < a.n_seq; ++i) {
+        start[i] = k;
+        for (int b = (int)blocks_of((long long)a.seq[i].n * a.rep, a.rows) - 1; b >= 0; --b, ++k) {
+            const int tiles = block_key_tiles(a.seq[i], b, a.rows, a.rep, a.tile);
+            a.full_at[k] = (uint16_t)full;
+            full += tiles / a.tiles;
+            if (full > 0xffff) return;
+            if (tiles % a.tiles) rest[n_rest++] = {tiles % a.tiles, k};
+        }
+    }
+    a.full_at[k] = (uint16_t)full;
+    std::sort(rest, rest + n_rest, [](const Rest& x, const Rest& y) {
+        return x.tiles != y.tiles ? x.tiles > y.tiles : x.block < y.block;
+    });
+    for (int r = 0; r < n_rest; ++r) a.rest[r] = (uint8_t)rest[r].block;
+    std::copy(start, start + a.n_seq, a.start);
+    a.n_blocks = k;
+    a.full = (int)full;
+    *items = full + n_rest;
+}
+
+}  // namespace
+
 size_t extend_blocks_ws(int n, const int32_t* counts, int n_q, int n_kv, int d, long long max_tokens) {
     const long long tiles = (max_tokens + kTermTile - 1) / kTermTile;
     if (tiles <= 1) return 0;
@@ -910,7 +965,7 @@ sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, co
             // All blocks' tiles in a row, cut evenly.
             long long blocks = 0, total = 0;
             for (int i = 0; i < a.n_seq; ++i) blocks += blocks_of((long long)a.seq[i].n * a.rep, a.rows);
-            if (q16 || blocks > kEvenBlocks || (w == 8 && c.d == 64)) continue;
+            if (q16 || blocks > kSortedBlocks || (w == 8 && c.d == 64)) continue;
             for (int i = 0; i < a.n_seq; ++i)
                 for (int b = 0, k = (int)blocks_of((long long)a.seq[i].n * a.rep, a.rows); b < k; ++b)
                     total += block_key_tiles(a.seq[i], b, a.rows, a.rep, a.tile);
@@ -941,6 +996,7 @@ sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, co
             at = (sum + a.even - 1) / a.even;
             parts = 2 * at * a.rows;
         }
+        if (!a.even) a.n_blocks = 0;
         for (int i = 0; i < a.n_seq && !a.even; ++i) {
             a.parts[i] = parts_of(i, a.tiles);
             a.start[i] = (int)at;
@@ -949,6 +1005,7 @@ sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, co
             if (a.parts[i] > 1) parts += (long long)a.parts[i] * a.seq[i].n * a.rep;
         }
         if (!a.even) a.start[a.n_seq] = (int)at;
+        if (!a.even && a.n_seq > 1) sort_parts(a, &at);
         const long long tokens = a.seq[a.n_seq - 1].first + a.seq[a.n_seq - 1].n - a.seq[0].first;
         // a grid has fewer than 2^32 threads
         if (at * a.n_kv >= (1LL << 32) / (waves * kWave) || parts > 0x7fffffffLL)
