@@ -397,3 +397,28 @@ def test_two_graphs_on_one_workspace(sa, q, kv):
             rows.cache.extend(0, x[1 - i], 0.125, calls[1 - i], ws=ws)
         torch.cuda.synchronize()
         assert all(torch.equal(o, w) for o, w in zip(out, want))
+
+
+@pytest.mark.parametrize("q,kv", PAIRS)
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 64), (16, 8, 128), (3, 1, 64)])
+def test_chunks_of_unequal_lengths(sa, q, kv, Hq, Hkv, D):
+    """Blocks in parts of all lengths, of sequences in no order of their lengths."""
+    lens, counts = [3000, 40, 1500, 0, 700, 5000], [400, 300, 1, 200, 90, 33]
+    rows = Rows(sa, kv, Hkv, D, lens, seed=29, room=400)
+    rows.append(counts)
+    x = rows.normal(sum(counts), Hq, D, dtype=TYPE[q])
+    check_all(rows, rows.cache.extend(0, x, 0.1, counts), x, counts, lens, 0.1)
+
+
+@pytest.mark.parametrize("q,kv", PAIRS)
+def test_many_blocks_of_two_sequences(sa, q, kv):
+    """More blocks than are put in order, and as many but one part each."""
+    for n, past in ((5000, 100), (600, 0)):
+        rows = Rows(sa, kv, 1, 64, [past, 0], seed=30, room=n)
+        rows.append([n, n])
+        x = rows.normal(2 * n, 8, 64, dtype=TYPE[q])
+        got = rows.cache.extend(0, x, 0.125, [n, n])
+        for r, first in ((0, 0), (1, n)):
+            for at in (0, 1, 31, 32, 255, n // 2, n - 2, n - 1):
+                i = first + at
+                check(got[i:i + 1], *attend(x[i:i + 1], rows.k[r], rows.v[r], 0.125, (past, 0)[r] + at))
