@@ -746,8 +746,10 @@ __global__ void __launch_bounds__(256) block_merge_kernel(BlockArgs a, long long
 
 constexpr int kMaxRounds = 4;    // of workgroups that a launch's tiles are cut into
 // What a workgroup costs besides its tiles, in tiles: its beginning and its output, or
-// where a block is cut a partial written and read again.
-constexpr int kWholeTiles = 2, kCutBf16 = 6, kCutF32 = 4, kCutTerms = 7;
+// where a block is cut a partial written and read again (bf16, 6 for both head sizes: 7 chunks
+// of 1 - 700 tokens, heads of 128, 216 us, 191 with 9; 16 of 100 - 1000, heads of 64, 397, 331 with
+// 4, which 9 leaves at 397).
+constexpr int kWholeTiles = 2, kCutBf16 = 9, kCutBf16Narrow = 4, kCutF32 = 4, kCutTerms = 7;
 // And a workgroup's further blocks where tiles are cut evenly.
 constexpr int kNextF32 = 4, kNextTerms = 14;
 
@@ -910,7 +912,7 @@ sa_status extend_blocks(const PagedView& c, const void* q, bool q16, int n_q, co
         // Eight or four waves, and the tiles of a workgroup: what is estimated cheapest, in
         // tiles of a workgroup of eight waves on a CU of its own.
         const long long cus = device_cu_count();
-        const int cut = q16 ? kCutBf16 : c.kv == SA_DTYPE_F32 ? kCutF32 : kCutTerms;
+        const int cut = q16 ? (c.d == 128 ? kCutBf16 : kCutBf16Narrow) : c.kv == SA_DTYPE_F32 ? kCutF32 : kCutTerms;
         const bool terms = !q16 && c.kv != SA_DTYPE_F32;   // in four waves always
         int waves = 8;
         double best = INFINITY;
