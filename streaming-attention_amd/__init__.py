@@ -543,8 +543,12 @@ class KVCache:
     def gather(self, layer: int, seq: int, length: int, stream=None):
         import torch
         H, D = self.desc.num_kv_heads, self.desc.head_dim
-        k = _alloc(stream, lambda: torch.empty(H, length, D, dtype=torch.float32, device="cuda"))
-        v = _alloc(stream, lambda: torch.empty_like(k))
+        if stream is None:
+            k = torch.empty(H, length, D, dtype=torch.float32, device="cuda")
+            v = torch.empty_like(k)
+        else:
+            k, v = (_alloc(stream, lambda: torch.empty(H, length, D, dtype=torch.float32, device="cuda"))
+                    for _ in range(2))
         check(lib().sa_kvcache_gather(self.handle, layer, seq, length, k.data_ptr(), v.data_ptr(), _stream(stream)))
         return k, v
 
