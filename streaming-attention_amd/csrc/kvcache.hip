@@ -1236,8 +1236,8 @@ extern "C" sa_status sa_paged_extend(const sa_kvcache* c, int layer, const void*
         if (!vd.ok()) return refused(vd);
         // nothing to do needs no tensors
         if (n_seq > 0 && std::all_of(counts, counts + n_seq, [](int32_t k) { return k == 0; })) return SA_OK;
-        SA_TRY(check_ranges(c, layer, q, n_seq, n_q_heads, out, ws, ws_bytes,
-                            sa_paged_extend_ws_bytes(c, n_seq, counts, n_q_heads)));
+        const size_t need = sa_paged_extend_ws_bytes(c, n_seq, counts, n_q_heads);
+        SA_TRY(check_ranges(c, layer, q, n_seq, n_q_heads, out, ws, ws_bytes, need));
         // Sequences of few and of many query rows go their own ways, one behind the
         // other, in the same workspace.
         const PagedView view = view_of(c, layer);
@@ -1255,6 +1255,9 @@ extern "C" sa_status sa_paged_extend(const sa_kvcache* c, int layer, const void*
             rows += counts[i];
         }
         split_chunks(view.kv, n_q_heads / view.n_kv, view.n_kv, seqs.data(), (int)seqs.size(), &many, &few);
+        // The second way's launch must not be refused behind the first's.
+        if (!many.empty() && !few.empty() && need > 0 && (!ws || ws_bytes < need))
+            return fail(SA_ENOMEM, "workspace too small for the partials");
         if (!many.empty())
             SA_TRY(extend_blocks(view, q, q16, n_q_heads, many.data(), (int)many.size(), scale, out, ws, ws_bytes,
                                  as_stream(stream)));
