@@ -372,7 +372,7 @@ sa_status sa_paged_decode_shared(const sa_kvcache* cache, int layer, const float
  * cache rows or NULL for 0..n_seq-1; a row may be listed more than once.  head_dim 64 or 128, at
  * most 64 query heads per KV head, at most 2^20 new tokens.  What a token does not see does not reach it,
  * NaN and infinities included; rows whose tiles hold such values take longer.
- * q, out and ws 16-byte aligned; out must not overlap q.  ws:
+ * q, out and ws 16-byte aligned, none overlapping another (SA_EINVAL).  ws:
  * sa_paged_extend_ws_bytes bytes, enough for any lengths of the same counts;
  * calls that overlap on one workspace race.  The tokens are those of the lengths
  * at the call, also where a graph that holds the call is replayed.

@@ -1254,6 +1254,9 @@ extern "C" sa_status sa_paged_extend(const sa_kvcache* c, int layer, const void*
             if (counts[i]) seqs.push_back(ChunkSeq{row, len, counts[i], (int)rows});
             rows += counts[i];
         }
+        const size_t bytes = (size_t)rows * n_q_heads * view.d * (q16 ? 2 : 4), used = std::min(ws_bytes, need);
+        if (overlap(out, bytes, q, bytes) || overlap(ws, used, q, bytes) || overlap(ws, used, out, bytes))
+            return fail(SA_EINVAL, "q, out and ws must not overlap");
         split_chunks(view.kv, n_q_heads / view.n_kv, view.n_kv, seqs.data(), (int)seqs.size(), &many, &few);
         // The second way's launch must not be refused behind the first's.
         if (!many.empty() && !few.empty() && need > 0 && (!ws || ws_bytes < need))

@@ -347,5 +347,10 @@ sa_status decode_paged_fused(const PagedView& c, const float* q, int n_seq, cons
                              void* ws, size_t ws_bytes, hipStream_t st);
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+// Whether na bytes at a and nb at b (none where NULL) have some in common.
+inline bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && na && nb && x < y + nb && y < x + na;
+}
 
 }  // namespace sa

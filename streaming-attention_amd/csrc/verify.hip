@@ -647,11 +647,6 @@ bool verify_sizes_ok(int n_seq, const int32_t* counts, int vocab, long long* dra
 
 int segments_of(int vocab) { return (vocab + 3 + kSeg - 1) / kSeg; }   // rows start up to 3 logits into the first
 
-bool overlap(const void* a, size_t na, const void* b, size_t nb) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return a && b && na && nb && x < y + nb && y < x + na;
-}
-
 }  // namespace
 }  // namespace sa
 
