@@ -606,7 +606,7 @@ sa_status sa_beam_select(const float* logits, int64_t row_stride, const float* s
  * a draft row without one rejects its token, whose place is drawn from p.  Drafted
  * tokens outside [0, vocab) are rejected.
  * vocab up to 2^30, n_seq up to 2^20; rows may start at any 4-byte address.  Outputs
- * must not overlap inputs or each other.  ws: 16-byte aligned,
+ * and ws must not overlap inputs or each other (SA_EINVAL).  ws: 16-byte aligned,
  * sa_draft_verify_ws_bytes bytes; calls that overlap on one workspace race.
  * ------------------------------------------------------------------------ */
 size_t sa_draft_verify_ws_bytes(int n_seq, const int32_t* counts, int vocab);

@@ -1014,7 +1014,7 @@ class Qwen3:
             draft.prefill(draft_cache, prompts)
         text = prompts.tolist()
         for t, new in zip(text, sample(logits, uniform(G), temperature).tolist()):
-            t.append(new)
+            t.append(_drawn(new))
         done = [False] * G
         while True:
             for g in range(G):
@@ -1050,9 +1050,7 @@ class Qwen3:
             accepted, new = draft_verify(target, drafts, uniform(sum(kept)), uniform(len(going)), kept, draft=q,
                                          temperature=temperature)
             for g, a, new_tokens in zip(going, accepted.tolist(), new.tolist()):
-                text[g] += new_tokens[:a + 1]
-                if new_tokens[a] < 0:
-                    raise ValueError("logits without a distribution (NaN or infinities)")
+                text[g] += new_tokens[:a] + [_drawn(new_tokens[a])]
             cache.set_lens(going, [len(text[g]) - 1 for g in going])
 
     def _drafts(self, cache, text, counts, temperature, uniform, ids):
@@ -1175,6 +1173,12 @@ class Qwen3:
             last = [(s, p) for s, p in zip(scores[g], paths[g]) if s > float("-inf")]
             out.append(sorted(done[g] + last, key=lambda x: -x[0])[:B])
         return out
+
+
+def _drawn(token: int) -> int:
+    if token < 0:
+        raise ValueError("logits without a distribution (NaN or infinities)")
+    return token
 
 
 def _looked_up(text, n: int):

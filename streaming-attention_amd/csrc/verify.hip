@@ -700,9 +700,13 @@ extern "C" sa_status sa_draft_verify(const float* target, int64_t target_stride,
     const long long wgs = split ? segs : (segs + kWaves - 1) / kWaves;
     // a grid has fewer than 2^32 threads
     if (wgs >= (1LL << 32) / kThreads) return fail(SA_EINVAL, "too many logits for one call");
-    if (!ws || ws_bytes < sa_draft_verify_ws_bytes(n_seq, counts, vocab))
-        return fail(SA_ENOMEM, "workspace too small for the segments");
+    const size_t need = sa_draft_verify_ws_bytes(n_seq, counts, vocab);
+    if (!ws || ws_bytes < need) return fail(SA_ENOMEM, "workspace too small for the segments");
     if (!aligned16(ws)) return fail(SA_EINVAL, "ws must be 16-byte aligned");
+    for (const auto& x : in)
+        if (overlap(ws, need, x.p, x.n)) return fail(SA_EINVAL, "ws must not overlap inputs");
+    if (overlap(ws, need, out_tokens, out_n) || overlap(ws, need, out_accepted, acc_n))
+        return fail(SA_EINVAL, "ws must not overlap outputs");
     a.target = target; a.draft = draft; a.tokens = tokens; a.u_accept = u_accept; a.u_sample = u_sample;
     a.target_stride = target_stride; a.draft_stride = draft_stride;
     a.seg = static_cast<Segment*>(ws);
