@@ -1014,7 +1014,7 @@ class Qwen3:
             draft.prefill(draft_cache, prompts)
         text = prompts.tolist()
         for t, new in zip(text, sample(logits, uniform(G), temperature).tolist()):
-            t.append(_drawn(new))
+            t.append(new)
         done = [False] * G
         while True:
             for g in range(G):
@@ -1022,6 +1022,8 @@ class Qwen3:
                 if eos is not None and eos in new:
                     text[g] = text[g][:L + new.index(eos) + 1]
                     done[g] = True
+                if text[g][-1] < 0:
+                    raise ValueError("logits without a distribution (NaN or infinities)")
                 done[g] = done[g] or len(text[g]) >= L + n_tokens
             if all(done):
                 return [t[L:L + n_tokens] for t in text]
@@ -1050,7 +1052,7 @@ class Qwen3:
             accepted, new = draft_verify(target, drafts, uniform(sum(kept)), uniform(len(going)), kept, draft=q,
                                          temperature=temperature)
             for g, a, new_tokens in zip(going, accepted.tolist(), new.tolist()):
-                text[g] += new_tokens[:a] + [_drawn(new_tokens[a])]
+                text[g] += new_tokens[:a + 1]
             cache.set_lens(going, [len(text[g]) - 1 for g in going])
 
     def _drafts(self, cache, text, counts, temperature, uniform, ids):
@@ -1173,12 +1175,6 @@ class Qwen3:
             last = [(s, p) for s, p in zip(scores[g], paths[g]) if s > float("-inf")]
             out.append(sorted(done[g] + last, key=lambda x: -x[0])[:B])
         return out
-
-
-def _drawn(token: int) -> int:
-    if token < 0:
-        raise ValueError("logits without a distribution (NaN or infinities)")
-    return token
 
 
 def _looked_up(text, n: int):

@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_speculative import CFG128, make_cache, make_model, tokens_of
+from test_gpu_speculative import CFG128, greedy, make_cache, make_model, tokens_of
 
 pytestmark = pytest.mark.gpu
 
@@ -115,3 +115,18 @@ def test_logits_without_a_distribution(sa, n_tokens, T):
     p = tokens_of(8, 1).view(2, 4).contiguous()
     with pytest.raises(ValueError, match="distribution"):
         model.speculative(make_cache(sa, "f32", 2, 64), p, n_tokens, n_draft=2, temperature=T)
+
+
+@pytest.mark.parametrize("drafter", ["itself", "lookup"])
+@pytest.mark.parametrize("n_draft", [0, 1, 3, 6])
+def test_what_follows_eos_does_not_matter(sa, drafter, n_draft):
+    """Logits behind an accepted eos are no token's, whatever they are."""
+    model = make_model(sa, 32, 200)
+    prompts = tokens_of(2 * 9, 11).view(2, 9).contiguous()
+    want = greedy(sa, model, "f32", prompts, 20)
+    eos = want[0][7]
+    assert not (prompts == eos).any()
+    model.tensor(sa.QW_EMBED).view(256, -1)[eos] = float("nan")
+    draft, caches = (model if drafter == "itself" else None), [make_cache(sa, "f32", 2, 60) for _ in range(2)]
+    got = model.speculative(caches[0], prompts, 20, draft, None if draft is None else caches[1], n_draft, 0.0, eos=eos)
+    assert got == [w[:w.index(eos) + 1] if eos in w else w for w in want]
