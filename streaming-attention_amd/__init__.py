@@ -978,7 +978,9 @@ class Qwen3:
         before; one forward of this model verifies them (extend, draft_verify).  generator: a
         CUDA torch.Generator of the uniform numbers.  Rounds need G * (n_draft + 1) <=
         max_batch; a generation that positions or a row's pages have no room for is refused
-        (ValueError) before it begins.  The caches hold the sequences afterwards: reset them."""
+        (ValueError) before it begins, as is one over caches that hold tokens or are another
+        model's; a pool that has too few pages ends it with an SaError.  The caches hold the
+        sequences afterwards: reset them."""
         import torch
         if prompts.dtype != torch.int32 or not prompts.is_cuda or prompts.dim() != 2:
             raise ValueError("prompts must be an int32 CUDA tensor [G, L]")
@@ -991,13 +993,18 @@ class Qwen3:
             raise ValueError("a draft model takes a cache and this model's vocabulary")
         if draft is not None and draft_cache is cache:
             raise ValueError("the draft model takes a cache of its own")
-        for m, c in ((self, cache), (draft, draft_cache)):
-            if m is None:
-                continue
+        pairs = [(self, cache)] if draft is None else [(self, cache), (draft, draft_cache)]
+        for m, c in pairs:
+            if any(getattr(m.desc, f) != getattr(c.desc, g) for f, g in (
+                    ("num_layers", "num_layers"), ("n_kv_heads", "num_kv_heads"), ("head_dim", "head_dim"))):
+                raise ValueError("the cache's geometry does not match the model")
             if G > c.desc.max_seqs or G * (n_draft + 1) > m.max_batch:
                 raise ValueError("the cache and the model need a row per sequence and drafted token")
             if L + n_tokens - 1 > m.desc.max_pos or L + n_tokens - 1 > c.desc.max_pages_per_seq * PAGE_TOKENS:
                 raise ValueError("prompt and tokens need more positions or pages than there are")
+            if any(c.length(g) for g in range(G)):
+                raise ValueError("the prompts take empty caches")
+        for _, c in pairs:
             for g in range(G):
                 c.reserve(g, L + n_tokens - 1)
         dev, V = prompts.device, self.desc.vocab

@@ -1,6 +1,7 @@
 """GPU tests of what speculative generation promises beyond equal greedy tokens: a model
 that drafts for itself is believed, tokens are distributed as the target's own
-whatever drafts them, and logits without a distribution end a generation with an error."""
+whatever drafts them, what cannot run is refused before it begins, and logits
+without a distribution end a generation with an error."""
 from __future__ import annotations
 
 import math
@@ -130,3 +131,27 @@ def test_what_follows_eos_does_not_matter(sa, drafter, n_draft):
     draft, caches = (model if drafter == "itself" else None), [make_cache(sa, "f32", 2, 60) for _ in range(2)]
     got = model.speculative(caches[0], prompts, 20, draft, None if draft is None else caches[1], n_draft, 0.0, eos=eos)
     assert got == [w[:w.index(eos) + 1] if eos in w else w for w in want]
+
+
+def test_refused_before_it_begins(sa):
+    """Neither cache has changed where either does not fit."""
+    model, short = make_model(sa, 16, 100), make_model(sa, 16, 10)
+    p = tokens_of(8, 1).view(2, 4).contiguous()
+    new = lambda pages=2, cfg=None: sa.KVCache(2, 2, 64 if cfg is None else cfg["head_dim"], 2, pages, 2 * pages)  # noqa: E731
+
+    def refused(draft, draft_cache, match, cache=None):
+        cache = new() if cache is None else cache
+        before = [[(c.length(r), c.capacity(r)) for r in range(2)] for c in (cache, draft_cache)]
+        with pytest.raises(ValueError, match=match):
+            model.speculative(cache, p, 20, draft=draft, draft_cache=draft_cache, n_draft=2)
+        assert [[(c.length(r), c.capacity(r)) for r in range(2)] for c in (cache, draft_cache)] == before
+
+    refused(short, new(), "positions")
+    refused(make_model(sa, 2, 100), new(), "row per sequence")
+    used = new()
+    used.reserve(1, 64)
+    used.set_len(1, 3)
+    refused(model, used, "empty")
+    refused(model, new(), "empty", cache=used)
+    refused(model, new(cfg=CFG128), "geometry")
+    refused(model, new(), "geometry", cache=new(cfg=CFG128))
