@@ -1065,20 +1065,20 @@ extern "C" sa_status sa_paged_decode(const sa_kvcache* c, int layer, const float
     if (!valid_cache(c)) return fail(SA_EINVAL, "invalid cache");
     if (layer < 0 || layer >= c->desc.num_layers) return fail(SA_ERANGE, "Layer index out of range");
     if (n_seq <= 0) return fail(SA_EINVAL, "n_seq must be positive");
-    if (c->scales)
-        return no_throw([&] {
+    return no_throw([&]() -> sa_status {
+        if (c->scales)
             return decode_fp8(c, layer, q, n_seq, seq_ids, n_q_heads, n_pending, scale, out, ws, ws_bytes,
                               as_stream(stream));
-        });
-    int max_len = 0;
-    long long total = 0;
-    const Verdict vd = c->pt.check_decode(seq_ids, n_seq, n_pending, &max_len, &total);
-    if (!vd.ok()) return refused(vd);
-    const PagedView pv = view_of(c, layer);
-    std::vector<int32_t> lens(n_seq);
-    for (int i = 0; i < n_seq; ++i) lens[i] = c->pt.len(seq_ids ? seq_ids[i] : i);
-    return decode_paged(pv, q, n_seq, seq_ids, lens.data(), n_q_heads, n_pending, max_len, total, scale, out, ws,
-                        ws_bytes, as_stream(stream));
+        int max_len = 0;
+        long long total = 0;
+        const Verdict vd = c->pt.check_decode(seq_ids, n_seq, n_pending, &max_len, &total);
+        if (!vd.ok()) return refused(vd);
+        const PagedView pv = view_of(c, layer);
+        std::vector<int32_t> lens(n_seq);
+        for (int i = 0; i < n_seq; ++i) lens[i] = c->pt.len(seq_ids ? seq_ids[i] : i);
+        return decode_paged(pv, q, n_seq, seq_ids, lens.data(), n_q_heads, n_pending, max_len, total, scale, out, ws,
+                            ws_bytes, as_stream(stream));
+    });
 }
 
 namespace sa {
@@ -1360,9 +1360,11 @@ extern "C" sa_status sa_append_decode(sa_kvcache* c, int layer, const float* q, 
                                       float* q_out, void* ws, size_t ws_bytes, int commit, sa_stream_t stream) {
     clear_error();
     if (!q || !k || !v) return fail(SA_EINVAL, "null q, k, v or out");
-    return append_decode_impl(c, layer, q, k, v, nullptr, 0, n_seq, seq_ids, n_q_heads, q_norm_w, k_norm_w, eps,
-                              rope_cos, rope_sin, rope_max_pos, scale, out, q_out, ws, ws_bytes, commit,
-                              as_stream(stream));
+    return no_throw([&] {
+        return append_decode_impl(c, layer, q, k, v, nullptr, 0, n_seq, seq_ids, n_q_heads, q_norm_w, k_norm_w, eps,
+                                  rope_cos, rope_sin, rope_max_pos, scale, out, q_out, ws, ws_bytes, commit,
+                                  as_stream(stream));
+    });
 }
 
 extern "C" sa_status sa_append_decode_partials(sa_kvcache* c, int layer, const float* part, int n_part,
@@ -1372,9 +1374,11 @@ extern "C" sa_status sa_append_decode_partials(sa_kvcache* c, int layer, const f
                                                float scale, float* out, float* q_out, void* ws, size_t ws_bytes,
                                                int commit, sa_stream_t stream) {
     clear_error();
-    return append_decode_partials(c, layer, part, n_part, n_seq, seq_ids, n_q_heads, q_norm_w, k_norm_w, eps,
-                                  rope_cos, rope_sin, rope_max_pos, scale, out, q_out, ws, ws_bytes, commit,
-                                  as_stream(stream));
+    return no_throw([&] {
+        return append_decode_partials(c, layer, part, n_part, n_seq, seq_ids, n_q_heads, q_norm_w, k_norm_w, eps,
+                                      rope_cos, rope_sin, rope_max_pos, scale, out, q_out, ws, ws_bytes, commit,
+                                      as_stream(stream));
+    });
 }
 
 extern "C" sa_status sa_kvcache_gather(const sa_kvcache* c, int layer, int seq, int len, float* k_out,
