@@ -249,6 +249,7 @@ struct AppendArgs {
     uint8_t* k_scale; uint8_t* v_scale;   // 8 bits
     int n_q, n_kv, max_pages, rope_max_pos;
     int s0, n_s;               // tokens [s0, s0 + n_s) of each sequence
+    int S;                     // tokens of each sequence; 0: as first[] says
     float eps;
     int32_t first[kRowsPerLaunch + 1];    // sequence i's tokens are first[i] .. first[i + 1] - 1 of q, k and v
 };
@@ -465,8 +466,12 @@ qknorm_rope_append_kernel(AppendArgs a) {
     const int s = a.s0 + (int)(idx / per_token);
     const int id = (int)(idx % per_token);   // query heads, key heads, value heads
     const int i_seq = blockIdx.y;
-    const int first = a.first[i_seq];
-    if (s >= min(a.s0 + a.n_s, a.first[i_seq + 1] - first)) return;
+    int first = i_seq * a.S, end = a.s0 + a.n_s;
+    if (a.S == 0) {
+        first = a.first[i_seq];
+        end = min(end, a.first[i_seq + 1] - first);
+    }
+    if (s >= end) return;
     const bool is_q = id < a.n_q, is_k = !is_q && id < a.n_q + a.n_kv;
     const int head = is_q ? id : is_k ? id - a.n_q : id - a.n_q - a.n_kv;
     const size_t token = (size_t)first + s;
@@ -915,6 +920,7 @@ sa_status append_impl(sa_kvcache* c, int layer, const float* q, const float* k, 
     a.k_scale = k_scales_of(c, layer); a.v_scale = v_scales_of(c, layer);
     a.n_q = q || part ? n_q_heads : 0; a.n_kv = c->desc.num_kv_heads;
     a.max_pages = c->desc.max_pages_per_seq; a.rope_max_pos = rope_max_pos; a.eps = eps;
+    a.S = counts ? 0 : S;
     const int rows = a.n_q + 2 * a.n_kv;
     const int D = c->desc.head_dim;
     const sa_dtype kv = c->desc.kv_dtype;
