@@ -908,6 +908,7 @@ sa_status append_impl(sa_kvcache* c, int layer, const float* q, const float* k, 
     const Verdict vd = counts ? c->pt.check_append(seq_ids, n_seq, counts, rope_cos ? rope_max_pos : 0)
                               : c->pt.check_append(seq_ids, n_seq, S, rope_cos ? rope_max_pos : 0);
     if (!vd.ok()) return refused(vd);
+    if (counts) SA_TRY(on_cache_device(c));
     long long tokens = 0;
     for (int i = 0; i < n_seq; ++i) tokens += counts ? counts[i] : S;
     if (tokens > 0x7fffffffLL) return fail(SA_EINVAL, "more than 2^31 - 1 new tokens");
@@ -1119,7 +1120,7 @@ sa_status sa::check_append(const sa_kvcache* c, int n, int S, int max_pos) {
 
 sa_status sa::check_append_ragged(const sa_kvcache* c, int n, const int32_t* counts, int max_pos) {
     const Verdict v = c->pt.check_append(nullptr, n, counts, max_pos);
-    return v.ok() ? SA_OK : refused(v);
+    return v.ok() ? on_cache_device(c) : refused(v);
 }
 
 long long sa::shared_tokens_saved(const sa_kvcache* c, const int32_t* sizes, int n_groups) {

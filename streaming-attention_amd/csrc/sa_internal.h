@@ -287,7 +287,7 @@ sa_status append_decode_partials(sa_kvcache* c, int layer, const float* part, in
 // Whether the next S tokens of rows 0 .. n - 1 can be appended: pages of their
 // own for them, and positions below max_pos.
 sa_status check_append(const sa_kvcache* c, int n, int S, int max_pos);
-// The same of counts[i] tokens of row i.
+// The same of counts[i] tokens of row i, on the cache's device.
 sa_status check_append_ragged(const sa_kvcache* c, int n, const int32_t* counts, int max_pos);
 
 constexpr int kMaxNewTokens = 1 << 20;   // of one call over chunks of new tokens
