@@ -196,7 +196,7 @@ __device__ __forceinline__ void block_plain(const BlockArgs& a, const Block& w, 
                            k0 % SA_PAGE_TOKENS;
         auto value = [&](const void* pool, int i) { return static_cast<const E*>(pool) + (key + i) * D; };
         auto scale = [&](const uint8_t* s, int i) {
-            if constexpr (KV == SA_DTYPE_FP8) return __uint_as_float((uint32_t)s[key + i] << 23);
+            if constexpr (KV == SA_DTYPE_FP8) return scale_of(s[key + i]);
             else return 1.f;
         };
         p.keys(min(TILE, end - k0), static_cast<const T*>(a.q) + o, a.factor,
@@ -218,16 +218,6 @@ __device__ __forceinline__ void block_plain(const BlockArgs& a, const Block& w, 
 }
 
 // ---------------------------------------------------------------- bf16
-
-// Sixteen codes of a row as two chunks of LDS.
-__device__ __forceinline__ bf16x8_t widen8(uint32_t lo, uint32_t hi, float scale) {
-    const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
-    const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
-    const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
-    const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
-    return __builtin_bit_cast(bf16x8_t, u32x4_t{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b),
-                                                __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)});
-}
 
 template <int D, int W, bool FP8>
 __global__ void __launch_bounds__(W * kWave, W == 8 && D == 64 ? 4 : 1) extend_bf16_kernel(BlockArgs a) {
@@ -299,9 +289,9 @@ __global__ void __launch_bounds__(W * kWave, W == 8 && D == 64 ? 4 : 1) extend_b
             for (int h = 0; h < 2; ++h) {
                 lds_u8_t* at = dst + r * G::ROWB + (((c + h) ^ G::swz(r & 15)) << 4);
                 *reinterpret_cast<__attribute__((address_space(3))) bf16x8_t*>(at) =
-                    widen8(rk[i][2 * h], rk[i][2 * h + 1], __uint_as_float(sk[i] << 23));
+                    codes_bf16x8(rk[i][2 * h], rk[i][2 * h + 1], scale_of(sk[i]));
                 *reinterpret_cast<__attribute__((address_space(3))) bf16x8_t*>(at + G::HALF) =
-                    widen8(rv[i][2 * h], rv[i][2 * h + 1], __uint_as_float(sv[i] << 23));
+                    codes_bf16x8(rv[i][2 * h], rv[i][2 * h + 1], scale_of(sv[i]));
             }
         }
     };
@@ -498,7 +488,7 @@ struct Staged {
         if constexpr (KV == SA_DTYPE_F32)
             split_terms(__builtin_bit_cast(f32x4_t, x[0]), __builtin_bit_cast(f32x4_t, x[1]), t);
         else if constexpr (KV == SA_DTYPE_BF16) t[0] = __builtin_bit_cast(bf16x8_t, x[0]);
-        else t[0] = widen8(x[0][0], x[0][1], __uint_as_float(scale << 23));
+        else t[0] = codes_bf16x8(x[0][0], x[0][1], scale_of(scale));
     }
 };
 
@@ -686,13 +676,6 @@ __global__ void __launch_bounds__(W * kWave) extend_f32_kernel(BlockArgs a) {
 
 // ---------------------------------------------------------------- partials
 
-__device__ __forceinline__ void put4(float* p, f32x4_t v) { *reinterpret_cast<f32x4_t*>(p) = v; }
-__device__ __forceinline__ void put4(uint16_t* p, f32x4_t v) {
-    const bf16x2_t lo = __builtin_convertvector(f32x2_t{v[0], v[1]}, bf16x2_t);
-    const bf16x2_t hi = __builtin_convertvector(f32x2_t{v[2], v[3]}, bf16x2_t);
-    *reinterpret_cast<uint2*>(p) = make_uint2(__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi));
-}
-
 // O = sum_c 2^(m_c - M) O_c / sum_c 2^(m_c - M) l_c, D / 4 lanes per row of 256 D / 4
 // consecutive (token, head) rows from the launch's first token on.
 template <int D, class T, bool EVEN>
@@ -739,7 +722,7 @@ __global__ void __launch_bounds__(256) block_merge_kernel(BlockArgs a, long long
         L = L * w0 + ml[1] * w1;
         M = m_new;
     }
-    put4(static_cast<T*>(a.out) + ((size_t)token * a.n_q + head) * D + 4 * c, o * (1.0f / L));
+    store4(static_cast<T*>(a.out) + ((size_t)token * a.n_q + head) * D + 4 * c, o * (1.0f / L));
 }
 
 // ---------------------------------------------------------------- launch

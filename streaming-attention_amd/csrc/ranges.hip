@@ -189,17 +189,6 @@ __device__ __forceinline__ void dma4_nt(const void* g, lds_u8_t* dst) {
     asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off nt" ::"v"(g), "s"(m) : "memory", "m0");
 }
 
-// Eight codes, times a power of two.
-__device__ __forceinline__ bf16x8_t codes_bf16x8(uint32_t lo, uint32_t hi, float scale) {
-    const bf16x2_t a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);
-    const bf16x2_t b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true);
-    const bf16x2_t c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false);
-    const bf16x2_t d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true);
-    return __builtin_bit_cast(bf16x8_t, u32x4_t{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b),
-                                                __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)});
-}
-__device__ __forceinline__ float scale_of(uint32_t byte) { return __uint_as_float(byte << 23); }
-
 template <int N>
 __device__ __forceinline__ void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -463,13 +452,6 @@ __device__ __forceinline__ int group_chunks(const RangeArgs& a, int g) {
 }
 __device__ __forceinline__ int own_chunks(const RangeArgs& a, int row) {
     return a.start[a.n_groups + row + 1] - a.start[a.n_groups + row];
-}
-
-__device__ __forceinline__ void store4(float* p, f32x4_t v) { *reinterpret_cast<f32x4_t*>(p) = v; }
-__device__ __forceinline__ void store4(uint16_t* p, f32x4_t v) {
-    const bf16x2_t lo = __builtin_convertvector(f32x2_t{v[0], v[1]}, bf16x2_t);
-    const bf16x2_t hi = __builtin_convertvector(f32x2_t{v[2], v[3]}, bf16x2_t);
-    *reinterpret_cast<u32x2_t*>(p) = u32x2_t{__builtin_bit_cast(uint32_t, lo), __builtin_bit_cast(uint32_t, hi)};
 }
 
 // O (unnormalised), m and l of query row j of an item: the output itself if it
