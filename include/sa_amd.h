@@ -306,6 +306,9 @@ sa_status sa_qk_norm_rope_ex(const float* x, int n_rows, int D, const int32_t* p
  * stream order); lengths written into sa_kvcache_seq_lens by other code are
  * not read.  q [n_seq][n_q_heads][D] fp32, out likewise.
  * ws must hold sa_paged_decode_ws_bytes(...) bytes.
+ * n_q_heads / num_kv_heads: 1, 2, 4 or 8; over a cache in 8 bits any up to 64, with
+ * q, out and ws 16-byte aligned and the cache's device current (SA_EINVAL
+ * otherwise).
  * ------------------------------------------------------------------------ */
 size_t sa_paged_decode_ws_bytes(const sa_kvcache* cache, int n_seq, int n_q_heads);
 sa_status sa_paged_decode(const sa_kvcache* cache, int layer, const float* q,
@@ -367,8 +370,10 @@ sa_status sa_paged_decode_shared(const sa_kvcache* cache, int layer, const float
  *   out_ij = softmax(scale q_ij k_t) v_t over t <= len + j.
  * q and out [sum counts][n_q_heads][D], the sequences' tokens one behind the
  * other, both in q_dtype: fp32 with any cache, accurate to fp32; bf16 with a bf16
- * or 8-bit cache, where large chunks take products of bf16 operands (weights
- * rounded to bf16) with fp32 sums and softmax.  seq_ids: host array [n_seq] of
+ * or 8-bit cache, where chunks of many query rows, and short ones beside them where they
+ * cost little more, take products of bf16 operands (weights rounded to bf16, 2^-8 of
+ * each) with fp32 sums and softmax: a sequence's bits depend on the others of its
+ * call, and equal calls give equal bits.  seq_ids: host array [n_seq] of
  * cache rows or NULL for 0..n_seq-1; a row may be listed more than once.  head_dim 64 or 128, at
  * most 64 query heads per KV head, at most 2^20 new tokens.  What a token does not see does not reach it,
  * NaN and infinities included; rows whose tiles hold such values take longer.
@@ -396,8 +401,10 @@ sa_status sa_paged_extend(const sa_kvcache* cache, int layer, const void* q, sa_
  * rotated q.  Other arguments as in sa_qknorm_rope_append and
  * sa_paged_decode (ws: sa_paged_decode_ws_bytes bytes).  Sequences whose
  * cache plus the new token fit one chunk take a single kernel launch per 64
- * sequences; longer ones add the LSE merge launch.  Rows are checked as for
- * an append of one token; a refused call enqueues nothing.
+ * sequences; longer ones add the LSE merge launch.  Over a cache in 8 bits the
+ * append, the decode and the commit are launches of their own, out, q_out and ws
+ * are 16-byte aligned, and head ratio and device are as in sa_paged_decode.  Rows
+ * are checked as for an append of one token; a refused call enqueues nothing.
  * ------------------------------------------------------------------------ */
 sa_status sa_append_decode(sa_kvcache* cache, int layer, const float* q, const float* k,
                            const float* v, int n_seq, const int32_t* seq_ids, int n_q_heads,

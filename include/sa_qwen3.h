@@ -170,8 +170,9 @@ sa_status sa_qwen3_beam_step(sa_qwen3* model, sa_kvcache* cache, const int32_t* 
  * appended is committed by sa_kvcache_set_lens as far as it is accepted
  * (sa_draft_verify), or overwritten by the next append.  The caller must have
  * reserved pages of every row's own for the new tokens; at most 2^20 of them.
- * Asynchronous on stream; a graph that holds a call repeats it for the lengths at
- * the call, also after larger calls.  Refused calls enqueue nothing. */
+ * Asynchronous on stream; the first call of a size allocates its workspace (capture
+ * a graph after one); a graph that holds a call repeats it for the lengths at the
+ * call, also after larger calls.  Refused calls enqueue nothing. */
 sa_status sa_qwen3_extend(sa_qwen3* model, sa_kvcache* cache, const int32_t* tokens, int n_seq,
                           const int32_t* counts, int all_rows, int32_t* next_tokens, float* logits, int commit,
                           sa_stream_t stream);

@@ -28,11 +28,13 @@
 // Rows whose sums are not finite are computed anew over what they see (plain_row.h).
 //
 // Bound, 16 / 8 heads of 128: MFMA and the softmax's VALU work beside it.  2048 bf16 tokens
-// behind 30720, 533 GF: 505 us, 1.06 PFLOP/s, MFMA 53 % and VALU 44 % busy, the second
-// launch 17 of them.  512 fp32 tokens behind 3584, 16.1 GF x 6: 92 us, 1.05 PFLOP/s of
-// products, MFMA 51 %, VALU 39 %.  Seven chunks of 1 - 700 tokens over 8 bits, 32 / 8 heads of
-// 64, 82.9 GF: 130 us; at 64 the softmax is as long as the products (VALU 63 %, MFMA 40 %),
-// and rounds of workgroups of unequal lengths cost a tenth.
+// behind 30720, 533 GF: 505 - 523 us, 1.02 - 1.06 PFLOP/s of 1.6 that a large product
+// reaches, MFMA 53 % and VALU 44 % busy, the second launch 17 of them.  512 fp32 tokens behind
+// 3584, 16.1 GF x 6: 92 - 94 us, 1.03 - 1.05 PFLOP/s of products, MFMA 51 %, VALU 39 %; fp32 over
+// bf16 or 8 bits, three products, 2048 behind 8192: 426 - 432 us, 1.08.  Seven chunks of
+// 1 - 700 tokens over 8 bits, 32 / 8 heads of 64, 82.9 GF: 130 - 134 us; at 64 the softmax is as
+// long as the products (VALU 63 %, MFMA 40 %), the joining launch takes 15, and rounds of
+// workgroups of unequal lengths cost a tenth.
 #include <algorithm>
 #include <cmath>
 #include <vector>
@@ -339,8 +341,9 @@ __global__ void __launch_bounds__(W * kWave, W == 8 && D == 64 ? 4 : 1) extend_b
                 const uint32_t hb = sb + kb * 32 * G::ROWB;
                 if (k > q_hi) continue;
                 // Eight waves come here only with the tiles at the diagonal: one form, with
-                // the mask, is enough, and without the other its registers spill no more
-                // (2048 tokens behind none 71 -> 45 us).
+                // the mask, is enough, and without the other the registers do (2048
+                // tokens behind none 71 -> 45 us), but for five that heads of 64 over 8 bits
+                // still spill around the ping-pong.
                 f32x16_t s = w.scores(hb);
                 if (W == 4 && k + 31 <= q_lo) {
                     w.template weigh<false>(s, hb);

@@ -47,7 +47,9 @@
 // 2.65 per tile of a wave; 4 rows behind 512 tokens, bf16: 9.0).  Over 8 bits 64 rows of
 // 512 - 32768 tokens, 2.12 GB, take 341 us (6.2 TB/s; MFMA 31 % and VALU 52 % busy), one row
 // of 5000 14.1; chunks of 5 tokens of each of 64 sequences of 512 - 16384, bf16, 2.18 GB, 363
-// (6.0 TB/s), 5 tokens behind 1000, fp32, 12.6 (9.2 and 4.4 in two launches).
+// (6.0 TB/s), 5 tokens behind 1000, fp32, 12.6 - 13.4 (9.2 and 4.4 alone under the kernel
+// tracer: arguments, table, page ids to LDS and a barrier, K, scores, V, a reduction
+// across the waves, each waiting for the one before it; then the joining launch).
 #include "ranges.h"
 
 #include <algorithm>

@@ -10,19 +10,24 @@
 // whose token also follows.
 //
 // A sum of probabilities decides which token is drawn, and tokens of a large
-// vocabulary lie as close as 1e-6: sums and exponentials are in 64 bits (fp64 FMA runs
-// at fp32's rate here), off by some 1e-13.
+// vocabulary lie as close as 1e-6: sums and exponentials are in 64 bits, off by some
+// 1e-13.
 //
-// Launches: (1) every row is cut into segments of 4096 logits, a workgroup each, which
-// leave their largest logit and sum of exponentials relative to it; (2) with draft
-// logits, what is accepted, and the rejected places' sums of w per segment; (3) a
-// workgroup per sequence finds the segment that the uniform number falls into, then
-// the token (without (2), after deciding what is accepted).
+// Launches: (1) every row is cut into segments of 2048 logits, a wave's each, or where a
+// call has fewer than 4096 of them a workgroup's, which leave a logit that no other
+// exceeds by far and the sum of exponentials relative to it (T = 0: the largest and its
+// token); (2) with draft logits, what is accepted, a workgroup per sequence, and the
+// rejected places' sums of w per segment; (3) a workgroup per sequence finds the
+// segment that the uniform number falls into, then the token (without (2), after
+// deciding what is accepted).
 //
-// Bound: fp64 arithmetic of the first launch (a logit's exponential and sum: VALU 95 %
-// busy; its reads alone would be 55), latency of the others.  64 sequences of 4 drafts, 576 rows
-// of 151,936 logits, 350 MB: 107 us, in launches of 73, 5, 21 and 8; one sequence 17.9 (4.6, 4.4,
-// 4.0, 6.0); 5 sequences of looked-up drafts, 32,003 logits, 11.7 (4.1 and 8.4).
+// Bound: 64-bit arithmetic of the first launch, per logit ten FMAs (2.33 ns per wave and
+// SIMD), four additions and a conversion (1.95) among some 21 instructions, VALU 95 % busy
+// (its reads alone would be 54 us); in the others a workgroup's chain of dependent reads,
+// scans and barriers.  64 sequences of 4 drafts, 576 rows of 151,936 logits, 350 MB: 100 -
+// 108 us; one sequence 17.6 - 18.2; 5 sequences of looked-up drafts, 32,003 logits, 11.7.
+// Alone under the kernel tracer, gaps between and the clock lower, the launches take 73, 5,
+// 21 and 8; 4.6, 4.4, 4.0 and 6.0; 4.1 and 8.4.
 #include "sa_internal.h"
 
 #include <algorithm>
