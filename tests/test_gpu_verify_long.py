@@ -19,7 +19,7 @@ SEG = 2048     # logits of a segment
 
 
 def probabilities(x, T):
-    x = np.asarray(x, np.float64) / T
+    x = np.asarray(x, np.float64) / np.float64(np.float32(T))      # the call's temperature is a float
     top = np.max(x)
     if not np.isfinite(top):
         return None
